@@ -20,6 +20,14 @@ from .abi import (  # noqa: F401
     lib_path,
     status_string,
 )
+from .attention import (  # noqa: F401
+    attend,
+    attend_backward,
+    attend_shared,
+    attention_mass,
+    check_attention_status,
+    evict,
+)
 from .index import B200IndexFlat, SearchToken, StandardB200Resources, device_caps  # noqa: F401
 from .sharded import MultiGpuIndexFlat, ShardedIndexFlat, shard_range  # noqa: F401
 from . import abi  # noqa: F401

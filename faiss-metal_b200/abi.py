@@ -54,6 +54,49 @@ class SearchArgs(ctypes.Structure):
     ]
 
 
+class AttendArgs(ctypes.Structure):
+    _fields_ = [
+        ("q", c_vp), ("q_stride", c_i64 * 3), ("shared_k", c_vp), ("shared_v", c_vp),
+        ("shared_k_stride", c_i64 * 2), ("shared_v_stride", c_i64 * 2), ("shared_n", c_i64),
+        ("k", c_vp), ("v", c_vp), ("k_stride", c_i64 * 3), ("v_stride", c_i64 * 3), ("n", c_i64),
+        ("key_lengths", c_vp), ("out", c_vp), ("lse", c_vp), ("scratch", c_vp), ("scratch_bytes", c_sz),
+        ("status", c_vp), ("stream", c_vp), ("batch", c_i64), ("queries", c_i64),
+        ("heads", c_i32), ("kv_heads", c_i32), ("d", c_i32), ("storage", c_i32), ("causal", c_i32),
+        ("scale", ctypes.c_float),
+    ]
+
+
+class AttendBackwardArgs(ctypes.Structure):
+    _fields_ = [
+        ("grad_out", c_vp), ("grad_out_stride", c_i64 * 3), ("q", c_vp), ("q_stride", c_i64 * 3),
+        ("k", c_vp), ("v", c_vp), ("k_stride", c_i64 * 3), ("v_stride", c_i64 * 3), ("n", c_i64),
+        ("key_lengths", c_vp), ("out", c_vp), ("lse", c_vp), ("grad_q", c_vp), ("grad_k", c_vp), ("grad_v", c_vp),
+        ("scratch", c_vp), ("scratch_bytes", c_sz), ("status", c_vp), ("stream", c_vp),
+        ("batch", c_i64), ("queries", c_i64),
+        ("heads", c_i32), ("kv_heads", c_i32), ("d", c_i32), ("storage", c_i32), ("scale", ctypes.c_float),
+    ]
+
+
+class AttentionMassArgs(ctypes.Structure):
+    _fields_ = [
+        ("q", c_vp), ("q_stride", c_i64 * 3), ("k", c_vp), ("k_stride", c_i64 * 3), ("n", c_i64),
+        ("key_lengths", c_vp), ("lse", c_vp), ("mass_in", c_vp), ("mass_out", c_vp),
+        ("scratch", c_vp), ("scratch_bytes", c_sz), ("status", c_vp), ("stream", c_vp),
+        ("batch", c_i64), ("queries", c_i64),
+        ("heads", c_i32), ("kv_heads", c_i32), ("d", c_i32), ("storage", c_i32), ("causal", c_i32),
+        ("scale", ctypes.c_float),
+    ]
+
+
+class EvictArgs(ctypes.Structure):
+    _fields_ = [
+        ("k", c_vp), ("v", c_vp), ("k_stride", c_i64 * 3), ("v_stride", c_i64 * 3), ("n", c_i64),
+        ("mass", c_vp), ("key_lengths", c_vp), ("keep", c_i64), ("recent", c_i64),
+        ("out_k", c_vp), ("out_v", c_vp), ("out_mass", c_vp), ("out_rows", c_vp), ("out_lengths", c_vp),
+        ("stream", c_vp), ("batch", c_i64), ("kv_heads", c_i32), ("d", c_i32), ("storage", c_i32),
+    ]
+
+
 # name -> (restype, argtypes); the symbol test checks this table against the header
 SIGNATURES = {
     "b200f_status_string": (ctypes.c_char_p, [c_int]),
@@ -82,6 +125,14 @@ SIGNATURES = {
     "b200f_merge_lists": (c_int, [c_vp, c_vp, c_int, c_i64, c_int, c_int, c_vp, c_vp, c_vp]),
     "b200f_merge_lists_strided": (c_int, [c_vp, c_vp, c_i64, c_i64, c_int, c_i64, c_int, c_int, c_vp, c_vp, c_vp]),
     "b200f_remap_labels_block_cyclic": (c_int, [c_vp, c_i64, c_i64, c_int, c_int, c_vp]),
+    "b200f_attend_scratch_bytes": (c_sz, [ctypes.POINTER(AttendArgs)]),
+    "b200f_attend": (c_int, [ctypes.POINTER(AttendArgs)]),
+    "b200f_attend_backward_scratch_bytes": (c_sz, [ctypes.POINTER(AttendBackwardArgs)]),
+    "b200f_attend_backward": (c_int, [ctypes.POINTER(AttendBackwardArgs)]),
+    "b200f_attention_mass_scratch_bytes": (c_sz, [ctypes.POINTER(AttentionMassArgs)]),
+    "b200f_attention_mass": (c_int, [ctypes.POINTER(AttentionMassArgs)]),
+    "b200f_evict": (c_int, [ctypes.POINTER(EvictArgs)]),
+    "b200f_attention_status": (c_vp, []),
     "b200f_fill_synthetic": (c_int, [c_vp, c_i64, c_int, c_i64, ctypes.c_uint64, c_int, ctypes.c_float, c_vp]),
     "b200f_profile_enable": (c_int, [c_int]),
     "b200f_profile_read": (c_int, [ctypes.POINTER(c_i64), ctypes.POINTER(c_i64), ctypes.POINTER(ctypes.c_double), c_int]),

@@ -1,0 +1,344 @@
+"""Soft reads of stored rows (the ``b200f_attend*`` / ``b200f_attention_mass`` / ``b200f_evict`` entry points).
+
+``B200IndexFlat.search`` reads a store the hard way: inner products with all rows, then the k largest.  A model that
+attends to stored states reads them the soft way, with a softmax in the place of the selection:
+
+``attend``           queries of a batch to keys of another length, each sequence its own
+``attend_backward``  its gradient
+``attend_shared``    one or a few new queries a sequence, to rows that all sequences share and to rows of their own
+``attention_mass``   the weight every row received, added up
+``evict``            the rows of largest weight and the most recent move to a smaller cache
+
+All tensors are torch CUDA tensors of one device, queries, keys and values float16 or bfloat16 in the layout [batch,
+rows, heads, width]; any strides whose last is 1 and whose others are multiples of 8 (0 repeats a sequence or a head).
+The work is queued on torch's current stream of that device; nothing waits for it.  A device-side error (a bounded wait that ran
+out) is raised by the next call after it happened, or by ``check_attention_status()``.
+
+The functions do not record gradients: inputs that require them are refused unless gradients are off
+(``torch.no_grad()``); ``attend_backward`` is the gradient.
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+
+from . import abi
+
+_STORAGE = {"float16": abi.STORAGE_F16, "bfloat16": abi.STORAGE_BF16}
+MAX_WIDTH = 128
+MAX_GROUP = 128
+
+
+def check_attention_status(synchronize: bool = True) -> None:
+    """Raises B200Error if a device-side check of an earlier call of this module failed.  synchronize: waits for
+    torch's current stream first."""
+    if synchronize:
+        import torch
+        torch.cuda.current_stream().synchronize()
+    p = _status()
+    bits = p[0]
+    if bits:
+        p[0] = 0
+        code = abi.ERR_DEVICE_WAIT if bits & 1 else abi.ERR_DEVICE_CHECK
+        raise abi.B200Error(code, "an earlier attention call: " + abi.status_string(code))
+
+
+_status_word = None
+
+
+def _status():
+    global _status_word
+    if _status_word is None:
+        p = abi.lib().b200f_attention_status()
+        if not p:
+            raise abi.B200Error(abi.ERR_NO_DEVICE, abi.status_string(abi.ERR_NO_DEVICE))
+        _status_word = ctypes.cast(p, ctypes.POINTER(ctypes.c_int32))
+    return _status_word
+
+
+class _Call:
+    """One call's arguments: checks tensors, holds the device and the stream."""
+
+    def __init__(self, what: str, first):
+        import torch
+        self.torch = torch
+        self.what = what
+        if not isinstance(first, torch.Tensor):
+            raise TypeError("%s: expected torch tensors" % what)
+        if not first.is_cuda:
+            raise ValueError("%s: expected CUDA tensors" % what)
+        self.device = first.device
+        self.dtype = first.dtype
+        name = str(first.dtype).replace("torch.", "")
+        if name not in _STORAGE:
+            raise ValueError("%s: expected float16 or bfloat16, got %s" % (what, name))
+        self.storage = _STORAGE[name]
+
+    def tensor(self, x, name: str, dims: int, dtype=None):
+        torch = self.torch
+        if not isinstance(x, torch.Tensor):
+            raise TypeError("%s: %s: expected a torch tensor" % (self.what, name))
+        if x.device != self.device:
+            raise ValueError("%s: %s: on %s, expected %s" % (self.what, name, x.device, self.device))
+        if x.dtype != (dtype or self.dtype):
+            raise ValueError("%s: %s: expected dtype %s, got %s" % (self.what, name, dtype or self.dtype, x.dtype))
+        if x.dim() != dims:
+            raise ValueError("%s: %s: expected %d dimensions, got %d" % (self.what, name, dims, x.dim()))
+        if x.requires_grad and torch.is_grad_enabled():
+            raise ValueError("%s: %s requires a gradient, which is not recorded; use torch.no_grad() and attend_backward"
+                             % (self.what, name))
+        return x
+
+    def shape(self, x, name: str, shape):
+        if tuple(x.shape) != tuple(shape):
+            raise ValueError("%s: %s: expected shape %s, got %s" % (self.what, name, tuple(shape), tuple(x.shape)))
+
+    def rows(self, x, name: str, dims: int = 4):
+        """A 16-bit operand; returns its strides but the last."""
+        self.tensor(x, name, dims)
+        if x.numel() and x.shape[-1] > 1 and x.stride(-1) != 1:
+            raise ValueError("%s: %s: the last dimension must be dense" % (self.what, name))
+        if x.numel() and x.data_ptr() % 16:
+            raise ValueError("%s: %s: must lie on a 16-byte boundary" % (self.what, name))
+        out = []
+        for i in range(dims - 1):
+            s = x.stride(i) if x.shape[i] > 1 else 0
+            if x.numel() and (s % 8 or (s == 0 and x.shape[i] > 1 and i == max(dims - 3, 0))):
+                raise ValueError("%s: %s: stride %d of dimension %d is no positive multiple of 8" % (self.what, name, s, i))
+            out.append(s)
+        return out
+
+    def dense(self, x, name: str, shape, dtype):
+        self.tensor(x, name, len(shape), dtype)
+        self.shape(x, name, shape)
+        if not x.is_contiguous():
+            raise ValueError("%s: %s: must be contiguous" % (self.what, name))
+        return x
+
+    def lengths(self, x, batch: int, name: str = "key_lengths"):
+        if x is None:
+            return None
+        return self.dense(x, name, (batch,), self.torch.int32).data_ptr()
+
+    def heads(self, h: int, hk: int, d: int):
+        if hk < 1 or h < 1 or h % hk or h // hk > MAX_GROUP:
+            raise ValueError("%s: %d heads do not divide into groups of %d key heads (at most %d heads a group)"
+                             % (self.what, h, hk, MAX_GROUP))
+        if d < 8 or d > MAX_WIDTH or d % 8:
+            raise ValueError("%s: width %d is no multiple of 8 up to %d" % (self.what, d, MAX_WIDTH))
+
+    def scale(self, scale, d: int) -> float:
+        s = 1.0 / math.sqrt(d) if scale is None else float(scale)
+        if not (0.0 < s < 3.0e38):
+            raise ValueError("%s: scale must be positive and finite" % self.what)
+        return s
+
+    def empty(self, shape, dtype=None):
+        return self.torch.empty(shape, dtype=dtype or self.dtype, device=self.device)
+
+    def run(self, fn, args, scratch_fn=None):
+        torch = self.torch
+        check_attention_status(synchronize=False)
+        with torch.cuda.device(self.device):
+            args.status = ctypes.addressof(_status().contents)
+            args.stream = torch.cuda.current_stream(self.device).cuda_stream
+            keep = None
+            if scratch_fn is not None:
+                n = scratch_fn(ctypes.byref(args))
+                keep = torch.empty(max(n, 256), dtype=torch.uint8, device=self.device)
+                args.scratch, args.scratch_bytes = keep.data_ptr(), keep.numel()
+            abi.check_op(fn(ctypes.byref(args)), self.what)
+
+
+def _set(args, name, strides):
+    for i, s in enumerate(strides):
+        getattr(args, name)[i] = s
+
+
+def attend(q, k, v, *, key_lengths=None, scale=None, return_lse=False):
+    """Cross attention: softmax(scale * q k^T) v.
+
+    q [batch, queries, heads, width]; k, v [batch, keys, key heads, width]; query head h reads key head
+    h // (heads // key heads).  key_lengths (int32 [batch], on the device): sequence b sees its first key_lengths[b]
+    keys; what lies behind them has no influence.  scale: 1 / sqrt(width) by default.  Returns the output, like q, and with
+    return_lse also the log of each row's sum of exponentials, float32 [batch, queries, heads].  A sequence that sees no
+    key has output 0 and log-sum -inf."""
+    c = _Call("attend", q)
+    a = abi.AttendArgs()
+    _set(a, "q_stride", c.rows(q, "q"))
+    _set(a, "k_stride", c.rows(k, "k"))
+    _set(a, "v_stride", c.rows(v, "v"))
+    b, t, h, d = q.shape
+    n, hk = k.shape[1], k.shape[2]
+    c.heads(h, hk, d)
+    c.shape(k, "k", (b, n, hk, d))
+    c.shape(v, "v", (b, n, hk, d))
+    a.key_lengths = c.lengths(key_lengths, b)
+    out = c.empty((b, t, h, d))
+    lse = c.empty((b, t, h), c.torch.float32) if return_lse else None
+    a.q, a.k, a.v, a.out = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()
+    a.lse = lse.data_ptr() if return_lse else None
+    a.n, a.batch, a.queries, a.heads, a.kv_heads, a.d, a.storage = n, b, t, h, hk, d, c.storage
+    a.scale = c.scale(scale, d)
+    c.run(abi.lib().b200f_attend, a, abi.lib().b200f_attend_scratch_bytes)
+    return (out, lse) if return_lse else out
+
+
+def attend_backward(grad_out, q, k, v, out, lse, *, key_lengths=None, scale=None):
+    """Gradient of attend(): (grad_q, grad_k, grad_v), dense, of the shapes of q, k and v.
+
+    out and lse are what attend() returned for the same q, k, v, key_lengths and scale; grad_out has the shape of out.
+    Keys that no query sees get 0.  Where k or v repeat sequences or heads (stride 0), their gradients come
+    for every repetition; add them up."""
+    c = _Call("attend_backward", q)
+    a = abi.AttendBackwardArgs()
+    _set(a, "grad_out_stride", c.rows(grad_out, "grad_out"))
+    _set(a, "q_stride", c.rows(q, "q"))
+    _set(a, "k_stride", c.rows(k, "k"))
+    _set(a, "v_stride", c.rows(v, "v"))
+    b, t, h, d = q.shape
+    n, hk = k.shape[1], k.shape[2]
+    c.heads(h, hk, d)
+    c.shape(k, "k", (b, n, hk, d))
+    c.shape(v, "v", (b, n, hk, d))
+    c.shape(grad_out, "grad_out", (b, t, h, d))
+    c.dense(out, "out", (b, t, h, d), c.dtype)
+    c.rows(out, "out")
+    c.dense(lse, "lse", (b, t, h), c.torch.float32)
+    a.key_lengths = c.lengths(key_lengths, b)
+    gq, gk, gv = c.empty((b, t, h, d)), c.empty((b, n, hk, d)), c.empty((b, n, hk, d))
+    a.grad_out, a.q, a.k, a.v, a.out = (x.data_ptr() for x in (grad_out, q, k, v, out))
+    a.lse, a.grad_q, a.grad_k, a.grad_v = (x.data_ptr() for x in (lse, gq, gk, gv))
+    a.n, a.batch, a.queries, a.heads, a.kv_heads, a.d, a.storage = n, b, t, h, hk, d, c.storage
+    a.scale = c.scale(scale, d)
+    c.run(abi.lib().b200f_attend_backward, a, abi.lib().b200f_attend_backward_scratch_bytes)
+    return gq, gk, gv
+
+
+def attend_shared(q, shared_k, shared_v, own_k, own_v, own_lengths=None, *, scale=None, return_lse=False):
+    """Attention of a batch whose sequences share a long prefix, which is read once for all of them.
+
+    q [batch, new, heads, width]: the last `new` tokens of every sequence, one when decoding; shared_k, shared_v [prefix,
+    key heads, width]; own_k, own_v [batch, rows, key heads, width], with the new tokens' rows already in them;
+    own_lengths (int32 [batch], on the device): rows of each sequence, the new ones included (default: all).  Query t sees
+    the whole prefix and the own rows j < own_lengths[b] - new + 1 + t.  Returns the output, like q, and with return_lse the log-sums
+    over both parts, float32 [batch, new, heads]."""
+    c = _Call("attend_shared", q)
+    a = abi.AttendArgs()
+    _set(a, "q_stride", c.rows(q, "q"))
+    _set(a, "shared_k_stride", c.rows(shared_k, "shared_k", 3))
+    _set(a, "shared_v_stride", c.rows(shared_v, "shared_v", 3))
+    _set(a, "k_stride", c.rows(own_k, "own_k"))
+    _set(a, "v_stride", c.rows(own_v, "own_v"))
+    b, t, h, d = q.shape
+    p, hk = shared_k.shape[0], shared_k.shape[1]
+    n = own_k.shape[1]
+    c.heads(h, hk, d)
+    c.shape(shared_k, "shared_k", (p, hk, d))
+    c.shape(shared_v, "shared_v", (p, hk, d))
+    c.shape(own_k, "own_k", (b, n, hk, d))
+    c.shape(own_v, "own_v", (b, n, hk, d))
+    a.key_lengths = c.lengths(own_lengths, b, "own_lengths")
+    out = c.empty((b, t, h, d))
+    lse = c.empty((b, t, h), c.torch.float32) if return_lse else None
+    a.q, a.shared_k, a.shared_v, a.k, a.v, a.out = (x.data_ptr() for x in (q, shared_k, shared_v, own_k, own_v, out))
+    a.lse = lse.data_ptr() if return_lse else None
+    a.shared_n, a.n, a.batch, a.queries, a.heads, a.kv_heads, a.d, a.storage = p, n, b, t, h, hk, d, c.storage
+    a.causal = 1
+    a.scale = c.scale(scale, d)
+    c.run(abi.lib().b200f_attend, a, abi.lib().b200f_attend_scratch_bytes)
+    return (out, lse) if return_lse else out
+
+
+def attention_mass(q, k, lse, *, key_lengths=None, scale=None, causal=False, mass=None):
+    """Accumulated attention weight: float32 [batch, key heads, keys], `mass` (zeros by default) plus what every key got from
+    the queries of its group, sum of exp(scale * q.k - lse).
+
+    q, k, key_lengths and scale as for attend(); lse float32 [batch, queries, heads] from attend(), or from attend_shared(), for which
+    k are the own rows and causal is True (query t sees j < key_lengths[b] - queries + 1 + t), or the prefix, as one
+    sequence."""
+    c = _Call("attention_mass", q)
+    a = abi.AttentionMassArgs()
+    _set(a, "q_stride", c.rows(q, "q"))
+    _set(a, "k_stride", c.rows(k, "k"))
+    b, t, h, d = q.shape
+    n, hk = k.shape[1], k.shape[2]
+    c.heads(h, hk, d)
+    c.shape(k, "k", (b, n, hk, d))
+    c.dense(lse, "lse", (b, t, h), c.torch.float32)
+    a.key_lengths = c.lengths(key_lengths, b)
+    if mass is not None:
+        a.mass_in = c.dense(mass, "mass", (b, hk, n), c.torch.float32).data_ptr()
+    out = c.empty((b, hk, n), c.torch.float32)
+    a.q, a.k, a.lse, a.mass_out = q.data_ptr(), k.data_ptr(), lse.data_ptr(), out.data_ptr()
+    a.n, a.batch, a.queries, a.heads, a.kv_heads, a.d, a.storage = n, b, t, h, hk, d, c.storage
+    a.causal = 1 if causal else 0
+    a.scale = c.scale(scale, d)
+    c.run(abi.lib().b200f_attention_mass, a, abi.lib().b200f_attention_mass_scratch_bytes)
+    return out
+
+
+def evict(k, v, mass, key_lengths=None, keep=1, *, recent=0):
+    """Cuts a cache down to `keep` rows a sequence and key head: the last `recent` rows and, of those before them, the ones of
+    largest mass (ties to the lower row, NaN counts as largest); all rows where there are no more than `keep`.
+
+    k, v [batch, rows, key heads, width]; mass float32 [batch, key heads, rows]; key_lengths int32 [batch] or None.  Returns
+    (k, v, mass, rows, lengths): caches of `keep` rows in the old order, zero behind the last one, their mass [batch, key heads,
+    keep], the row each slot was (int32, -1 behind the last one) and the new lengths (int32 [batch])."""
+    c = _Call("evict", k)
+    a = abi.EvictArgs()
+    _set(a, "k_stride", c.rows(k, "k"))
+    _set(a, "v_stride", c.rows(v, "v"))
+    b, n, hk, d = k.shape
+    c.shape(v, "v", (b, n, hk, d))
+    if hk < 1 or d < 8 or d % 8:
+        raise ValueError("evict: width %d of %d key heads: expected a multiple of 8, and a head" % (d, hk))
+    keep, recent = int(keep), int(recent)
+    if keep < 1 or recent < 0 or recent > keep:
+        raise ValueError("evict: expected keep >= 1 and 0 <= recent <= keep, got %d and %d" % (keep, recent))
+    c.dense(mass, "mass", (b, hk, n), c.torch.float32)
+    a.key_lengths = c.lengths(key_lengths, b)
+    out_k, out_v = c.empty((b, keep, hk, d)), c.empty((b, keep, hk, d))
+    out_mass = c.empty((b, hk, keep), c.torch.float32)
+    out_rows = c.empty((b, hk, keep), c.torch.int32)
+    out_lengths = c.empty((b,), c.torch.int32)
+    a.k, a.v, a.mass = k.data_ptr(), v.data_ptr(), mass.data_ptr()
+    a.out_k, a.out_v, a.out_mass, a.out_rows, a.out_lengths = (
+        x.data_ptr() for x in (out_k, out_v, out_mass, out_rows, out_lengths))
+    a.n, a.keep, a.recent, a.batch, a.kv_heads, a.d, a.storage = n, keep, recent, b, hk, d, c.storage
+    with c.torch.cuda.device(c.device):
+        a.stream = c.torch.cuda.current_stream(c.device).cuda_stream
+        abi.check_op(abi.lib().b200f_evict(ctypes.byref(a)), "evict")
+    return out_k, out_v, out_mass, out_rows, out_lengths
+
+
+def attend_index(index, x, values, scale, return_lse):
+    """B200IndexFlat.attend()."""
+    c = _Call("attend", x)
+    if index.metric_type != abi.METRIC_INNER_PRODUCT:
+        raise ValueError("attend: the index must be one of inner products")
+    if index.storage != c.storage:
+        raise ValueError("attend: x must have the index's storage type (float16 or bfloat16), got %s" % c.dtype)
+    if c.device.index != index.resources.device:
+        raise ValueError("attend: x is on %s, the index on device %d" % (c.device, index.resources.device))
+    if c.torch.cuda.is_current_stream_capturing():
+        raise ValueError("attend: the rows of an index may move, a graph cannot hold their address")
+    n, d = index.ntotal, index.d
+    a = abi.AttendArgs()
+    xs, vs = c.rows(x, "x", 2), c.rows(values, "values", 2)
+    nq = x.shape[0]
+    c.shape(x, "x", (nq, d))
+    c.shape(values, "values", (n, d))
+    c.heads(1, 1, d)
+    out = c.empty((nq, d))
+    lse = c.empty((nq,), c.torch.float32) if return_lse else None
+    a.q_stride[1] = xs[0]
+    a.k_stride[1], a.v_stride[1] = d, vs[0]   # 16-bit rows of an inner-product index lie side by side
+    a.q, a.k, a.v, a.out = x.data_ptr(), index.device_rows(), values.data_ptr(), out.data_ptr()
+    a.lse = lse.data_ptr() if return_lse else None
+    a.n, a.batch, a.queries, a.heads, a.kv_heads, a.d, a.storage = n, 1, nq, 1, 1, d, c.storage
+    a.scale = c.scale(scale, d)
+    c.run(abi.lib().b200f_attend, a, abi.lib().b200f_attend_scratch_bytes)
+    # adds and resets run on the index's own stream, and have completed when they return
+    index.resources.wait_stream(c.torch.cuda.current_stream(c.device).cuda_stream)
+    return (out, lse) if return_lse else out

@@ -220,6 +220,16 @@ class B200IndexFlat:
                   "search_async")
         return SearchToken(t, (distances, labels))
 
+    def attend(self, x, values, *, scale=None, return_lse=False):
+        """Reads all rows the soft way: softmax(scale * x rows^T) values, where search() takes the k largest inner products.
+
+        Inner-product indexes with FP16 or BF16 storage and d a multiple of 8 up to 128.  x [n, d] and values [ntotal, d]: torch
+        CUDA tensors of the storage's type on the index's device.  scale: 1 / sqrt(d) by default.  Returns [n, d] and, with
+        return_lse, the log-sums, float32 [n].  Queued on torch's current stream; later calls of the index wait for it.  Not
+        while that stream is captured."""
+        from . import attention
+        return attention.attend_index(self, x, values, scale, return_lse)
+
     def reset(self):
         """Removes all rows.  Their device memory stays mapped for the next add(), up to 8 GiB a device;
         StandardB200Resources.release_retained() gives it back."""

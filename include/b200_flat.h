@@ -318,6 +318,142 @@ int b200f_merge_lists_strided(const float* dist, const int64_t* labels, int64_t 
 int b200f_remap_labels_block_cyclic(int64_t* labels, int64_t count, int64_t block_rows, int nshards, int shard,
                                     void* stream);
 
+/* ---- soft reads of stored rows (device pointers, async on `stream`) ------ */
+/* b200f_search reads a store the hard way: inner products with all rows, then the k largest.  These entry
+ * points read it the soft way, with a softmax over the inner products in the place of the selection, as a
+ * model does that attends to stored states.  The reference has no counterpart.
+ *
+ * Layouts (elements of the 16-bit type `storage`, B200F_STORAGE_F16 or B200F_STORAGE_BF16; the last
+ * dimension is dense, the others have the strides given, in elements):
+ *   queries [batch][queries][heads][d], keys and values [batch][n][kv_heads][d];
+ *   query head h reads key head h / (heads / kv_heads);
+ *   log-sums [batch][queries][heads] and weights [batch][kv_heads][n], fp32, dense.
+ * Limits: d a multiple of 8 up to 128, heads a multiple of kv_heads with at most 128 heads a key head, pointers
+ * on 16 bytes, strides multiples of 8; a stride of 0 repeats a sequence or a head, rows do not repeat.
+ * B200F_ERR_BAD_ARG otherwise.  batch * queries * heads and n below 2^31 (B200F_ERR_UNSUPPORTED).
+ *
+ * key_lengths (device int32[batch] or NULL): sequence b sees its first key_lengths[b] keys (clamped to
+ * 0..n); what lies behind them is never read into a result, NaN included.  causal: query t of T
+ * sees only the keys j < key_lengths[b] - T + 1 + t, as when the T queries belong to the sequence's last T rows.
+ * A query that sees nothing has output 0 and log-sum -INF.
+ *
+ * Arithmetic: products of 16-bit operands, fp32 accumulation; weights and, in the backward pass, score
+ * gradients are rounded to the operands' type before they are multiplied; sums, log-sums and normalisation
+ * are fp32; outputs are rounded once.  No result depends on the order in which CTAs run.
+ *
+ * status: as for b200f_search (int32[4], [0] != 0: a bounded wait ran out), but never cleared here. */
+typedef struct B200FAttendArgs {
+    const void* q;
+    int64_t q_stride[3];        /* batch, query, head */
+    const void* shared_k;       /* [shared_n][kv_heads][d]: keys that every sequence sees whole, before its own; */
+    const void* shared_v;       /* read once for the whole batch                                                 */
+    int64_t shared_k_stride[2]; /* row, head */
+    int64_t shared_v_stride[2];
+    int64_t shared_n;           /* 0: none */
+    const void* k;              /* own keys of every sequence */
+    const void* v;
+    int64_t k_stride[3];        /* batch, row, head */
+    int64_t v_stride[3];
+    int64_t n;                  /* 0: none */
+    const int32_t* key_lengths; /* of the own keys */
+    void* out;                  /* [batch][queries][heads][d], dense */
+    float* lse;                 /* optional: log of the sum of exp(scale * q.k), natural */
+    void* scratch;              /* b200f_attend_scratch_bytes(), 256-byte aligned */
+    size_t scratch_bytes;
+    int32_t* status;
+    void* stream;
+    int64_t batch, queries;
+    int32_t heads, kv_heads, d, storage;
+    int32_t causal;             /* of the own keys */
+    float scale;                /* > 0 */
+} B200FAttendArgs;
+size_t b200f_attend_scratch_bytes(const B200FAttendArgs* args);   /* pointers are not looked at; 0 also on bad arguments */
+/* out = softmax(scale * q k^T) v over the shared and the own keys together. */
+int b200f_attend(const B200FAttendArgs* args);
+
+/* Gradient of b200f_attend without shared keys and causal: grad_out -> grad_q, grad_k, grad_v (dense, whole: rows
+ * that no query sees get 0).  out and lse are what b200f_attend gave for the same q, k, v, key_lengths and scale. */
+typedef struct B200FAttendBackwardArgs {
+    const void* grad_out;
+    int64_t grad_out_stride[3]; /* batch, query, head */
+    const void* q;
+    int64_t q_stride[3];
+    const void* k;
+    const void* v;
+    int64_t k_stride[3];        /* batch, row, head */
+    int64_t v_stride[3];
+    int64_t n;
+    const int32_t* key_lengths;
+    const void* out;            /* as b200f_attend wrote it */
+    const float* lse;
+    void* grad_q;               /* [batch][queries][heads][d] */
+    void* grad_k;               /* [batch][n][kv_heads][d]    */
+    void* grad_v;
+    void* scratch;
+    size_t scratch_bytes;
+    int32_t* status;
+    void* stream;
+    int64_t batch, queries;
+    int32_t heads, kv_heads, d, storage;
+    float scale;
+} B200FAttendBackwardArgs;
+size_t b200f_attend_backward_scratch_bytes(const B200FAttendBackwardArgs* args);
+int b200f_attend_backward(const B200FAttendBackwardArgs* args);
+
+/* mass_out[b][h][j] = mass_in[b][h][j] + sum of the weights exp(scale * q.k_j - lse) that key j of key head h gets
+ * from all queries of that head's group; keys that nobody sees keep mass_in.  lse is b200f_attend's, over
+ * whatever it ran over: with shared keys too, this gives the own keys' part. */
+typedef struct B200FAttentionMassArgs {
+    const void* q;
+    int64_t q_stride[3];
+    const void* k;
+    int64_t k_stride[3];
+    int64_t n;
+    const int32_t* key_lengths;
+    const float* lse;
+    const float* mass_in;       /* NULL: zeros */
+    float* mass_out;            /* may be mass_in */
+    void* scratch;
+    size_t scratch_bytes;
+    int32_t* status;
+    void* stream;
+    int64_t batch, queries;
+    int32_t heads, kv_heads, d, storage;
+    int32_t causal;
+    float scale;
+} B200FAttentionMassArgs;
+size_t b200f_attention_mass_scratch_bytes(const B200FAttentionMassArgs* args);
+int b200f_attention_mass(const B200FAttentionMassArgs* args);
+
+/* Cuts every (sequence, key head) down to `keep` rows: where it has more, the last `recent` ones and, of those
+ * before them, the keep - recent of largest mass (ties to the lower row, NaN counts as largest); else all.  Kept
+ * rows keep their order.  out_rows[b][h][i]: the row that slot i was; slots behind the last kept row
+ * are zero in out_k / out_v / out_mass and -1 in out_rows.  Outputs must not overlap the inputs.  Any d that is a multiple
+ * of 8. */
+typedef struct B200FEvictArgs {
+    const void* k;
+    const void* v;
+    int64_t k_stride[3];        /* batch, row, head */
+    int64_t v_stride[3];
+    int64_t n;
+    const float* mass;          /* [batch][kv_heads][n], dense */
+    const int32_t* key_lengths; /* device int32[batch] or NULL (all n rows) */
+    int64_t keep, recent;       /* 0 <= recent <= keep, keep >= 1 */
+    void* out_k;                /* [batch][keep][kv_heads][d] */
+    void* out_v;
+    float* out_mass;            /* [batch][kv_heads][keep] */
+    int32_t* out_rows;          /* [batch][kv_heads][keep] */
+    int32_t* out_lengths;       /* [batch] */
+    void* stream;
+    int64_t batch;
+    int32_t kv_heads, d, storage;
+} B200FEvictArgs;
+int b200f_evict(const B200FEvictArgs* args);
+
+/* A status word (int32[4], pinned host memory, usable on every device) that lasts as long as the process, for
+ * callers that keep none of their own; the Python functions use it.  NULL without a GPU. */
+int32_t* b200f_attention_status(void);
+
 /* Deterministic synthetic rows on the device (benchmark inputs): element
  * (row, col) depends only on (seed, row0 + row, col).
  * dist: 0 = U[0,1), 1 = N(0,1) * scale, 2 = N(0,1) then row-normalised,
