@@ -1,0 +1,585 @@
+// Attention: softmax(scale * q k^T) v over keys that all sequences share and keys of each sequence.
+//
+// The query rows of a key head (queries x heads of its group; for shared keys those of all sequences) are packed into
+// tiles of 128, so that a tensor-core tile is full whatever the head layout, and keys are read once for all rows that see them.
+#include "attention_mma.cuh"
+
+#include <math.h>
+
+namespace b200f {
+
+namespace {
+
+// ---- attend_tile_kernel ------------------------------------------------------------------
+// One CTA takes two streams of score tiles [128 rows][128 keys] in turn, each with its own softmax warps (a row a thread) and its
+// own half of tensor memory: S (128 columns, whose first half then holds the weights P) and O.  While one stream's warps
+// exponentiate, the tensor cores work for the other.  PAIR: two row tiles over the same keys, each key tile fetched once for both.
+// SPLIT (no more than 128 rows): one row tile, the streams have different keys.
+// O is rescaled only when a row's maximum grew by more than 2^8 over the one its weights refer to; sums stay in fp32.
+constexpr int TILE_THREADS = 384;          // TMA, MMA, two spare warps; 2 x 4 softmax warps
+constexpr int TILE_MAX_STAGES = 10;
+template <int DP>
+constexpr int TILE_STAGE_BYTES = DP / 64 * ATT_CHUNK;
+template <int DP>
+constexpr int TILE_STAGES = DP == 128 ? 5 : 10;
+template <int DP>
+constexpr int TILE_SM_BAR = (2 + TILE_STAGES<DP>)*TILE_STAGE_BYTES<DP>;
+template <int DP>
+constexpr int TILE_SMEM = TILE_SM_BAR<DP> + (2 * TILE_MAX_STAGES + 6) * 8 + 16;
+static_assert(TILE_SMEM<128> <= 232448 && TILE_SMEM<64> <= 232448, "shared memory of a CTA");
+constexpr uint32_t TM_S = 0, TM_O = 256;   // stream t: S at 128 t, O at 256 + 128 t
+
+// A set of keys and the query rows that read them.  Work items: (unit, block of rows, range of keys).
+struct Segment {
+    int64_t n;             // keys of a unit
+    AttMap km, vm;
+    int rows;              // packed query rows of a unit
+    int row_blocks;        // of 256 rows, or 128 (split)
+    int splits;            // ranges of keys
+    int split;             // SPLIT: streams take different keys
+    int part0;             // first partial result
+    int64_t first;         // first work item
+};
+
+struct TileParams {
+    Segment seg[2];        // shared, own
+    AttView q;
+    AttLengths len;        // own keys
+    int64_t queries, batch, rows_total;
+    int heads, kv_heads, group, d;
+    float scale;
+    uint16_t* out;
+    float* lse;
+    float* part_o;         // [parts][rows_total][d], null: the one part is the result
+    float* part_lse;       // [parts][rows_total], base 2
+    int32_t* status;
+};
+
+struct RowAt {
+    int64_t b, t;
+    int h;
+};
+// packed row r of a unit
+__device__ __forceinline__ RowAt row_at(const TileParams& p, int shared, int64_t unit, int64_t r) {
+    const int64_t tt = r / p.group;
+    RowAt a;
+    a.h = (int)(unit % p.kv_heads) * p.group + (int)(r - tt * p.group);
+    a.b = shared ? tt / p.queries : unit / p.kv_heads;
+    a.t = shared ? tt % p.queries : tt;
+    return a;
+}
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(TILE_THREADS, 1)
+attend_tile_kernel(const __grid_constant__ CUtensorMap map_sk, const __grid_constant__ CUtensorMap map_sv,
+                   const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const TileParams p) {
+    extern __shared__ __align__(1024) uint8_t smem[];
+    constexpr int STAGES = TILE_STAGES<DP>, STAGE = TILE_STAGE_BYTES<DP>, CHUNKS = DP / 64;
+    const uint32_t sbase = smem_u32(smem);
+    const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0);
+    const int lane = threadIdx.x & 31;
+    const uint32_t bar_full = sbase + TILE_SM_BAR<DP>, bar_empty = bar_full + TILE_MAX_STAGES * 8;
+    const uint32_t bar_s = bar_empty + TILE_MAX_STAGES * 8, bar_p = bar_s + 16, bar_o = bar_p + 16;
+    volatile uint32_t* tmem_ptr = reinterpret_cast<volatile uint32_t*>(smem + TILE_SM_BAR<DP> + (2 * TILE_MAX_STAGES + 6) * 8);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_ptr + 1);
+
+    pdl_wait();
+    pdl_trigger();
+    if ((sbase & 1023u) != 0) {
+        if (threadIdx.x == 0) atomicOr(p.status, kDevErrSmemAlign);
+        return;
+    }
+    // ---- this CTA's item
+    const int shared = (int64_t)blockIdx.x < p.seg[1].first ? 1 : 0;
+    const Segment& sg = p.seg[shared ? 0 : 1];
+    int64_t item = (int64_t)blockIdx.x - sg.first;
+    const int rb = (int)(item % sg.row_blocks);
+    item /= sg.row_blocks;
+    const int sp = (int)(item % sg.splits);
+    const int64_t unit = item / sg.splits;
+    const int64_t row0 = (int64_t)rb * (sg.split ? 128 : 256);
+    const int kvh = (int)(unit % p.kv_heads);
+    const int64_t ub = shared ? 0 : unit / p.kv_heads;
+    const int64_t seq_len = shared ? sg.n : p.len.of(ub);
+    // keys that any row of this block sees
+    int64_t seen_max = seq_len;
+    if (!shared && p.len.causal) {
+        const int64_t last = min((int64_t)sg.rows, row0 + (sg.split ? 128 : 256)) - 1;
+        seen_max = p.len.seen(seq_len, last / p.group);
+    }
+    const int64_t ntiles = (seen_max + ATT_TILE - 1) / ATT_TILE;
+    const int pieces = sg.split ? 2 * sg.splits : sg.splits;
+    const int64_t per = (ntiles + pieces - 1) / pieces;
+    const int64_t ka = min(ntiles, per * (sg.split ? 2 * sp : sp)), kb = min(ntiles, ka + per);
+    const int64_t kb2 = min(ntiles, kb + per);
+    // stream t: tiles first[t] .. first[t] + n[t]
+    const int first0 = (int)ka, n0 = (int)(kb - ka);
+    const int first1 = sg.split ? (int)kb : (int)ka;
+    const int n1 = sg.split ? (int)(kb2 - kb) : (row0 + 128 < sg.rows ? n0 : 0);
+
+    if (threadIdx.x == 0) {
+        *abort_flag = 0;
+        for (int s = 0; s < STAGES; s++) {
+            mbar_init(bar_full + s * 8, 1);
+            mbar_init(bar_empty + s * 8, 1);
+        }
+        for (int t = 0; t < 2; t++) {
+            mbar_init(bar_s + t * 8, 1);
+            mbar_init(bar_p + t * 8, 4);
+            mbar_init(bar_o + t * 8, 1);
+        }
+        mbar_fence_init();
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32((const void*)tmem_ptr)),
+                     "r"(TMEM_COLS)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_ptr;
+    const uint32_t ring = sbase + 2 * STAGE;
+    auto wait = [&](uint32_t bar, uint32_t parity) { return mbar_wait(bar, parity, abort_flag, p.status); };
+
+    if (warp != 0) {
+        // query rows to shared memory, swizzled as TMA would: 16-byte piece c of row r goes to piece c ^ (r & 7)
+        const int nrows = sg.split ? 128 : 256;
+        for (int i = threadIdx.x - 32; i < nrows * (DP / 8); i += TILE_THREADS - 32) {
+            const int r = i / (DP / 8), c = i % (DP / 8);
+            uint4 x = make_uint4(0, 0, 0, 0);
+            if (row0 + r < sg.rows && c * 8 < p.d) {
+                const RowAt a = row_at(p, shared, unit, row0 + r);
+                x = *reinterpret_cast<const uint4*>(p.q.at(a.b, a.t, a.h) + c * 8);
+            }
+            *reinterpret_cast<uint4*>(smem + (r >> 7) * STAGE + (c >> 3) * ATT_CHUNK + (r & 127) * 128 + (((c & 7) ^ (r & 7)) << 4)) = x;
+        }
+        fence_proxy_async_shared();
+        asm volatile("bar.sync 1, %0;" ::"n"(TILE_THREADS - 32) : "memory");
+    }
+
+    if (warp == 0) {
+        // ------------------------------ keys and values in the order of their use ------------------------------
+        if (elect_one()) {
+            int slot = 0;
+            uint32_t phase = 0;
+            bool ok = true;
+            auto load = [&](const CUtensorMap* m, const AttMap& am, int tile) {
+                if (!ok || !(ok = wait(bar_empty + slot * 8, phase ^ 1))) return;
+                mbar_arrive_expect_tx(bar_full + slot * 8, STAGE);
+                for (int c = 0; c < CHUNKS; c++)
+                    tma_load_4d(ring + slot * STAGE + c * ATT_CHUNK, m, bar_full + slot * 8, c * 64, tile * ATT_TILE, kvh * am.head_step,
+                                (int)ub * am.batch_step);
+                if (++slot == STAGES) {
+                    slot = 0;
+                    phase ^= 1;
+                }
+            };
+            const CUtensorMap* mk = shared ? &map_sk : &map_k;
+            const CUtensorMap* mv = shared ? &map_sv : &map_v;
+            if (n0 > 0) load(mk, sg.km, first0);
+            if (sg.split && n1 > 0) load(mk, sg.km, first1);
+            for (int j = 0; j < n0 && ok; j++) {
+                load(mv, sg.vm, first0 + j);
+                if (j + 1 < n0) load(mk, sg.km, first0 + j + 1);
+                if (sg.split && j < n1) {
+                    load(mv, sg.vm, first1 + j);
+                    if (j + 1 < n1) load(mk, sg.km, first1 + j + 1);
+                }
+            }
+            if (!ok) {   // let the copies in flight land before shared memory goes away
+                const long long t0 = clock64();
+                while (clock64() - t0 < 2000000LL) {
+                }
+            }
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        // ------------------------------ MMA issuer ------------------------------
+        const bool leader = elect_one();
+        int cur = 0;
+        uint32_t phase = 0;
+        bool ok = true;
+        const int boundary = seq_len < sg.n && (seq_len & (ATT_TILE - 1)) ? (int)(seq_len / ATT_TILE) : -1;
+        auto take = [&]() {   // the next stage, once it is full
+            const int s = cur;
+            ok = ok && wait(bar_full + s * 8, phase);
+            if (++cur == STAGES) {
+                cur = 0;
+                phase ^= 1;
+            }
+            return s;
+        };
+        int kslot = 0, vslot = 0;
+        const int last = n1 > 0 && !sg.split ? 1 : 0;   // the stream that uses a stage last
+        auto scores = [&](int t) {
+            if (t == 0 || sg.split) kslot = take();
+            tc_fence_after();
+            mma_rows<T, DP, ATT_TILE>(leader && ok, tmem + TM_S + 128 * t, sbase + (sg.split ? 0 : t) * STAGE, ring + kslot * STAGE);
+            tc_commit_by<false>(leader, bar_s + t * 8);
+            if (t == last || sg.split) tc_commit_by<false>(leader, bar_empty + kslot * 8);
+        };
+        if (n0 > 0) scores(0);
+        if (n1 > 0) scores(1);
+        for (int j = 0; j < n0 && ok; j++) {
+            for (int t = 0; t < 2 && ok; t++) {
+                if (j >= (t ? n1 : n0)) continue;
+                if (t == 0 || sg.split) {
+                    vslot = take();
+                    // rows behind the sequence's end, within the tensor: whatever they hold, 0 * it must be 0
+                    if (ok && (t ? first1 : first0) + j == boundary)
+                        zero_tile_rows(smem + 2 * STAGE + vslot * STAGE, CHUNKS, (int)(seq_len & (ATT_TILE - 1)));
+                }
+                ok = ok && wait(bar_p + t * 8, j & 1);
+                ok = __all_sync(0xffffffffu, ok);
+                tc_fence_after();
+                mma_weights<T, DP, ATT_TILE>(leader && ok, tmem + TM_O + 128 * t, tmem + TM_S + 128 * t, ring + vslot * STAGE, j > 0);
+                if (t == last || sg.split) tc_commit_by<false>(leader, bar_empty + vslot * 8);
+                if (j + 1 < (t ? n1 : n0)) scores(t);
+                else tc_commit_by<false>(leader, bar_o + t * 8);
+            }
+            ok = __all_sync(0xffffffffu, ok);
+        }
+        if (!ok) {   // let the MMAs in flight retire before tensor memory goes away
+            const long long t0 = clock64();
+            while (clock64() - t0 < 200000LL) {
+            }
+        }
+    } else if (warp >= 4) {
+        // ------------------------------ softmax, a row a thread ------------------------------
+        const int t = (warp - 4) >> 2, ew = warp & 3;
+        const int nt = t ? n1 : n0, kt0 = t ? first1 : first0;
+        const int64_t r = row0 + (sg.split ? 0 : t * 128) + ew * 32 + lane;
+        const bool live = r < sg.rows;
+        const bool warp_live = row0 + (sg.split ? 0 : t * 128) + ew * 32 < sg.rows;
+        RowAt at{0, 0, 0};
+        if (live) at = row_at(p, shared, unit, r);
+        // keys this row sees; rows that do not exist are not masked
+        const int64_t end = !live ? (int64_t)1 << 40 : shared ? seq_len : p.len.seen(seq_len, at.t);
+        const uint32_t ts = tmem + TM_S + 128 * t + ((uint32_t)(ew * 32) << 16);
+        const uint32_t to = tmem + TM_O + 128 * t + ((uint32_t)(ew * 32) << 16);
+        const float c = p.scale * kLog2e;
+        const float slack = fminf(8.f / c, 1e30f);
+        float m = -CUDART_INF_F, l = 0.f;   // weights are exp2(c (s - m))
+        bool ok = true;
+        for (int j = 0; j < nt; j++) {
+            ok = __all_sync(0xffffffffu, wait(bar_s + t * 8, j & 1));
+            if (!ok) break;
+            if (warp_live) {
+                tc_fence_after();
+                uint32_t s[4][32];
+#pragma unroll
+                for (int i = 0; i < 4; i++) tc_ld32(ts + 32 * i, s[i]);
+#pragma unroll
+                for (int i = 0; i < 4; i++) tc_wait_ld32(s[i]);
+                const int64_t key0 = (int64_t)(kt0 + j) * ATT_TILE;
+                if (__any_sync(0xffffffffu, key0 + ATT_TILE > end)) {
+                    const int lim = (int)max(min(end - key0, (int64_t)ATT_TILE), (int64_t)0);
+#pragma unroll
+                    for (int i = 0; i < 128; i++)
+                        if (i >= lim) s[i >> 5][i & 31] = 0xff800000u;   // -INF
+                }
+                float mx[4];
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    float a = max3(__uint_as_float(s[i][0]), __uint_as_float(s[i][1]), __uint_as_float(s[i][2]));
+                    float b = max3(__uint_as_float(s[i][3]), __uint_as_float(s[i][4]), __uint_as_float(s[i][5]));
+#pragma unroll
+                    for (int e = 6; e < 30; e += 4) {
+                        a = max3(a, __uint_as_float(s[i][e]), __uint_as_float(s[i][e + 1]));
+                        b = max3(b, __uint_as_float(s[i][e + 2]), __uint_as_float(s[i][e + 3]));
+                    }
+                    mx[i] = max3(max3(a, b, __uint_as_float(s[i][30])), __uint_as_float(s[i][31]), -CUDART_INF_F);
+                }
+                const float top = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]);
+                const bool grown = top > m + slack;
+                if (__any_sync(0xffffffffu, grown)) {
+                    const float f = grown ? ex2((m - top) * c) : 1.f;   // 0 where nothing was seen before
+                    if (grown) m = top;
+                    l *= f;
+                    if (j > 0) {
+#pragma unroll 1
+                        for (int i = 0; i < DP / 32; i++) {
+                            uint32_t o[32];
+                            tc_ld32(to + 32 * i, o);
+                            tc_wait_ld32(o);
+#pragma unroll
+                            for (int e = 0; e < 32; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                            tc_st32(to + 32 * i, o);
+                        }
+                    }
+                }
+                const float mc = m == -CUDART_INF_F ? 0.f : -m * c;
+                float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    uint32_t w[32];
+#pragma unroll
+                    for (int e = 0; e < 32; e++) {
+                        const float a = ex2(fmaf(__uint_as_float(s[2 * h + (e >> 4)][(2 * e) & 31]), c, mc));
+                        const float b = ex2(fmaf(__uint_as_float(s[2 * h + (e >> 4)][(2 * e + 1) & 31]), c, mc));
+                        sum[e & 1] += a;
+                        sum[2 + (e & 1)] += b;
+                        w[e] = pack2<T>(a, b);
+                    }
+                    tc_st32(ts + 32 * h, w);
+                }
+                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                tc_wait_st();
+                tc_fence_before();
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar_p + t * 8);
+        }
+        // ------------------------------ this row's output ------------------------------
+        if (ok && nt > 0) ok = __all_sync(0xffffffffu, wait(bar_o + t * 8, 0));
+        const bool empty_stream = nt == 0;
+        if (ok && warp_live) {
+            tc_fence_after();
+            const int64_t grow = (at.b * p.queries + at.t) * p.heads + at.h;
+            const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+            const float lse2 = l > 0.f || l != l ? log2f(l) + (m == -CUDART_INF_F ? 0.f : m * c) : -CUDART_INF_F;
+            const bool whole = p.part_o == nullptr;
+            const int part = sg.part0 + (sg.split ? 2 * sp + t : sp);
+            {
+                if (live) {
+                    if (whole) {
+                        if (p.lse) p.lse[grow] = lse2 * kLn2;
+                    } else {
+                        p.part_lse[part * p.rows_total + grow] = lse2;
+                    }
+                }
+#pragma unroll 1
+                for (int i = 0; i < DP / 32; i++) {
+                    uint32_t o[32];
+                    if (!empty_stream) {
+                        tc_ld32(to + 32 * i, o);
+                        tc_wait_ld32(o);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 32; e++) o[e] = inv == 0.f ? 0u : __float_as_uint(__uint_as_float(o[e]) * inv);
+                    if (!live) continue;
+                    if (whole) {
+#pragma unroll
+                        for (int e = 0; e < 32; e += 8)
+                            if (32 * i + e < p.d)
+                                *reinterpret_cast<uint4*>(p.out + grow * p.d + 32 * i + e) =
+                                        make_uint4(pack2<T>(__uint_as_float(o[e]), __uint_as_float(o[e + 1])),
+                                                   pack2<T>(__uint_as_float(o[e + 2]), __uint_as_float(o[e + 3])),
+                                                   pack2<T>(__uint_as_float(o[e + 4]), __uint_as_float(o[e + 5])),
+                                                   pack2<T>(__uint_as_float(o[e + 6]), __uint_as_float(o[e + 7])));
+                    } else if (!empty_stream) {
+                        float* const po = p.part_o + (part * p.rows_total + grow) * p.d;
+#pragma unroll
+                        for (int e = 0; e < 32; e += 4)
+                            if (32 * i + e < p.d)
+                                *reinterpret_cast<uint4*>(po + 32 * i + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                    }
+                }
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1)
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS) : "memory");
+}
+
+// ---- attend_join_kernel: partial results of a row become its result, a warp a row ------------------
+template <typename T>
+__global__ void __launch_bounds__(256) attend_join_kernel(const float* part_o, const float* part_lse, int parts, int64_t rows, int d,
+                                                          uint16_t* out, float* lse) {
+    const int lane = threadIdx.x & 31;
+    const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+    pdl_wait();
+    pdl_trigger();
+    if (row >= rows) return;
+    float top = -CUDART_INF_F;
+    bool nan = false;
+    for (int i = lane; i < parts; i += 32) {
+        const float x = __ldcg(part_lse + i * rows + row);
+        top = fmaxf(top, x);
+        nan |= x != x;
+    }
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    nan = __any_sync(0xffffffffu, nan);
+    float total = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    const bool mine = lane * 4 < d;
+    if (top != -CUDART_INF_F || nan) {
+#pragma unroll 4
+        for (int i = 0; i < parts; i++) {
+            const float x = __ldcg(part_lse + i * rows + row);
+            if (x == -CUDART_INF_F) continue;   // nothing was written there
+            const float w = ex2(x - top);
+            total += w;
+            if (mine) {
+                const float4 o = __ldcg(reinterpret_cast<const float4*>(part_o + (i * rows + row) * d) + lane);
+                acc.x = fmaf(w, o.x, acc.x);
+                acc.y = fmaf(w, o.y, acc.y);
+                acc.z = fmaf(w, o.z, acc.z);
+                acc.w = fmaf(w, o.w, acc.w);
+            }
+        }
+    }
+    const float inv = top != -CUDART_INF_F || nan ? 1.f / total : 0.f;
+    if (mine)
+        *reinterpret_cast<uint2*>(out + row * d + lane * 4) =
+                make_uint2(pack2<T>(acc.x * inv, acc.y * inv), pack2<T>(acc.z * inv, acc.w * inv));
+    if (lane == 0 && lse) lse[row] = inv == 0.f ? -CUDART_INF_F : (top + log2f(total)) * kLn2;
+}
+
+// ---- host ---------------------------------------------------------------------------------------
+
+struct AttendPlan {
+    Segment seg[2];
+    int64_t items;
+    int parts;
+    size_t scratch;
+};
+
+// Ranges of keys: as many as fill the SMs once, of at least MIN_TILES tiles; a segment's share goes by its tiles.
+constexpr int MIN_TILES = 2;
+AttendPlan plan_attend(const B200FAttendArgs& a) {
+    AttendPlan pl{};
+    const int group = a.heads / a.kv_heads;
+    const int64_t sm = cached_sm_count();
+    int64_t weight[2], base[2], total = 0;
+    for (int i = 0; i < 2; i++) {
+        Segment& s = pl.seg[i];
+        const int64_t units = i == 0 ? a.kv_heads : a.batch * a.kv_heads;
+        s.n = i == 0 ? a.shared_n : a.n;
+        s.rows = (int)((i == 0 ? a.batch : 1) * a.queries * group);
+        const int64_t tiles = ceil_div64(s.n, ATT_TILE);
+        s.split = s.rows <= 128 && tiles >= 2;
+        s.row_blocks = (int)ceil_div64(s.rows, s.split ? 128 : 256);
+        base[i] = s.n > 0 ? units * s.row_blocks : 0;
+        weight[i] = base[i] * tiles;
+        total += weight[i];
+    }
+    if (total == 0) {   // no keys: rows of zeros, written by the own segment
+        base[1] = (a.batch * a.kv_heads) * pl.seg[1].row_blocks;
+        pl.seg[1].splits = 1;
+    }
+    for (int i = 0; i < 2; i++) {
+        Segment& s = pl.seg[i];
+        s.first = pl.items;
+        s.part0 = pl.parts;
+        if (base[i] == 0) {
+            s.splits = 1;
+            s.row_blocks = 1;
+            continue;
+        }
+        if (total > 0) {
+            const int64_t tiles = ceil_div64(s.n, ATT_TILE);
+            const int64_t share = (int64_t)((double)sm * weight[i] / total / base[i]);
+            const int64_t most = tiles / (s.split ? 2 * MIN_TILES : MIN_TILES);
+            s.splits = (int)(share < most ? share : most);
+            if (s.splits < 1) s.splits = 1;
+        }
+        pl.items += base[i] * s.splits;
+        pl.parts += s.split ? 2 * s.splits : s.splits;
+    }
+    const int64_t rows = a.batch * a.queries * a.heads;
+    pl.scratch = 256;
+    if (pl.parts > 1) pl.scratch = (size_t)(round_up64(pl.parts * rows * 4, 256) + pl.parts * rows * a.d * 4);
+    return pl;
+}
+
+int check_attend(const B200FAttendArgs* a) {
+    if (!a) return B200F_ERR_BAD_ARG;
+    const int rc = att_sizes_ok(a->batch, a->queries, a->n, a->heads, a->kv_heads, a->d, a->storage, a->scale);
+    if (rc != B200F_OK) return rc;
+    if (a->shared_n < 0) return B200F_ERR_BAD_ARG;
+    return a->shared_n > ((int64_t)1 << 31) - 1025 ? B200F_ERR_UNSUPPORTED : B200F_OK;
+}
+
+template <typename T, int DP>
+int launch_tiles(const CUtensorMap* maps, const TileParams& p, int64_t items, cudaStream_t st) {
+    static bool attr_set[kMaxDevices] = {false};
+    const int slot = device_slot();
+    if (!attr_set[slot]) {
+        B200F_CUDA_TRY(cudaFuncSetAttribute(attend_tile_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, TILE_SMEM<DP>));
+        attr_set[slot] = true;
+    }
+    const cudaError_t e = launch_kernel(attend_tile_kernel<T, DP>, dim3((unsigned)items), TILE_THREADS, TILE_SMEM<DP>, Launch(st), maps[0],
+                                        maps[1], maps[2], maps[3], p);
+    if (e != cudaSuccess) {
+        (void)cudaGetLastError();
+        return B200F_ERR_CUDA;
+    }
+    count_launch();
+    return B200F_OK;
+}
+
+}  // namespace
+
+}  // namespace b200f
+
+using namespace b200f;
+
+extern "C" size_t b200f_attend_scratch_bytes(const B200FAttendArgs* a) {
+    if (check_attend(a) != B200F_OK) return 0;
+    return a->batch == 0 || a->queries == 0 ? 256 : plan_attend(*a).scratch;
+}
+
+extern "C" int b200f_attend(const B200FAttendArgs* a) {
+    int rc = check_attend(a);
+    if (rc != B200F_OK) return rc;
+    if (a->batch == 0 || a->queries == 0) return B200F_OK;
+    const AttView q = att_view(a->q, a->q_stride), k = att_view(a->k, a->k_stride), v = att_view(a->v, a->v_stride);
+    const AttView sk{static_cast<const uint16_t*>(a->shared_k), 0, a->shared_k_stride[0], a->shared_k_stride[1]};
+    const AttView sv{static_cast<const uint16_t*>(a->shared_v), 0, a->shared_v_stride[0], a->shared_v_stride[1]};
+    if (!att_view_ok(q, a->batch, a->queries, a->heads) || !a->out || (reinterpret_cast<uintptr_t>(a->out) & 15) != 0 || !a->status ||
+        (a->n > 0 && (!att_view_ok(k, a->batch, a->n, a->kv_heads) || !att_view_ok(v, a->batch, a->n, a->kv_heads))) ||
+        (a->shared_n > 0 && (!att_view_ok(sk, 1, a->shared_n, a->kv_heads) || !att_view_ok(sv, 1, a->shared_n, a->kv_heads))))
+        return B200F_ERR_BAD_ARG;
+    AttendPlan pl = plan_attend(*a);
+    if (!a->scratch || (reinterpret_cast<uintptr_t>(a->scratch) & 255) != 0 || a->scratch_bytes < pl.scratch) return B200F_ERR_SCRATCH;
+    if (pl.items > 0x7fffffff) return B200F_ERR_UNSUPPORTED;
+    CUtensorMap maps[4] = {};
+    if (a->shared_n > 0) {
+        rc = make_rows_map(&maps[0], &pl.seg[0].km, sk, a->storage, a->d, a->shared_n, a->kv_heads, 1);
+        if (rc == B200F_OK) rc = make_rows_map(&maps[1], &pl.seg[0].vm, sv, a->storage, a->d, a->shared_n, a->kv_heads, 1);
+    }
+    if (a->n > 0 && rc == B200F_OK) {
+        rc = make_rows_map(&maps[2], &pl.seg[1].km, k, a->storage, a->d, a->n, a->kv_heads, a->batch);
+        if (rc == B200F_OK) rc = make_rows_map(&maps[3], &pl.seg[1].vm, v, a->storage, a->d, a->n, a->kv_heads, a->batch);
+    }
+    if (rc != B200F_OK) return rc;
+    TileParams p{};
+    p.seg[0] = pl.seg[0];
+    p.seg[1] = pl.seg[1];
+    p.q = q;
+    p.len = AttLengths{a->key_lengths, a->n, a->queries, a->causal};
+    p.queries = a->queries;
+    p.batch = a->batch;
+    p.rows_total = a->batch * a->queries * a->heads;
+    p.heads = a->heads;
+    p.kv_heads = a->kv_heads;
+    p.group = a->heads / a->kv_heads;
+    p.d = a->d;
+    p.scale = a->scale;
+    p.out = static_cast<uint16_t*>(a->out);
+    p.lse = a->lse;
+    p.status = a->status;
+    if (pl.parts > 1) {
+        p.part_lse = static_cast<float*>(a->scratch);
+        p.part_o = p.part_lse + round_up64(pl.parts * p.rows_total, 64);
+    }
+    const cudaStream_t st = (cudaStream_t)a->stream;
+    const bool half = a->storage == B200F_STORAGE_F16, wide = a->d > 64;
+    rc = half ? (wide ? launch_tiles<__half, 128>(maps, p, pl.items, st) : launch_tiles<__half, 64>(maps, p, pl.items, st))
+              : (wide ? launch_tiles<__nv_bfloat16, 128>(maps, p, pl.items, st) : launch_tiles<__nv_bfloat16, 64>(maps, p, pl.items, st));
+    if (rc != B200F_OK || pl.parts == 1) return rc;
+    const cudaError_t e = launch_kernel(half ? attend_join_kernel<__half> : attend_join_kernel<__nv_bfloat16>,
+                                        dim3((unsigned)ceil_div64(p.rows_total, 8)), 256, 0, Launch(st, true), p.part_o, p.part_lse, pl.parts,
+                                        p.rows_total, a->d, p.out, p.lse);
+    if (e != cudaSuccess) {
+        (void)cudaGetLastError();
+        return B200F_ERR_CUDA;
+    }
+    count_launch();
+    return B200F_OK;
+}

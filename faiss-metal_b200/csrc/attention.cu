@@ -1,5 +1,4 @@
-// Soft reads of stored rows: attention, its gradient, accumulated weights.  One CTA per row, dot products by
-// warp shuffles, online softmax; right for every case.
+// Gradient of attention and accumulated weights: a CTA a row or a key, dot products by warp shuffles.
 #include "attention.cuh"
 
 #include <math.h>
@@ -23,64 +22,11 @@ __device__ __forceinline__ float dot(const float (&a)[LD], const float (&b)[LD])
     return warp_sum(s);
 }
 
-struct Softmax {
-    float m = -kHostInf, l = 0.f, o[LD] = {};
-    __device__ void add(float s, const float (&v)[LD]) {
-        const float mn = fmaxf(m, s);
-        if (mn == -CUDART_INF_F) return;
-        const float c = expf(m - mn), p = expf(s - mn);
-        l = l * c + p;
-#pragma unroll
-        for (int i = 0; i < LD; i++) o[i] = o[i] * c + p * v[i];
-        m = mn;
-    }
-};
-
 struct Dims {
     int64_t batch, queries;
     int heads, group, d;
     float scale;
 };
-
-template <typename T>
-__global__ void attend_kernel(AttView q, AttView sk, AttView sv, int64_t shared_n, AttView k, AttView v, AttLengths len, Dims dm,
-                              uint16_t* out, float* lse) {
-    __shared__ float part[WARPS][ATT_MAX_D + 2];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int64_t row = blockIdx.x;
-    const int h = (int)(row % dm.heads);
-    const int64_t t = row / dm.heads % dm.queries, b = row / dm.heads / dm.queries;
-    float x[LD], y[LD], z[LD];
-    load_row<T>(q.at(b, t, h), dm.d, lane, x);
-    Softmax sm;
-    for (int64_t j = warp; j < shared_n; j += WARPS) {
-        load_row<T>(sk.at(0, j, h / dm.group), dm.d, lane, y);
-        load_row<T>(sv.at(0, j, h / dm.group), dm.d, lane, z);
-        sm.add(dot(x, y) * dm.scale, z);
-    }
-    const int64_t end = len.n ? len.seen(len.of(b), t) : 0;
-    for (int64_t j = warp; j < end; j += WARPS) {
-        load_row<T>(k.at(b, j, h / dm.group), dm.d, lane, y);
-        load_row<T>(v.at(b, j, h / dm.group), dm.d, lane, z);
-        sm.add(dot(x, y) * dm.scale, z);
-    }
-#pragma unroll
-    for (int i = 0; i < LD; i++) part[warp][lane + 32 * i] = sm.o[i];
-    if (lane == 0) {
-        part[warp][ATT_MAX_D] = sm.m;
-        part[warp][ATT_MAX_D + 1] = sm.l;
-    }
-    __syncthreads();
-    float m = -CUDART_INF_F, l = 0.f, o = 0.f;
-    for (int w = 0; w < WARPS; w++) m = fmaxf(m, part[w][ATT_MAX_D]);
-    for (int w = 0; w < WARPS; w++) {
-        const float c = m == -CUDART_INF_F ? 0.f : expf(part[w][ATT_MAX_D] - m);
-        l += c * part[w][ATT_MAX_D + 1];
-        o += c * part[w][threadIdx.x];
-    }
-    if ((int)threadIdx.x < dm.d) out[row * dm.d + threadIdx.x] = from_f32<T>(l == 0.f ? 0.f : o / l);
-    if (threadIdx.x == 0 && lse) lse[row] = l == 0.f ? -CUDART_INF_F : m + logf(l);
-}
 
 template <typename T>
 __global__ void grad_q_kernel(AttView g, AttView q, AttView k, AttView v, AttLengths len, Dims dm, const uint16_t* out,
@@ -171,42 +117,11 @@ __global__ void key_kernel(AttView g, AttView q, AttView k, AttView v, AttLength
     }
 }
 
-int check_attend(const B200FAttendArgs* a) {
-    if (!a) return B200F_ERR_BAD_ARG;
-    const int rc = att_sizes_ok(a->batch, a->queries, a->n, a->heads, a->kv_heads, a->d, a->storage, a->scale);
-    if (rc != B200F_OK) return rc;
-    if (a->shared_n < 0) return B200F_ERR_BAD_ARG;
-    return a->shared_n > ((int64_t)1 << 31) - 1025 ? B200F_ERR_UNSUPPORTED : B200F_OK;
-}
-
 }  // namespace
 
 }  // namespace b200f
 
 using namespace b200f;
-
-extern "C" size_t b200f_attend_scratch_bytes(const B200FAttendArgs* a) { return check_attend(a) == B200F_OK ? 256 : 0; }
-
-extern "C" int b200f_attend(const B200FAttendArgs* a) {
-    const int rc = check_attend(a);
-    if (rc != B200F_OK) return rc;
-    if (a->batch == 0 || a->queries == 0) return B200F_OK;
-    const AttView q = att_view(a->q, a->q_stride), k = att_view(a->k, a->k_stride), v = att_view(a->v, a->v_stride);
-    const AttView sk{static_cast<const uint16_t*>(a->shared_k), 0, a->shared_k_stride[0], a->shared_k_stride[1]};
-    const AttView sv{static_cast<const uint16_t*>(a->shared_v), 0, a->shared_v_stride[0], a->shared_v_stride[1]};
-    if (!att_view_ok(q, a->batch, a->queries, a->heads) || !a->out || !a->status ||
-        (a->n > 0 && (!att_view_ok(k, a->batch, a->n, a->kv_heads) || !att_view_ok(v, a->batch, a->n, a->kv_heads))) ||
-        (a->shared_n > 0 && (!att_view_ok(sk, 1, a->shared_n, a->kv_heads) || !att_view_ok(sv, 1, a->shared_n, a->kv_heads))))
-        return B200F_ERR_BAD_ARG;
-    const Dims dm{a->batch, a->queries, a->heads, a->heads / a->kv_heads, a->d, a->scale};
-    const AttLengths len{a->key_lengths, a->n, a->queries, a->causal};
-    const auto kernel = a->storage == B200F_STORAGE_F16 ? attend_kernel<__half> : attend_kernel<__nv_bfloat16>;
-    kernel<<<(unsigned)(a->batch * a->queries * a->heads), 32 * WARPS, 0, (cudaStream_t)a->stream>>>(
-            q, sk, sv, a->shared_n, k, v, len, dm, static_cast<uint16_t*>(a->out), a->lse);
-    count_launch();
-    B200F_LAUNCH_CHECK();
-    return B200F_OK;
-}
 
 extern "C" size_t b200f_attend_backward_scratch_bytes(const B200FAttendBackwardArgs* a) {
     if (!a || att_sizes_ok(a->batch, a->queries, a->n, a->heads, a->kv_heads, a->d, a->storage, a->scale) != B200F_OK) return 0;

@@ -1,0 +1,161 @@
+// tcgen05 pieces of the soft reads: operand tiles of 128 rows, products with an operand in tensor memory, masks.
+#pragma once
+
+#include "attention.cuh"
+#include "gemm_common.cuh"
+
+namespace b200f {
+
+constexpr int ATT_TILE = 128;              // keys, or packed query rows, of a tile
+constexpr int ATT_CHUNK = ATT_TILE * 128;  // bytes of 64 columns of a tile: a swizzled box of 128-byte rows
+
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1, int c2, int c3) {
+    asm volatile(
+            "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+            " [%0], [%1, {%3, %4, %5, %6}], [%2];"
+            ::"r"(dst), "l"(map), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+            : "memory");
+}
+__device__ __forceinline__ void tma_load_5d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1, int c2, int c3,
+                                            int c4) {
+    asm volatile(
+            "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+            " [%0], [%1, {%3, %4, %5, %6, %7}], [%2];"
+            ::"r"(dst), "l"(map), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(c4)
+            : "memory");
+}
+
+// Shared-memory writes of this thread become visible to TMA and tcgen05.
+__device__ __forceinline__ void fence_proxy_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// The A operand in tensor memory: 16-bit elements, two a column, row i in lane i.
+__device__ __forceinline__ void tc_mma_ts_by(bool leader, uint32_t d_tmem, uint32_t a_tmem, uint64_t desc_b, uint32_t idesc,
+                                             uint32_t accumulate) {
+    asm volatile(
+            "{\n\t"
+            ".reg .pred p, q;\n\t"
+            "setp.ne.b32 p, %4, 0;\n\t"
+            "setp.ne.b32 q, %5, 0;\n\t"
+            "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t"
+            "}\n" ::"r"(d_tmem),
+            "r"(a_tmem), "l"(desc_b), "r"(idesc), "r"(accumulate), "r"((uint32_t)leader)
+            : "memory");
+}
+
+// 32 registers a thread -> 32 lanes x 32 consecutive columns
+__device__ __forceinline__ void tc_st32(uint32_t taddr, const uint32_t (&r)[32]) {
+    asm volatile(
+            "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+            "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+            "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
+            ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+              "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]),
+              "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]),
+              "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+            : "memory");
+}
+__device__ __forceinline__ void tc_st16(uint32_t taddr, const uint32_t* r) {
+    asm volatile(
+            "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+            "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+            ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+              "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+            : "memory");
+}
+__device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi);
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// Descriptor of an operand tile whose rows (128 bytes, swizzled) run along K: 64 elements of M or N a row, 8-row
+// groups 1024 bytes apart, the next 64 elements a chunk further on.  A K step of 16 rows is 2048 bytes.
+__device__ __forceinline__ uint64_t make_smem_desc_mn(uint32_t saddr) {
+    uint64_t desc = 0;
+    desc |= (uint64_t)((saddr & 0x3FFFFu) >> 4);
+    desc |= (uint64_t)(ATT_CHUNK >> 4) << 16;
+    desc |= (uint64_t)(1024 >> 4) << 32;
+    desc |= (uint64_t)1 << 46;
+    desc |= (uint64_t)2 << 61;
+    return desc;
+}
+
+// fp32 accumulate, M = 128
+template <typename T>
+__host__ __device__ constexpr uint32_t att_idesc(int n, bool b_mn_major) {
+    const uint32_t fmt = sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+    return (1u << 4) | (fmt << 7) | (fmt << 10) | ((b_mn_major ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | (8u << 24);
+}
+
+// D[128][N] (+)= A B^T over DP columns, both operands tiles in shared memory with K along their rows.
+template <typename T, int DP, int N>
+__device__ __forceinline__ void mma_rows(bool leader, uint32_t d_tmem, uint32_t a_smem, uint32_t b_smem) {
+#pragma unroll
+    for (int c = 0; c < DP / 64; c++) {
+        const uint64_t da = make_smem_desc(a_smem + c * ATT_CHUNK), db = make_smem_desc(b_smem + c * ATT_CHUNK);
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+            tc_mma_f16_by<false>(leader, d_tmem, da + 2 * k, db + 2 * k, att_idesc<T>(N, false), c + k > 0);
+    }
+}
+// D[128][DP] (+)= P B over K rows of the tile B; P [128][K] in tensor memory.
+template <typename T, int DP, int K>
+__device__ __forceinline__ void mma_weights(bool leader, uint32_t d_tmem, uint32_t p_tmem, uint32_t b_smem, bool accumulate) {
+    const uint64_t db = make_smem_desc_mn(b_smem);
+#pragma unroll
+    for (int k = 0; k < K / 16; k++)
+        tc_mma_ts_by(leader, d_tmem, p_tmem + 8 * k, db + 128 * k, att_idesc<T>(DP, true), accumulate || k > 0);
+}
+
+// Rows [first, ATT_TILE) of a tile in shared memory become zero; a warp calls it.
+__device__ __forceinline__ void zero_tile_rows(uint8_t* tile, int chunks, int first) {
+    const int lane = threadIdx.x & 31;
+    for (int c = 0; c < chunks; c++)
+        for (int i = first * 8 + lane; i < ATT_TILE * 8; i += 32)
+            *reinterpret_cast<uint4*>(tile + c * ATT_CHUNK + i * 16) = make_uint4(0, 0, 0, 0);
+    fence_proxy_async_shared();
+    __syncwarp();
+}
+
+// ---- host side -------------------------------------------------------------------------
+
+// Coordinates of a repeated sequence or head stay 0.
+struct AttMap {
+    int batch_step, head_step;
+};
+
+// 4-D map {column, row, head, sequence} of keys or values, box {64, ATT_TILE, 1, 1}; columns and rows beyond the end read 0.
+inline int make_rows_map(CUtensorMap* map, AttMap* am, const AttView& v, int storage, int d, int64_t rows, int64_t heads, int64_t batch) {
+    EncodeTiledFn fn = get_encode_fn();
+    if (!fn) return B200F_ERR_CUDA;
+    am->batch_step = batch > 1 && v.sb == 0 ? 0 : 1;
+    am->head_step = heads > 1 && v.sh == 0 ? 0 : 1;
+    const int64_t nh = am->head_step ? heads : 1, nb = am->batch_step ? batch : 1;
+    cuuint64_t dims[4] = {(cuuint64_t)d, (cuuint64_t)rows, (cuuint64_t)nh, (cuuint64_t)nb};
+    // strides of dimensions of one element are not used, but checked
+    cuuint64_t strides[3] = {(cuuint64_t)(rows > 1 ? v.sr * 2 : 256), (cuuint64_t)(nh > 1 ? v.sh * 2 : 256),
+                             (cuuint64_t)(nb > 1 ? v.sb * 2 : 256)};
+    cuuint32_t box[4] = {64, (cuuint32_t)ATT_TILE, 1, 1};
+    cuuint32_t estr[4] = {1, 1, 1, 1};
+    const CUresult r = fn(map, storage == B200F_STORAGE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
+                          const_cast<uint16_t*>(v.p), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? B200F_OK : B200F_ERR_CUDA;
+}
+
+}  // namespace b200f
