@@ -127,6 +127,10 @@ class _Call:
         if d < 8 or d > MAX_WIDTH or d % 8:
             raise ValueError("%s: width %d is no multiple of 8 up to %d" % (self.what, d, MAX_WIDTH))
 
+    def distinct_heads(self, x, name: str, hk: int):
+        if x.numel() and x.shape[2] > hk and x.stride(2) == 0:
+            raise ValueError("%s: %s: query heads of one key head must not repeat" % (self.what, name))
+
     def scale(self, scale, d: int) -> float:
         s = 1.0 / math.sqrt(d) if scale is None else float(scale)
         if not (0.0 < s < 3.0e38):
@@ -202,6 +206,8 @@ def attend_backward(grad_out, q, k, v, out, lse, *, key_lengths=None, scale=None
     c.shape(k, "k", (b, n, hk, d))
     c.shape(v, "v", (b, n, hk, d))
     c.shape(grad_out, "grad_out", (b, t, h, d))
+    c.distinct_heads(q, "q", hk)
+    c.distinct_heads(grad_out, "grad_out", hk)
     c.dense(out, "out", (b, t, h, d), c.dtype)
     c.rows(out, "out")
     c.dense(lse, "lse", (b, t, h), c.torch.float32)
@@ -265,6 +271,7 @@ def attention_mass(q, k, lse, *, key_lengths=None, scale=None, causal=False, mas
     n, hk = k.shape[1], k.shape[2]
     c.heads(h, hk, d)
     c.shape(k, "k", (b, n, hk, d))
+    c.distinct_heads(q, "q", hk)
     c.dense(lse, "lse", (b, t, h), c.torch.float32)
     a.key_lengths = c.lengths(key_lengths, b)
     if mass is not None:

@@ -229,7 +229,7 @@ attend_tile_kernel(const __grid_constant__ CUtensorMap map_sk, const __grid_cons
                     vslot = take();
                     // rows behind the sequence's end, within the tensor: whatever they hold, 0 * it must be 0
                     if (ok && (t ? first1 : first0) + j == boundary)
-                        zero_tile_rows(smem + 2 * STAGE + vslot * STAGE, CHUNKS, (int)(seq_len & (ATT_TILE - 1)));
+                        zero_tile_rows(smem + 2 * STAGE + vslot * STAGE, CHUNKS, (int)(seq_len & (ATT_TILE - 1)), ATT_TILE);
                 }
                 ok = ok && wait(bar_p + t * 8, j & 1);
                 ok = __all_sync(0xffffffffu, ok);

@@ -1,0 +1,590 @@
+// Gradient of attention.  With s = scale q k^T, p = exp(s - lse), dp = do v^T, ds = p (dp - delta), delta = rowsum(do o):
+//   dv = p^T do, dk = scale ds^T q   (summed over the query heads of a key head)      grad_kernel<KEYS = true>
+//   dq = scale ds k                                                                  grad_kernel<KEYS = false>
+// Scores are computed twice (7 products instead of 5) so that every sum has one owner: adding dq tile by tile from the key side
+// would take atomics, whose order changes results.
+#include "attention_mma.cuh"
+
+#include <math.h>
+
+namespace b200f {
+
+namespace {
+
+// ---- grad_kernel ------------------------------------------------------------------------------
+// A CTA keeps a pair of tiles of 128 rows (A1, A2) in shared memory and streams pairs of 64 rows (B1, B2) past them:
+//   KEYS:  A1 = k, A2 = v, B1 = q, B2 = do     S = A1 B1^T, P' = A2 B2^T, acc1 (dk) += ds B1, acc2 (dv) += p B2
+//   else:  A1 = q, A2 = do, B1 = k, B2 = v     acc1 (dq) += ds B1
+// S and P' have two buffers, each with its own group of four warps (a row of A a thread) that turns them into p and ds in place; the
+// tensor cores compute the next pair of scores and add the previous pair's products meanwhile.
+constexpr int GRAD_THREADS = 384;   // TMA, MMA, two spare warps; 2 x 4 warps
+constexpr int GRAD_ROWS = 64;       // rows of a streamed tile
+constexpr int GRAD_MAX_STAGES = 8;
+template <int DP>
+constexpr int GRAD_A_BYTES = DP / 64 * ATT_CHUNK;
+template <int DP>
+constexpr int GRAD_B_BYTES = DP / 64 * GRAD_ROWS * 128;
+constexpr int GRAD_STAT_BYTES = GRAD_ROWS * 8;
+template <int DP>
+constexpr int GRAD_STAGES = DP == 128 ? 4 : 8;
+template <int DP>
+constexpr int GRAD_SM_STAT = 2 * GRAD_A_BYTES<DP> + GRAD_STAGES<DP> * 2 * GRAD_B_BYTES<DP>;
+template <int DP>
+constexpr int GRAD_SM_BAR = GRAD_SM_STAT<DP> + GRAD_STAGES<DP> * GRAD_STAT_BYTES;
+template <int DP>
+constexpr int GRAD_SMEM = GRAD_SM_BAR<DP> + (2 * GRAD_MAX_STAGES + 6) * 8 + 16;
+static_assert(GRAD_SMEM<128> <= 232448 && GRAD_SMEM<64> <= 232448, "shared memory of a CTA");
+constexpr uint32_t TG_S = 0, TG_P = 128, TG_ACC1 = 256, TG_ACC2 = 384;   // S and P' of buffer b at + 64 b
+
+struct GradParams {
+    AttMap a1m, a2m, b1m, b2m;
+    AttView q, g;            // queries and output gradients (KEYS = false: A1 and A2 are read with plain loads)
+    AttLengths len;
+    RowTiles rt;             // query rows in tiles of GRAD_ROWS
+    const float2* stat;      // [unit][tile][slot]: lse in base 2 (+INF: a slot without a row), delta
+    const uint32_t* gmax;    // fp16: bit pattern of the largest |do|
+    int64_t batch, queries;
+    int heads, kv_heads, group, d;
+    float scale;
+    int splits;              // ranges of the streamed tiles
+    int64_t blocks;          // blocks of 128 rows a unit
+    uint16_t* out1;          // dk or dq; dense
+    uint16_t* out2;          // dv
+    float* part;             // splits > 1: [split][out1 | out2] in fp32
+    int64_t part_stride, part2;
+    int32_t* status;
+};
+
+// fp16 score gradients are multiplied by a power of two that brings the largest |do| near 2^-3: they stay clear of fp16's
+// subnormals and, while a value row's norm stays below 2^18, of its end.
+__device__ __forceinline__ float grad_factor(uint32_t max_bits) {
+    const int e = (int)(max_bits >> 23) - 127;
+    return max_bits == 0 || e > 126 ? 1.f : exp2f((float)min(max(-3 - e, -100), 100));
+}
+
+template <typename T, int DP, bool KEYS>
+__global__ void __launch_bounds__(GRAD_THREADS, 1)
+grad_kernel(const __grid_constant__ CUtensorMap map_a1, const __grid_constant__ CUtensorMap map_a2,
+            const __grid_constant__ CUtensorMap map_b1, const __grid_constant__ CUtensorMap map_b2, const GradParams p) {
+    extern __shared__ __align__(1024) uint8_t smem[];
+    constexpr int STAGES = GRAD_STAGES<DP>, ABYTES = GRAD_A_BYTES<DP>, BBYTES = GRAD_B_BYTES<DP>, CHUNKS = DP / 64;
+    constexpr bool HALF = std::is_same<T, __half>::value;
+    const uint32_t sbase = smem_u32(smem);
+    const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0);
+    const int lane = threadIdx.x & 31;
+    const uint32_t bar_full = sbase + GRAD_SM_BAR<DP>, bar_empty = bar_full + GRAD_MAX_STAGES * 8;
+    const uint32_t bar_a = bar_empty + GRAD_MAX_STAGES * 8, bar_s = bar_a + 8, bar_p = bar_s + 16, bar_done = bar_p + 16;
+    volatile uint32_t* tmem_ptr = reinterpret_cast<volatile uint32_t*>(smem + GRAD_SM_BAR<DP> + (2 * GRAD_MAX_STAGES + 6) * 8);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_ptr + 1);
+    const uint32_t ring = sbase + 2 * ABYTES;
+
+    pdl_wait();
+    pdl_trigger();
+    if ((sbase & 1023u) != 0) {
+        if (threadIdx.x == 0) atomicOr(p.status, kDevErrSmemAlign);
+        return;
+    }
+    // ---- this CTA's item: a block of 128 rows of A, a range of B's tiles
+    const int64_t blk = blockIdx.x % p.blocks;
+    const int64_t rest = blockIdx.x / p.blocks;
+    const int sp = (int)(rest % p.splits);
+    const int64_t unit = rest / p.splits;
+    const int kvh = (int)(unit % p.kv_heads);
+    const int64_t b = unit / p.kv_heads;
+    const int64_t len = p.len.of(b);
+    const int64_t row0 = blk * 128;
+    const int64_t tiles = KEYS ? (row0 < len ? p.rt.tiles : 0) : (len + GRAD_ROWS - 1) / GRAD_ROWS;
+    const int64_t per = (tiles + p.splits - 1) / p.splits;
+    const int64_t first = min(tiles, per * sp);
+    const int n = (int)(min(tiles, first + per) - first);
+
+    if (threadIdx.x == 0) {
+        *abort_flag = 0;
+        for (int s = 0; s < STAGES; s++) {
+            mbar_init(bar_full + s * 8, 1);
+            mbar_init(bar_empty + s * 8, 1);
+        }
+        mbar_init(bar_a, 1);
+        for (int t = 0; t < 2; t++) {
+            mbar_init(bar_s + t * 8, 1);
+            mbar_init(bar_p + t * 8, 4);
+        }
+        mbar_init(bar_done, 1);
+        mbar_fence_init();
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32((const void*)tmem_ptr)),
+                     "r"(TMEM_COLS)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    if (KEYS) {
+        // slots that no box fills hold zeros: they are K rows of the products
+        const int fill = p.rt.gb * p.rt.bt;
+        if (fill < GRAD_ROWS) {
+            for (int s = warp; s < 2 * STAGES; s += GRAD_THREADS / 32)
+                zero_tile_rows(smem + 2 * ABYTES + s * BBYTES, CHUNKS, fill, GRAD_ROWS);
+        }
+    } else if (n > 0) {
+        // A1 and A2: packed query rows, swizzled as TMA would
+        const int64_t rows = p.queries * p.group;
+        for (int i = threadIdx.x; i < 2 * 128 * (DP / 8); i += GRAD_THREADS) {
+            const int which = i / (128 * (DP / 8)), r = i / (DP / 8) % 128, c = i % (DP / 8);
+            uint4 x = make_uint4(0, 0, 0, 0);
+            if (row0 + r < rows && c * 8 < p.d) {
+                const int64_t t = (row0 + r) / p.group;
+                const int h = kvh * p.group + (int)(row0 + r - t * p.group);
+                x = *reinterpret_cast<const uint4*>((which ? p.g : p.q).at(b, t, h) + c * 8);
+            }
+            *reinterpret_cast<uint4*>(smem + which * ABYTES + (c >> 3) * ATT_CHUNK + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = x;
+        }
+        fence_proxy_async_shared();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_ptr;
+    auto wait = [&](uint32_t bar, uint32_t parity) { return mbar_wait(bar, parity, abort_flag, p.status); };
+
+    if (warp == 0) {
+        if (elect_one() && n > 0) {
+            bool ok = true;
+            if (KEYS) {
+                mbar_arrive_expect_tx(bar_a, 2 * ABYTES);
+                for (int c = 0; c < CHUNKS; c++) {
+                    tma_load_4d(sbase + c * ATT_CHUNK, &map_a1, bar_a, c * 64, (int)row0, kvh * p.a1m.head_step, (int)b * p.a1m.batch_step);
+                    tma_load_4d(sbase + ABYTES + c * ATT_CHUNK, &map_a2, bar_a, c * 64, (int)row0, kvh * p.a2m.head_step,
+                                (int)b * p.a2m.batch_step);
+                }
+            }
+            const uint32_t bytes = KEYS ? 2 * CHUNKS * p.rt.gb * p.rt.bt * 128 + GRAD_STAT_BYTES : 2 * BBYTES;
+            int slot = 0;
+            uint32_t phase = 0;
+            for (int i = 0; i < n && ok; i++) {
+                ok = wait(bar_empty + slot * 8, phase ^ 1);
+                if (!ok) break;
+                const uint32_t full = bar_full + slot * 8, b1 = ring + slot * 2 * BBYTES, b2 = b1 + BBYTES;
+                mbar_arrive_expect_tx(full, bytes);
+                const int64_t tile = first + i;
+                if (KEYS) {
+                    const int g0 = (int)(tile % p.rt.gchunks) * p.rt.gb, t0 = (int)(tile / p.rt.gchunks) * p.rt.bt;
+                    for (int c = 0; c < CHUNKS; c++) {
+                        tma_load_5d(b1 + c * GRAD_ROWS * 128, &map_b1, full, c * 64, g0, t0, kvh * p.b1m.head_step,
+                                    (int)b * p.b1m.batch_step);
+                        tma_load_5d(b2 + c * GRAD_ROWS * 128, &map_b2, full, c * 64, g0, t0, kvh * p.b2m.head_step,
+                                    (int)b * p.b2m.batch_step);
+                    }
+                    bulk_load(sbase + GRAD_SM_STAT<DP> + slot * GRAD_STAT_BYTES, p.stat + (unit * p.rt.tiles + tile) * GRAD_ROWS,
+                              GRAD_STAT_BYTES, full);
+                } else {
+                    for (int c = 0; c < CHUNKS; c++) {
+                        tma_load_4d(b1 + c * GRAD_ROWS * 128, &map_b1, full, c * 64, (int)tile * GRAD_ROWS, kvh * p.b1m.head_step,
+                                    (int)b * p.b1m.batch_step);
+                        tma_load_4d(b2 + c * GRAD_ROWS * 128, &map_b2, full, c * 64, (int)tile * GRAD_ROWS, kvh * p.b2m.head_step,
+                                    (int)b * p.b2m.batch_step);
+                    }
+                }
+                if (++slot == STAGES) {
+                    slot = 0;
+                    phase ^= 1;
+                }
+            }
+            if (!ok) {   // let the copies in flight land before shared memory goes away
+                const long long t0 = clock64();
+                while (clock64() - t0 < 2000000LL) {
+                }
+            }
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        const bool leader = elect_one();
+        bool ok = true;
+        if (KEYS && n > 0) ok = wait(bar_a, 0);
+        const int64_t boundary = !KEYS && len < p.len.n && (len & (GRAD_ROWS - 1)) ? len / GRAD_ROWS : -1;
+        int slot = 0;
+        uint32_t phase = 0;
+        auto scores = [&](int i) {   // S and P' of the next stage
+            ok = ok && wait(bar_full + slot * 8, phase);
+            if (!KEYS && ok && first + i == boundary) {
+                // keys behind the sequence's end, within the tensor: K rows of the products
+                zero_tile_rows(smem + 2 * ABYTES + slot * 2 * BBYTES, CHUNKS, (int)(len & (GRAD_ROWS - 1)), GRAD_ROWS);
+            }
+            ok = __all_sync(0xffffffffu, ok);
+            const uint32_t b1 = ring + slot * 2 * BBYTES;
+            mma_rows<T, DP, GRAD_ROWS>(leader && ok, tmem + TG_S + 64 * (i & 1), sbase, b1);
+            mma_rows<T, DP, GRAD_ROWS>(leader && ok, tmem + TG_P + 64 * (i & 1), sbase + ABYTES, b1 + BBYTES);
+            tc_commit_by<false>(leader, bar_s + (i & 1) * 8);
+            if (++slot == STAGES) {
+                slot = 0;
+                phase ^= 1;
+            }
+        };
+        if (n > 0) scores(0);
+        if (n > 1) scores(1);
+        int used = 0;
+        for (int i = 0; i < n && ok; i++) {
+            ok = __all_sync(0xffffffffu, wait(bar_p + (i & 1) * 8, (i >> 1) & 1));
+            tc_fence_after();
+            const uint32_t b1 = ring + used * 2 * BBYTES;
+            mma_weights<T, DP, GRAD_ROWS>(leader && ok, tmem + TG_ACC1, tmem + TG_P + 64 * (i & 1), b1, i > 0);
+            if (KEYS) mma_weights<T, DP, GRAD_ROWS>(leader && ok, tmem + TG_ACC2, tmem + TG_S + 64 * (i & 1), b1 + BBYTES, i > 0);
+            tc_commit_by<false>(leader, bar_empty + used * 8);
+            if (++used == STAGES) used = 0;
+            if (i + 2 < n) scores(i + 2);
+        }
+        if (n > 0) tc_commit_by<false>(leader, bar_done);
+        if (!ok) {   // let the MMAs in flight retire before tensor memory goes away
+            const long long t0 = clock64();
+            while (clock64() - t0 < 200000LL) {
+            }
+        }
+    } else if (warp >= 4) {
+        const int wg = (warp - 4) >> 2, ew = warp & 3;
+        const uint32_t lanes = (uint32_t)(ew * 32) << 16;
+        const int64_t r = row0 + ew * 32 + lane;   // key, or packed query row
+        const float c = p.scale * kLog2e;
+        const float factor = HALF ? grad_factor(__ldcg(p.gmax)) : 1.f;
+        float my_lse = 0.f, my_delta = 0.f;
+        bool live = KEYS ? r < p.len.n : r < p.queries * p.group;
+        int64_t t = 0;
+        int g = 0;
+        if (!KEYS && live) {
+            t = r / p.group;
+            g = (int)(r - t * p.group);
+            const float2 st = __ldcg(p.stat + unit * p.rt.tiles * GRAD_ROWS + p.rt.place(t, g));
+            my_lse = st.x;
+            my_delta = st.y * factor;
+        }
+        bool ok = true;
+        for (int i = wg; i < n; i += 2) {
+            ok = wait(bar_s + wg * 8, (i >> 1) & 1);
+            // the stage's statistics: complete since the scores are there, and not refilled before this tile's products
+            if (KEYS) ok = ok && wait(bar_full + (i % STAGES) * 8, (i / STAGES) & 1);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            tc_fence_after();
+            const uint32_t ts = tmem + TG_S + 64 * wg + lanes, tp = tmem + TG_P + 64 * wg + lanes;
+            const uint32_t stat = sbase + GRAD_SM_STAT<DP> + (i % STAGES) * GRAD_STAT_BYTES;
+            const int lim = KEYS ? GRAD_ROWS : (int)min(len - (first + i) * GRAD_ROWS, (int64_t)GRAD_ROWS);
+            uint32_t s[2][32], dp[2][32];
+            tc_ld32(ts, s[0]);
+            tc_ld32(tp, dp[0]);
+            tc_ld32(ts + 32, s[1]);
+            tc_ld32(tp + 32, dp[1]);
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                tc_wait_ld32(s[h]);
+                tc_wait_ld32(dp[h]);
+            }
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                uint32_t wp[16], ws[16];
+#pragma unroll
+                for (int e = 0; e < 32; e += 2) {
+                    float l0 = my_lse, l1 = my_lse, d0 = my_delta, d1 = my_delta;
+                    if (KEYS) {
+                        const uint4 x = lds128(stat + (32 * h + e) * 8);
+                        l0 = __uint_as_float(x.x);
+                        d0 = __uint_as_float(x.y) * factor;
+                        l1 = __uint_as_float(x.z);
+                        d1 = __uint_as_float(x.w) * factor;
+                    }
+                    const float p0 = ex2(fmaf(__uint_as_float(s[h][e]), c, -l0)), p1 = ex2(fmaf(__uint_as_float(s[h][e + 1]), c, -l1));
+                    float s0 = p0 * fmaf(__uint_as_float(dp[h][e]), factor, -d0), s1 = p1 * fmaf(__uint_as_float(dp[h][e + 1]), factor, -d1);
+                    if (!KEYS) {
+                        if (32 * h + e >= lim) s0 = 0.f;
+                        if (32 * h + e + 1 >= lim) s1 = 0.f;
+                    }
+                    wp[e >> 1] = pack2<T>(p0, p1);
+                    ws[e >> 1] = pack2<T>(s0, s1);
+                }
+                if (KEYS) tc_st16(ts + 16 * h, wp);
+                tc_st16(tp + 16 * h, ws);
+            }
+            tc_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar_p + wg * 8);
+        }
+        // ------------------------------ results: KEYS: a group of warps an accumulator, else half of its columns each
+        if (ok && n > 0) ok = __all_sync(0xffffffffu, wait(bar_done, 0));
+        if (ok) {
+            tc_fence_after();
+            const bool zero = n == 0 || (KEYS && r >= len);
+            const float mul = (KEYS && wg == 1) ? 1.f : p.scale / factor;
+            const int64_t at = KEYS ? ((b * p.len.n + r) * p.kv_heads + kvh) * p.d
+                                    : ((b * p.queries + t) * p.heads + kvh * p.group + g) * p.d;
+            const uint32_t acc = tmem + (KEYS && wg ? TG_ACC2 : TG_ACC1) + lanes;
+            constexpr int NCH = KEYS ? DP / 32 : DP / 64;
+#pragma unroll 1
+            for (int ch = 0; ch < NCH; ch++) {
+                const int col = 32 * (KEYS ? ch : wg * NCH + ch);
+                uint32_t o[32];
+                if (n > 0) {
+                    tc_ld32(acc + col, o);
+                    tc_wait_ld32(o);
+                }
+#pragma unroll
+                for (int e = 0; e < 32; e++) o[e] = zero ? 0u : __float_as_uint(__uint_as_float(o[e]) * mul);
+                if (!live) continue;
+                if (p.part) {
+                    float* const po = p.part + sp * p.part_stride + (KEYS && wg ? p.part2 : 0) + at;
+#pragma unroll
+                    for (int e = 0; e < 32; e += 4)
+                        if (col + e < p.d) *reinterpret_cast<uint4*>(po + col + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                } else {
+                    uint16_t* const po = (KEYS && wg ? p.out2 : p.out1) + at;
+#pragma unroll
+                    for (int e = 0; e < 32; e += 8)
+                        if (col + e < p.d)
+                            *reinterpret_cast<uint4*>(po + col + e) =
+                                    make_uint4(pack2<T>(__uint_as_float(o[e]), __uint_as_float(o[e + 1])),
+                                               pack2<T>(__uint_as_float(o[e + 2]), __uint_as_float(o[e + 3])),
+                                               pack2<T>(__uint_as_float(o[e + 4]), __uint_as_float(o[e + 5])),
+                                               pack2<T>(__uint_as_float(o[e + 6]), __uint_as_float(o[e + 7])));
+                }
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1)
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS) : "memory");
+}
+
+// ---- grad_stat_kernel: what the gradients need of every query row, 16 lanes a slot ----------------------
+template <typename T>
+__global__ void __launch_bounds__(256) grad_stat_kernel(AttView g, const uint16_t* out, const float* lse, RowTiles rt, int64_t units, int heads,
+                                                        int kv_heads, int d, float2* stat, uint32_t* gmax) {
+    const int sub = threadIdx.x & 15;
+    const int64_t i = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
+    const bool in = i < units * rt.tiles * rt.slots;
+    const int64_t unit = in ? i / (rt.tiles * rt.slots) : 0, tile = i / rt.slots % rt.tiles;
+    int64_t t;
+    int gg;
+    const bool live = in && rt.at(tile, (int)(i % rt.slots), &t, &gg);
+    float dot = 0.f;
+    uint32_t top = 0;
+    const int h = (int)(unit % kv_heads) * rt.group + (live ? gg : 0);
+    const int64_t b = unit / kv_heads;
+    const int64_t row = live ? (b * rt.queries + t) * heads + h : 0;
+    if (live && sub * 8 < d) {
+        const uint4 x = *reinterpret_cast<const uint4*>(g.at(b, t, h) + sub * 8);
+        const uint4 y = *reinterpret_cast<const uint4*>(out + row * d + sub * 8);
+        const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const float a = to_f32<T>((uint16_t)xs[e]), c = to_f32<T>((uint16_t)(xs[e] >> 16));
+            dot = fmaf(a, to_f32<T>((uint16_t)ys[e]), dot);
+            dot = fmaf(c, to_f32<T>((uint16_t)(ys[e] >> 16)), dot);
+            top = max(top, max(__float_as_uint(a) & 0x7fffffffu, __float_as_uint(c) & 0x7fffffffu));
+        }
+    }
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
+    if (in && sub == 0) {
+        const float l = live ? lse[row] * kLog2e : CUDART_INF_F;
+        stat[i] = make_float2(l == -CUDART_INF_F ? CUDART_INF_F : l, live ? dot : 0.f);
+    }
+    if (gmax) {   // the largest finite one; the order does not matter
+        if (top >= 0x7f800000u) top = 0;
+        top = __reduce_max_sync(0xffffffffu, top);
+        if ((threadIdx.x & 31) == 0 && top > __ldcg(gmax)) atomicMax(gmax, top);
+    }
+}
+
+// Sums of partial gradients, in order.
+template <typename T>
+__global__ void __launch_bounds__(256) grad_join_kernel(const float* part, int splits, int64_t stride, int64_t n1, int64_t n2, uint16_t* out1,
+                                                        uint16_t* out2) {
+    pdl_wait();
+    pdl_trigger();
+    const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+    if (i >= n1 + n2) return;
+    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int k = 0; k < splits; k++) {
+        const float4 x = __ldcg(reinterpret_cast<const float4*>(part + k * stride + i));
+        s.x += x.x;
+        s.y += x.y;
+        s.z += x.z;
+        s.w += x.w;
+    }
+    *reinterpret_cast<uint2*>(i < n1 ? out1 + i : out2 + (i - n1)) = make_uint2(pack2<T>(s.x, s.y), pack2<T>(s.z, s.w));
+}
+
+// ---- host ---------------------------------------------------------------------------------------
+
+struct GradPlan {
+    RowTiles rt;
+    int64_t key_blocks, row_blocks;
+    int key_splits, row_splits;
+    size_t stat_bytes, part_bytes, scratch;
+};
+// Ranges of the streamed tiles: as many as fill the SMs once, of at least MIN_TILES tiles of 64 rows.
+constexpr int MIN_TILES = 4;
+GradPlan plan_grad(const B200FAttendBackwardArgs& a) {
+    GradPlan pl{};
+    const int group = a.heads / a.kv_heads;
+    const int64_t units = a.batch * a.kv_heads, sm = cached_sm_count();
+    pl.rt = row_tiles(GRAD_ROWS, a.queries, group);
+    pl.key_blocks = ceil_div64(a.n, 128);
+    pl.row_blocks = ceil_div64(a.queries * group, 128);
+    auto splits = [&](int64_t items, int64_t tiles) {
+        int64_t s = items > 0 ? sm / items : 1;
+        if (s > tiles / MIN_TILES) s = tiles / MIN_TILES;
+        return (int)(s < 1 ? 1 : s);
+    };
+    pl.key_splits = splits(units * pl.key_blocks, pl.rt.tiles);
+    pl.row_splits = splits(units * pl.row_blocks, ceil_div64(a.n, GRAD_ROWS));
+    pl.stat_bytes = (size_t)round_up64(units * pl.rt.tiles * GRAD_ROWS * 8, 256);
+    const int64_t keys = units * a.n * a.d, rows = a.batch * a.queries * a.heads * a.d;
+    size_t kp = pl.key_splits > 1 ? (size_t)pl.key_splits * 2 * keys * 4 : 0, rp = pl.row_splits > 1 ? (size_t)pl.row_splits * rows * 4 : 0;
+    pl.part_bytes = kp > rp ? kp : rp;   // one after the other
+    pl.scratch = 256 + pl.stat_bytes + pl.part_bytes;
+    return pl;
+}
+
+int check_grad(const B200FAttendBackwardArgs* a) {
+    if (!a) return B200F_ERR_BAD_ARG;
+    return att_sizes_ok(a->batch, a->queries, a->n, a->heads, a->kv_heads, a->d, a->storage, a->scale);
+}
+
+template <typename T, int DP, bool KEYS>
+int launch_grad(const CUtensorMap* maps, const GradParams& p, int64_t items, cudaStream_t st) {
+    static bool attr_set[kMaxDevices] = {false};
+    const int slot = device_slot();
+    if (!attr_set[slot]) {
+        B200F_CUDA_TRY(cudaFuncSetAttribute(grad_kernel<T, DP, KEYS>, cudaFuncAttributeMaxDynamicSharedMemorySize, GRAD_SMEM<DP>));
+        attr_set[slot] = true;
+    }
+    const cudaError_t e = launch_kernel(grad_kernel<T, DP, KEYS>, dim3((unsigned)items), GRAD_THREADS, GRAD_SMEM<DP>, Launch(st), maps[0],
+                                        maps[1], maps[2], maps[3], p);
+    if (e != cudaSuccess) {
+        (void)cudaGetLastError();
+        return B200F_ERR_CUDA;
+    }
+    count_launch();
+    return B200F_OK;
+}
+
+template <typename T>
+int launch_backward(const B200FAttendBackwardArgs& a, const GradPlan& pl, GradParams p, const uint16_t* out, float2* stat, uint32_t* gmax,
+                    float* part, const AttView& k, const AttView& v) {
+    const cudaStream_t st = (cudaStream_t)a.stream;
+    const bool wide = a.d > 64;
+    int rc = B200F_OK;
+    if (pl.rt.tiles > 0) {
+        if (gmax) B200F_CUDA_TRY(cudaMemsetAsync(gmax, 0, 4, st));
+        const int64_t slots = a.batch * a.kv_heads * pl.rt.tiles * GRAD_ROWS;
+        grad_stat_kernel<T><<<(unsigned)ceil_div64(slots, 16), 256, 0, st>>>(p.g, out, a.lse, pl.rt, a.batch * a.kv_heads, a.heads, a.kv_heads,
+                                                                           a.d, stat, gmax);
+        count_launch();
+        B200F_LAUNCH_CHECK();
+    }
+    auto join = [&](int splits, int64_t n1, int64_t n2, void* o1, void* o2) {
+        const cudaError_t e = launch_kernel(grad_join_kernel<T>, dim3((unsigned)ceil_div64((n1 + n2) / 4, 256)), 256, 0, Launch(st, true), part,
+                                            splits, n1 + n2, n1, n2, static_cast<uint16_t*>(o1), static_cast<uint16_t*>(o2));
+        if (e != cudaSuccess) {
+            (void)cudaGetLastError();
+            return B200F_ERR_CUDA;
+        }
+        count_launch();
+        return B200F_OK;
+    };
+    const int64_t units = a.batch * a.kv_heads;
+    if (a.n > 0) {
+        CUtensorMap maps[4] = {};
+        rc = make_rows_map(&maps[0], &p.a1m, k, a.storage, a.d, a.n, a.kv_heads, a.batch);
+        if (rc == B200F_OK) rc = make_rows_map(&maps[1], &p.a2m, v, a.storage, a.d, a.n, a.kv_heads, a.batch);
+        if (rc == B200F_OK && a.queries > 0) rc = make_queries_map(&maps[2], &p.b1m, p.q, a.storage, a.d, pl.rt, a.kv_heads, a.batch);
+        if (rc == B200F_OK && a.queries > 0) rc = make_queries_map(&maps[3], &p.b2m, p.g, a.storage, a.d, pl.rt, a.kv_heads, a.batch);
+        if (rc != B200F_OK) return rc;
+        const int64_t keys = units * a.n * a.d;
+        p.splits = pl.key_splits;
+        p.blocks = pl.key_blocks;
+        p.out1 = static_cast<uint16_t*>(a.grad_k);
+        p.out2 = static_cast<uint16_t*>(a.grad_v);
+        p.part = pl.key_splits > 1 ? part : nullptr;
+        p.part_stride = 2 * keys;
+        p.part2 = keys;
+        const int64_t items = units * pl.key_blocks * pl.key_splits;
+        rc = wide ? launch_grad<T, 128, true>(maps, p, items, st) : launch_grad<T, 64, true>(maps, p, items, st);
+        if (rc == B200F_OK && p.part) rc = join(p.splits, keys, keys, a.grad_k, a.grad_v);
+        if (rc != B200F_OK) return rc;
+    }
+    if (a.queries > 0) {
+        CUtensorMap maps[4] = {};
+        if (a.n > 0) {
+            rc = make_rows_map(&maps[2], &p.b1m, k, a.storage, a.d, a.n, a.kv_heads, a.batch, GRAD_ROWS);
+            if (rc == B200F_OK) rc = make_rows_map(&maps[3], &p.b2m, v, a.storage, a.d, a.n, a.kv_heads, a.batch, GRAD_ROWS);
+            if (rc != B200F_OK) return rc;
+        }
+        const int64_t rows = a.batch * a.queries * a.heads * a.d;
+        p.splits = pl.row_splits;
+        p.blocks = pl.row_blocks;
+        p.out1 = static_cast<uint16_t*>(a.grad_q);
+        p.out2 = nullptr;
+        p.part = pl.row_splits > 1 ? part : nullptr;
+        p.part_stride = rows;
+        p.part2 = 0;
+        const int64_t items = units * pl.row_blocks * pl.row_splits;
+        rc = wide ? launch_grad<T, 128, false>(maps, p, items, st) : launch_grad<T, 64, false>(maps, p, items, st);
+        if (rc == B200F_OK && p.part) rc = join(p.splits, rows, 0, a.grad_q, nullptr);
+    }
+    return rc;
+}
+
+}  // namespace
+
+}  // namespace b200f
+
+using namespace b200f;
+
+extern "C" size_t b200f_attend_backward_scratch_bytes(const B200FAttendBackwardArgs* a) {
+    return check_grad(a) == B200F_OK ? plan_grad(*a).scratch : 0;
+}
+
+extern "C" int b200f_attend_backward(const B200FAttendBackwardArgs* a) {
+    const int rc = check_grad(a);
+    if (rc != B200F_OK) return rc;
+    if (a->batch == 0) return B200F_OK;
+    const AttView g = att_view(a->grad_out, a->grad_out_stride), q = att_view(a->q, a->q_stride);
+    const AttView k = att_view(a->k, a->k_stride), v = att_view(a->v, a->v_stride);
+    auto aligned = [](const void* x) { return x && (reinterpret_cast<uintptr_t>(x) & 15) == 0; };
+    const int group = a->heads / a->kv_heads;
+    if (!a->status ||
+        (a->queries > 0 && (!att_view_ok(g, a->batch, a->queries, a->heads) || !att_view_ok(q, a->batch, a->queries, a->heads) ||
+                            (group > 1 && (q.sh == 0 || g.sh == 0)) || !aligned(a->out) || !a->lse || !aligned(a->grad_q))) ||
+        (a->n > 0 && (!att_view_ok(k, a->batch, a->n, a->kv_heads) || !att_view_ok(v, a->batch, a->n, a->kv_heads) ||
+                      !aligned(a->grad_k) || !aligned(a->grad_v))))
+        return B200F_ERR_BAD_ARG;
+    const GradPlan pl = plan_grad(*a);
+    if (!a->scratch || (reinterpret_cast<uintptr_t>(a->scratch) & 255) != 0 || a->scratch_bytes < pl.scratch) return B200F_ERR_SCRATCH;
+    const int64_t units = a->batch * a->kv_heads, lim = 0x7fffffff;
+    if (units * pl.key_blocks * pl.key_splits > lim || units * pl.row_blocks * pl.row_splits > lim ||
+        units * pl.rt.tiles * GRAD_ROWS / 16 > lim || units * a->n * a->d / 512 > lim)
+        return B200F_ERR_UNSUPPORTED;
+    uint8_t* const scratch = static_cast<uint8_t*>(a->scratch);
+    uint32_t* const gmax = a->storage == B200F_STORAGE_F16 ? reinterpret_cast<uint32_t*>(scratch) : nullptr;
+    float2* const stat = reinterpret_cast<float2*>(scratch + 256);
+    float* const part = reinterpret_cast<float*>(scratch + 256 + pl.stat_bytes);
+    GradParams p{};
+    p.q = q;
+    p.g = g;
+    p.len = AttLengths{a->key_lengths, a->n, a->queries, 0};
+    p.rt = pl.rt;
+    p.stat = stat;
+    p.gmax = gmax;
+    p.batch = a->batch;
+    p.queries = a->queries;
+    p.heads = a->heads;
+    p.kv_heads = a->kv_heads;
+    p.group = group;
+    p.d = a->d;
+    p.scale = a->scale;
+    p.status = a->status;
+    const uint16_t* const out = static_cast<const uint16_t*>(a->out);
+    return gmax ? launch_backward<__half>(*a, pl, p, out, stat, gmax, part, k, v)
+                : launch_backward<__nv_bfloat16>(*a, pl, p, out, stat, gmax, part, k, v);
+}

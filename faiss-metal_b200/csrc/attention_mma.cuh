@@ -84,11 +84,11 @@ __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
 }
 
 // Descriptor of an operand tile whose rows (128 bytes, swizzled) run along K: 64 elements of M or N a row, 8-row
-// groups 1024 bytes apart, the next 64 elements a chunk further on.  A K step of 16 rows is 2048 bytes.
-__device__ __forceinline__ uint64_t make_smem_desc_mn(uint32_t saddr) {
+// groups 1024 bytes apart, the next 64 elements `chunk` bytes further on.  A K step of 16 rows is 2048 bytes.
+__device__ __forceinline__ uint64_t make_smem_desc_mn(uint32_t saddr, uint32_t chunk) {
     uint64_t desc = 0;
     desc |= (uint64_t)((saddr & 0x3FFFFu) >> 4);
-    desc |= (uint64_t)(ATT_CHUNK >> 4) << 16;
+    desc |= (uint64_t)(chunk >> 4) << 16;
     desc |= (uint64_t)(1024 >> 4) << 32;
     desc |= (uint64_t)1 << 46;
     desc |= (uint64_t)2 << 61;
@@ -102,32 +102,32 @@ __host__ __device__ constexpr uint32_t att_idesc(int n, bool b_mn_major) {
     return (1u << 4) | (fmt << 7) | (fmt << 10) | ((b_mn_major ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | (8u << 24);
 }
 
-// D[128][N] (+)= A B^T over DP columns, both operands tiles in shared memory with K along their rows.
+// D[128][N] = A B^T over DP columns, both operands tiles (of 128 and N rows) in shared memory with K along their rows.
 template <typename T, int DP, int N>
 __device__ __forceinline__ void mma_rows(bool leader, uint32_t d_tmem, uint32_t a_smem, uint32_t b_smem) {
 #pragma unroll
     for (int c = 0; c < DP / 64; c++) {
-        const uint64_t da = make_smem_desc(a_smem + c * ATT_CHUNK), db = make_smem_desc(b_smem + c * ATT_CHUNK);
+        const uint64_t da = make_smem_desc(a_smem + c * ATT_CHUNK), db = make_smem_desc(b_smem + c * (N * 128));
 #pragma unroll
         for (int k = 0; k < 4; k++)
             tc_mma_f16_by<false>(leader, d_tmem, da + 2 * k, db + 2 * k, att_idesc<T>(N, false), c + k > 0);
     }
 }
-// D[128][DP] (+)= P B over K rows of the tile B; P [128][K] in tensor memory.
+// D[128][DP] (+)= P B over the K rows of the tile B; P [128][K] in tensor memory.
 template <typename T, int DP, int K>
 __device__ __forceinline__ void mma_weights(bool leader, uint32_t d_tmem, uint32_t p_tmem, uint32_t b_smem, bool accumulate) {
-    const uint64_t db = make_smem_desc_mn(b_smem);
+    const uint64_t db = make_smem_desc_mn(b_smem, K * 128);
 #pragma unroll
     for (int k = 0; k < K / 16; k++)
         tc_mma_ts_by(leader, d_tmem, p_tmem + 8 * k, db + 128 * k, att_idesc<T>(DP, true), accumulate || k > 0);
 }
 
-// Rows [first, ATT_TILE) of a tile in shared memory become zero; a warp calls it.
-__device__ __forceinline__ void zero_tile_rows(uint8_t* tile, int chunks, int first) {
+// Rows [first, rows) of a tile in shared memory become zero; a warp calls it.
+__device__ __forceinline__ void zero_tile_rows(uint8_t* tile, int chunks, int first, int rows) {
     const int lane = threadIdx.x & 31;
     for (int c = 0; c < chunks; c++)
-        for (int i = first * 8 + lane; i < ATT_TILE * 8; i += 32)
-            *reinterpret_cast<uint4*>(tile + c * ATT_CHUNK + i * 16) = make_uint4(0, 0, 0, 0);
+        for (int i = first * 8 + lane; i < rows * 8; i += 32)
+            *reinterpret_cast<uint4*>(tile + c * rows * 128 + i * 16) = make_uint4(0, 0, 0, 0);
     fence_proxy_async_shared();
     __syncwarp();
 }
@@ -139,8 +139,9 @@ struct AttMap {
     int batch_step, head_step;
 };
 
-// 4-D map {column, row, head, sequence} of keys or values, box {64, ATT_TILE, 1, 1}; columns and rows beyond the end read 0.
-inline int make_rows_map(CUtensorMap* map, AttMap* am, const AttView& v, int storage, int d, int64_t rows, int64_t heads, int64_t batch) {
+// 4-D map {column, row, head, sequence} of keys or values, box {64, box_rows, 1, 1}; columns and rows beyond the end read 0.
+inline int make_rows_map(CUtensorMap* map, AttMap* am, const AttView& v, int storage, int d, int64_t rows, int64_t heads, int64_t batch,
+                         int box_rows = ATT_TILE) {
     EncodeTiledFn fn = get_encode_fn();
     if (!fn) return B200F_ERR_CUDA;
     am->batch_step = batch > 1 && v.sb == 0 ? 0 : 1;
@@ -150,9 +151,55 @@ inline int make_rows_map(CUtensorMap* map, AttMap* am, const AttView& v, int sto
     // strides of dimensions of one element are not used, but checked
     cuuint64_t strides[3] = {(cuuint64_t)(rows > 1 ? v.sr * 2 : 256), (cuuint64_t)(nh > 1 ? v.sh * 2 : 256),
                              (cuuint64_t)(nb > 1 ? v.sb * 2 : 256)};
-    cuuint32_t box[4] = {64, (cuuint32_t)ATT_TILE, 1, 1};
+    cuuint32_t box[4] = {64, (cuuint32_t)box_rows, 1, 1};
     cuuint32_t estr[4] = {1, 1, 1, 1};
     const CUresult r = fn(map, storage == B200F_STORAGE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
+                          const_cast<uint16_t*>(v.p), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? B200F_OK : B200F_ERR_CUDA;
+}
+
+// How the query rows of a key head are packed into tiles that TMA fetches: `bt` queries of `gb` heads a tile, the group in
+// `gchunks` pieces.  Slot s of tile i is query (i / gchunks) * bt + s / gb, head (i % gchunks) * gb + s % gb of the group.
+struct RowTiles {
+    int slots, gb, bt, gchunks, group;
+    int64_t queries, tiles;
+    __host__ __device__ bool at(int64_t tile, int slot, int64_t* t, int* g) const {
+        const int q = slot / gb;
+        *t = tile / gchunks * bt + q;
+        *g = (int)(tile % gchunks) * gb + (slot - q * gb);
+        return q < bt && *t < queries && *g < group;
+    }
+    __host__ __device__ int64_t place(int64_t t, int g) const {   // tile * slots + slot
+        return (t / bt * gchunks + g / gb) * slots + t % bt * gb + g % gb;
+    }
+};
+inline RowTiles row_tiles(int slots, int64_t queries, int group) {
+    RowTiles r;
+    r.slots = slots;
+    r.group = group;
+    r.queries = queries;
+    r.gb = group < slots ? group : slots;
+    r.bt = slots / r.gb;
+    r.gchunks = (group + r.gb - 1) / r.gb;
+    r.tiles = ceil_div64(queries, r.bt) * r.gchunks;
+    return r;
+}
+// 5-D map {column, head of the group, query, key head, sequence} of queries, box {64, gb, bt, 1, 1}.  Heads of a group do not repeat.
+inline int make_queries_map(CUtensorMap* map, AttMap* am, const AttView& v, int storage, int d, const RowTiles& rt, int kv_heads,
+                            int64_t batch) {
+    EncodeTiledFn fn = get_encode_fn();
+    if (!fn) return B200F_ERR_CUDA;
+    if (rt.group > 1 && v.sh == 0) return B200F_ERR_BAD_ARG;
+    am->batch_step = batch > 1 && v.sb == 0 ? 0 : 1;
+    am->head_step = kv_heads > 1 && v.sh == 0 ? 0 : 1;
+    const int64_t nh = am->head_step ? kv_heads : 1, nb = am->batch_step ? batch : 1;
+    cuuint64_t dims[5] = {(cuuint64_t)d, (cuuint64_t)rt.group, (cuuint64_t)rt.queries, (cuuint64_t)nh, (cuuint64_t)nb};
+    cuuint64_t strides[4] = {(cuuint64_t)(rt.group > 1 ? v.sh * 2 : 256), (cuuint64_t)(rt.queries > 1 ? v.sr * 2 : 256),
+                             (cuuint64_t)(nh > 1 ? v.sh * rt.group * 2 : 256), (cuuint64_t)(nb > 1 ? v.sb * 2 : 256)};
+    cuuint32_t box[5] = {64, (cuuint32_t)rt.gb, (cuuint32_t)rt.bt, 1, 1};
+    cuuint32_t estr[5] = {1, 1, 1, 1, 1};
+    const CUresult r = fn(map, storage == B200F_STORAGE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 5,
                           const_cast<uint16_t*>(v.p), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                           CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     return r == CUDA_SUCCESS ? B200F_OK : B200F_ERR_CUDA;

@@ -329,7 +329,8 @@ int b200f_remap_labels_block_cyclic(int64_t* labels, int64_t count, int64_t bloc
  *   query head h reads key head h / (heads / kv_heads);
  *   log-sums [batch][queries][heads] and weights [batch][kv_heads][n], fp32, dense.
  * Limits: d a multiple of 8 up to 128, heads a multiple of kv_heads with at most 128 heads a key head, pointers
- * on 16 bytes, strides multiples of 8; a stride of 0 repeats a sequence or a head, rows do not repeat.
+ * on 16 bytes, strides multiples of 8; a stride of 0 repeats a sequence or a head (not, in the gradient and
+ * the accumulated weights, query heads of one key head), rows do not repeat.
  * B200F_ERR_BAD_ARG otherwise.  batch * queries * heads and n below 2^31 (B200F_ERR_UNSUPPORTED).
  *
  * key_lengths (device int32[batch] or NULL): sequence b sees its first key_lengths[b] keys (clamped to
