@@ -23,7 +23,7 @@ HOST_CXX = shutil.which("g++") or "g++"
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 CU_SOURCES = ["csrc/rows.cu", "csrc/scan.cu", "csrc/select.cu", "csrc/select_rank.cu", "csrc/gemm_topk.cu", "csrc/gemm_resident.cu",
-              "csrc/search.cu", "csrc/attend.cu", "csrc/attend_backward.cu", "csrc/attention.cu", "csrc/evict.cu"]
+              "csrc/search.cu", "csrc/attend.cu", "csrc/attend_backward.cu", "csrc/attention_mass.cu", "csrc/evict.cu"]
 CPP_SOURCES = ["host/Resources.cpp", "host/GrowableArray.cpp", "host/IndexFlat.cpp", "host/Sharded.cpp", "host/capi.cpp",
                "faiss_compat/compat_impl.cpp"]
 def _headers():

@@ -583,3 +583,24 @@ extern "C" int b200f_attend(const B200FAttendArgs* a) {
     count_launch();
     return B200F_OK;
 }
+
+extern "C" int32_t* b200f_attention_status(void) {
+    static int32_t* const word = []() -> int32_t* {
+        // allowed while a stream of this thread is being captured: nothing of the capture depends on it
+        cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+        if (cudaThreadExchangeStreamCaptureMode(&mode) != cudaSuccess) {
+            (void)cudaGetLastError();
+            return nullptr;
+        }
+        void* p = nullptr;
+        const cudaError_t e = cudaHostAlloc(&p, 4 * sizeof(int32_t), cudaHostAllocPortable | cudaHostAllocMapped);
+        (void)cudaThreadExchangeStreamCaptureMode(&mode);
+        if (e != cudaSuccess) {
+            (void)cudaGetLastError();
+            return nullptr;
+        }
+        for (int i = 0; i < 4; i++) static_cast<int32_t*>(p)[i] = 0;
+        return static_cast<int32_t*>(p);
+    }();
+    return word;
+}
