@@ -21,6 +21,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+from types import SimpleNamespace
 
 from . import abi
 
@@ -56,15 +57,13 @@ def _status():
     return _status_word
 
 
-class _Call:
-    """One call's arguments: checks tensors, holds the device and the stream."""
+class _Check:
+    """Checks one call's operands: everything about them but their addresses."""
 
     def __init__(self, what: str, first):
         import torch
         self.torch = torch
         self.what = what
-        if not isinstance(first, torch.Tensor):
-            raise TypeError("%s: expected torch tensors" % what)
         if not first.is_cuda:
             raise ValueError("%s: expected CUDA tensors" % what)
         self.device = first.device
@@ -75,19 +74,12 @@ class _Call:
         self.storage = _STORAGE[name]
 
     def tensor(self, x, name: str, dims: int, dtype=None):
-        torch = self.torch
-        if not isinstance(x, torch.Tensor):
-            raise TypeError("%s: %s: expected a torch tensor" % (self.what, name))
         if x.device != self.device:
             raise ValueError("%s: %s: on %s, expected %s" % (self.what, name, x.device, self.device))
         if x.dtype != (dtype or self.dtype):
             raise ValueError("%s: %s: expected dtype %s, got %s" % (self.what, name, dtype or self.dtype, x.dtype))
         if x.dim() != dims:
             raise ValueError("%s: %s: expected %d dimensions, got %d" % (self.what, name, dims, x.dim()))
-        if x.requires_grad and torch.is_grad_enabled():
-            raise ValueError("%s: %s requires a gradient, which is not recorded; use torch.no_grad() and attend_backward"
-                             % (self.what, name))
-        return x
 
     def shape(self, x, name: str, shape):
         if tuple(x.shape) != tuple(shape):
@@ -98,8 +90,6 @@ class _Call:
         self.tensor(x, name, dims)
         if x.numel() and x.shape[-1] > 1 and x.stride(-1) != 1:
             raise ValueError("%s: %s: the last dimension must be dense" % (self.what, name))
-        if x.numel() and x.data_ptr() % 16:
-            raise ValueError("%s: %s: must lie on a 16-byte boundary" % (self.what, name))
         out = []
         for i in range(dims - 1):
             s = x.stride(i) if x.shape[i] > 1 else 0
@@ -113,12 +103,10 @@ class _Call:
         self.shape(x, name, shape)
         if not x.is_contiguous():
             raise ValueError("%s: %s: must be contiguous" % (self.what, name))
-        return x
 
     def lengths(self, x, batch: int, name: str = "key_lengths"):
-        if x is None:
-            return None
-        return self.dense(x, name, (batch,), self.torch.int32).data_ptr()
+        if x is not None:
+            self.dense(x, name, (batch,), self.torch.int32)
 
     def heads(self, h: int, hk: int, d: int):
         if hk < 1 or h < 1 or h % hk or h // hk > MAX_GROUP:
@@ -137,26 +125,80 @@ class _Call:
             raise ValueError("%s: scale must be positive and finite" % self.what)
         return s
 
-    def empty(self, shape, dtype=None):
-        return self.torch.empty(shape, dtype=dtype or self.dtype, device=self.device)
-
-    def run(self, fn, args, scratch_fn=None):
-        torch = self.torch
-        check_attention_status(synchronize=False)
-        with torch.cuda.device(self.device):
+    def plan(self, args, fn: str, with_scratch: bool = True):
+        """What calls of these shapes share: the argument block without addresses, the scratch they need."""
+        lib = abi.lib()
+        scratch = 0
+        if with_scratch:
             args.status = ctypes.addressof(_status().contents)
-            args.stream = torch.cuda.current_stream(self.device).cuda_stream
-            keep = None
-            if scratch_fn is not None:
-                n = scratch_fn(ctypes.byref(args))
-                keep = torch.empty(max(n, 256), dtype=torch.uint8, device=self.device)
-                args.scratch, args.scratch_bytes = keep.data_ptr(), keep.numel()
-            abi.check_op(fn(ctypes.byref(args)), self.what)
+            with self.torch.cuda.device(self.device):
+                scratch = getattr(lib, fn + "_scratch_bytes")(ctypes.byref(args))
+                if scratch == 0:   # sizes that the library refuses: it says which way
+                    abi.check_op(getattr(lib, fn)(ctypes.byref(args)), self.what)
+        return SimpleNamespace(what=self.what, proto=bytes(args), fn=getattr(lib, fn), device=self.device, dtype=self.dtype,
+                               index=self.device.index, scratch=scratch)
+
+
+# Plans by operator, shapes, strides, types and options; never by address.  A server meets few of them; one that meets
+# many starts over.
+_plans: dict = {}
+_MAX_PLANS = 4096
+
+
+def _keep(key, plan):
+    if len(_plans) >= _MAX_PLANS:
+        _plans.clear()
+    _plans[key] = plan
+    return plan
+
+
+def _look(what: str, *tensors):
+    """The part of a plan's key that comes from tensors (None: not given)."""
+    import torch
+    grad = torch.is_grad_enabled()
+    key = [what]
+    for x in tensors:
+        if x is None:
+            key.append(None)
+            continue
+        if not isinstance(x, torch.Tensor):
+            raise TypeError("%s: expected torch tensors, got %s" % (what, type(x).__name__))
+        if grad and x.requires_grad:
+            raise ValueError("%s: a tensor requires a gradient, which is not recorded; use torch.no_grad() and attend_backward"
+                             % what)
+        key.append((x.dtype, x.shape, x.stride(), x.device))
+    return key
+
+
+def _run(plan, args, addresses: int, unused_scratch: int = 0):
+    """addresses: all 16-bit operands' addresses, or-ed."""
+    import torch
+    if addresses & 15:
+        raise ValueError("%s: operands must lie on 16-byte boundaries" % plan.what)
+    if (_status_word or _status())[0]:
+        check_attention_status(synchronize=False)
+    if torch.cuda.current_device() != plan.index:
+        with torch.cuda.device(plan.index):
+            return _run(plan, args, 0, unused_scratch)
+    args.stream = torch._C._cuda_getCurrentRawStream(plan.index)
+    if plan.scratch > unused_scratch:
+        keep = torch.empty(plan.scratch, dtype=torch.uint8, device=plan.device)
+        args.scratch, args.scratch_bytes = keep.data_ptr(), plan.scratch
+    status = plan.fn(ctypes.byref(args))
+    if status:
+        abi.check_op(status, plan.what)
+
+
+_NO_SCRATCH = 256   # scratch sizes up to this are not used by attend and attention_mass
 
 
 def _set(args, name, strides):
     for i, s in enumerate(strides):
         getattr(args, name)[i] = s
+
+
+def _sizes(a, b, t, n, h, hk, d, storage, scale):
+    a.batch, a.queries, a.n, a.heads, a.kv_heads, a.d, a.storage, a.scale = b, t, n, h, hk, d, storage, scale
 
 
 def attend(q, k, v, *, key_lengths=None, scale=None, return_lse=False):
@@ -167,24 +209,30 @@ def attend(q, k, v, *, key_lengths=None, scale=None, return_lse=False):
     keys; what lies behind them has no influence.  scale: 1 / sqrt(width) by default.  Returns the output, like q, and with
     return_lse also the log of each row's sum of exponentials, float32 [batch, queries, heads].  A sequence that sees no
     key has output 0 and log-sum -inf."""
-    c = _Call("attend", q)
-    a = abi.AttendArgs()
-    _set(a, "q_stride", c.rows(q, "q"))
-    _set(a, "k_stride", c.rows(k, "k"))
-    _set(a, "v_stride", c.rows(v, "v"))
-    b, t, h, d = q.shape
-    n, hk = k.shape[1], k.shape[2]
-    c.heads(h, hk, d)
-    c.shape(k, "k", (b, n, hk, d))
-    c.shape(v, "v", (b, n, hk, d))
-    a.key_lengths = c.lengths(key_lengths, b)
-    out = c.empty((b, t, h, d))
-    lse = c.empty((b, t, h), c.torch.float32) if return_lse else None
-    a.q, a.k, a.v, a.out = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()
+    import torch
+    key = tuple(_look("attend", q, k, v, key_lengths) + [scale])
+    plan = _plans.get(key)
+    if plan is None:
+        c = _Check("attend", q)
+        a = abi.AttendArgs()
+        _set(a, "q_stride", c.rows(q, "q"))
+        _set(a, "k_stride", c.rows(k, "k"))
+        _set(a, "v_stride", c.rows(v, "v"))
+        b, t, h, d = q.shape
+        n, hk = k.shape[1], k.shape[2]
+        c.heads(h, hk, d)
+        c.shape(k, "k", (b, n, hk, d))
+        c.shape(v, "v", (b, n, hk, d))
+        c.lengths(key_lengths, b)
+        _sizes(a, b, t, n, h, hk, d, c.storage, c.scale(scale, d))
+        plan = _keep(key, c.plan(a, "b200f_attend"))
+    a = abi.AttendArgs.from_buffer_copy(plan.proto)
+    out = torch.empty(q.shape, dtype=plan.dtype, device=plan.device)
+    lse = torch.empty(q.shape[:3], dtype=torch.float32, device=plan.device) if return_lse else None
+    a.q, a.k, a.v, a.out = pq, pk, pv, _ = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()
+    a.key_lengths = key_lengths.data_ptr() if key_lengths is not None else None
     a.lse = lse.data_ptr() if return_lse else None
-    a.n, a.batch, a.queries, a.heads, a.kv_heads, a.d, a.storage = n, b, t, h, hk, d, c.storage
-    a.scale = c.scale(scale, d)
-    c.run(abi.lib().b200f_attend, a, abi.lib().b200f_attend_scratch_bytes)
+    _run(plan, a, pq | pk | pv, _NO_SCRATCH)
     return (out, lse) if return_lse else out
 
 
@@ -194,30 +242,36 @@ def attend_backward(grad_out, q, k, v, out, lse, *, key_lengths=None, scale=None
     out and lse are what attend() returned for the same q, k, v, key_lengths and scale; grad_out has the shape of out.
     Keys that no query sees get 0.  Where k or v repeat sequences or heads (stride 0), their gradients come
     for every repetition; add them up."""
-    c = _Call("attend_backward", q)
-    a = abi.AttendBackwardArgs()
-    _set(a, "grad_out_stride", c.rows(grad_out, "grad_out"))
-    _set(a, "q_stride", c.rows(q, "q"))
-    _set(a, "k_stride", c.rows(k, "k"))
-    _set(a, "v_stride", c.rows(v, "v"))
-    b, t, h, d = q.shape
-    n, hk = k.shape[1], k.shape[2]
-    c.heads(h, hk, d)
-    c.shape(k, "k", (b, n, hk, d))
-    c.shape(v, "v", (b, n, hk, d))
-    c.shape(grad_out, "grad_out", (b, t, h, d))
-    c.distinct_heads(q, "q", hk)
-    c.distinct_heads(grad_out, "grad_out", hk)
-    c.dense(out, "out", (b, t, h, d), c.dtype)
-    c.rows(out, "out")
-    c.dense(lse, "lse", (b, t, h), c.torch.float32)
-    a.key_lengths = c.lengths(key_lengths, b)
-    gq, gk, gv = c.empty((b, t, h, d)), c.empty((b, n, hk, d)), c.empty((b, n, hk, d))
-    a.grad_out, a.q, a.k, a.v, a.out = (x.data_ptr() for x in (grad_out, q, k, v, out))
-    a.lse, a.grad_q, a.grad_k, a.grad_v = (x.data_ptr() for x in (lse, gq, gk, gv))
-    a.n, a.batch, a.queries, a.heads, a.kv_heads, a.d, a.storage = n, b, t, h, hk, d, c.storage
-    a.scale = c.scale(scale, d)
-    c.run(abi.lib().b200f_attend_backward, a, abi.lib().b200f_attend_backward_scratch_bytes)
+    import torch
+    key = tuple(_look("attend_backward", grad_out, q, k, v, out, lse, key_lengths) + [scale])
+    plan = _plans.get(key)
+    if plan is None:
+        c = _Check("attend_backward", q)
+        a = abi.AttendBackwardArgs()
+        _set(a, "grad_out_stride", c.rows(grad_out, "grad_out"))
+        _set(a, "q_stride", c.rows(q, "q"))
+        _set(a, "k_stride", c.rows(k, "k"))
+        _set(a, "v_stride", c.rows(v, "v"))
+        b, t, h, d = q.shape
+        n, hk = k.shape[1], k.shape[2]
+        c.heads(h, hk, d)
+        c.shape(k, "k", (b, n, hk, d))
+        c.shape(v, "v", (b, n, hk, d))
+        c.shape(grad_out, "grad_out", (b, t, h, d))
+        c.distinct_heads(q, "q", hk)
+        c.distinct_heads(grad_out, "grad_out", hk)
+        c.dense(out, "out", (b, t, h, d), c.dtype)
+        c.dense(lse, "lse", (b, t, h), torch.float32)
+        c.lengths(key_lengths, b)
+        _sizes(a, b, t, n, h, hk, d, c.storage, c.scale(scale, d))
+        plan = _keep(key, c.plan(a, "b200f_attend_backward"))
+    a = abi.AttendBackwardArgs.from_buffer_copy(plan.proto)
+    gq, gk, gv = (torch.empty(x.shape, dtype=plan.dtype, device=plan.device) for x in (q, k, v))
+    a.grad_out, a.q, a.k, a.v, a.out = pg, pq, pk, pv, po = (
+        grad_out.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr())
+    a.lse, a.grad_q, a.grad_k, a.grad_v = lse.data_ptr(), gq.data_ptr(), gk.data_ptr(), gv.data_ptr()
+    a.key_lengths = key_lengths.data_ptr() if key_lengths is not None else None
+    _run(plan, a, pg | pq | pk | pv | po)
     return gq, gk, gv
 
 
@@ -229,30 +283,38 @@ def attend_shared(q, shared_k, shared_v, own_k, own_v, own_lengths=None, *, scal
     own_lengths (int32 [batch], on the device): rows of each sequence, the new ones included (default: all).  Query t sees
     the whole prefix and the own rows j < own_lengths[b] - new + 1 + t.  Returns the output, like q, and with return_lse the log-sums
     over both parts, float32 [batch, new, heads]."""
-    c = _Call("attend_shared", q)
-    a = abi.AttendArgs()
-    _set(a, "q_stride", c.rows(q, "q"))
-    _set(a, "shared_k_stride", c.rows(shared_k, "shared_k", 3))
-    _set(a, "shared_v_stride", c.rows(shared_v, "shared_v", 3))
-    _set(a, "k_stride", c.rows(own_k, "own_k"))
-    _set(a, "v_stride", c.rows(own_v, "own_v"))
-    b, t, h, d = q.shape
-    p, hk = shared_k.shape[0], shared_k.shape[1]
-    n = own_k.shape[1]
-    c.heads(h, hk, d)
-    c.shape(shared_k, "shared_k", (p, hk, d))
-    c.shape(shared_v, "shared_v", (p, hk, d))
-    c.shape(own_k, "own_k", (b, n, hk, d))
-    c.shape(own_v, "own_v", (b, n, hk, d))
-    a.key_lengths = c.lengths(own_lengths, b, "own_lengths")
-    out = c.empty((b, t, h, d))
-    lse = c.empty((b, t, h), c.torch.float32) if return_lse else None
-    a.q, a.shared_k, a.shared_v, a.k, a.v, a.out = (x.data_ptr() for x in (q, shared_k, shared_v, own_k, own_v, out))
+    import torch
+    key = tuple(_look("attend_shared", q, shared_k, shared_v, own_k, own_v, own_lengths) + [scale])
+    plan = _plans.get(key)
+    if plan is None:
+        c = _Check("attend_shared", q)
+        a = abi.AttendArgs()
+        _set(a, "q_stride", c.rows(q, "q"))
+        _set(a, "shared_k_stride", c.rows(shared_k, "shared_k", 3))
+        _set(a, "shared_v_stride", c.rows(shared_v, "shared_v", 3))
+        _set(a, "k_stride", c.rows(own_k, "own_k"))
+        _set(a, "v_stride", c.rows(own_v, "own_v"))
+        b, t, h, d = q.shape
+        p, hk = shared_k.shape[0], shared_k.shape[1]
+        n = own_k.shape[1]
+        c.heads(h, hk, d)
+        c.shape(shared_k, "shared_k", (p, hk, d))
+        c.shape(shared_v, "shared_v", (p, hk, d))
+        c.shape(own_k, "own_k", (b, n, hk, d))
+        c.shape(own_v, "own_v", (b, n, hk, d))
+        c.lengths(own_lengths, b, "own_lengths")
+        _sizes(a, b, t, n, h, hk, d, c.storage, c.scale(scale, d))
+        a.shared_n, a.causal = p, 1
+        plan = _keep(key, c.plan(a, "b200f_attend"))
+    a = abi.AttendArgs.from_buffer_copy(plan.proto)
+    out = torch.empty(q.shape, dtype=plan.dtype, device=plan.device)
+    lse = torch.empty(q.shape[:3], dtype=torch.float32, device=plan.device) if return_lse else None
+    a.q, a.shared_k, a.shared_v, a.k, a.v = pq, psk, psv, pk, pv = (
+        q.data_ptr(), shared_k.data_ptr(), shared_v.data_ptr(), own_k.data_ptr(), own_v.data_ptr())
+    a.out = out.data_ptr()
+    a.key_lengths = own_lengths.data_ptr() if own_lengths is not None else None
     a.lse = lse.data_ptr() if return_lse else None
-    a.shared_n, a.n, a.batch, a.queries, a.heads, a.kv_heads, a.d, a.storage = p, n, b, t, h, hk, d, c.storage
-    a.causal = 1
-    a.scale = c.scale(scale, d)
-    c.run(abi.lib().b200f_attend, a, abi.lib().b200f_attend_scratch_bytes)
+    _run(plan, a, pq | psk | psv | pk | pv, _NO_SCRATCH)
     return (out, lse) if return_lse else out
 
 
@@ -263,25 +325,32 @@ def attention_mass(q, k, lse, *, key_lengths=None, scale=None, causal=False, mas
     q, k, key_lengths and scale as for attend(); lse float32 [batch, queries, heads] from attend(), or from attend_shared(), for which
     k are the own rows and causal is True (query t sees j < key_lengths[b] - queries + 1 + t), or the prefix, as one
     sequence."""
-    c = _Call("attention_mass", q)
-    a = abi.AttentionMassArgs()
-    _set(a, "q_stride", c.rows(q, "q"))
-    _set(a, "k_stride", c.rows(k, "k"))
-    b, t, h, d = q.shape
-    n, hk = k.shape[1], k.shape[2]
-    c.heads(h, hk, d)
-    c.shape(k, "k", (b, n, hk, d))
-    c.distinct_heads(q, "q", hk)
-    c.dense(lse, "lse", (b, t, h), c.torch.float32)
-    a.key_lengths = c.lengths(key_lengths, b)
-    if mass is not None:
-        a.mass_in = c.dense(mass, "mass", (b, hk, n), c.torch.float32).data_ptr()
-    out = c.empty((b, hk, n), c.torch.float32)
-    a.q, a.k, a.lse, a.mass_out = q.data_ptr(), k.data_ptr(), lse.data_ptr(), out.data_ptr()
-    a.n, a.batch, a.queries, a.heads, a.kv_heads, a.d, a.storage = n, b, t, h, hk, d, c.storage
-    a.causal = 1 if causal else 0
-    a.scale = c.scale(scale, d)
-    c.run(abi.lib().b200f_attention_mass, a, abi.lib().b200f_attention_mass_scratch_bytes)
+    import torch
+    key = tuple(_look("attention_mass", q, k, lse, key_lengths, mass) + [scale, bool(causal)])
+    plan = _plans.get(key)
+    if plan is None:
+        c = _Check("attention_mass", q)
+        a = abi.AttentionMassArgs()
+        _set(a, "q_stride", c.rows(q, "q"))
+        _set(a, "k_stride", c.rows(k, "k"))
+        b, t, h, d = q.shape
+        n, hk = k.shape[1], k.shape[2]
+        c.heads(h, hk, d)
+        c.shape(k, "k", (b, n, hk, d))
+        c.distinct_heads(q, "q", hk)
+        c.dense(lse, "lse", (b, t, h), torch.float32)
+        c.lengths(key_lengths, b)
+        if mass is not None:
+            c.dense(mass, "mass", (b, hk, n), torch.float32)
+        _sizes(a, b, t, n, h, hk, d, c.storage, c.scale(scale, d))
+        a.causal = 1 if causal else 0
+        plan = _keep(key, c.plan(a, "b200f_attention_mass"))
+    a = abi.AttentionMassArgs.from_buffer_copy(plan.proto)
+    out = torch.empty((q.shape[0], k.shape[2], k.shape[1]), dtype=torch.float32, device=plan.device)
+    a.q, a.k, a.lse, a.mass_out = pq, pk, _, _ = q.data_ptr(), k.data_ptr(), lse.data_ptr(), out.data_ptr()
+    a.key_lengths = key_lengths.data_ptr() if key_lengths is not None else None
+    a.mass_in = mass.data_ptr() if mass is not None else None
+    _run(plan, a, pq | pk, _NO_SCRATCH)
     return out
 
 
@@ -292,60 +361,71 @@ def evict(k, v, mass, key_lengths=None, keep=1, *, recent=0):
     k, v [batch, rows, key heads, width]; mass float32 [batch, key heads, rows]; key_lengths int32 [batch] or None.  Returns
     (k, v, mass, rows, lengths): caches of `keep` rows in the old order, zero behind the last one, their mass [batch, key heads,
     keep], the row each slot was (int32, -1 behind the last one) and the new lengths (int32 [batch])."""
-    c = _Call("evict", k)
-    a = abi.EvictArgs()
-    _set(a, "k_stride", c.rows(k, "k"))
-    _set(a, "v_stride", c.rows(v, "v"))
-    b, n, hk, d = k.shape
-    c.shape(v, "v", (b, n, hk, d))
-    if hk < 1 or d < 8 or d % 8:
-        raise ValueError("evict: width %d of %d key heads: expected a multiple of 8, and a head" % (d, hk))
-    keep, recent = int(keep), int(recent)
-    if keep < 1 or recent < 0 or recent > keep:
-        raise ValueError("evict: expected keep >= 1 and 0 <= recent <= keep, got %d and %d" % (keep, recent))
-    c.dense(mass, "mass", (b, hk, n), c.torch.float32)
-    a.key_lengths = c.lengths(key_lengths, b)
-    out_k, out_v = c.empty((b, keep, hk, d)), c.empty((b, keep, hk, d))
-    out_mass = c.empty((b, hk, keep), c.torch.float32)
-    out_rows = c.empty((b, hk, keep), c.torch.int32)
-    out_lengths = c.empty((b,), c.torch.int32)
-    a.k, a.v, a.mass = k.data_ptr(), v.data_ptr(), mass.data_ptr()
+    import torch
+    key = tuple(_look("evict", k, v, mass, key_lengths) + [keep, recent])
+    plan = _plans.get(key)
+    if plan is None:
+        c = _Check("evict", k)
+        a = abi.EvictArgs()
+        _set(a, "k_stride", c.rows(k, "k"))
+        _set(a, "v_stride", c.rows(v, "v"))
+        b, n, hk, d = k.shape
+        c.shape(v, "v", (b, n, hk, d))
+        if hk < 1 or d < 8 or d % 8:
+            raise ValueError("evict: width %d of %d key heads: expected a multiple of 8, and a head" % (d, hk))
+        if int(keep) < 1 or int(recent) < 0 or int(recent) > int(keep):
+            raise ValueError("evict: expected keep >= 1 and 0 <= recent <= keep, got %d and %d" % (keep, recent))
+        c.dense(mass, "mass", (b, hk, n), torch.float32)
+        c.lengths(key_lengths, b)
+        a.batch, a.n, a.kv_heads, a.d, a.storage, a.keep, a.recent = b, n, hk, d, c.storage, int(keep), int(recent)
+        plan = _keep(key, c.plan(a, "b200f_evict", with_scratch=False))
+    a = abi.EvictArgs.from_buffer_copy(plan.proto)
+    b, _, hk, d = k.shape
+    keep = a.keep
+    out_k = torch.empty((b, keep, hk, d), dtype=plan.dtype, device=plan.device)
+    out_v = torch.empty((b, keep, hk, d), dtype=plan.dtype, device=plan.device)
+    out_mass = torch.empty((b, hk, keep), dtype=torch.float32, device=plan.device)
+    out_rows = torch.empty((b, hk, keep), dtype=torch.int32, device=plan.device)
+    out_lengths = torch.empty((b,), dtype=torch.int32, device=plan.device)
+    a.k, a.v, a.mass = pk, pv, _ = k.data_ptr(), v.data_ptr(), mass.data_ptr()
+    a.key_lengths = key_lengths.data_ptr() if key_lengths is not None else None
     a.out_k, a.out_v, a.out_mass, a.out_rows, a.out_lengths = (
-        x.data_ptr() for x in (out_k, out_v, out_mass, out_rows, out_lengths))
-    a.n, a.keep, a.recent, a.batch, a.kv_heads, a.d, a.storage = n, keep, recent, b, hk, d, c.storage
-    with c.torch.cuda.device(c.device):
-        a.stream = c.torch.cuda.current_stream(c.device).cuda_stream
-        abi.check_op(abi.lib().b200f_evict(ctypes.byref(a)), "evict")
+        out_k.data_ptr(), out_v.data_ptr(), out_mass.data_ptr(), out_rows.data_ptr(), out_lengths.data_ptr())
+    _run(plan, a, pk | pv)
     return out_k, out_v, out_mass, out_rows, out_lengths
 
 
 def attend_index(index, x, values, scale, return_lse):
     """B200IndexFlat.attend()."""
-    c = _Call("attend", x)
-    if index.metric_type != abi.METRIC_INNER_PRODUCT:
-        raise ValueError("attend: the index must be one of inner products")
-    if index.storage != c.storage:
-        raise ValueError("attend: x must have the index's storage type (float16 or bfloat16), got %s" % c.dtype)
-    if c.device.index != index.resources.device:
-        raise ValueError("attend: x is on %s, the index on device %d" % (c.device, index.resources.device))
-    if c.torch.cuda.is_current_stream_capturing():
-        raise ValueError("attend: the rows of an index may move, a graph cannot hold their address")
+    import torch
     n, d = index.ntotal, index.d
-    a = abi.AttendArgs()
-    xs, vs = c.rows(x, "x", 2), c.rows(values, "values", 2)
-    nq = x.shape[0]
-    c.shape(x, "x", (nq, d))
-    c.shape(values, "values", (n, d))
-    c.heads(1, 1, d)
-    out = c.empty((nq, d))
-    lse = c.empty((nq,), c.torch.float32) if return_lse else None
-    a.q_stride[1] = xs[0]
-    a.k_stride[1], a.v_stride[1] = d, vs[0]   # 16-bit rows of an inner-product index lie side by side
-    a.q, a.k, a.v, a.out = x.data_ptr(), index.device_rows(), values.data_ptr(), out.data_ptr()
+    key = tuple(_look("attend", x, values) + [scale, n, d, index.storage, index.metric_type, index.resources.device])
+    plan = _plans.get(key)
+    if plan is None:
+        c = _Check("attend", x)
+        if index.metric_type != abi.METRIC_INNER_PRODUCT:
+            raise ValueError("attend: the index must be one of inner products")
+        if index.storage != c.storage:
+            raise ValueError("attend: x must have the index's storage type (float16 or bfloat16), got %s" % c.dtype)
+        if c.device.index != index.resources.device:
+            raise ValueError("attend: x is on %s, the index on device %d" % (c.device, index.resources.device))
+        a = abi.AttendArgs()
+        xs, vs = c.rows(x, "x", 2), c.rows(values, "values", 2)
+        c.shape(x, "x", (x.shape[0], d))
+        c.shape(values, "values", (n, d))
+        c.heads(1, 1, d)
+        a.q_stride[1] = xs[0]
+        a.k_stride[1], a.v_stride[1] = d, vs[0]   # 16-bit rows of an inner-product index lie side by side
+        _sizes(a, 1, x.shape[0], n, 1, 1, d, c.storage, c.scale(scale, d))
+        plan = _keep(key, c.plan(a, "b200f_attend"))
+    if torch.cuda.is_current_stream_capturing():
+        raise ValueError("attend: the rows of an index may move, a graph cannot hold their address")
+    a = abi.AttendArgs.from_buffer_copy(plan.proto)
+    out = torch.empty(x.shape, dtype=plan.dtype, device=plan.device)
+    lse = torch.empty(x.shape[:1], dtype=torch.float32, device=plan.device) if return_lse else None
+    a.q, a.k, a.v, a.out = px, _, pv, _ = x.data_ptr(), index.device_rows(), values.data_ptr(), out.data_ptr()
     a.lse = lse.data_ptr() if return_lse else None
-    a.n, a.batch, a.queries, a.heads, a.kv_heads, a.d, a.storage = n, 1, nq, 1, 1, d, c.storage
-    a.scale = c.scale(scale, d)
-    c.run(abi.lib().b200f_attend, a, abi.lib().b200f_attend_scratch_bytes)
+    _run(plan, a, px | pv, _NO_SCRATCH)
     # adds and resets run on the index's own stream, and have completed when they return
-    index.resources.wait_stream(c.torch.cuda.current_stream(c.device).cuda_stream)
+    index.resources.wait_stream(torch.cuda.current_stream(plan.device).cuda_stream)
     return (out, lse) if return_lse else out

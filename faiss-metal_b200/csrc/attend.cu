@@ -37,8 +37,9 @@ struct Segment {
     int row_blocks;        // of 256 rows, or 128 (split)
     int splits;            // ranges of keys
     int split;             // SPLIT: streams take different keys
+    int few;               // attend_few_kernel takes it
     int part0;             // first partial result
-    int64_t first;         // first work item
+    int64_t items;         // CTAs
 };
 
 struct TileParams {
@@ -90,9 +91,10 @@ attend_tile_kernel(const __grid_constant__ CUtensorMap map_sk, const __grid_cons
         return;
     }
     // ---- this CTA's item
-    const int shared = (int64_t)blockIdx.x < p.seg[1].first ? 1 : 0;
+    const int64_t before = p.seg[0].few ? 0 : p.seg[0].items;   // CTAs of the shared keys
+    const int shared = (int64_t)blockIdx.x < before ? 1 : 0;
     const Segment& sg = p.seg[shared ? 0 : 1];
-    int64_t item = (int64_t)blockIdx.x - sg.first;
+    int64_t item = (int64_t)blockIdx.x - (shared ? 0 : before);
     const int rb = (int)(item % sg.row_blocks);
     item /= sg.row_blocks;
     const int sp = (int)(item % sg.splits);
@@ -386,6 +388,300 @@ attend_tile_kernel(const __grid_constant__ CUtensorMap map_sk, const __grid_cons
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS) : "memory");
 }
 
+// ---- attend_few_kernel ---------------------------------------------------------------------------------
+// At most 16 packed query rows a unit, as when decoding: reading keys and values once is the bound, 3 us of HBM time for every
+// us of tensor work even on mma.sync, whose 16-row tile wastes nothing here (a tcgen05 tile has 128).  Four warps share tiles of
+// 64 keys that TMA streams in, 16 keys a warp, each with a softmax of its own; they are joined once at the end.  Two
+// CTAs an SM, so that one streams while the other starts or ends.
+constexpr int FEW_ROWS = 16;
+constexpr int FEW_KEYS = 64;            // keys of a tile
+constexpr int FEW_THREADS = 160;        // four warps, TMA
+template <int DP>
+constexpr int FEW_TILE = DP / 64 * FEW_KEYS * 128;
+template <int DP>
+constexpr int FEW_STAGES = DP == 128 ? 3 : 6;
+template <int DP>
+constexpr int FEW_SM_BAR = FEW_STAGES<DP> * 2 * FEW_TILE<DP>;
+template <int DP>
+constexpr int FEW_SMEM = FEW_SM_BAR<DP> + 2 * FEW_STAGES<DP> * 8 + 16;
+static_assert(4 * FEW_ROWS * (128 + 2) * 4 <= FEW_SM_BAR<128> && 4 * FEW_ROWS * (64 + 2) * 4 <= FEW_SM_BAR<64>, "the warps' results fit the ring");
+
+__device__ __forceinline__ void ldmatrix4(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ void ldmatrix4_trans(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+template <typename T>
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if (std::is_same<T, __half>::value)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(FEW_THREADS, 2)
+attend_few_kernel(const __grid_constant__ CUtensorMap map_sk, const __grid_constant__ CUtensorMap map_sv,
+                  const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const TileParams p) {
+    extern __shared__ __align__(1024) uint8_t smem[];
+    constexpr int STAGES = FEW_STAGES<DP>, TILE = FEW_TILE<DP>, CHUNK = FEW_KEYS * 128;
+    const uint32_t sbase = smem_u32(smem);
+    const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0);
+    const int lane = threadIdx.x & 31;
+    const uint32_t bar_full = sbase + FEW_SM_BAR<DP>, bar_empty = bar_full + STAGES * 8;
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + FEW_SM_BAR<DP> + 2 * STAGES * 8);
+
+    // Launched behind the tile kernel of the same call, whose inputs are complete and whose results it does not read: it waits for
+    // that kernel only when it ends, so that whoever waits for it has both.
+    pdl_trigger();
+    if ((sbase & 1023u) != 0) {
+        if (threadIdx.x == 0) atomicOr(p.status, kDevErrSmemAlign);
+        return;
+    }
+    const int shared = p.seg[0].few && (int64_t)blockIdx.x < p.seg[0].items ? 1 : 0;
+    const Segment& sg = p.seg[shared ? 0 : 1];
+    const int64_t item = (int64_t)blockIdx.x - (shared || !p.seg[0].few ? 0 : p.seg[0].items);
+    const int sp = (int)(item % sg.splits);
+    const int64_t unit = item / sg.splits;
+    const int kvh = (int)(unit % p.kv_heads);
+    const int64_t ub = shared ? 0 : unit / p.kv_heads;
+    const int64_t seq_len = shared ? sg.n : p.len.of(ub);
+    const int64_t ntiles = (seq_len + FEW_KEYS - 1) / FEW_KEYS;   // causal ends lie in the last tiles
+    const int64_t per = (ntiles + sg.splits - 1) / sg.splits;
+    const int64_t first = min(ntiles, per * sp);
+    const int n = (int)(min(ntiles, first + per) - first);
+
+    if (threadIdx.x == 0) {
+        *abort_flag = 0;
+        for (int s = 0; s < STAGES; s++) {
+            mbar_init(bar_full + s * 8, 1);
+            mbar_init(bar_empty + s * 8, 4);
+        }
+        mbar_fence_init();
+    }
+    __syncthreads();
+    auto wait = [&](uint32_t bar, uint32_t parity) { return mbar_wait(bar, parity, abort_flag, p.status); };
+    bool ok = true;
+    float m[2] = {-CUDART_INF_F, -CUDART_INF_F}, l[2] = {0.f, 0.f};   // rows lane / 4 and 8 more
+    float o[DP / 8][4];
+#pragma unroll
+    for (int i = 0; i < DP / 8; i++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) o[i][e] = 0.f;
+
+    if (warp == 4) {
+        if (elect_one()) {
+            const CUtensorMap* mk = shared ? &map_sk : &map_k;
+            const CUtensorMap* mv = shared ? &map_sv : &map_v;
+            int slot = 0;
+            uint32_t phase = 0;
+            for (int i = 0; i < n && ok; i++) {
+                ok = wait(bar_empty + slot * 8, phase ^ 1);
+                if (!ok) break;
+                const uint32_t dst = sbase + slot * 2 * TILE, full = bar_full + slot * 8;
+                mbar_arrive_expect_tx(full, 2 * TILE);
+                for (int c = 0; c < DP / 64; c++)
+                    tma_load_4d(dst + c * CHUNK, mk, full, c * 64, (int)(first + i) * FEW_KEYS, kvh * sg.km.head_step,
+                                (int)ub * sg.km.batch_step);
+                for (int c = 0; c < DP / 64; c++)
+                    tma_load_4d(dst + TILE + c * CHUNK, mv, full, c * 64, (int)(first + i) * FEW_KEYS, kvh * sg.vm.head_step,
+                                (int)ub * sg.vm.batch_step);
+                if (++slot == STAGES) {
+                    slot = 0;
+                    phase ^= 1;
+                }
+            }
+            if (!ok) {   // let the copies in flight land before shared memory goes away
+                const long long t0 = clock64();
+                while (clock64() - t0 < 2000000LL) {
+                }
+            }
+        }
+        __syncwarp();
+    } else {
+        // query fragments: rows lane / 4 and 8 more, columns 16 i + 2 (lane % 4) and 8 more
+        uint32_t q[DP / 16][4];
+        int64_t end[2];
+        const int col = (lane & 3) * 2;
+#pragma unroll
+        for (int i = 0; i < DP / 16; i++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) q[i][e] = 0;
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            const int r = (lane >> 2) + 8 * e;
+            end[e] = (int64_t)1 << 40;   // rows that do not exist are not masked
+            if (r < sg.rows) {
+                const RowAt at = row_at(p, shared, unit, r);
+                end[e] = shared ? seq_len : p.len.seen(seq_len, at.t);
+                const uint16_t* const src = p.q.at(at.b, at.t, at.h);
+#pragma unroll
+                for (int i = 0; i < DP / 16; i++) {
+                    if (16 * i < p.d) q[i][e] = *reinterpret_cast<const uint32_t*>(src + 16 * i + col);
+                    if (16 * i + 8 < p.d) q[i][2 + e] = *reinterpret_cast<const uint32_t*>(src + 16 * i + 8 + col);
+                }
+            }
+        }
+        const float c = p.scale * kLog2e;
+        const float slack = fminf(8.f / c, 1e30f);
+        // this lane's row address in ldmatrix: matrix lane / 8, row lane % 8 of the warp's 16 keys
+        const int mi = lane >> 3, mr = lane & 7;
+        const int krow = warp * 16 + (mi >> 1) * 8 + mr, kpiece = mi & 1;   // keys: (0-7, d 0-7), (0-7, d 8-15), (8-15, ..)
+        const int vrow = warp * 16 + (mi & 1) * 8 + mr, vpiece = mi >> 1;   // values: (keys 0-7, d 0-7), (8-15, d 0-7), ..
+        int slot = 0;
+        uint32_t phase = 0;
+        for (int i = 0; i < n; i++) {
+            ok = __all_sync(0xffffffffu, wait(bar_full + slot * 8, phase));
+            if (!ok) break;
+            const uint32_t kt = sbase + slot * 2 * TILE, vt = kt + TILE;
+            const int64_t key0 = (first + i) * FEW_KEYS + warp * 16;
+            float s[2][4] = {};
+#pragma unroll
+            for (int ks = 0; ks < DP / 16; ks++) {
+                uint32_t b[4];
+                ldmatrix4(kt + (ks >> 2) * CHUNK + krow * 128 + ((((ks & 3) * 2 + kpiece) ^ mr) << 4), b);
+                mma16816<T>(s[0], q[ks], b[0], b[1]);
+                mma16816<T>(s[1], q[ks], b[2], b[3]);
+            }
+            if (key0 + 16 > seq_len && seq_len < sg.n) {
+                // rows behind the sequence's end, within the tensor: whatever they hold, 0 * it must be 0
+                const int dead = (int)max(seq_len - key0, (int64_t)0);
+                for (int x = lane; x < (16 - dead) * (DP / 8); x += 32) {
+                    const int rr = warp * 16 + dead + x / (DP / 8), pc = x % (DP / 8);
+                    *reinterpret_cast<uint4*>(smem + slot * 2 * TILE + TILE + (pc >> 3) * CHUNK + rr * 128 + (pc & 7) * 16) =
+                            make_uint4(0, 0, 0, 0);
+                }
+                __syncwarp();
+            }
+            // s[h][2 e + x]: row lane / 4 + 8 e, key key0 + 8 h + col + x
+            if (__any_sync(0xffffffffu, key0 + 16 > end[0] || key0 + 16 > end[1])) {
+#pragma unroll
+                for (int h = 0; h < 2; h++)
+#pragma unroll
+                    for (int x = 0; x < 4; x++)
+                        if (key0 + 8 * h + col + (x & 1) >= end[x >> 1]) s[h][x] = -CUDART_INF_F;
+            }
+            float top[2];
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                top[e] = fmaxf(fmaxf(s[0][2 * e], s[0][2 * e + 1]), fmaxf(s[1][2 * e], s[1][2 * e + 1]));
+                top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 1));
+                top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 2));
+            }
+            const bool g0 = top[0] > m[0] + slack, g1 = top[1] > m[1] + slack;
+            if (__any_sync(0xffffffffu, g0 || g1)) {
+                const float f0 = g0 ? ex2((m[0] - top[0]) * c) : 1.f, f1 = g1 ? ex2((m[1] - top[1]) * c) : 1.f;
+                if (g0) m[0] = top[0];
+                if (g1) m[1] = top[1];
+                l[0] *= f0;
+                l[1] *= f1;
+#pragma unroll
+                for (int t = 0; t < DP / 8; t++) {
+                    o[t][0] *= f0;
+                    o[t][1] *= f0;
+                    o[t][2] *= f1;
+                    o[t][3] *= f1;
+                }
+            }
+            uint32_t w[4];
+#pragma unroll
+            for (int h = 0; h < 2; h++)
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    const float mc = m[e] == -CUDART_INF_F ? 0.f : -m[e] * c;
+                    const float x = ex2(fmaf(s[h][2 * e], c, mc)), y = ex2(fmaf(s[h][2 * e + 1], c, mc));
+                    l[e] += x + y;
+                    w[2 * h + e] = pack2<T>(x, y);
+                }
+#pragma unroll
+            for (int t = 0; t < DP / 16; t++) {
+                uint32_t b[4];
+                ldmatrix4_trans(vt + (t >> 2) * CHUNK + vrow * 128 + ((((t & 3) * 2 + vpiece) ^ mr) << 4), b);
+                mma16816<T>(o[2 * t], w, b[0], b[1]);
+                mma16816<T>(o[2 * t + 1], w, b[2], b[3]);
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar_empty + slot * 8);
+            if (++slot == STAGES) {
+                slot = 0;
+                phase ^= 1;
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            l[e] += __shfl_xor_sync(0xffffffffu, l[e], 1);
+            l[e] += __shfl_xor_sync(0xffffffffu, l[e], 2);
+        }
+    }
+    // ---- the four warps' results become one, through the ring, which nobody uses any more
+    __syncthreads();
+    if (!*abort_flag) {
+        float* const po = reinterpret_cast<float*>(smem);                       // [4][FEW_ROWS][DP]
+        float* const pm = po + 4 * FEW_ROWS * DP, * const pl = pm + 4 * FEW_ROWS;   // base-2 maximum, sum
+        if (warp < 4) {
+            const float c = p.scale * kLog2e;
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                const int r = (lane >> 2) + 8 * e;
+                if ((lane & 3) == 0) {
+                    pm[warp * FEW_ROWS + r] = m[e] == -CUDART_INF_F ? -CUDART_INF_F : m[e] * c;
+                    pl[warp * FEW_ROWS + r] = l[e];
+                }
+#pragma unroll
+                for (int t = 0; t < DP / 8; t++)
+                    *reinterpret_cast<float2*>(po + (warp * FEW_ROWS + r) * DP + 8 * t + (lane & 3) * 2) = make_float2(o[t][2 * e], o[t][2 * e + 1]);
+            }
+        }
+        __syncthreads();
+        const int part = sg.part0 + sp;
+        for (int i = threadIdx.x; i < sg.rows * (DP / 8); i += FEW_THREADS) {
+            const int r = i / (DP / 8), c0 = i % (DP / 8) * 8;
+            if (c0 >= p.d) continue;
+            float top = -CUDART_INF_F, total = 0.f, acc[8] = {};
+            for (int x = 0; x < 4; x++) top = fmaxf(top, pm[x * FEW_ROWS + r]);
+            for (int x = 0; x < 4; x++) {
+                const float lx = pl[x * FEW_ROWS + r];
+                if (lx == 0.f) continue;   // saw nothing
+                // a sum that is not 0 with maximum -INF: NaN came in
+                const float mx = pm[x * FEW_ROWS + r], f = mx == top ? 1.f : ex2(mx - top);
+                total = fmaf(f, lx, total);
+                const float* const src = po + (x * FEW_ROWS + r) * DP + c0;
+#pragma unroll
+                for (int e = 0; e < 8; e++) acc[e] = fmaf(f, src[e], acc[e]);
+            }
+            const bool none = total == 0.f;
+            const float inv = none ? 0.f : 1.f / total;
+            const RowAt at = row_at(p, shared, unit, r);
+            const int64_t grow = (at.b * p.queries + at.t) * p.heads + at.h;
+            const float lse2 = none ? -CUDART_INF_F : log2f(total) + (top == -CUDART_INF_F ? 0.f : top);
+#pragma unroll
+            for (int e = 0; e < 8; e++) acc[e] = none ? 0.f : acc[e] * inv;
+            if (!p.part_o) {
+                *reinterpret_cast<uint4*>(p.out + grow * p.d + c0) = make_uint4(pack2<T>(acc[0], acc[1]), pack2<T>(acc[2], acc[3]),
+                                                                              pack2<T>(acc[4], acc[5]), pack2<T>(acc[6], acc[7]));
+                if (c0 == 0 && p.lse) p.lse[grow] = lse2 * kLn2;
+            } else {
+                float4* const dst = reinterpret_cast<float4*>(p.part_o + (part * p.rows_total + grow) * p.d + c0);
+                dst[0] = make_float4(acc[0], acc[1], acc[2], acc[3]);
+                dst[1] = make_float4(acc[4], acc[5], acc[6], acc[7]);
+                if (c0 == 0) p.part_lse[part * p.rows_total + grow] = lse2;
+            }
+        }
+    }
+    pdl_wait();
+}
+
 // ---- attend_join_kernel: partial results of a row become its result, a warp a row ------------------
 template <typename T>
 __global__ void __launch_bounds__(256) attend_join_kernel(const float* part_o, const float* part_lse, int parts, int64_t rows, int d,
@@ -434,52 +730,59 @@ __global__ void __launch_bounds__(256) attend_join_kernel(const float* part_o, c
 
 struct AttendPlan {
     Segment seg[2];
-    int64_t items;
+    int64_t items[2];   // CTAs of the tile kernel, of the few-rows kernel
     int parts;
     size_t scratch;
 };
 
-// Ranges of keys: as many as fill the SMs once, of at least MIN_TILES tiles; a segment's share goes by its tiles.
+// Ranges of keys.  Tiles: as many as fill the SMs once, of at least MIN_TILES tiles; a segment's share goes by its tiles.  Few
+// rows: about four turns of the two CTAs an SM takes, of at least FEW_MIN_TILES tiles.
 constexpr int MIN_TILES = 2;
+constexpr int FEW_MIN_TILES = 4;
 AttendPlan plan_attend(const B200FAttendArgs& a) {
     AttendPlan pl{};
     const int group = a.heads / a.kv_heads;
     const int64_t sm = cached_sm_count();
-    int64_t weight[2], base[2], total = 0;
+    int64_t weight[2] = {0, 0}, base[2] = {0, 0}, total = 0;
     for (int i = 0; i < 2; i++) {
         Segment& s = pl.seg[i];
         const int64_t units = i == 0 ? a.kv_heads : a.batch * a.kv_heads;
         s.n = i == 0 ? a.shared_n : a.n;
-        s.rows = (int)((i == 0 ? a.batch : 1) * a.queries * group);
+        const int64_t rows = (i == 0 ? a.batch : 1) * a.queries * group;
+        s.rows = (int)rows;
+        s.splits = s.row_blocks = 1;
+        // without any keys rows of zeros are written by the own segment
+        const bool on = s.n > 0 || (i == 1 && a.shared_n == 0);
+        s.few = rows <= FEW_ROWS;
+        if (!on) continue;
+        if (s.few) {
+            const int64_t tiles = ceil_div64(s.n, FEW_KEYS);
+            int64_t want = 8 * sm / units;
+            if (want > tiles / FEW_MIN_TILES) want = tiles / FEW_MIN_TILES;
+            s.splits = (int)(want < 1 ? 1 : want);
+            s.items = units * s.splits;
+            continue;
+        }
         const int64_t tiles = ceil_div64(s.n, ATT_TILE);
-        s.split = s.rows <= 128 && tiles >= 2;
-        s.row_blocks = (int)ceil_div64(s.rows, s.split ? 128 : 256);
-        base[i] = s.n > 0 ? units * s.row_blocks : 0;
+        s.split = rows <= 128 && tiles >= 2;
+        s.row_blocks = (int)ceil_div64(rows, s.split ? 128 : 256);
+        base[i] = units * s.row_blocks;
         weight[i] = base[i] * tiles;
         total += weight[i];
     }
-    if (total == 0) {   // no keys: rows of zeros, written by the own segment
-        base[1] = (a.batch * a.kv_heads) * pl.seg[1].row_blocks;
-        pl.seg[1].splits = 1;
-    }
     for (int i = 0; i < 2; i++) {
         Segment& s = pl.seg[i];
-        s.first = pl.items;
         s.part0 = pl.parts;
-        if (base[i] == 0) {
-            s.splits = 1;
-            s.row_blocks = 1;
-            continue;
-        }
-        if (total > 0) {
+        if (base[i] > 0) {
             const int64_t tiles = ceil_div64(s.n, ATT_TILE);
-            const int64_t share = (int64_t)((double)sm * weight[i] / total / base[i]);
+            const int64_t share = total > 0 ? (int64_t)((double)sm * weight[i] / total / base[i]) : 1;
             const int64_t most = tiles / (s.split ? 2 * MIN_TILES : MIN_TILES);
             s.splits = (int)(share < most ? share : most);
             if (s.splits < 1) s.splits = 1;
+            s.items = base[i] * s.splits;
         }
-        pl.items += base[i] * s.splits;
-        pl.parts += s.split ? 2 * s.splits : s.splits;
+        pl.items[s.few] += s.items;
+        if (s.items > 0) pl.parts += s.split ? 2 * s.splits : s.splits;
     }
     const int64_t rows = a.batch * a.queries * a.heads;
     pl.scratch = 256;
@@ -496,20 +799,34 @@ int check_attend(const B200FAttendArgs* a) {
 }
 
 template <typename T, int DP>
-int launch_tiles(const CUtensorMap* maps, const TileParams& p, int64_t items, cudaStream_t st) {
+int launch_attend(const CUtensorMap* maps, const TileParams& p, const AttendPlan& pl, cudaStream_t st) {
     static bool attr_set[kMaxDevices] = {false};
     const int slot = device_slot();
     if (!attr_set[slot]) {
         B200F_CUDA_TRY(cudaFuncSetAttribute(attend_tile_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, TILE_SMEM<DP>));
+        B200F_CUDA_TRY(cudaFuncSetAttribute(attend_few_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, FEW_SMEM<DP>));
         attr_set[slot] = true;
     }
-    const cudaError_t e = launch_kernel(attend_tile_kernel<T, DP>, dim3((unsigned)items), TILE_THREADS, TILE_SMEM<DP>, Launch(st), maps[0],
-                                        maps[1], maps[2], maps[3], p);
+    cudaError_t e = cudaSuccess;
+    if (pl.items[0] > 0) {
+        e = launch_kernel(attend_tile_kernel<T, DP>, dim3((unsigned)pl.items[0]), TILE_THREADS, TILE_SMEM<DP>, Launch(st), maps[0], maps[1],
+                          maps[2], maps[3], p);
+        count_launch();
+    }
+    if (e == cudaSuccess && pl.items[1] > 0) {
+        e = launch_kernel(attend_few_kernel<T, DP>, dim3((unsigned)pl.items[1]), FEW_THREADS, FEW_SMEM<DP>, Launch(st, pl.items[0] > 0),
+                          maps[0], maps[1], maps[2], maps[3], p);
+        count_launch();
+    }
+    if (e == cudaSuccess && pl.parts > 1) {
+        e = launch_kernel(attend_join_kernel<T>, dim3((unsigned)ceil_div64(p.rows_total, 8)), 256, 0, Launch(st, true),
+                          static_cast<const float*>(p.part_o), static_cast<const float*>(p.part_lse), pl.parts, p.rows_total, p.d, p.out, p.lse);
+        count_launch();
+    }
     if (e != cudaSuccess) {
         (void)cudaGetLastError();
         return B200F_ERR_CUDA;
     }
-    count_launch();
     return B200F_OK;
 }
 
@@ -536,16 +853,17 @@ extern "C" int b200f_attend(const B200FAttendArgs* a) {
         (a->shared_n > 0 && (!att_view_ok(sk, 1, a->shared_n, a->kv_heads) || !att_view_ok(sv, 1, a->shared_n, a->kv_heads))))
         return B200F_ERR_BAD_ARG;
     AttendPlan pl = plan_attend(*a);
-    if (!a->scratch || (reinterpret_cast<uintptr_t>(a->scratch) & 255) != 0 || a->scratch_bytes < pl.scratch) return B200F_ERR_SCRATCH;
-    if (pl.items > 0x7fffffff) return B200F_ERR_UNSUPPORTED;
+    if (pl.parts > 1 && (!a->scratch || (reinterpret_cast<uintptr_t>(a->scratch) & 255) != 0 || a->scratch_bytes < pl.scratch))
+        return B200F_ERR_SCRATCH;
+    if (pl.items[0] > 0x7fffffff || pl.items[1] > 0x7fffffff) return B200F_ERR_UNSUPPORTED;
     CUtensorMap maps[4] = {};
     if (a->shared_n > 0) {
-        rc = make_rows_map(&maps[0], &pl.seg[0].km, sk, a->storage, a->d, a->shared_n, a->kv_heads, 1);
-        if (rc == B200F_OK) rc = make_rows_map(&maps[1], &pl.seg[0].vm, sv, a->storage, a->d, a->shared_n, a->kv_heads, 1);
+        rc = make_rows_map(&maps[0], &pl.seg[0].km, sk, a->storage, a->d, a->shared_n, a->kv_heads, 1, pl.seg[0].few ? FEW_KEYS : ATT_TILE);
+        if (rc == B200F_OK) rc = make_rows_map(&maps[1], &pl.seg[0].vm, sv, a->storage, a->d, a->shared_n, a->kv_heads, 1, pl.seg[0].few ? FEW_KEYS : ATT_TILE);
     }
     if (a->n > 0 && rc == B200F_OK) {
-        rc = make_rows_map(&maps[2], &pl.seg[1].km, k, a->storage, a->d, a->n, a->kv_heads, a->batch);
-        if (rc == B200F_OK) rc = make_rows_map(&maps[3], &pl.seg[1].vm, v, a->storage, a->d, a->n, a->kv_heads, a->batch);
+        rc = make_rows_map(&maps[2], &pl.seg[1].km, k, a->storage, a->d, a->n, a->kv_heads, a->batch, pl.seg[1].few ? FEW_KEYS : ATT_TILE);
+        if (rc == B200F_OK) rc = make_rows_map(&maps[3], &pl.seg[1].vm, v, a->storage, a->d, a->n, a->kv_heads, a->batch, pl.seg[1].few ? FEW_KEYS : ATT_TILE);
     }
     if (rc != B200F_OK) return rc;
     TileParams p{};
@@ -569,19 +887,9 @@ extern "C" int b200f_attend(const B200FAttendArgs* a) {
         p.part_o = p.part_lse + round_up64(pl.parts * p.rows_total, 64);
     }
     const cudaStream_t st = (cudaStream_t)a->stream;
-    const bool half = a->storage == B200F_STORAGE_F16, wide = a->d > 64;
-    rc = half ? (wide ? launch_tiles<__half, 128>(maps, p, pl.items, st) : launch_tiles<__half, 64>(maps, p, pl.items, st))
-              : (wide ? launch_tiles<__nv_bfloat16, 128>(maps, p, pl.items, st) : launch_tiles<__nv_bfloat16, 64>(maps, p, pl.items, st));
-    if (rc != B200F_OK || pl.parts == 1) return rc;
-    const cudaError_t e = launch_kernel(half ? attend_join_kernel<__half> : attend_join_kernel<__nv_bfloat16>,
-                                        dim3((unsigned)ceil_div64(p.rows_total, 8)), 256, 0, Launch(st, true), p.part_o, p.part_lse, pl.parts,
-                                        p.rows_total, a->d, p.out, p.lse);
-    if (e != cudaSuccess) {
-        (void)cudaGetLastError();
-        return B200F_ERR_CUDA;
-    }
-    count_launch();
-    return B200F_OK;
+    if (a->storage == B200F_STORAGE_F16)
+        return a->d > 64 ? launch_attend<__half, 128>(maps, p, pl, st) : launch_attend<__half, 64>(maps, p, pl, st);
+    return a->d > 64 ? launch_attend<__nv_bfloat16, 128>(maps, p, pl, st) : launch_attend<__nv_bfloat16, 64>(maps, p, pl, st);
 }
 
 extern "C" int32_t* b200f_attention_status(void) {

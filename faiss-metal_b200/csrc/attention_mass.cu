@@ -383,7 +383,8 @@ extern "C" int b200f_attention_mass(const B200FAttentionMassArgs* a) {
         (a->queries > 0 && (!att_view_ok(q, a->batch, a->queries, a->heads) || (group > 1 && q.sh == 0) || !a->lse)))
         return B200F_ERR_BAD_ARG;
     const MassPlan pl = plan_mass(*a);
-    if (!a->scratch || (reinterpret_cast<uintptr_t>(a->scratch) & 255) != 0 || a->scratch_bytes < pl.scratch) return B200F_ERR_SCRATCH;
+    if (pl.splits > 1 && (!a->scratch || (reinterpret_cast<uintptr_t>(a->scratch) & 255) != 0 || a->scratch_bytes < pl.scratch))
+        return B200F_ERR_SCRATCH;
     const cudaStream_t st = (cudaStream_t)a->stream;
     const int64_t units = a->batch * a->kv_heads, total = units * a->n, items = units * pl.blocks * pl.splits;
     if (items > 0x7fffffff || ceil_div64(total, 256) > 0x7fffffff) return B200F_ERR_UNSUPPORTED;

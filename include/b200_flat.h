@@ -359,7 +359,8 @@ typedef struct B200FAttendArgs {
     const int32_t* key_lengths; /* of the own keys */
     void* out;                  /* [batch][queries][heads][d], dense */
     float* lse;                 /* optional: log of the sum of exp(scale * q.k), natural */
-    void* scratch;              /* b200f_attend_scratch_bytes(), 256-byte aligned */
+    void* scratch;              /* b200f_attend_scratch_bytes(), 256-byte aligned; at most 256 bytes: not used, may
+                                   be NULL (here and for the accumulated weights) */
     size_t scratch_bytes;
     int32_t* status;
     void* stream;
