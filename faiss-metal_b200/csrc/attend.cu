@@ -11,19 +11,26 @@ namespace b200f {
 namespace {
 
 // ---- attend_tile_kernel ------------------------------------------------------------------
-// One CTA takes two streams of score tiles [128 rows][128 keys] in turn, each with its own softmax warps (a row a thread) and its
-// own half of tensor memory: S (128 columns, whose first half then holds the weights P) and O.  While one stream's warps
-// exponentiate, the tensor cores work for the other.  PAIR: two row tiles over the same keys, each key tile fetched once for both.
-// SPLIT (no more than 128 rows): one row tile, the streams have different keys.
-// O is rescaled only when a row's maximum grew by more than 2^8 over the one its weights refer to; sums stay in fp32.
-constexpr int TILE_THREADS = 384;          // TMA, MMA, two spare warps; 2 x 4 softmax warps
+// One CTA takes two streams of score tiles [128 rows][128 keys], each with its own issuing warp, its own four softmax warps (a row a
+// thread) and its own half of tensor memory: S (128 columns, whose first half then holds the weights P) and O.  PAIR: two row tiles
+// over the same keys, each key tile fetched once for both.  SPLIT (no more than 128 rows): one row tile, the streams have
+// different keys.  While one stream exponentiates, the tensor cores work for the other.
+// Weights are exp2(c (s - m)) for a reference m that is taken from a row's first tile and moves, with O rescaled, only when a tile's
+// weights add up to 2^15 or more: no maximum is looked for before the exponentials.  Sums stay in fp32.
+constexpr int TILE_THREADS = 384;          // TMA, an issuer of MMAs a stream, a spare warp; 2 x 4 softmax warps
+constexpr int TILE_REGS_FEW = 80, TILE_REGS_MANY = 208;   // 128 and 256 threads of the 384 x 168 at launch
+static_assert(128 * TILE_REGS_FEW + 256 * TILE_REGS_MANY <= 384 * 168, "registers of a CTA");
+constexpr float WEIGHTS_MAX = 32768.f;     // fp16 weights end at 65504
+constexpr int TILE_KEYS = 128;
 constexpr int TILE_MAX_STAGES = 10;
 template <int DP>
-constexpr int TILE_STAGE_BYTES = DP / 64 * ATT_CHUNK;
+constexpr int TILE_Q_BYTES = DP / 64 * ATT_CHUNK;
+template <int DP>
+constexpr int TILE_STAGE_BYTES = DP / 64 * TILE_KEYS * 128;
 template <int DP>
 constexpr int TILE_STAGES = DP == 128 ? 5 : 10;
 template <int DP>
-constexpr int TILE_SM_BAR = (2 + TILE_STAGES<DP>)*TILE_STAGE_BYTES<DP>;
+constexpr int TILE_SM_BAR = 2 * TILE_Q_BYTES<DP> + TILE_STAGES<DP>*TILE_STAGE_BYTES<DP>;
 template <int DP>
 constexpr int TILE_SMEM = TILE_SM_BAR<DP> + (2 * TILE_MAX_STAGES + 6) * 8 + 16;
 static_assert(TILE_SMEM<128> <= 232448 && TILE_SMEM<64> <= 232448, "shared memory of a CTA");
@@ -75,13 +82,14 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
 attend_tile_kernel(const __grid_constant__ CUtensorMap map_sk, const __grid_constant__ CUtensorMap map_sv,
                    const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const TileParams p) {
     extern __shared__ __align__(1024) uint8_t smem[];
-    constexpr int STAGES = TILE_STAGES<DP>, STAGE = TILE_STAGE_BYTES<DP>, CHUNKS = DP / 64;
+    constexpr int STAGES = TILE_STAGES<DP>, STAGE = TILE_STAGE_BYTES<DP>, QBYTES = TILE_Q_BYTES<DP>, CHUNKS = DP / 64;
+    constexpr int HALF_RING = (STAGES + 1) / 2;
     const uint32_t sbase = smem_u32(smem);
     const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0);
     const int lane = threadIdx.x & 31;
     const uint32_t bar_full = sbase + TILE_SM_BAR<DP>, bar_empty = bar_full + TILE_MAX_STAGES * 8;
-    const uint32_t bar_s = bar_empty + TILE_MAX_STAGES * 8, bar_p = bar_s + 16, bar_o = bar_p + 16;
-    volatile uint32_t* tmem_ptr = reinterpret_cast<volatile uint32_t*>(smem + TILE_SM_BAR<DP> + (2 * TILE_MAX_STAGES + 6) * 8);
+    const uint32_t bar_s = bar_empty + TILE_MAX_STAGES * 8, bar_p = bar_s + 16, bar_done = bar_p + 16;   // [stream]
+    volatile uint32_t* tmem_ptr = reinterpret_cast<volatile uint32_t*>(smem + TILE_SMEM<DP> - 16);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_ptr + 1);
 
     pdl_wait();
@@ -109,7 +117,7 @@ attend_tile_kernel(const __grid_constant__ CUtensorMap map_sk, const __grid_cons
         const int64_t last = min((int64_t)sg.rows, row0 + (sg.split ? 128 : 256)) - 1;
         seen_max = p.len.seen(seq_len, last / p.group);
     }
-    const int64_t ntiles = (seen_max + ATT_TILE - 1) / ATT_TILE;
+    const int64_t ntiles = (seen_max + TILE_KEYS - 1) / TILE_KEYS;
     const int pieces = sg.split ? 2 * sg.splits : sg.splits;
     const int64_t per = (ntiles + pieces - 1) / pieces;
     const int64_t ka = min(ntiles, per * (sg.split ? 2 * sp : sp)), kb = min(ntiles, ka + per);
@@ -125,10 +133,10 @@ attend_tile_kernel(const __grid_constant__ CUtensorMap map_sk, const __grid_cons
             mbar_init(bar_full + s * 8, 1);
             mbar_init(bar_empty + s * 8, 1);
         }
-        for (int t = 0; t < 2; t++) {
-            mbar_init(bar_s + t * 8, 1);
-            mbar_init(bar_p + t * 8, 4);
-            mbar_init(bar_o + t * 8, 1);
+        for (int i = 0; i < 2; i++) {
+            mbar_init(bar_s + i * 8, 1);
+            mbar_init(bar_p + i * 8, 4);
+            mbar_init(bar_done + i * 8, 1);
         }
         mbar_fence_init();
     }
@@ -142,52 +150,57 @@ attend_tile_kernel(const __grid_constant__ CUtensorMap map_sk, const __grid_cons
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_ptr;
-    const uint32_t ring = sbase + 2 * STAGE;
+    const uint32_t ring = sbase + 2 * QBYTES;
     auto wait = [&](uint32_t bar, uint32_t parity) { return mbar_wait(bar, parity, abort_flag, p.status); };
 
     if (warp != 0) {
         // query rows to shared memory, swizzled as TMA would: 16-byte piece c of row r goes to piece c ^ (r & 7)
-        const int nrows = sg.split ? 128 : 256;
-        for (int i = threadIdx.x - 32; i < nrows * (DP / 8); i += TILE_THREADS - 32) {
-            const int r = i / (DP / 8), c = i % (DP / 8);
+        // DP / 8 threads a row
+        constexpr int PER_ROW = DP / 8, AT_ONCE = (TILE_THREADS - 32) / PER_ROW;
+        const int nrows = sg.split ? 128 : 256, c = (threadIdx.x - 32) % PER_ROW;
+        for (int r = (threadIdx.x - 32) / PER_ROW; r < nrows; r += AT_ONCE) {
             uint4 x = make_uint4(0, 0, 0, 0);
             if (row0 + r < sg.rows && c * 8 < p.d) {
                 const RowAt a = row_at(p, shared, unit, row0 + r);
                 x = *reinterpret_cast<const uint4*>(p.q.at(a.b, a.t, a.h) + c * 8);
             }
-            *reinterpret_cast<uint4*>(smem + (r >> 7) * STAGE + (c >> 3) * ATT_CHUNK + (r & 127) * 128 + (((c & 7) ^ (r & 7)) << 4)) = x;
+            *reinterpret_cast<uint4*>(smem + (r >> 7) * QBYTES + (c >> 3) * ATT_CHUNK + (r & 127) * 128 + (((c & 7) ^ (r & 7)) << 4)) = x;
         }
         fence_proxy_async_shared();
         asm volatile("bar.sync 1, %0;" ::"n"(TILE_THREADS - 32) : "memory");
     }
 
+    if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(TILE_REGS_FEW));
     if (warp == 0) {
         // ------------------------------ keys and values in the order of their use ------------------------------
         if (elect_one()) {
-            int slot = 0;
-            uint32_t phase = 0;
+            int slot[2] = {0, HALF_RING};   // SPLIT: a half of the ring a stream
+            uint32_t phase[2] = {0, 0};
             bool ok = true;
-            auto load = [&](const CUtensorMap* m, const AttMap& am, int tile) {
-                if (!ok || !(ok = wait(bar_empty + slot * 8, phase ^ 1))) return;
-                mbar_arrive_expect_tx(bar_full + slot * 8, STAGE);
+            auto load = [&](int t, const CUtensorMap* m, const AttMap& am, int tile) {
+                const int s = slot[t];
+                if (!ok || !(ok = wait(bar_empty + s * 8, phase[t] ^ 1))) return;
+                mbar_arrive_expect_tx(bar_full + s * 8, STAGE);
                 for (int c = 0; c < CHUNKS; c++)
-                    tma_load_4d(ring + slot * STAGE + c * ATT_CHUNK, m, bar_full + slot * 8, c * 64, tile * ATT_TILE, kvh * am.head_step,
-                                (int)ub * am.batch_step);
-                if (++slot == STAGES) {
-                    slot = 0;
-                    phase ^= 1;
+                    tma_load_4d(ring + s * STAGE + c * TILE_KEYS * 128, m, bar_full + s * 8, c * 64, tile * TILE_KEYS,
+                                kvh * am.head_step, (int)ub * am.batch_step);
+                const int end = sg.split && t == 0 ? HALF_RING : STAGES;
+                if (++slot[t] == end) {
+                    slot[t] = t == 0 ? 0 : HALF_RING;
+                    phase[t] ^= 1;
                 }
             };
             const CUtensorMap* mk = shared ? &map_sk : &map_k;
             const CUtensorMap* mv = shared ? &map_sv : &map_v;
-            if (n0 > 0) load(mk, sg.km, first0);
-            if (sg.split && n1 > 0) load(mk, sg.km, first1);
+            if (n0 > 0) load(0, mk, sg.km, first0);
+            if (sg.split && n1 > 0) load(1, mk, sg.km, first1);
             for (int j = 0; j < n0 && ok; j++) {
-                load(mv, sg.vm, first0 + j);
-                if (j + 1 < n0) load(mk, sg.km, first0 + j + 1);
+                load(0, mv, sg.vm, first0 + j);
+                if (j + 1 < n0) load(0, mk, sg.km, first0 + j + 1);
                 if (sg.split && j < n1) {
-                    load(mv, sg.vm, first1 + j);
-                    if (j + 1 < n1) load(mk, sg.km, first1 + j + 1);
+                    load(1, mv, sg.vm, first1 + j);
+                    if (j + 1 < n1) load(1, mk, sg.km, first1 + j + 1);
                 }
             }
             if (!ok) {   // let the copies in flight land before shared memory goes away
@@ -200,56 +213,71 @@ attend_tile_kernel(const __grid_constant__ CUtensorMap map_sk, const __grid_cons
     } else if (warp == 1) {
         // ------------------------------ MMA issuer ------------------------------
         const bool leader = elect_one();
-        int cur = 0;
-        uint32_t phase = 0;
         bool ok = true;
-        const int boundary = seq_len < sg.n && (seq_len & (ATT_TILE - 1)) ? (int)(seq_len / ATT_TILE) : -1;
-        auto take = [&]() {   // the next stage, once it is full
-            const int s = cur;
-            ok = ok && wait(bar_full + s * 8, phase);
-            if (++cur == STAGES) {
-                cur = 0;
-                phase ^= 1;
+        const int tail = (int)(seq_len & (TILE_KEYS - 1));
+        const int boundary = seq_len < sg.n && tail ? (int)(seq_len / TILE_KEYS) : -1;
+        const uint64_t dq = make_smem_desc(sbase), dk = make_smem_desc(ring), dv = make_smem_desc_mn(ring, TILE_KEYS * 128);
+        constexpr uint64_t QCHUNK = ATT_CHUNK >> 4, KCHUNK = (TILE_KEYS * 128) >> 4;
+        const int last = n1 > 0 && !sg.split ? 1 : 0;   // PAIR: the stream that uses a stage last
+        int slot[2] = {0, sg.split ? HALF_RING : 0};
+        uint32_t phase[2] = {0, 0};
+        auto next = [&](int t) __attribute__((always_inline)) {
+            if (++slot[t] == (sg.split && t == 0 ? HALF_RING : STAGES)) {
+                slot[t] = sg.split && t == 1 ? HALF_RING : 0;
+                phase[t] ^= 1;
             }
-            return s;
         };
-        int kslot = 0, vslot = 0;
-        const int last = n1 > 0 && !sg.split ? 1 : 0;   // the stream that uses a stage last
-        auto scores = [&](int t) {
-            if (t == 0 || sg.split) kslot = take();
+        auto scores = [&](int t) __attribute__((always_inline)) {   // from the next stage
+            if (t == 0 || sg.split) ok = ok && wait(bar_full + slot[t] * 8, phase[t]);
             tc_fence_after();
-            mma_rows<T, DP, ATT_TILE>(leader && ok, tmem + TM_S + 128 * t, sbase + (sg.split ? 0 : t) * STAGE, ring + kslot * STAGE);
+            const uint64_t da = dq + (sg.split ? 0 : t * (uint64_t)(QBYTES >> 4)), db = dk + (uint64_t)(slot[t] * (STAGE >> 4));
+#pragma unroll
+            for (int c = 0; c < CHUNKS; c++)
+#pragma unroll
+                for (int k = 0; k < 4; k++)
+                    tc_mma_f16_by<false>(leader, tmem + TM_S + 128 * t, da + c * QCHUNK + 2 * k, db + c * KCHUNK + 2 * k,
+                                         att_idesc<T>(TILE_KEYS, false), c + k > 0);
             tc_commit_by<false>(leader, bar_s + t * 8);
-            if (t == last || sg.split) tc_commit_by<false>(leader, bar_empty + kslot * 8);
+            if (t == last || sg.split) tc_commit_by<false>(leader, bar_empty + slot[t] * 8);
+            next(t);
+        };
+        auto values = [&](int t, int j) __attribute__((always_inline)) {
+            if (t == 0 || sg.split) {
+                ok = ok && wait(bar_full + slot[t] * 8, phase[t]);
+                // rows behind the sequence's end, within the tensor: whatever they hold, 0 * it must be 0
+                if ((t ? first1 : first0) + j == boundary && __all_sync(0xffffffffu, ok))
+                    zero_tile_rows(smem + 2 * QBYTES + slot[t] * STAGE, CHUNKS, tail, TILE_KEYS);
+            }
+            ok = ok && wait(bar_p + t * 8, j & 1);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) return;
+            tc_fence_after();
+            const uint64_t db = dv + (uint64_t)(slot[t] * (STAGE >> 4));
+#pragma unroll
+            for (int k = 0; k < TILE_KEYS / 16; k++)
+                tc_mma_ts_by(leader, tmem + TM_O + 128 * t, tmem + TM_S + 128 * t + 8 * k, db + 128 * k, att_idesc<T>(DP, true),
+                             k > 0 ? 1u : (uint32_t)(j > 0));
+            if (j + 1 == (t ? n1 : n0)) tc_commit_by<false>(leader, bar_done + t * 8);
+            if (t == last || sg.split) tc_commit_by<false>(leader, bar_empty + slot[t] * 8);
+            next(t);
         };
         if (n0 > 0) scores(0);
         if (n1 > 0) scores(1);
         for (int j = 0; j < n0 && ok; j++) {
-            for (int t = 0; t < 2 && ok; t++) {
-                if (j >= (t ? n1 : n0)) continue;
-                if (t == 0 || sg.split) {
-                    vslot = take();
-                    // rows behind the sequence's end, within the tensor: whatever they hold, 0 * it must be 0
-                    if (ok && (t ? first1 : first0) + j == boundary)
-                        zero_tile_rows(smem + 2 * STAGE + vslot * STAGE, CHUNKS, (int)(seq_len & (ATT_TILE - 1)), ATT_TILE);
-                }
-                ok = ok && wait(bar_p + t * 8, j & 1);
-                ok = __all_sync(0xffffffffu, ok);
-                tc_fence_after();
-                mma_weights<T, DP, ATT_TILE>(leader && ok, tmem + TM_O + 128 * t, tmem + TM_S + 128 * t, ring + vslot * STAGE, j > 0);
-                if (t == last || sg.split) tc_commit_by<false>(leader, bar_empty + vslot * 8);
-                if (j + 1 < (t ? n1 : n0)) scores(t);
-                else tc_commit_by<false>(leader, bar_o + t * 8);
-            }
-            ok = __all_sync(0xffffffffu, ok);
+            values(0, j);
+            if (ok && j + 1 < n0) scores(0);
+            if (ok && j < n1) values(1, j);
+            if (ok && j + 1 < n1) scores(1);
         }
         if (!ok) {   // let the MMAs in flight retire before tensor memory goes away
             const long long t0 = clock64();
             while (clock64() - t0 < 200000LL) {
             }
         }
-    } else if (warp >= 4) {
+    }
+    } else {
         // ------------------------------ softmax, a row a thread ------------------------------
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(TILE_REGS_MANY));
         const int t = (warp - 4) >> 2, ew = warp & 3;
         const int nt = t ? n1 : n0, kt0 = t ? first1 : first0;
         const int64_t r = row0 + (sg.split ? 0 : t * 128) + ew * 32 + lane;
@@ -258,76 +286,79 @@ attend_tile_kernel(const __grid_constant__ CUtensorMap map_sk, const __grid_cons
         RowAt at{0, 0, 0};
         if (live) at = row_at(p, shared, unit, r);
         // keys this row sees; rows that do not exist are not masked
-        const int64_t end = !live ? (int64_t)1 << 40 : shared ? seq_len : p.len.seen(seq_len, at.t);
+        const int end = !live ? 0x7ffffff0 : (int)(shared ? seq_len : p.len.seen(seq_len, at.t));
         const uint32_t ts = tmem + TM_S + 128 * t + ((uint32_t)(ew * 32) << 16);
         const uint32_t to = tmem + TM_O + 128 * t + ((uint32_t)(ew * 32) << 16);
         const float c = p.scale * kLog2e;
-        const float slack = fminf(8.f / c, 1e30f);
-        float m = -CUDART_INF_F, l = 0.f;   // weights are exp2(c (s - m))
+        float m = -CUDART_INF_F, l = 0.f;
+        float mc = CUDART_NAN_F;   // -c m; no reference yet: the first tile's sum fails the test below
         bool ok = true;
+        uint32_t s[4][32];
+        // weights of 32 keys to tensor memory; returns their sum
+        auto weigh = [&](uint32_t (&x)[32], float mc_now, int i) __attribute__((always_inline)) {
+            const float2 c2 = make_float2(c, c), mc2 = make_float2(mc_now, mc_now);
+            float2 sum[2];
+            uint32_t w[16];
+#pragma unroll
+            for (int e = 0; e < 16; e++) {
+                float2 y = fma2(make_float2(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1])), c2, mc2);
+                y.x = ex2(y.x);
+                y.y = ex2(y.y);
+                sum[e & 1] = e < 2 ? y : add2(sum[e & 1], y);
+                w[e] = pack2<T>(y.x, y.y);
+            }
+            tc_st16(ts + 16 * i, w);
+            const float2 z = add2(sum[0], sum[1]);
+            return z.x + z.y;
+        };
         for (int j = 0; j < nt; j++) {
             ok = __all_sync(0xffffffffu, wait(bar_s + t * 8, j & 1));
             if (!ok) break;
             if (warp_live) {
                 tc_fence_after();
-                uint32_t s[4][32];
-#pragma unroll
-                for (int i = 0; i < 4; i++) tc_ld32(ts + 32 * i, s[i]);
-#pragma unroll
-                for (int i = 0; i < 4; i++) tc_wait_ld32(s[i]);
-                const int64_t key0 = (int64_t)(kt0 + j) * ATT_TILE;
-                if (__any_sync(0xffffffffu, key0 + ATT_TILE > end)) {
-                    const int lim = (int)max(min(end - key0, (int64_t)ATT_TILE), (int64_t)0);
-#pragma unroll
-                    for (int i = 0; i < 128; i++)
-                        if (i >= lim) s[i >> 5][i & 31] = 0xff800000u;   // -INF
-                }
-                float mx[4];
+                const int lim = end - (kt0 + j) * TILE_KEYS;
+                const bool masked = __any_sync(0xffffffffu, lim < TILE_KEYS);
+                float sum = 0.f;
+                tc_ld32(ts, s[0]);
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    float a = max3(__uint_as_float(s[i][0]), __uint_as_float(s[i][1]), __uint_as_float(s[i][2]));
-                    float b = max3(__uint_as_float(s[i][3]), __uint_as_float(s[i][4]), __uint_as_float(s[i][5]));
+                    tc_wait_ld32(s[i]);
+                    if (i < 3) tc_ld32(ts + 32 * (i + 1), s[i + 1]);   // under the exponentials of this chunk
+                    if (masked) {
 #pragma unroll
-                    for (int e = 6; e < 30; e += 4) {
-                        a = max3(a, __uint_as_float(s[i][e]), __uint_as_float(s[i][e + 1]));
-                        b = max3(b, __uint_as_float(s[i][e + 2]), __uint_as_float(s[i][e + 3]));
+                        for (int e = 0; e < 32; e++)
+                            if (32 * i + e >= lim) s[i][e] = 0xff800000u;   // -INF
                     }
-                    mx[i] = max3(max3(a, b, __uint_as_float(s[i][30])), __uint_as_float(s[i][31]), -CUDART_INF_F);
+                    sum += weigh(s[i], mc, i);
                 }
-                const float top = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]);
-                const bool grown = top > m + slack;
-                if (__any_sync(0xffffffffu, grown)) {
-                    const float f = grown ? ex2((m - top) * c) : 1.f;   // 0 where nothing was seen before
-                    if (grown) m = top;
-                    l *= f;
-                    if (j > 0) {
-#pragma unroll 1
-                        for (int i = 0; i < DP / 32; i++) {
-                            uint32_t o[32];
-                            tc_ld32(to + 32 * i, o);
-                            tc_wait_ld32(o);
+                if (__any_sync(0xffffffffu, !(sum < WEIGHTS_MAX))) {
+                    // a new reference, from this tile's maximum; the tile once more
+                    const bool grown = !(sum < WEIGHTS_MAX);
+                    float top = -CUDART_INF_F;
 #pragma unroll
-                            for (int e = 0; e < 32; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-                            tc_st32(to + 32 * i, o);
+                    for (int i = 0; i < 4; i++)
+#pragma unroll
+                        for (int e = 0; e < 32; e += 2) top = max3(top, __uint_as_float(s[i][e]), __uint_as_float(s[i][e + 1]));
+                    const float now = grown ? fmaxf(top, m) : m;
+                    const float f = now == m ? 1.f : ex2((m - now) * c);   // 0 where nothing was seen before
+                    m = now;
+                    l *= f;
+                    mc = m == -CUDART_INF_F ? CUDART_NAN_F : -m * c;
+                    if (j > 0) {   // the scores are there, so the previous tile's product is done
+#pragma unroll 1
+                        for (int i = 0; i < DP / 16; i++) {
+                            uint32_t o[16];
+                            tc_ld16_wait(to + 16 * i, o);
+#pragma unroll
+                            for (int e = 0; e < 16; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                            tc_st16(to + 16 * i, o);
                         }
                     }
-                }
-                const float mc = m == -CUDART_INF_F ? 0.f : -m * c;
-                float sum[4] = {0.f, 0.f, 0.f, 0.f};
+                    sum = 0.f;
 #pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    uint32_t w[32];
-#pragma unroll
-                    for (int e = 0; e < 32; e++) {
-                        const float a = ex2(fmaf(__uint_as_float(s[2 * h + (e >> 4)][(2 * e) & 31]), c, mc));
-                        const float b = ex2(fmaf(__uint_as_float(s[2 * h + (e >> 4)][(2 * e + 1) & 31]), c, mc));
-                        sum[e & 1] += a;
-                        sum[2 + (e & 1)] += b;
-                        w[e] = pack2<T>(a, b);
-                    }
-                    tc_st32(ts + 32 * h, w);
+                    for (int i = 0; i < 4; i++) sum += weigh(s[i], m == -CUDART_INF_F ? 0.f : mc, i);
                 }
-                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                l += sum;
                 tc_wait_st();
                 tc_fence_before();
             }
@@ -335,49 +366,44 @@ attend_tile_kernel(const __grid_constant__ CUtensorMap map_sk, const __grid_cons
             if (lane == 0) mbar_arrive(bar_p + t * 8);
         }
         // ------------------------------ this row's output ------------------------------
-        if (ok && nt > 0) ok = __all_sync(0xffffffffu, wait(bar_o + t * 8, 0));
-        const bool empty_stream = nt == 0;
+        if (ok && nt > 0) ok = wait(bar_done + t * 8, 0);
+        ok = __all_sync(0xffffffffu, ok);
         if (ok && warp_live) {
             tc_fence_after();
+            const bool none = nt == 0;
             const int64_t grow = (at.b * p.queries + at.t) * p.heads + at.h;
             const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
             const float lse2 = l > 0.f || l != l ? log2f(l) + (m == -CUDART_INF_F ? 0.f : m * c) : -CUDART_INF_F;
             const bool whole = p.part_o == nullptr;
             const int part = sg.part0 + (sg.split ? 2 * sp + t : sp);
-            {
-                if (live) {
-                    if (whole) {
-                        if (p.lse) p.lse[grow] = lse2 * kLn2;
-                    } else {
-                        p.part_lse[part * p.rows_total + grow] = lse2;
-                    }
+            if (live) {
+                if (whole) {
+                    if (p.lse) p.lse[grow] = lse2 * kLn2;
+                } else {
+                    p.part_lse[part * p.rows_total + grow] = lse2;
                 }
+            }
 #pragma unroll 1
-                for (int i = 0; i < DP / 32; i++) {
-                    uint32_t o[32];
-                    if (!empty_stream) {
-                        tc_ld32(to + 32 * i, o);
-                        tc_wait_ld32(o);
-                    }
+            for (int i = 0; i < DP / 16; i++) {
+                uint32_t o[16];
+                if (!none) tc_ld16_wait(to + 16 * i, o);
 #pragma unroll
-                    for (int e = 0; e < 32; e++) o[e] = inv == 0.f ? 0u : __float_as_uint(__uint_as_float(o[e]) * inv);
-                    if (!live) continue;
-                    if (whole) {
+                for (int e = 0; e < 16; e++) o[e] = inv == 0.f ? 0u : __float_as_uint(__uint_as_float(o[e]) * inv);
+                if (!live) continue;
+                if (whole) {
 #pragma unroll
-                        for (int e = 0; e < 32; e += 8)
-                            if (32 * i + e < p.d)
-                                *reinterpret_cast<uint4*>(p.out + grow * p.d + 32 * i + e) =
-                                        make_uint4(pack2<T>(__uint_as_float(o[e]), __uint_as_float(o[e + 1])),
-                                                   pack2<T>(__uint_as_float(o[e + 2]), __uint_as_float(o[e + 3])),
-                                                   pack2<T>(__uint_as_float(o[e + 4]), __uint_as_float(o[e + 5])),
-                                                   pack2<T>(__uint_as_float(o[e + 6]), __uint_as_float(o[e + 7])));
-                    } else if (!empty_stream) {
-                        float* const po = p.part_o + (part * p.rows_total + grow) * p.d;
+                    for (int e = 0; e < 16; e += 8)
+                        if (16 * i + e < p.d)
+                            *reinterpret_cast<uint4*>(p.out + grow * p.d + 16 * i + e) =
+                                    make_uint4(pack2<T>(__uint_as_float(o[e]), __uint_as_float(o[e + 1])),
+                                               pack2<T>(__uint_as_float(o[e + 2]), __uint_as_float(o[e + 3])),
+                                               pack2<T>(__uint_as_float(o[e + 4]), __uint_as_float(o[e + 5])),
+                                               pack2<T>(__uint_as_float(o[e + 6]), __uint_as_float(o[e + 7])));
+                } else if (!none) {
+                    float* const po = p.part_o + (part * p.rows_total + grow) * p.d;
 #pragma unroll
-                        for (int e = 0; e < 32; e += 4)
-                            if (32 * i + e < p.d)
-                                *reinterpret_cast<uint4*>(po + 32 * i + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
-                    }
+                    for (int e = 0; e < 16; e += 4)
+                        if (16 * i + e < p.d) *reinterpret_cast<uint4*>(po + 16 * i + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
                 }
             }
         }
@@ -763,7 +789,7 @@ AttendPlan plan_attend(const B200FAttendArgs& a) {
             s.items = units * s.splits;
             continue;
         }
-        const int64_t tiles = ceil_div64(s.n, ATT_TILE);
+        const int64_t tiles = ceil_div64(s.n, TILE_KEYS);
         s.split = rows <= 128 && tiles >= 2;
         s.row_blocks = (int)ceil_div64(rows, s.split ? 128 : 256);
         base[i] = units * s.row_blocks;
@@ -774,7 +800,7 @@ AttendPlan plan_attend(const B200FAttendArgs& a) {
         Segment& s = pl.seg[i];
         s.part0 = pl.parts;
         if (base[i] > 0) {
-            const int64_t tiles = ceil_div64(s.n, ATT_TILE);
+            const int64_t tiles = ceil_div64(s.n, TILE_KEYS);
             const int64_t share = total > 0 ? (int64_t)((double)sm * weight[i] / total / base[i]) : 1;
             const int64_t most = tiles / (s.split ? 2 * MIN_TILES : MIN_TILES);
             s.splits = (int)(share < most ? share : most);
@@ -858,12 +884,12 @@ extern "C" int b200f_attend(const B200FAttendArgs* a) {
     if (pl.items[0] > 0x7fffffff || pl.items[1] > 0x7fffffff) return B200F_ERR_UNSUPPORTED;
     CUtensorMap maps[4] = {};
     if (a->shared_n > 0) {
-        rc = make_rows_map(&maps[0], &pl.seg[0].km, sk, a->storage, a->d, a->shared_n, a->kv_heads, 1, pl.seg[0].few ? FEW_KEYS : ATT_TILE);
-        if (rc == B200F_OK) rc = make_rows_map(&maps[1], &pl.seg[0].vm, sv, a->storage, a->d, a->shared_n, a->kv_heads, 1, pl.seg[0].few ? FEW_KEYS : ATT_TILE);
+        rc = make_rows_map(&maps[0], &pl.seg[0].km, sk, a->storage, a->d, a->shared_n, a->kv_heads, 1, pl.seg[0].few ? FEW_KEYS : TILE_KEYS);
+        if (rc == B200F_OK) rc = make_rows_map(&maps[1], &pl.seg[0].vm, sv, a->storage, a->d, a->shared_n, a->kv_heads, 1, pl.seg[0].few ? FEW_KEYS : TILE_KEYS);
     }
     if (a->n > 0 && rc == B200F_OK) {
-        rc = make_rows_map(&maps[2], &pl.seg[1].km, k, a->storage, a->d, a->n, a->kv_heads, a->batch, pl.seg[1].few ? FEW_KEYS : ATT_TILE);
-        if (rc == B200F_OK) rc = make_rows_map(&maps[3], &pl.seg[1].vm, v, a->storage, a->d, a->n, a->kv_heads, a->batch, pl.seg[1].few ? FEW_KEYS : ATT_TILE);
+        rc = make_rows_map(&maps[2], &pl.seg[1].km, k, a->storage, a->d, a->n, a->kv_heads, a->batch, pl.seg[1].few ? FEW_KEYS : TILE_KEYS);
+        if (rc == B200F_OK) rc = make_rows_map(&maps[3], &pl.seg[1].vm, v, a->storage, a->d, a->n, a->kv_heads, a->batch, pl.seg[1].few ? FEW_KEYS : TILE_KEYS);
     }
     if (rc != B200F_OK) return rc;
     TileParams p{};

@@ -75,6 +75,45 @@ __device__ __forceinline__ void tc_ld16_wait(uint32_t taddr, uint32_t (&r)[16]) 
 }
 __device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// 32 lanes x 64 consecutive columns, complete on return
+__device__ __forceinline__ void tc_ld64_wait(uint32_t taddr, uint32_t (&r)[64]) {
+    uint32_t (&a)[32] = *reinterpret_cast<uint32_t (*)[32]>(&r[0]);
+    uint32_t (&b)[32] = *reinterpret_cast<uint32_t (*)[32]>(&r[32]);
+    tc_ld32(taddr, a);
+    tc_ld32(taddr + 32, b);
+    tc_wait_ld32(a);
+    tc_wait_ld32(b);
+}
+
+// two at once
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{\n\t"
+        ".reg .b64 a, b, c, d;\n\t"
+        "mov.b64 a, {%2, %3};\n\t"
+        "mov.b64 b, {%4, %5};\n\t"
+        "mov.b64 c, {%6, %7};\n\t"
+        "fma.rn.f32x2 d, a, b, c;\n\t"
+        "mov.b64 {%0, %1}, d;\n\t"
+        "}\n"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n\t"
+        ".reg .b64 a, b, d;\n\t"
+        "mov.b64 a, {%2, %3};\n\t"
+        "mov.b64 b, {%4, %5};\n\t"
+        "add.rn.f32x2 d, a, b;\n\t"
+        "mov.b64 {%0, %1}, d;\n\t"
+        "}\n"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
