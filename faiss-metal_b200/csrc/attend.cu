@@ -16,7 +16,8 @@ namespace {
 // over the same keys, each key tile fetched once for both.  SPLIT (no more than 128 rows): one row tile, the streams have
 // different keys.  While one stream exponentiates, the tensor cores work for the other.
 // Weights are exp2(c (s - m)) for a reference m that is taken from a row's first tile and moves, with O rescaled, only when a tile's
-// weights add up to 2^15 or more: no maximum is looked for before the exponentials.  Sums stay in fp32.
+// weights add up to 2^15 or more: no maximum is looked for before the exponentials.  Sums stay in fp32.  The weights of the first 64
+// keys go to the tensor cores while those of the others are computed.
 constexpr int TILE_THREADS = 384;          // TMA, an issuer of MMAs a stream, a spare warp; 2 x 4 softmax warps
 constexpr int TILE_REGS_FEW = 80, TILE_REGS_MANY = 208;   // 128 and 256 threads of the 384 x 168 at launch
 static_assert(128 * TILE_REGS_FEW + 256 * TILE_REGS_MANY <= 384 * 168, "registers of a CTA");
@@ -32,7 +33,7 @@ constexpr int TILE_STAGES = DP == 128 ? 5 : 10;
 template <int DP>
 constexpr int TILE_SM_BAR = 2 * TILE_Q_BYTES<DP> + TILE_STAGES<DP>*TILE_STAGE_BYTES<DP>;
 template <int DP>
-constexpr int TILE_SMEM = TILE_SM_BAR<DP> + (2 * TILE_MAX_STAGES + 6) * 8 + 16;
+constexpr int TILE_SMEM = TILE_SM_BAR<DP> + (2 * TILE_MAX_STAGES + 10) * 8 + 16;
 static_assert(TILE_SMEM<128> <= 232448 && TILE_SMEM<64> <= 232448, "shared memory of a CTA");
 constexpr uint32_t TM_S = 0, TM_O = 256;   // stream t: S at 128 t, O at 256 + 128 t
 
@@ -88,7 +89,7 @@ attend_tile_kernel(const __grid_constant__ CUtensorMap map_sk, const __grid_cons
     const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0);
     const int lane = threadIdx.x & 31;
     const uint32_t bar_full = sbase + TILE_SM_BAR<DP>, bar_empty = bar_full + TILE_MAX_STAGES * 8;
-    const uint32_t bar_s = bar_empty + TILE_MAX_STAGES * 8, bar_p = bar_s + 16, bar_done = bar_p + 16;   // [stream]
+    const uint32_t bar_s = bar_empty + TILE_MAX_STAGES * 8, bar_p = bar_s + 16, bar_half = bar_p + 32, bar_done = bar_half + 16;   // [stream]; P: [stream][half]
     volatile uint32_t* tmem_ptr = reinterpret_cast<volatile uint32_t*>(smem + TILE_SMEM<DP> - 16);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_ptr + 1);
 
@@ -135,9 +136,10 @@ attend_tile_kernel(const __grid_constant__ CUtensorMap map_sk, const __grid_cons
         }
         for (int i = 0; i < 2; i++) {
             mbar_init(bar_s + i * 8, 1);
-            mbar_init(bar_p + i * 8, 4);
+            mbar_init(bar_half + i * 8, 1);
             mbar_init(bar_done + i * 8, 1);
         }
+        for (int i = 0; i < 4; i++) mbar_init(bar_p + i * 8, 4);
         mbar_fence_init();
     }
     if (warp == 1) {
@@ -212,63 +214,79 @@ attend_tile_kernel(const __grid_constant__ CUtensorMap map_sk, const __grid_cons
         __syncwarp();
     } else if (warp == 1) {
         // ------------------------------ MMA issuer ------------------------------
+        // Lean, and in control flow that the compiler knows to be uniform (every wait is voted on): what this warp does between a barrier and
+        // the product behind it is time the tensor cores stand still.
         const bool leader = elect_one();
         bool ok = true;
         const int tail = (int)(seq_len & (TILE_KEYS - 1));
         const int boundary = seq_len < sg.n && tail ? (int)(seq_len / TILE_KEYS) : -1;
-        const uint64_t dq = make_smem_desc(sbase), dk = make_smem_desc(ring), dv = make_smem_desc_mn(ring, TILE_KEYS * 128);
-        constexpr uint64_t QCHUNK = ATT_CHUNK >> 4, KCHUNK = (TILE_KEYS * 128) >> 4;
-        const int last = n1 > 0 && !sg.split ? 1 : 0;   // PAIR: the stream that uses a stage last
-        int slot[2] = {0, sg.split ? HALF_RING : 0};
-        uint32_t phase[2] = {0, 0};
-        auto next = [&](int t) __attribute__((always_inline)) {
-            if (++slot[t] == (sg.split && t == 0 ? HALF_RING : STAGES)) {
-                slot[t] = sg.split && t == 1 ? HALF_RING : 0;
-                phase[t] ^= 1;
+        auto issue = [&](auto split_c) __attribute__((always_inline)) {
+            constexpr bool SPLIT = decltype(split_c)::value;
+            const uint64_t dq = make_smem_desc(sbase), dk = make_smem_desc(ring), dv = make_smem_desc_mn(ring, TILE_KEYS * 128);
+            constexpr uint64_t QCHUNK = ATT_CHUNK >> 4, KCHUNK = (TILE_KEYS * 128) >> 4;
+            const bool gives[2] = {SPLIT || n1 == 0, true};   // PAIR: the stream that uses a stage last gives it back
+            int slot[2] = {0, SPLIT ? HALF_RING : 0};
+            uint32_t phase[2] = {0, 0};
+            auto waits = [&](uint32_t bar, uint32_t parity) __attribute__((always_inline)) {
+                return (bool)__all_sync(0xffffffffu, wait(bar, parity));
+            };
+            auto next = [&](int t) __attribute__((always_inline)) {
+                if (++slot[t] == (SPLIT && t == 0 ? HALF_RING : STAGES)) {
+                    slot[t] = SPLIT && t == 1 ? HALF_RING : 0;
+                    phase[t] ^= 1;
+                }
+            };
+            auto scores = [&](int t) __attribute__((always_inline)) {   // from the next stage
+                if (t == 0 || SPLIT) {
+                    if (!waits(bar_full + slot[t] * 8, phase[t])) return false;
+                }
+                tc_fence_after();
+                const uint64_t da = dq + (SPLIT ? 0 : t * (uint64_t)(QBYTES >> 4)), db = dk + (uint64_t)(slot[t] * (STAGE >> 4));
+#pragma unroll
+                for (int c = 0; c < CHUNKS; c++)
+#pragma unroll
+                    for (int k = 0; k < 4; k++)
+                        tc_mma_f16_by<false>(leader, tmem + TM_S + 128 * t, da + c * QCHUNK + 2 * k, db + c * KCHUNK + 2 * k,
+                                             att_idesc<T>(TILE_KEYS, false), c + k > 0);
+                tc_commit_by<false>(leader, bar_s + t * 8);
+                if (gives[t]) tc_commit_by<false>(leader, bar_empty + slot[t] * 8);
+                next(t);
+                return true;
+            };
+            auto values = [&](int t, int j) __attribute__((always_inline)) {
+                if (t == 0 || SPLIT) {
+                    if (!waits(bar_full + slot[t] * 8, phase[t])) return false;
+                    // rows behind the sequence's end, within the tensor: whatever they hold, 0 * it must be 0
+                    if ((t ? first1 : first0) + j == boundary)
+                        zero_tile_rows(smem + 2 * QBYTES + slot[t] * STAGE, CHUNKS, tail, TILE_KEYS);
+                }
+                const uint64_t db = dv + (uint64_t)(slot[t] * (STAGE >> 4));
+#pragma unroll
+                for (int h = 0; h < 2; h++) {   // the weights come in halves, of 64 keys
+                    if (!waits(bar_p + (2 * t + h) * 8, j & 1)) return false;
+                    tc_fence_after();
+#pragma unroll
+                    for (int k = 4 * h; k < 4 * h + 4; k++)
+                        tc_mma_ts_by(leader, tmem + TM_O + 128 * t, tmem + TM_S + 128 * t + 8 * k, db + 128 * k, att_idesc<T>(DP, true),
+                                     k > 0 ? 1u : (uint32_t)(j > 0));
+                    if (h == 0) tc_commit_by<false>(leader, bar_half + t * 8);
+                }
+                if (j + 1 == (t ? n1 : n0)) tc_commit_by<false>(leader, bar_done + t * 8);
+                if (gives[t]) tc_commit_by<false>(leader, bar_empty + slot[t] * 8);
+                next(t);
+                return true;
+            };
+            if (n0 > 0 && !scores(0)) return false;
+            if (n1 > 0 && !scores(1)) return false;
+            for (int j = 0; j < n0; j++) {
+                if (!values(0, j)) return false;
+                if (j + 1 < n0 && !scores(0)) return false;
+                if (j < n1 && !values(1, j)) return false;
+                if (j + 1 < n1 && !scores(1)) return false;
             }
+            return true;
         };
-        auto scores = [&](int t) __attribute__((always_inline)) {   // from the next stage
-            if (t == 0 || sg.split) ok = ok && wait(bar_full + slot[t] * 8, phase[t]);
-            tc_fence_after();
-            const uint64_t da = dq + (sg.split ? 0 : t * (uint64_t)(QBYTES >> 4)), db = dk + (uint64_t)(slot[t] * (STAGE >> 4));
-#pragma unroll
-            for (int c = 0; c < CHUNKS; c++)
-#pragma unroll
-                for (int k = 0; k < 4; k++)
-                    tc_mma_f16_by<false>(leader, tmem + TM_S + 128 * t, da + c * QCHUNK + 2 * k, db + c * KCHUNK + 2 * k,
-                                         att_idesc<T>(TILE_KEYS, false), c + k > 0);
-            tc_commit_by<false>(leader, bar_s + t * 8);
-            if (t == last || sg.split) tc_commit_by<false>(leader, bar_empty + slot[t] * 8);
-            next(t);
-        };
-        auto values = [&](int t, int j) __attribute__((always_inline)) {
-            if (t == 0 || sg.split) {
-                ok = ok && wait(bar_full + slot[t] * 8, phase[t]);
-                // rows behind the sequence's end, within the tensor: whatever they hold, 0 * it must be 0
-                if ((t ? first1 : first0) + j == boundary && __all_sync(0xffffffffu, ok))
-                    zero_tile_rows(smem + 2 * QBYTES + slot[t] * STAGE, CHUNKS, tail, TILE_KEYS);
-            }
-            ok = ok && wait(bar_p + t * 8, j & 1);
-            ok = __all_sync(0xffffffffu, ok);
-            if (!ok) return;
-            tc_fence_after();
-            const uint64_t db = dv + (uint64_t)(slot[t] * (STAGE >> 4));
-#pragma unroll
-            for (int k = 0; k < TILE_KEYS / 16; k++)
-                tc_mma_ts_by(leader, tmem + TM_O + 128 * t, tmem + TM_S + 128 * t + 8 * k, db + 128 * k, att_idesc<T>(DP, true),
-                             k > 0 ? 1u : (uint32_t)(j > 0));
-            if (j + 1 == (t ? n1 : n0)) tc_commit_by<false>(leader, bar_done + t * 8);
-            if (t == last || sg.split) tc_commit_by<false>(leader, bar_empty + slot[t] * 8);
-            next(t);
-        };
-        if (n0 > 0) scores(0);
-        if (n1 > 0) scores(1);
-        for (int j = 0; j < n0 && ok; j++) {
-            values(0, j);
-            if (ok && j + 1 < n0) scores(0);
-            if (ok && j < n1) values(1, j);
-            if (ok && j + 1 < n1) scores(1);
-        }
+        ok = sg.split ? issue(std::true_type()) : issue(std::false_type());
         if (!ok) {   // let the MMAs in flight retire before tensor memory goes away
             const long long t0 = clock64();
             while (clock64() - t0 < 200000LL) {
@@ -314,56 +332,65 @@ attend_tile_kernel(const __grid_constant__ CUtensorMap map_sk, const __grid_cons
         for (int j = 0; j < nt; j++) {
             ok = __all_sync(0xffffffffu, wait(bar_s + t * 8, j & 1));
             if (!ok) break;
-            if (warp_live) {
-                tc_fence_after();
-                const int lim = end - (kt0 + j) * TILE_KEYS;
-                const bool masked = __any_sync(0xffffffffu, lim < TILE_KEYS);
-                float sum = 0.f;
-                tc_ld32(ts, s[0]);
+            tc_fence_after();
+            const int lim = end - (kt0 + j) * TILE_KEYS;
+            const bool masked = __any_sync(0xffffffffu, lim < TILE_KEYS);
+            if (warp_live) tc_ld32(ts, s[0]);
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    tc_wait_ld32(s[i]);
-                    if (i < 3) tc_ld32(ts + 32 * (i + 1), s[i + 1]);   // under the exponentials of this chunk
-                    if (masked) {
+            for (int h = 0; h < 2; h++) {
+                if (warp_live) {
+                    float sum = 0.f;
 #pragma unroll
-                        for (int e = 0; e < 32; e++)
-                            if (32 * i + e >= lim) s[i][e] = 0xff800000u;   // -INF
-                    }
-                    sum += weigh(s[i], mc, i);
-                }
-                if (__any_sync(0xffffffffu, !(sum < WEIGHTS_MAX))) {
-                    // a new reference, from this tile's maximum; the tile once more
-                    const bool grown = !(sum < WEIGHTS_MAX);
-                    float top = -CUDART_INF_F;
+                    for (int i = 2 * h; i < 2 * h + 2; i++) {
+                        tc_wait_ld32(s[i]);
+                        if (i < 3) tc_ld32(ts + 32 * (i + 1), s[i + 1]);   // under the exponentials of this chunk
+                        if (masked) {
 #pragma unroll
-                    for (int i = 0; i < 4; i++)
-#pragma unroll
-                        for (int e = 0; e < 32; e += 2) top = max3(top, __uint_as_float(s[i][e]), __uint_as_float(s[i][e + 1]));
-                    const float now = grown ? fmaxf(top, m) : m;
-                    const float f = now == m ? 1.f : ex2((m - now) * c);   // 0 where nothing was seen before
-                    m = now;
-                    l *= f;
-                    mc = m == -CUDART_INF_F ? CUDART_NAN_F : -m * c;
-                    if (j > 0) {   // the scores are there, so the previous tile's product is done
-#pragma unroll 1
-                        for (int i = 0; i < DP / 16; i++) {
-                            uint32_t o[16];
-                            tc_ld16_wait(to + 16 * i, o);
-#pragma unroll
-                            for (int e = 0; e < 16; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-                            tc_st16(to + 16 * i, o);
+                            for (int e = 0; e < 32; e++)
+                                if (32 * i + e >= lim) s[i][e] = 0xff800000u;   // -INF
                         }
+                        sum += weigh(s[i], mc, i);
                     }
-                    sum = 0.f;
+                    if (__any_sync(0xffffffffu, !(sum < WEIGHTS_MAX))) {
+                        // a new reference, from the maximum of these 64 keys, which are then weighed once more
+                        const bool grown = !(sum < WEIGHTS_MAX);
+                        float top = -CUDART_INF_F;
 #pragma unroll
-                    for (int i = 0; i < 4; i++) sum += weigh(s[i], m == -CUDART_INF_F ? 0.f : mc, i);
+                        for (int i = 2 * h; i < 2 * h + 2; i++)
+#pragma unroll
+                            for (int e = 0; e < 32; e += 2) top = max3(top, __uint_as_float(s[i][e]), __uint_as_float(s[i][e + 1]));
+                        const float now = grown ? fmaxf(top, m) : m;
+                        const float f = now == m ? 1.f : ex2((m - now) * c);   // 0 where nothing was seen before
+                        m = now;
+                        l *= f;
+                        mc = m == -CUDART_INF_F ? CUDART_NAN_F : -m * c;
+                        // O holds what came before: the previous tile's product is done, since the scores are there; the first half's
+                        // may be under way
+                        if (h == 1) {
+                            ok = __all_sync(0xffffffffu, wait(bar_half + t * 8, j & 1));
+                            tc_fence_after();
+                        }
+                        if (h == 1 || j > 0) {
+#pragma unroll 1
+                            for (int i = 0; i < DP / 16; i++) {
+                                uint32_t o[16];
+                                tc_ld16_wait(to + 16 * i, o);
+#pragma unroll
+                                for (int e = 0; e < 16; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                                tc_st16(to + 16 * i, o);
+                            }
+                        }
+                        sum = 0.f;
+#pragma unroll
+                        for (int i = 2 * h; i < 2 * h + 2; i++) sum += weigh(s[i], m == -CUDART_INF_F ? 0.f : mc, i);
+                    }
+                    l += sum;
+                    tc_wait_st();
+                    tc_fence_before();
                 }
-                l += sum;
-                tc_wait_st();
-                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar_p + (2 * t + h) * 8);
             }
-            __syncwarp();
-            if (lane == 0) mbar_arrive(bar_p + t * 8);
         }
         // ------------------------------ this row's output ------------------------------
         if (ok && nt > 0) ok = wait(bar_done + t * 8, 0);
