@@ -16,11 +16,12 @@ namespace {
 // over the same keys, each key tile fetched once for both.  SPLIT (no more than 128 rows): one row tile, the streams have
 // different keys.  While one stream exponentiates, the tensor cores work for the other.
 // Weights are exp2(c (s - m)) for a reference m that is taken from a row's first tile and moves, with O rescaled, only when a tile's
-// weights add up to 2^15 or more: no maximum is looked for before the exponentials.  Sums stay in fp32.  The weights of the first 64
+// weights add up to 2^15 or more: no maximum is looked for before the exponentials.  Sums stay in fp32.  The weights of the first 96
 // keys go to the tensor cores while those of the others are computed.
 constexpr int TILE_THREADS = 384;          // TMA, an issuer of MMAs a stream, a spare warp; 2 x 4 softmax warps
 constexpr int TILE_REGS_FEW = 80, TILE_REGS_MANY = 208;   // 128 and 256 threads of the 384 x 168 at launch
 static_assert(128 * TILE_REGS_FEW + 256 * TILE_REGS_MANY <= 384 * 168, "registers of a CTA");
+constexpr int PART_KEYS = 96;             // keys whose weights are handed on first
 constexpr float WEIGHTS_MAX = 32768.f;     // fp16 weights end at 65504
 constexpr int TILE_KEYS = 128;
 constexpr int TILE_MAX_STAGES = 10;
@@ -89,7 +90,7 @@ attend_tile_kernel(const __grid_constant__ CUtensorMap map_sk, const __grid_cons
     const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0);
     const int lane = threadIdx.x & 31;
     const uint32_t bar_full = sbase + TILE_SM_BAR<DP>, bar_empty = bar_full + TILE_MAX_STAGES * 8;
-    const uint32_t bar_s = bar_empty + TILE_MAX_STAGES * 8, bar_p = bar_s + 16, bar_half = bar_p + 32, bar_done = bar_half + 16;   // [stream]; P: [stream][half]
+    const uint32_t bar_s = bar_empty + TILE_MAX_STAGES * 8, bar_p = bar_s + 16, bar_part = bar_p + 32, bar_done = bar_part + 16;   // [stream]; P: [stream][part]
     volatile uint32_t* tmem_ptr = reinterpret_cast<volatile uint32_t*>(smem + TILE_SMEM<DP> - 16);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_ptr + 1);
 
@@ -136,7 +137,7 @@ attend_tile_kernel(const __grid_constant__ CUtensorMap map_sk, const __grid_cons
         }
         for (int i = 0; i < 2; i++) {
             mbar_init(bar_s + i * 8, 1);
-            mbar_init(bar_half + i * 8, 1);
+            mbar_init(bar_part + i * 8, 1);
             mbar_init(bar_done + i * 8, 1);
         }
         for (int i = 0; i < 4; i++) mbar_init(bar_p + i * 8, 4);
@@ -236,11 +237,10 @@ attend_tile_kernel(const __grid_constant__ CUtensorMap map_sk, const __grid_cons
                     phase[t] ^= 1;
                 }
             };
-            auto scores = [&](int t) __attribute__((always_inline)) {   // from the next stage
-                if (t == 0 || SPLIT) {
-                    if (!waits(bar_full + slot[t] * 8, phase[t])) return false;
-                }
-                tc_fence_after();
+            auto keys_there = [&](int t) __attribute__((always_inline)) {
+                return !(t == 0 || SPLIT) || waits(bar_full + slot[t] * 8, phase[t]);
+            };
+            auto scores = [&](int t) __attribute__((always_inline)) {   // from the next stage, which is there
                 const uint64_t da = dq + (SPLIT ? 0 : t * (uint64_t)(QBYTES >> 4)), db = dk + (uint64_t)(slot[t] * (STAGE >> 4));
 #pragma unroll
                 for (int c = 0; c < CHUNKS; c++)
@@ -251,38 +251,48 @@ attend_tile_kernel(const __grid_constant__ CUtensorMap map_sk, const __grid_cons
                 tc_commit_by<false>(leader, bar_s + t * 8);
                 if (gives[t]) tc_commit_by<false>(leader, bar_empty + slot[t] * 8);
                 next(t);
-                return true;
             };
-            auto values = [&](int t, int j) __attribute__((always_inline)) {
+            // P V of tile j and, more, the scores of the next
+            auto turn = [&](int t, int j, bool more) __attribute__((always_inline)) {
                 if (t == 0 || SPLIT) {
                     if (!waits(bar_full + slot[t] * 8, phase[t])) return false;
                     // rows behind the sequence's end, within the tensor: whatever they hold, 0 * it must be 0
                     if ((t ? first1 : first0) + j == boundary)
                         zero_tile_rows(smem + 2 * QBYTES + slot[t] * STAGE, CHUNKS, tail, TILE_KEYS);
                 }
-                const uint64_t db = dv + (uint64_t)(slot[t] * (STAGE >> 4));
+                const int s = slot[t];
+                const uint64_t db = dv + (uint64_t)(s * (STAGE >> 4));
+                auto product = [&](int k) __attribute__((always_inline)) {   // 16 keys
+                    tc_mma_ts_by(leader, tmem + TM_O + 128 * t, tmem + TM_S + 128 * t + 8 * k, db + 128 * k, att_idesc<T>(DP, true),
+                                 k > 0 ? 1u : (uint32_t)(j > 0));
+                };
+                if (!waits(bar_p + 2 * t * 8, j & 1)) return false;
+                tc_fence_after();
 #pragma unroll
-                for (int h = 0; h < 2; h++) {   // the weights come in halves, of 64 keys
-                    if (!waits(bar_p + (2 * t + h) * 8, j & 1)) return false;
-                    tc_fence_after();
-#pragma unroll
-                    for (int k = 4 * h; k < 4 * h + 4; k++)
-                        tc_mma_ts_by(leader, tmem + TM_O + 128 * t, tmem + TM_S + 128 * t + 8 * k, db + 128 * k, att_idesc<T>(DP, true),
-                                     k > 0 ? 1u : (uint32_t)(j > 0));
-                    if (h == 0) tc_commit_by<false>(leader, bar_half + t * 8);
-                }
-                if (j + 1 == (t ? n1 : n0)) tc_commit_by<false>(leader, bar_done + t * 8);
-                if (gives[t]) tc_commit_by<false>(leader, bar_empty + slot[t] * 8);
+                for (int k = 0; k < PART_KEYS / 16; k++) product(k);
+                tc_commit_by<false>(leader, bar_part + t * 8);
                 next(t);
+                if (more && !keys_there(t)) return false;
+                if (!waits(bar_p + (2 * t + 1) * 8, j & 1)) return false;
+                tc_fence_after();
+#pragma unroll
+                for (int k = PART_KEYS / 16; k < TILE_KEYS / 16; k++) product(k);
+                if (more) scores(t);
+                else tc_commit_by<false>(leader, bar_done + t * 8);
+                if (gives[t]) tc_commit_by<false>(leader, bar_empty + s * 8);
                 return true;
             };
-            if (n0 > 0 && !scores(0)) return false;
-            if (n1 > 0 && !scores(1)) return false;
+            if (n0 > 0) {
+                if (!keys_there(0)) return false;
+                scores(0);
+            }
+            if (n1 > 0) {
+                if (!keys_there(1)) return false;
+                scores(1);
+            }
             for (int j = 0; j < n0; j++) {
-                if (!values(0, j)) return false;
-                if (j + 1 < n0 && !scores(0)) return false;
-                if (j < n1 && !values(1, j)) return false;
-                if (j + 1 < n1 && !scores(1)) return false;
+                if (!turn(0, j, j + 1 < n0)) return false;
+                if (j < n1 && !turn(1, j, j + 1 < n1)) return false;
             }
             return true;
         };
@@ -314,19 +324,9 @@ attend_tile_kernel(const __grid_constant__ CUtensorMap map_sk, const __grid_cons
         uint32_t s[4][32];
         // weights of 32 keys to tensor memory; returns their sum
         auto weigh = [&](uint32_t (&x)[32], float mc_now, int i) __attribute__((always_inline)) {
-            const float2 c2 = make_float2(c, c), mc2 = make_float2(mc_now, mc_now);
-            float2 sum[2];
             uint32_t w[16];
-#pragma unroll
-            for (int e = 0; e < 16; e++) {
-                float2 y = fma2(make_float2(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1])), c2, mc2);
-                y.x = ex2(y.x);
-                y.y = ex2(y.y);
-                sum[e & 1] = e < 2 ? y : add2(sum[e & 1], y);
-                w[e] = pack2<T>(y.x, y.y);
-            }
+            const float2 z = weigh32<T>(x, c, mc_now, w);
             tc_st16(ts + 16 * i, w);
-            const float2 z = add2(sum[0], sum[1]);
             return z.x + z.y;
         };
         for (int j = 0; j < nt; j++) {
@@ -335,61 +335,60 @@ attend_tile_kernel(const __grid_constant__ CUtensorMap map_sk, const __grid_cons
             tc_fence_after();
             const int lim = end - (kt0 + j) * TILE_KEYS;
             const bool masked = __any_sync(0xffffffffu, lim < TILE_KEYS);
-            if (warp_live) tc_ld32(ts, s[0]);
+            tc_ld32(ts, s[0]);
 #pragma unroll
             for (int h = 0; h < 2; h++) {
-                if (warp_live) {
-                    float sum = 0.f;
+                constexpr int PART = PART_KEYS / 32;
+                float sum = 0.f;
 #pragma unroll
-                    for (int i = 2 * h; i < 2 * h + 2; i++) {
-                        tc_wait_ld32(s[i]);
-                        if (i < 3) tc_ld32(ts + 32 * (i + 1), s[i + 1]);   // under the exponentials of this chunk
-                        if (masked) {
+                for (int i = h ? PART : 0; i < (h ? 4 : PART); i++) {
+                    tc_wait_ld32(s[i]);
+                    if (i < 3) tc_ld32(ts + 32 * (i + 1), s[i + 1]);   // under the exponentials of this chunk
+                    if (masked) {
 #pragma unroll
-                            for (int e = 0; e < 32; e++)
-                                if (32 * i + e >= lim) s[i][e] = 0xff800000u;   // -INF
-                        }
-                        sum += weigh(s[i], mc, i);
+                        for (int e = 0; e < 32; e++)
+                            if (32 * i + e >= lim) s[i][e] = 0xff800000u;   // -INF
                     }
-                    if (__any_sync(0xffffffffu, !(sum < WEIGHTS_MAX))) {
-                        // a new reference, from the maximum of these 64 keys, which are then weighed once more
-                        const bool grown = !(sum < WEIGHTS_MAX);
-                        float top = -CUDART_INF_F;
-#pragma unroll
-                        for (int i = 2 * h; i < 2 * h + 2; i++)
-#pragma unroll
-                            for (int e = 0; e < 32; e += 2) top = max3(top, __uint_as_float(s[i][e]), __uint_as_float(s[i][e + 1]));
-                        const float now = grown ? fmaxf(top, m) : m;
-                        const float f = now == m ? 1.f : ex2((m - now) * c);   // 0 where nothing was seen before
-                        m = now;
-                        l *= f;
-                        mc = m == -CUDART_INF_F ? CUDART_NAN_F : -m * c;
-                        // O holds what came before: the previous tile's product is done, since the scores are there; the first half's
-                        // may be under way
-                        if (h == 1) {
-                            ok = __all_sync(0xffffffffu, wait(bar_half + t * 8, j & 1));
-                            tc_fence_after();
-                        }
-                        if (h == 1 || j > 0) {
-#pragma unroll 1
-                            for (int i = 0; i < DP / 16; i++) {
-                                uint32_t o[16];
-                                tc_ld16_wait(to + 16 * i, o);
-#pragma unroll
-                                for (int e = 0; e < 16; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-                                tc_st16(to + 16 * i, o);
-                            }
-                        }
-                        sum = 0.f;
-#pragma unroll
-                        for (int i = 2 * h; i < 2 * h + 2; i++) sum += weigh(s[i], m == -CUDART_INF_F ? 0.f : mc, i);
-                    }
-                    l += sum;
-                    tc_wait_st();
-                    tc_fence_before();
+                    sum += weigh(s[i], mc, i);
                 }
+                if (__any_sync(0xffffffffu, !(sum < WEIGHTS_MAX))) {
+                    // a new reference, from the maximum of these keys, which are then weighed once more
+                    const bool grown = !(sum < WEIGHTS_MAX);
+                    float top = -CUDART_INF_F;
+#pragma unroll
+                    for (int i = h ? PART : 0; i < (h ? 4 : PART); i++)
+#pragma unroll
+                        for (int e = 0; e < 32; e += 2) top = max3(top, __uint_as_float(s[i][e]), __uint_as_float(s[i][e + 1]));
+                    const float now = grown ? fmaxf(top, m) : m;
+                    const float f = now == m ? 1.f : ex2((m - now) * c);   // 0 where nothing was seen before
+                    m = now;
+                    l *= f;
+                    mc = m == -CUDART_INF_F ? CUDART_NAN_F : -m * c;
+                    // O holds what came before: the previous tile's product is done, since the scores are there; the first part's
+                    // may be under way
+                    if (h == 1) {
+                        ok = __all_sync(0xffffffffu, wait(bar_part + t * 8, j & 1));
+                        tc_fence_after();
+                    }
+                    if (h == 1 || j > 0) {
+#pragma unroll 1
+                        for (int i = 0; i < DP / 16; i++) {
+                            uint32_t o[16];
+                            tc_ld16_wait(to + 16 * i, o);
+#pragma unroll
+                            for (int e = 0; e < 16; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                            tc_st16(to + 16 * i, o);
+                        }
+                    }
+                    sum = 0.f;
+#pragma unroll
+                    for (int i = h ? PART : 0; i < (h ? 4 : PART); i++) sum += weigh(s[i], m == -CUDART_INF_F ? 0.f : mc, i);
+                }
+                l += sum;
+                tc_wait_st();
+                tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(bar_p + (2 * t + h) * 8);
+                mbar_arrive_if(lane == 0, bar_p + (2 * t + h) * 8);
             }
         }
         // ------------------------------ this row's output ------------------------------

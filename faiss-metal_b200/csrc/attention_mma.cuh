@@ -28,6 +28,17 @@ __device__ __forceinline__ void tma_load_5d(uint32_t dst, const CUtensorMap* map
 // Shared-memory writes of this thread become visible to TMA and tcgen05.
 __device__ __forceinline__ void fence_proxy_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
+__device__ __forceinline__ void mbar_arrive_if(bool on, uint32_t bar) {
+    asm volatile(
+            "{\n\t"
+            ".reg .pred p;\n\t"
+            "setp.ne.b32 p, %1, 0;\n\t"
+            "@p mbarrier.arrive.shared::cta.b64 _, [%0];\n\t"
+            "}\n" ::"r"(bar),
+            "r"((uint32_t)on)
+            : "memory");
+}
+
 // The A operand in tensor memory: 16-bit elements, two a column, row i in lane i.
 __device__ __forceinline__ void tc_mma_ts_by(bool leader, uint32_t d_tmem, uint32_t a_tmem, uint64_t desc_b, uint32_t idesc,
                                              uint32_t accumulate) {
@@ -131,6 +142,33 @@ template <>
 __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
     const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// w = exp2(x c + mc) of 32 values, packed; returns their sums.  In groups of eight, and each step for the whole group before the next:
+// the compiler keeps this order, and an exponential's result takes some 40 cycles (a warp alone on its scheduler: 1,090
+// cycles for 64 values step by step, 600 this way; the exponential unit takes 512).
+template <typename T>
+__device__ __forceinline__ float2 weigh32(const uint32_t (&x)[32], float c, float mc, uint32_t* w) {
+    const float2 c2 = make_float2(c, c), mc2 = make_float2(mc, mc);
+    float2 add[4];
+#pragma unroll
+    for (int g = 0; g < 16; g += 4) {
+        float2 y[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            y[e] = fma2(make_float2(__uint_as_float(x[2 * (g + e)]), __uint_as_float(x[2 * (g + e) + 1])), c2, mc2);
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            y[e].x = ex2(y[e].x);
+            y[e].y = ex2(y[e].y);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            add[e] = g == 0 ? y[e] : add2(add[e], y[e]);
+            w[g + e] = pack2<T>(y[e].x, y[e].y);
+        }
+    }
+    return add2(add2(add[0], add[1]), add2(add[2], add[3]));
 }
 
 // Descriptor of an operand tile whose rows (128 bytes, swizzled) run along K: 64 elements of M or N a row, 8-row
