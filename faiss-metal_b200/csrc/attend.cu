@@ -71,11 +71,12 @@ struct RowAt {
 };
 // packed row r of a unit
 __device__ __forceinline__ RowAt row_at(const TileParams& p, int shared, int64_t unit, int64_t r) {
-    const int64_t tt = r / p.group;
+    // below 2^31: batch * queries * heads
+    const uint32_t tt = (uint32_t)r / (uint32_t)p.group, ub = (uint32_t)unit / (uint32_t)p.kv_heads;
     RowAt a;
-    a.h = (int)(unit % p.kv_heads) * p.group + (int)(r - tt * p.group);
-    a.b = shared ? tt / p.queries : unit / p.kv_heads;
-    a.t = shared ? tt % p.queries : tt;
+    a.h = (int)(((uint32_t)unit - ub * p.kv_heads) * p.group + ((uint32_t)r - tt * p.group));
+    a.b = shared ? tt / (uint32_t)p.queries : ub;
+    a.t = shared ? tt % (uint32_t)p.queries : tt;
     return a;
 }
 
@@ -158,17 +159,16 @@ attend_tile_kernel(const __grid_constant__ CUtensorMap map_sk, const __grid_cons
 
     if (warp != 0) {
         // query rows to shared memory, swizzled as TMA would: 16-byte piece c of row r goes to piece c ^ (r & 7)
-        // DP / 8 threads a row
+        // DP / 8 threads a row; asynchronous, so that the rows are all on their way at once
         constexpr int PER_ROW = DP / 8, AT_ONCE = (TILE_THREADS - 32) / PER_ROW;
         const int nrows = sg.split ? 128 : 256, c = (threadIdx.x - 32) % PER_ROW;
         for (int r = (threadIdx.x - 32) / PER_ROW; r < nrows; r += AT_ONCE) {
-            uint4 x = make_uint4(0, 0, 0, 0);
-            if (row0 + r < sg.rows && c * 8 < p.d) {
-                const RowAt a = row_at(p, shared, unit, row0 + r);
-                x = *reinterpret_cast<const uint4*>(p.q.at(a.b, a.t, a.h) + c * 8);
-            }
-            *reinterpret_cast<uint4*>(smem + (r >> 7) * QBYTES + (c >> 3) * ATT_CHUNK + (r & 127) * 128 + (((c & 7) ^ (r & 7)) << 4)) = x;
+            const bool there = row0 + r < sg.rows && c * 8 < p.d;
+            const RowAt a = there ? row_at(p, shared, unit, row0 + r) : RowAt{0, 0, 0};
+            cp_async16(sbase + (r >> 7) * QBYTES + (c >> 3) * ATT_CHUNK + (r & 127) * 128 + (((c & 7) ^ (r & 7)) << 4),
+                       p.q.at(a.b, a.t, a.h) + (there ? c * 8 : 0), there);
         }
+        asm volatile("cp.async.wait_all;" ::: "memory");
         fence_proxy_async_shared();
         asm volatile("bar.sync 1, %0;" ::"n"(TILE_THREADS - 32) : "memory");
     }
@@ -323,9 +323,9 @@ attend_tile_kernel(const __grid_constant__ CUtensorMap map_sk, const __grid_cons
         bool ok = true;
         uint32_t s[4][32];
         // weights of 32 keys to tensor memory; returns their sum
-        auto weigh = [&](uint32_t (&x)[32], float mc_now, int i) __attribute__((always_inline)) {
+        auto weigh = [&](auto mix, uint32_t (&x)[32], float mc_now, int i) __attribute__((always_inline)) {
             uint32_t w[16];
-            const float2 z = weigh32<T>(x, c, mc_now, w);
+            const float2 z = weigh32<T, decltype(mix)::value>(x, c, mc_now, w);
             tc_st16(ts + 16 * i, w);
             return z.x + z.y;
         };
@@ -344,33 +344,35 @@ attend_tile_kernel(const __grid_constant__ CUtensorMap map_sk, const __grid_cons
                 for (int i = h ? PART : 0; i < (h ? 4 : PART); i++) {
                     tc_wait_ld32(s[i]);
                     if (i < 3) tc_ld32(ts + 32 * (i + 1), s[i + 1]);   // under the exponentials of this chunk
-                    if (masked) {
+                    if (!masked) {
+                        sum += weigh(std::true_type(), s[i], mc, i);
+                    } else {
 #pragma unroll
                         for (int e = 0; e < 32; e++)
                             if (32 * i + e >= lim) s[i][e] = 0xff800000u;   // -INF
                     }
-                    sum += weigh(s[i], mc, i);
                 }
-                if (__any_sync(0xffffffffu, !(sum < WEIGHTS_MAX))) {
-                    // a new reference, from the maximum of these keys, which are then weighed once more
-                    const bool grown = !(sum < WEIGHTS_MAX);
+                if (masked || __any_sync(0xffffffffu, !(sum < WEIGHTS_MAX))) {
+                    // perhaps a new reference, from the maximum of these keys, which are then weighed (once more)
                     float top = -CUDART_INF_F;
 #pragma unroll
                     for (int i = h ? PART : 0; i < (h ? 4 : PART); i++)
 #pragma unroll
                         for (int e = 0; e < 32; e += 2) top = max3(top, __uint_as_float(s[i][e]), __uint_as_float(s[i][e + 1]));
+                    const bool grown = masked ? !(fmaf(top, c, mc) <= 8.f) : !(sum < WEIGHTS_MAX);
                     const float now = grown ? fmaxf(top, m) : m;
+                    const bool moved = __any_sync(0xffffffffu, now != m);
                     const float f = now == m ? 1.f : ex2((m - now) * c);   // 0 where nothing was seen before
                     m = now;
                     l *= f;
                     mc = m == -CUDART_INF_F ? CUDART_NAN_F : -m * c;
                     // O holds what came before: the previous tile's product is done, since the scores are there; the first part's
                     // may be under way
-                    if (h == 1) {
+                    if (moved && h == 1) {
                         ok = __all_sync(0xffffffffu, wait(bar_part + t * 8, j & 1));
                         tc_fence_after();
                     }
-                    if (h == 1 || j > 0) {
+                    if (moved && (h == 1 || j > 0)) {
 #pragma unroll 1
                         for (int i = 0; i < DP / 16; i++) {
                             uint32_t o[16];
@@ -382,7 +384,8 @@ attend_tile_kernel(const __grid_constant__ CUtensorMap map_sk, const __grid_cons
                     }
                     sum = 0.f;
 #pragma unroll
-                    for (int i = h ? PART : 0; i < (h ? 4 : PART); i++) sum += weigh(s[i], m == -CUDART_INF_F ? 0.f : mc, i);
+                    for (int i = h ? PART : 0; i < (h ? 4 : PART); i++) 
+                        sum += weigh(std::false_type(), s[i], m == -CUDART_INF_F ? 0.f : mc, i);
                 }
                 l += sum;
                 tc_wait_st();

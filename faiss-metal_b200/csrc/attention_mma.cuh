@@ -25,6 +25,11 @@ __device__ __forceinline__ void tma_load_5d(uint32_t dst, const CUtensorMap* map
             : "memory");
 }
 
+// 16 bytes global -> shared, zeros where not `there` (src is not read then)
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool there) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+
 // Shared-memory writes of this thread become visible to TMA and tcgen05.
 __device__ __forceinline__ void fence_proxy_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
@@ -144,10 +149,29 @@ __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 
+// 2^y of two values on the FMA pipe: y = n + f with n the nearest integer (Cody and Waite's range reduction, the rounding by adding
+// 1.5 * 2^23), 2^f by a polynomial of degree 4 (fitted here to the relative error on [-1/2, 1/2], 2.7e-6 in fp32), n added to the
+// exponent.  Down to 2^-126; for y up to 126.
+__device__ __forceinline__ float2 ex2_fma(float2 y) {
+    constexpr float ROUND = 12582912.f;
+    y.x = fmaxf(y.x, -126.f);
+    y.y = fmaxf(y.y, -126.f);
+    const float2 r = add2(y, make_float2(ROUND, ROUND));
+    const float2 f = add2(y, fma2(r, make_float2(-1.f, -1.f), make_float2(ROUND, ROUND)));
+    float2 z = fma2(f, make_float2(0.009570104735915316f, 0.009570104735915316f), make_float2(0.05591786050289549f, 0.05591786050289549f));
+    z = fma2(z, f, make_float2(0.2402474475630491f, 0.2402474475630491f));
+    z = fma2(z, f, make_float2(0.6931218146697293f, 0.6931218146697293f));
+    z = fma2(z, f, make_float2(0.9999992614616359f, 0.9999992614616359f));
+    // the low bits of r are n
+    return make_float2(__uint_as_float(__float_as_uint(r.x) * 8388608u + __float_as_uint(z.x)),
+                       __uint_as_float(__float_as_uint(r.y) * 8388608u + __float_as_uint(z.y)));
+}
+
 // w = exp2(x c + mc) of 32 values, packed; returns their sums.  In groups of eight, and each step for the whole group before the next:
 // the compiler keeps this order, and an exponential's result takes some 40 cycles (a warp alone on its scheduler: 1,090
 // cycles for 64 values step by step, 600 this way; the exponential unit takes 512).
-template <typename T>
+// MIX: two of eight by ex2_fma, which takes the load off that unit; for finite values only.
+template <typename T, bool MIX>
 __device__ __forceinline__ float2 weigh32(const uint32_t (&x)[32], float c, float mc, uint32_t* w) {
     const float2 c2 = make_float2(c, c), mc2 = make_float2(mc, mc);
     float2 add[4];
@@ -158,10 +182,11 @@ __device__ __forceinline__ float2 weigh32(const uint32_t (&x)[32], float c, floa
         for (int e = 0; e < 4; e++)
             y[e] = fma2(make_float2(__uint_as_float(x[2 * (g + e)]), __uint_as_float(x[2 * (g + e) + 1])), c2, mc2);
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
+        for (int e = 0; e < (MIX ? 3 : 4); e++) {
             y[e].x = ex2(y[e].x);
             y[e].y = ex2(y[e].y);
         }
+        if (MIX) y[3] = ex2_fma(y[3]);
 #pragma unroll
         for (int e = 0; e < 4; e++) {
             add[e] = g == 0 ? y[e] : add2(add[e], y[e]);
