@@ -130,6 +130,28 @@ attend_tile_kernel(const __grid_constant__ CUtensorMap map_sk, const __grid_cons
     const int first1 = sg.split ? (int)kb : (int)ka;
     const int n1 = sg.split ? (int)(kb2 - kb) : (row0 + 128 < sg.rows ? n0 : 0);
 
+    if (warp != 0) {
+        // query rows to shared memory, swizzled as TMA would: 16-byte piece c of row r goes to piece c ^ (r & 7).  DP / 8 threads a row;
+        // asynchronous, so that all rows are on their way at once, and without a division a row
+        constexpr int PER_ROW = DP / 8, AT_ONCE = (TILE_THREADS - 32) / PER_ROW;
+        const int nrows = sg.split ? 128 : 256, c = (threadIdx.x - 32) % PER_ROW;
+        int r = (threadIdx.x - 32) / PER_ROW;
+        uint32_t tt = (uint32_t)(row0 + r) / (uint32_t)p.group, g = (uint32_t)(row0 + r) - tt * p.group;
+        const uint32_t dt = AT_ONCE / (uint32_t)p.group, dg = AT_ONCE - dt * p.group;
+        const uint16_t* const base = p.q.at(ub, 0, (int64_t)kvh * p.group) + c * 8;
+        for (; r < nrows; r += AT_ONCE) {
+            const bool there = row0 + r < sg.rows && c * 8 < p.d;
+            const uint32_t b = shared ? tt / (uint32_t)p.queries : 0, t = shared ? tt - b * (uint32_t)p.queries : tt;
+            const uint16_t* const src = there ? base + b * p.q.sb + t * p.q.sr + g * p.q.sh : p.q.p;
+            cp_async16(sbase + (r >> 7) * QBYTES + (c >> 3) * ATT_CHUNK + (r & 127) * 128 + (((c & 7) ^ (r & 7)) << 4), src, there);
+            tt += dt;
+            g += dg;
+            if (g >= (uint32_t)p.group) {
+                g -= p.group;
+                tt++;
+            }
+        }
+    }
     if (threadIdx.x == 0) {
         *abort_flag = 0;
         for (int s = 0; s < STAGES; s++) {
@@ -158,21 +180,10 @@ attend_tile_kernel(const __grid_constant__ CUtensorMap map_sk, const __grid_cons
     auto wait = [&](uint32_t bar, uint32_t parity) { return mbar_wait(bar, parity, abort_flag, p.status); };
 
     if (warp != 0) {
-        // query rows to shared memory, swizzled as TMA would: 16-byte piece c of row r goes to piece c ^ (r & 7)
-        // DP / 8 threads a row; asynchronous, so that the rows are all on their way at once
-        constexpr int PER_ROW = DP / 8, AT_ONCE = (TILE_THREADS - 32) / PER_ROW;
-        const int nrows = sg.split ? 128 : 256, c = (threadIdx.x - 32) % PER_ROW;
-        for (int r = (threadIdx.x - 32) / PER_ROW; r < nrows; r += AT_ONCE) {
-            const bool there = row0 + r < sg.rows && c * 8 < p.d;
-            const RowAt a = there ? row_at(p, shared, unit, row0 + r) : RowAt{0, 0, 0};
-            cp_async16(sbase + (r >> 7) * QBYTES + (c >> 3) * ATT_CHUNK + (r & 127) * 128 + (((c & 7) ^ (r & 7)) << 4),
-                       p.q.at(a.b, a.t, a.h) + (there ? c * 8 : 0), there);
-        }
         asm volatile("cp.async.wait_all;" ::: "memory");
         fence_proxy_async_shared();
         asm volatile("bar.sync 1, %0;" ::"n"(TILE_THREADS - 32) : "memory");
     }
-
     if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(TILE_REGS_FEW));
     if (warp == 0) {
@@ -412,27 +423,47 @@ attend_tile_kernel(const __grid_constant__ CUtensorMap map_sk, const __grid_cons
                     p.part_lse[part * p.rows_total + grow] = lse2;
                 }
             }
+            // results: through shared memory (the stream's query tile is done with), so that whole rows are written
+            uint8_t* const stage = smem + t * QBYTES + ew * 32 * (DP * 2);
 #pragma unroll 1
-            for (int i = 0; i < DP / 16; i++) {
-                uint32_t o[16];
-                if (!none) tc_ld16_wait(to + 16 * i, o);
+            for (int i = 0; i < DP / 32; i++) {
+                uint32_t o[32];
+                if (!none) {
+                    tc_ld32(to + 32 * i, o);
+                    tc_wait_ld32(o);
+                }
 #pragma unroll
-                for (int e = 0; e < 16; e++) o[e] = inv == 0.f ? 0u : __float_as_uint(__uint_as_float(o[e]) * inv);
-                if (!live) continue;
+                for (int e = 0; e < 32; e++) o[e] = inv == 0.f ? 0u : __float_as_uint(__uint_as_float(o[e]) * inv);
                 if (whole) {
 #pragma unroll
-                    for (int e = 0; e < 16; e += 8)
-                        if (16 * i + e < p.d)
-                            *reinterpret_cast<uint4*>(p.out + grow * p.d + 16 * i + e) =
-                                    make_uint4(pack2<T>(__uint_as_float(o[e]), __uint_as_float(o[e + 1])),
-                                               pack2<T>(__uint_as_float(o[e + 2]), __uint_as_float(o[e + 3])),
-                                               pack2<T>(__uint_as_float(o[e + 4]), __uint_as_float(o[e + 5])),
-                                               pack2<T>(__uint_as_float(o[e + 6]), __uint_as_float(o[e + 7])));
-                } else if (!none) {
+                    for (int e = 0; e < 4; e++)
+                        *reinterpret_cast<uint4*>(stage + lane * (DP * 2) + (((4 * i + e) ^ (lane & 7)) << 4)) =
+                                make_uint4(pack2<T>(__uint_as_float(o[8 * e]), __uint_as_float(o[8 * e + 1])),
+                                           pack2<T>(__uint_as_float(o[8 * e + 2]), __uint_as_float(o[8 * e + 3])),
+                                           pack2<T>(__uint_as_float(o[8 * e + 4]), __uint_as_float(o[8 * e + 5])),
+                                           pack2<T>(__uint_as_float(o[8 * e + 6]), __uint_as_float(o[8 * e + 7])));
+                } else if (live && !none) {
                     float* const po = p.part_o + (part * p.rows_total + grow) * p.d;
 #pragma unroll
-                    for (int e = 0; e < 16; e += 4)
-                        if (16 * i + e < p.d) *reinterpret_cast<uint4*>(po + 16 * i + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                    for (int e = 0; e < 32; e += 8)
+                        if (32 * i + e < p.d) {
+                            const float v[8] = {__uint_as_float(o[e]),     __uint_as_float(o[e + 1]), __uint_as_float(o[e + 2]),
+                                                __uint_as_float(o[e + 3]), __uint_as_float(o[e + 4]), __uint_as_float(o[e + 5]),
+                                                __uint_as_float(o[e + 6]), __uint_as_float(o[e + 7])};
+                            st_global_v8(po + 32 * i + e, v);
+                        }
+                }
+            }
+            if (whole) {
+                __syncwarp();
+                constexpr int PER_ROW = DP / 8;   // lanes a row
+                const int piece = lane % PER_ROW;
+#pragma unroll 4
+                for (int rr = lane / PER_ROW; rr < 32; rr += 32 / PER_ROW) {
+                    const int64_t to_row = __shfl_sync(0xffffffffu, live ? grow : -1, rr);
+                    if (to_row >= 0 && piece * 8 < p.d)
+                        *reinterpret_cast<uint4*>(p.out + to_row * p.d + piece * 8) =
+                                *reinterpret_cast<const uint4*>(stage + rr * (DP * 2) + ((piece ^ (rr & 7)) << 4));
                 }
             }
         }
