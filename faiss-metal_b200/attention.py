@@ -371,8 +371,8 @@ def evict(k, v, mass, key_lengths=None, keep=1, *, recent=0):
         _set(a, "v_stride", c.rows(v, "v"))
         b, n, hk, d = k.shape
         c.shape(v, "v", (b, n, hk, d))
-        if hk < 1 or d < 8 or d % 8:
-            raise ValueError("evict: width %d of %d key heads: expected a multiple of 8, and a head" % (d, hk))
+        if hk < 1 or d < 8 or d > 1024 or d % 8:
+            raise ValueError("evict: width %d of %d key heads: expected a multiple of 8 up to 1024, and a head" % (d, hk))
         if int(keep) < 1 or int(recent) < 0 or int(recent) > int(keep):
             raise ValueError("evict: expected keep >= 1 and 0 <= recent <= keep, got %d and %d" % (keep, recent))
         c.dense(mass, "mass", (b, hk, n), torch.float32)

@@ -768,33 +768,40 @@ attend_few_kernel(const __grid_constant__ CUtensorMap map_sk, const __grid_const
     pdl_wait();
 }
 
-// ---- attend_join_kernel: partial results of a row become its result, a warp a row ------------------
+// ---- attend_join_kernel: partial results of a row become its result ------------------
+// W warps a row, each W-th part, so that many parts are on their way at once (1,000 rows of 37 parts: 31 us with a warp a row).
 template <typename T>
-__global__ void __launch_bounds__(256) attend_join_kernel(const float* part_o, const float* part_lse, int parts, int64_t rows, int d,
+__global__ void __launch_bounds__(256) attend_join_kernel(const float* part_o, const float* part_lse, int parts, int64_t rows, int d, int W,
                                                           uint16_t* out, float* lse) {
-    const int lane = threadIdx.x & 31;
-    const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+    __shared__ float4 acc_s[8][32];
+    __shared__ float total_s[8];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t row = (int64_t)blockIdx.x * (8 / W) + warp / W;
     pdl_wait();
     pdl_trigger();
-    if (row >= rows) return;
+    const bool in = row < rows;
     float top = -CUDART_INF_F;
     bool nan = false;
-    for (int i = lane; i < parts; i += 32) {
-        const float x = __ldcg(part_lse + i * rows + row);
-        top = fmaxf(top, x);
-        nan |= x != x;
+    if (in) {
+        for (int i = lane; i < parts; i += 32) {
+            const float x = __ldcg(part_lse + i * rows + row);
+            top = fmaxf(top, x);
+            nan |= x != x;
+        }
     }
+#pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     nan = __any_sync(0xffffffffu, nan);
+    const bool some = top != -CUDART_INF_F || nan;
     float total = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
     const bool mine = lane * 4 < d;
-    if (top != -CUDART_INF_F || nan) {
+    if (in && some) {
 #pragma unroll 4
-        for (int i = 0; i < parts; i++) {
+        for (int i = warp % W; i < parts; i += W) {
             const float x = __ldcg(part_lse + i * rows + row);
-            if (x == -CUDART_INF_F) continue;   // nothing was written there
             const float w = ex2(x - top);
+            if (x == -CUDART_INF_F) continue;   // nothing was written there
             total += w;
             if (mine) {
                 const float4 o = __ldcg(reinterpret_cast<const float4*>(part_o + (i * rows + row) * d) + lane);
@@ -805,11 +812,26 @@ __global__ void __launch_bounds__(256) attend_join_kernel(const float* part_o, c
             }
         }
     }
-    const float inv = top != -CUDART_INF_F || nan ? 1.f / total : 0.f;
+    if (W > 1) {
+        acc_s[warp][lane] = acc;
+        if (lane == 0) total_s[warp] = total;
+        __syncthreads();
+        if (warp % W != 0) return;
+        for (int x = 1; x < W; x++) {
+            const float4 o = acc_s[warp + x][lane];
+            acc.x += o.x;
+            acc.y += o.y;
+            acc.z += o.z;
+            acc.w += o.w;
+            total += total_s[warp + x];
+        }
+    }
+    if (!in) return;
+    const float inv = some ? 1.f / total : 0.f;
     if (mine)
         *reinterpret_cast<uint2*>(out + row * d + lane * 4) =
                 make_uint2(pack2<T>(acc.x * inv, acc.y * inv), pack2<T>(acc.z * inv, acc.w * inv));
-    if (lane == 0 && lse) lse[row] = inv == 0.f ? -CUDART_INF_F : (top + log2f(total)) * kLn2;
+    if (lane == 0 && lse) lse[row] = some ? (top + log2f(total)) * kLn2 : -CUDART_INF_F;
 }
 
 // ---- host ---------------------------------------------------------------------------------------
@@ -905,8 +927,10 @@ int launch_attend(const CUtensorMap* maps, const TileParams& p, const AttendPlan
         count_launch();
     }
     if (e == cudaSuccess && pl.parts > 1) {
-        e = launch_kernel(attend_join_kernel<T>, dim3((unsigned)ceil_div64(p.rows_total, 8)), 256, 0, Launch(st, true),
-                          static_cast<const float*>(p.part_o), static_cast<const float*>(p.part_lse), pl.parts, p.rows_total, p.d, p.out, p.lse);
+        const int W = pl.parts > 16 ? 8 : pl.parts > 8 ? 4 : pl.parts > 4 ? 2 : 1;
+        e = launch_kernel(attend_join_kernel<T>, dim3((unsigned)ceil_div64(p.rows_total, 8 / W)), 256, 0, Launch(st, true),
+                          static_cast<const float*>(p.part_o), static_cast<const float*>(p.part_lse), pl.parts, p.rows_total, p.d, W, p.out,
+                          p.lse);
         count_launch();
     }
     if (e != cudaSuccess) {

@@ -251,7 +251,7 @@ grad_kernel(const __grid_constant__ CUtensorMap map_a1, const __grid_constant__ 
         if (!KEYS && live) {
             t = r / p.group;
             g = (int)(r - t * p.group);
-            const float2 st = __ldcg(p.stat + unit * p.rt.tiles * GRAD_ROWS + p.rt.place(t, g));
+            const float2 st = __ldcg(p.stat + unit * p.rt.tiles * GRAD_ROWS + p.rt.place((int)t, g));
             my_lse = st.x;
             my_delta = st.y * factor;
         }
@@ -359,10 +359,9 @@ __global__ void __launch_bounds__(256) grad_stat_kernel(AttView g, const uint16_
     const int sub = threadIdx.x & 15;
     const int64_t i = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
     const bool in = i < units * rt.tiles * rt.slots;
-    const int64_t unit = in ? i / (rt.tiles * rt.slots) : 0, tile = i / rt.slots % rt.tiles;
-    int64_t t;
-    int gg;
-    const bool live = in && rt.at(tile, (int)(i % rt.slots), &t, &gg);
+    const int64_t tile_of = in ? i / rt.slots : 0, unit = tile_of / rt.tiles;
+    int t, gg;
+    const bool live = in && rt.at((int)(tile_of - unit * rt.tiles), (int)(i % rt.slots), &t, &gg);
     float dot = 0.f;
     uint32_t top = 0;
     const int h = (int)(unit % kv_heads) * rt.group + (live ? gg : 0);

@@ -15,7 +15,8 @@ namespace {
 constexpr int MASS_THREADS = 384;   // TMA, MMA, two warps for log-sums; 2 x 4 warps
 constexpr int MASS_SLOTS = 128;     // query rows of a tile
 constexpr int MASS_RING = 3;        // streamed tiles: three of keys, or two of queries
-constexpr int MASS_STAT = 2 * MASS_SLOTS * 8;
+constexpr int MASS_STATS = 4;       // query tiles whose log-sums are fetched ahead
+constexpr int MASS_STAT = MASS_STATS * MASS_SLOTS * 8;
 
 struct MassParams {
     AttView q;
@@ -39,18 +40,17 @@ struct MassParams {
     int32_t* status;
 };
 
-// log-sum (base 2; +INF: no row) and end of visible keys of a slot
-__device__ __forceinline__ void slot_stat(const MassParams& p, int64_t unit, int64_t len, int64_t tile, int slot, float* lse2, int* end) {
-    int64_t t;
-    int g;
+// minus the log-sum (base 2; -INF: no row) and end of visible keys of a slot
+__device__ __forceinline__ void slot_stat(const MassParams& p, int64_t b, int kvh, int64_t len, int tile, int slot, float* lse2, int* end) {
+    int t, g;
     float l = CUDART_INF_F;
     int e = 0;
     if (p.rt.at(tile, slot, &t, &g)) {
-        l = __ldg(p.lse + (unit / p.kv_heads * p.queries + t) * p.heads + unit % p.kv_heads * p.group + g) * kLog2e;
+        l = __ldg(p.lse + (b * p.queries + t) * p.heads + kvh * p.group + g) * kLog2e;
         if (l == -CUDART_INF_F) l = CUDART_INF_F;
         e = (int)p.len.seen(len, t);
     }
-    lse2[slot] = l;
+    lse2[slot] = -l;
     end[slot] = e;
 }
 
@@ -64,11 +64,11 @@ mass_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ C
     const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0);
     const int lane = threadIdx.x & 31;
     const uint32_t bar_full = sbase + p.bar_off, bar_empty = bar_full + MASS_RING * 8, bar_a = bar_empty + MASS_RING * 8;
-    const uint32_t bar_s = bar_a + 8, bar_free = bar_s + 16, bar_stat = bar_free + 16;
-    volatile uint32_t* tmem_ptr = reinterpret_cast<volatile uint32_t*>(smem + p.bar_off + (2 * MASS_RING + 7) * 8);
+    const uint32_t bar_s = bar_a + 8, bar_free = bar_s + 16, bar_stat = bar_free + 16, bar_used = bar_stat + MASS_STATS * 8;
+    volatile uint32_t* tmem_ptr = reinterpret_cast<volatile uint32_t*>(smem + p.bar_off + (2 * MASS_RING + 5 + 2 * MASS_STATS) * 8);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_ptr + 1);
-    float* const stat_lse = reinterpret_cast<float*>(smem + p.stat_off);            // [2][MASS_SLOTS]
-    int* const stat_end = reinterpret_cast<int*>(smem + p.stat_off) + 2 * MASS_SLOTS;
+    float* const stat_lse = reinterpret_cast<float*>(smem + p.stat_off);            // [MASS_STATS][MASS_SLOTS]
+    int* const stat_end = reinterpret_cast<int*>(smem + p.stat_off) + MASS_STATS * MASS_SLOTS;
 
     if ((sbase & 1023u) != 0) {
         if (threadIdx.x == 0) atomicOr(p.status, kDevErrSmemAlign);
@@ -116,7 +116,10 @@ mass_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ C
         for (int t = 0; t < 2; t++) {
             mbar_init(bar_s + t * 8, 1);
             mbar_init(bar_free + t * 8, 4);
+        }
+        for (int t = 0; t < MASS_STATS; t++) {
             mbar_init(bar_stat + t * 8, 2);
+            mbar_init(bar_used + t * 8, 4);
         }
         mbar_fence_init();
     }
@@ -137,7 +140,7 @@ mass_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ C
             }
         }
     }
-    if (FEW && threadIdx.x >= 128 && threadIdx.x < 128 + MASS_SLOTS) slot_stat(p, unit, len, 0, threadIdx.x - 128, stat_lse, stat_end);
+    if (FEW && threadIdx.x >= 128 && threadIdx.x < 128 + MASS_SLOTS) slot_stat(p, b, kvh, len, 0, threadIdx.x - 128, stat_lse, stat_end);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -215,11 +218,13 @@ mass_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ C
         // ------------------------------ log-sums of the streamed query rows
         if (!FEW) {
             for (int i = 0; i < n; i++) {
-                if (!__all_sync(0xffffffffu, wait(bar_free + (i & 1) * 8, ((i >> 1) & 1) ^ 1))) break;
-                for (int s = threadIdx.x - 64; s < MASS_SLOTS; s += 64)
-                    slot_stat(p, unit, len, first + i, s, stat_lse + (i & 1) * MASS_SLOTS, stat_end + (i & 1) * MASS_SLOTS);
+                const int x = i % MASS_STATS;
+                if (!__all_sync(0xffffffffu, wait(bar_used + x * 8, ((i / MASS_STATS) & 1) ^ 1))) break;
+#pragma unroll
+                for (int s = 0; s < MASS_SLOTS; s += 64)
+                    slot_stat(p, b, kvh, len, (int)first + i, threadIdx.x - 64 + s, stat_lse + x * MASS_SLOTS, stat_end + x * MASS_SLOTS);
                 __syncwarp();
-                if (lane == 0) mbar_arrive(bar_stat + (i & 1) * 8);
+                mbar_arrive_if(lane == 0, bar_stat + x * 8);
             }
         }
     } else {
@@ -229,45 +234,60 @@ mass_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ C
         bool ok = true;
         for (int i = wg; i < n; i += 2) {
             ok = wait(bar_s + wg * 8, (i >> 1) & 1);
-            if (!FEW) ok = ok && wait(bar_stat + wg * 8, (i >> 1) & 1);
+            if (!FEW) ok = ok && wait(bar_stat + (i % MASS_STATS) * 8, (i / MASS_STATS) & 1);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             tc_fence_after();
             const int64_t key = (FEW ? first + i : (int64_t)blk) * 128 + ew * 32 + lane;
             const uint32_t ts = tmem + p.cols * wg + ((uint32_t)(ew * 32) << 16);
-            const uint32_t lse = sbase + p.stat_off + (FEW ? 0 : wg * MASS_SLOTS * 4), ends = lse + 2 * MASS_SLOTS * 4;
+            const uint32_t lse = sbase + p.stat_off + (FEW ? 0 : i % MASS_STATS * MASS_SLOTS * 4), ends = lse + MASS_STATS * MASS_SLOTS * 4;
             // causal: some query of the tile does not see some key of this warp
             bool masked = false;
             if (p.len.causal) {
                 const int64_t tmin = FEW ? 0 : (first + i) / p.rt.gchunks * p.rt.bt;
                 masked = key - lane + 32 > p.len.seen(len, tmin);
             }
-            float part[2] = {0.f, 0.f};
+            // in groups of eight, each step for the whole group (see weigh32)
+            float2 part[4] = {};
             for (int c0 = 0; c0 < p.cols; c0 += 16) {
                 uint32_t s[16];
                 tc_ld16_wait(ts + c0, s);
 #pragma unroll
-                for (int e = 0; e < 16; e += 4) {
-                    const uint4 l = lds128(lse + (c0 + e) * 4);
-                    float x0 = ex2(fmaf(__uint_as_float(s[e]), c, -__uint_as_float(l.x)));
-                    float x1 = ex2(fmaf(__uint_as_float(s[e + 1]), c, -__uint_as_float(l.y)));
-                    float x2 = ex2(fmaf(__uint_as_float(s[e + 2]), c, -__uint_as_float(l.z)));
-                    float x3 = ex2(fmaf(__uint_as_float(s[e + 3]), c, -__uint_as_float(l.w)));
-                    if (masked) {
-                        const uint4 z = lds128(ends + (c0 + e) * 4);
-                        if (key >= (int)z.x) x0 = 0.f;
-                        if (key >= (int)z.y) x1 = 0.f;
-                        if (key >= (int)z.z) x2 = 0.f;
-                        if (key >= (int)z.w) x3 = 0.f;
+                for (int h = 0; h < 16; h += 8) {
+                    float2 y[4];
+#pragma unroll
+                    for (int e = 0; e < 4; e += 2) {
+                        const uint4 l = lds128(lse + (c0 + h + 2 * e) * 4);   // the negated log-sums
+                        y[e] = fma2(make_float2(__uint_as_float(s[h + 2 * e]), __uint_as_float(s[h + 2 * e + 1])), make_float2(c, c),
+                                    make_float2(__uint_as_float(l.x), __uint_as_float(l.y)));
+                        y[e + 1] = fma2(make_float2(__uint_as_float(s[h + 2 * e + 2]), __uint_as_float(s[h + 2 * e + 3])),
+                                        make_float2(c, c), make_float2(__uint_as_float(l.z), __uint_as_float(l.w)));
                     }
-                    part[0] += x0 + x1;
-                    part[1] += x2 + x3;
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        y[e].x = ex2(y[e].x);
+                        y[e].y = ex2(y[e].y);
+                    }
+                    if (masked) {
+#pragma unroll
+                        for (int e = 0; e < 4; e += 2) {
+                            const uint4 z = lds128(ends + (c0 + h + 2 * e) * 4);
+                            if (key >= (int)z.x) y[e].x = 0.f;
+                            if (key >= (int)z.y) y[e].y = 0.f;
+                            if (key >= (int)z.z) y[e + 1].x = 0.f;
+                            if (key >= (int)z.w) y[e + 1].y = 0.f;
+                        }
+                    }
+#pragma unroll
+                    for (int e = 0; e < 4; e++) part[e] = add2(part[e], y[e]);
                 }
             }
-            sum += part[0] + part[1];
+            const float2 both = add2(add2(part[0], part[1]), add2(part[2], part[3]));
+            sum += both.x + both.y;
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(bar_free + wg * 8);
+            mbar_arrive_if(lane == 0, bar_free + wg * 8);
+            if (!FEW) mbar_arrive_if(lane == 0, bar_used + (i % MASS_STATS) * 8);
             if (FEW) {
                 if (key < len) p.mass_out[unit * p.len.n + key] = (p.mass_in ? p.mass_in[unit * p.len.n + key] : 0.f) + sum;
                 sum = 0.f;
@@ -324,7 +344,7 @@ MassPlan plan_mass(const B200FAttentionMassArgs& a) {
         pl.blocks = (int)ceil_div64(tiles, pl.chunk);
     } else {
         pl.blocks = (int)tiles;
-        int64_t s = units * tiles > 0 ? 2 * sm / (units * tiles) : 1;
+        int64_t s = units * tiles > 0 ? 4 * sm / (units * tiles) : 1;
         if (s > pl.rt.tiles / 2) s = pl.rt.tiles / 2;
         pl.splits = (int)(s < 1 ? 1 : s);
     }
@@ -348,7 +368,7 @@ int launch_mass(const CUtensorMap* maps, MassParams p, int64_t items, cudaStream
     p.bar_off = p.stat_off + MASS_STAT;
     p.tmem_cols = 32;
     while (p.tmem_cols < 2 * p.cols) p.tmem_cols *= 2;
-    const int smem = p.bar_off + (2 * MASS_RING + 7) * 8 + 16;
+    const int smem = p.bar_off + (2 * MASS_RING + 5 + 2 * MASS_STATS) * 8 + 16;
     static bool attr_set[kMaxDevices] = {false};
     const int slot = device_slot();
     if (!attr_set[slot]) {

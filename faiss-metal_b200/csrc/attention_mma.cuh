@@ -276,27 +276,27 @@ inline int make_rows_map(CUtensorMap* map, AttMap* am, const AttView& v, int sto
 // `gchunks` pieces.  Slot s of tile i is query (i / gchunks) * bt + s / gb, head (i % gchunks) * gb + s % gb of the group.
 struct RowTiles {
     int slots, gb, bt, gchunks, group;
-    int64_t queries, tiles;
-    __host__ __device__ bool at(int64_t tile, int slot, int64_t* t, int* g) const {
-        const int q = slot / gb;
-        *t = tile / gchunks * bt + q;
-        *g = (int)(tile % gchunks) * gb + (slot - q * gb);
+    int queries, tiles;   // batch * queries * heads is below 2^31
+    __host__ __device__ bool at(int tile, int slot, int* t, int* g) const {
+        const int q = (int)((unsigned)slot / (unsigned)gb), block = (int)((unsigned)tile / (unsigned)gchunks);
+        *t = block * bt + q;
+        *g = (tile - block * gchunks) * gb + (slot - q * gb);
         return q < bt && *t < queries && *g < group;
     }
-    __host__ __device__ int64_t place(int64_t t, int g) const {   // tile * slots + slot
-        return (t / bt * gchunks + g / gb) * slots + t % bt * gb + g % gb;
+    __host__ __device__ int64_t place(int t, int g) const {   // tile * slots + slot
+        return ((int64_t)(t / bt) * gchunks + g / gb) * slots + t % bt * gb + g % gb;
     }
 };
 inline RowTiles row_tiles(int slots, int64_t queries, int group) {
     RowTiles r;
     r.slots = slots;
     r.group = group;
-    r.queries = queries;
+    r.queries = (int)queries;
     r.gb = group < slots ? group : slots;
     r.bt = slots / r.gb;
     if (r.bt > queries) r.bt = queries > 0 ? (int)queries : 1;
     r.gchunks = (group + r.gb - 1) / r.gb;
-    r.tiles = ceil_div64(queries, r.bt) * r.gchunks;
+    r.tiles = (int)(ceil_div64(queries, r.bt) * r.gchunks);
     return r;
 }
 // 5-D map {column, head of the group, query, key head, sequence} of queries, box {64, gb, bt, 1, 1}.  Heads of a group do not repeat.

@@ -431,7 +431,7 @@ int b200f_attention_mass(const B200FAttentionMassArgs* args);
  * before them, the keep - recent of largest mass (ties to the lower row, NaN counts as largest); else all.  Kept
  * rows keep their order.  out_rows[b][h][i]: the row that slot i was; slots behind the last kept row
  * are zero in out_k / out_v / out_mass and -1 in out_rows.  Outputs must not overlap the inputs.  Any d that is a multiple
- * of 8. */
+ * of 8 up to 1,024. */
 typedef struct B200FEvictArgs {
     const void* k;
     const void* v;
