@@ -14,7 +14,7 @@ namespace {
 // its own four warps.  Two CTAs share an SM, so that one's start and end hide behind the other.
 constexpr int MASS_THREADS = 384;   // TMA, MMA, two warps for log-sums; 2 x 4 warps
 constexpr int MASS_SLOTS = 128;     // query rows of a tile
-constexpr int MASS_RING = 3;        // streamed tiles: three of keys, or two of queries
+constexpr int MASS_RING = 5;        // streamed tiles at most: what half an SM's shared memory takes
 constexpr int MASS_STATS = 4;       // query tiles whose log-sums are fetched ahead
 constexpr int MASS_STAT = MASS_STATS * MASS_SLOTS * 8;
 
@@ -360,7 +360,7 @@ int check_mass(const B200FAttentionMassArgs* a) {
 template <typename T, int DP, bool FEW>
 int launch_mass(const CUtensorMap* maps, MassParams p, int64_t items, cudaStream_t st) {
     const int key_bytes = DP / 64 * ATT_CHUNK, query_bytes = DP / 64 * p.cols * 128;   // multiples of 1024
-    p.ring = FEW ? MASS_RING : 2;
+    p.ring = DP == 64 ? 5 : FEW ? 3 : 2;
     p.a_off = 0;
     p.ring_off = FEW ? query_bytes : key_bytes;
     p.stage = FEW ? key_bytes : query_bytes;
@@ -372,9 +372,9 @@ int launch_mass(const CUtensorMap* maps, MassParams p, int64_t items, cudaStream
     static bool attr_set[kMaxDevices] = {false};
     const int slot = device_slot();
     if (!attr_set[slot]) {
-        // the largest layout: three key tiles and a query tile of 128 rows
+        // the largest layout: the ring of key tiles and a query tile of 128 rows
         B200F_CUDA_TRY(cudaFuncSetAttribute(mass_kernel<T, DP, FEW>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                            (MASS_RING + 1) * DP / 64 * ATT_CHUNK + MASS_STAT + 256));
+                                            (DP == 64 ? 6 : 4) * DP / 64 * ATT_CHUNK + MASS_STAT + 256));
         attr_set[slot] = true;
     }
     mass_kernel<T, DP, FEW><<<(unsigned)items, MASS_THREADS, smem, st>>>(maps[0], maps[1], p);
