@@ -435,13 +435,7 @@ attend_tile_kernel(const __grid_constant__ CUtensorMap map_sk, const __grid_cons
 #pragma unroll
                 for (int e = 0; e < 32; e++) o[e] = inv == 0.f ? 0u : __float_as_uint(__uint_as_float(o[e]) * inv);
                 if (whole) {
-#pragma unroll
-                    for (int e = 0; e < 4; e++)
-                        *reinterpret_cast<uint4*>(stage + lane * (DP * 2) + (((4 * i + e) ^ (lane & 7)) << 4)) =
-                                make_uint4(pack2<T>(__uint_as_float(o[8 * e]), __uint_as_float(o[8 * e + 1])),
-                                           pack2<T>(__uint_as_float(o[8 * e + 2]), __uint_as_float(o[8 * e + 3])),
-                                           pack2<T>(__uint_as_float(o[8 * e + 4]), __uint_as_float(o[8 * e + 5])),
-                                           pack2<T>(__uint_as_float(o[8 * e + 6]), __uint_as_float(o[8 * e + 7])));
+                    stage_columns32<T, DP>(stage, o, 4 * i);
                 } else if (live && !none) {
                     float* const po = p.part_o + (part * p.rows_total + grow) * p.d;
 #pragma unroll
@@ -454,18 +448,7 @@ attend_tile_kernel(const __grid_constant__ CUtensorMap map_sk, const __grid_cons
                         }
                 }
             }
-            if (whole) {
-                __syncwarp();
-                constexpr int PER_ROW = DP / 8;   // lanes a row
-                const int piece = lane % PER_ROW;
-#pragma unroll 4
-                for (int rr = lane / PER_ROW; rr < 32; rr += 32 / PER_ROW) {
-                    const int64_t to_row = __shfl_sync(0xffffffffu, live ? grow : -1, rr);
-                    if (to_row >= 0 && piece * 8 < p.d)
-                        *reinterpret_cast<uint4*>(p.out + to_row * p.d + piece * 8) =
-                                *reinterpret_cast<const uint4*>(stage + rr * (DP * 2) + ((piece ^ (rr & 7)) << 4));
-                }
-            }
+            if (whole) store_rows<DP>(stage, p.out, live ? grow * p.d : -1, 0, p.d);
         }
     }
     tc_fence_before();

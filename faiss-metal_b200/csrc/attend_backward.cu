@@ -12,11 +12,14 @@ namespace b200f {
 namespace {
 
 // ---- grad_kernel ------------------------------------------------------------------------------
-// A CTA keeps a pair of tiles of 128 rows (A1, A2) in shared memory and streams pairs of 64 rows (B1, B2) past them:
+// A CTA keeps a pair of tiles of 128 rows (A1, A2) and streams pairs of 64 rows (B1, B2) past them:
 //   KEYS:  A1 = k, A2 = v, B1 = q, B2 = do     S = A1 B1^T, P' = A2 B2^T, acc1 (dk) += ds B1, acc2 (dv) += p B2
 //   else:  A1 = q, A2 = do, B1 = k, B2 = v     acc1 (dq) += ds B1
 // S and P' have two buffers, each with its own group of four warps (a row of A a thread) that turns them into p and ds in place; the
 // tensor cores compute the next pair of scores and add the previous pair's products meanwhile.
+// Products of 64 columns with both operands in shared memory run at 2/3 of the full rate, which its bandwidth bounds: KEYS spends 1,280
+// of its 1,400 cycles a tile on them (1,024 at full rate), tensor memory being full.  Without acc2 there is room: A1 and A2 lie in
+// tensor memory, and the tile takes 768.
 constexpr int GRAD_THREADS = 384;   // TMA, MMA, two spare warps; 2 x 4 warps
 constexpr int GRAD_ROWS = 64;       // rows of a streamed tile
 constexpr int GRAD_MAX_STAGES = 8;
@@ -25,23 +28,27 @@ constexpr int GRAD_A_BYTES = DP / 64 * ATT_CHUNK;
 template <int DP>
 constexpr int GRAD_B_BYTES = DP / 64 * GRAD_ROWS * 128;
 constexpr int GRAD_STAT_BYTES = GRAD_ROWS * 8;
-template <int DP>
-constexpr int GRAD_STAGES = DP == 128 ? 4 : 8;
-template <int DP>
-constexpr int GRAD_SM_STAT = 2 * GRAD_A_BYTES<DP> + GRAD_STAGES<DP> * 2 * GRAD_B_BYTES<DP>;
-template <int DP>
-constexpr int GRAD_SM_BAR = GRAD_SM_STAT<DP> + GRAD_STAGES<DP> * GRAD_STAT_BYTES;
-template <int DP>
-constexpr int GRAD_SMEM = GRAD_SM_BAR<DP> + (2 * GRAD_MAX_STAGES + 6) * 8 + 16;
-static_assert(GRAD_SMEM<128> <= 232448 && GRAD_SMEM<64> <= 232448, "shared memory of a CTA");
+template <int DP, bool KEYS>
+constexpr int GRAD_STAGES = DP == 64 ? 8 : KEYS ? 4 : 6;
+template <int DP, bool KEYS>
+constexpr int GRAD_SM_RING = KEYS ? 2 * GRAD_A_BYTES<DP> : 0;
+template <int DP, bool KEYS>
+constexpr int GRAD_SM_STAT = GRAD_SM_RING<DP, KEYS> + GRAD_STAGES<DP, KEYS> * 2 * GRAD_B_BYTES<DP>;
+template <int DP, bool KEYS>
+constexpr int GRAD_SM_BAR = GRAD_SM_STAT<DP, KEYS> + GRAD_STAGES<DP, KEYS> * GRAD_STAT_BYTES;
+template <int DP, bool KEYS>
+constexpr int GRAD_SMEM = GRAD_SM_BAR<DP, KEYS> + (2 * GRAD_MAX_STAGES + 8) * 8 + 16;
+static_assert(GRAD_SMEM<128, true> <= 232448 && GRAD_SMEM<128, false> <= 232448 && GRAD_SMEM<64, true> <= 232448, "shared memory of a CTA");
+static_assert(GRAD_SM_STAT<64, false> >= 256 * 128, "the results' stage");
 constexpr uint32_t TG_S = 0, TG_P = 128, TG_ACC1 = 256, TG_ACC2 = 384;   // S and P' of buffer b at + 64 b
+constexpr uint32_t TG_A1 = 384, TG_A2 = 448;                             // not KEYS
 
 struct GradParams {
     AttMap a1m, a2m, b1m, b2m;
     AttView q, g;            // queries and output gradients (KEYS = false: A1 and A2 are read with plain loads)
     AttLengths len;
     RowTiles rt;             // query rows in tiles of GRAD_ROWS
-    const float2* stat;      // [unit][tile][slot]: lse in base 2 (+INF: a slot without a row), delta
+    const float* stat;       // [unit][tile]: of every slot minus the lse in base 2 (-INF: no row), then minus delta
     const uint32_t* gmax;    // fp16: bit pattern of the largest |do|
     int64_t batch, queries;
     int heads, kv_heads, group, d;
@@ -62,21 +69,68 @@ __device__ __forceinline__ float grad_factor(uint32_t max_bits) {
     return max_bits == 0 || e > 126 ? 1.f : exp2f((float)min(max(-3 - e, -100), 100));
 }
 
+// Score gradients of 32 columns, ds = p (dp - delta), and the weights p; mstat = minus log-sums and deltas, of the columns (KEYS; an
+// address in shared memory, the deltas behind the log-sums) or the row's.  Steps by groups, as in weigh32.
+template <typename T, bool KEYS>
+__device__ __forceinline__ void grad32(const uint32_t (&s)[32], const uint32_t (&dp)[32], float c, float factor, uint32_t mstat, float mlse,
+                                       float mdelta, uint32_t (&wp)[16], uint32_t (&ws)[16]) {
+    constexpr bool HALF = std::is_same<T, __half>::value;
+    const float2 c2 = make_float2(c, c), f2 = make_float2(factor, factor);
+#pragma unroll
+    for (int g = 0; g < 16; g += 4) {
+        float2 l[4], d[4], y[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) l[e] = make_float2(mlse, mlse), d[e] = make_float2(mdelta, mdelta);
+        if (KEYS) {
+#pragma unroll
+            for (int e = 0; e < 4; e += 2) {
+                const uint4 a = lds128(mstat + (2 * (g + e)) * 4), b = lds128(mstat + GRAD_ROWS * 4 + (2 * (g + e)) * 4);
+                l[e] = make_float2(__uint_as_float(a.x), __uint_as_float(a.y));
+                l[e + 1] = make_float2(__uint_as_float(a.z), __uint_as_float(a.w));
+                d[e] = make_float2(__uint_as_float(b.x), __uint_as_float(b.y));
+                d[e + 1] = make_float2(__uint_as_float(b.z), __uint_as_float(b.w));
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            y[e] = fma2(make_float2(__uint_as_float(s[2 * (g + e)]), __uint_as_float(s[2 * (g + e) + 1])), c2, l[e]);
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            y[e].x = ex2(y[e].x);
+            y[e].y = ex2(y[e].y);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; e++) d[e] = add2(make_float2(__uint_as_float(dp[2 * (g + e)]), __uint_as_float(dp[2 * (g + e) + 1])), d[e]);
+        if (HALF) {
+#pragma unroll
+            for (int e = 0; e < 4; e++) d[e] = mul2(d[e], f2);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            d[e] = mul2(y[e], d[e]);
+            wp[g + e] = pack2<T>(y[e].x, y[e].y);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; e++) ws[g + e] = pack2<T>(d[e].x, d[e].y);
+    }
+}
+
 template <typename T, int DP, bool KEYS>
 __global__ void __launch_bounds__(GRAD_THREADS, 1)
 grad_kernel(const __grid_constant__ CUtensorMap map_a1, const __grid_constant__ CUtensorMap map_a2,
             const __grid_constant__ CUtensorMap map_b1, const __grid_constant__ CUtensorMap map_b2, const GradParams p) {
     extern __shared__ __align__(1024) uint8_t smem[];
-    constexpr int STAGES = GRAD_STAGES<DP>, ABYTES = GRAD_A_BYTES<DP>, BBYTES = GRAD_B_BYTES<DP>, CHUNKS = DP / 64;
+    constexpr int STAGES = GRAD_STAGES<DP, KEYS>, ABYTES = GRAD_A_BYTES<DP>, BBYTES = GRAD_B_BYTES<DP>, CHUNKS = DP / 64;
+    constexpr int RING = GRAD_SM_RING<DP, KEYS>;
     constexpr bool HALF = std::is_same<T, __half>::value;
     const uint32_t sbase = smem_u32(smem);
     const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0);
     const int lane = threadIdx.x & 31;
-    const uint32_t bar_full = sbase + GRAD_SM_BAR<DP>, bar_empty = bar_full + GRAD_MAX_STAGES * 8;
-    const uint32_t bar_a = bar_empty + GRAD_MAX_STAGES * 8, bar_s = bar_a + 8, bar_p = bar_s + 16, bar_done = bar_p + 16;
-    volatile uint32_t* tmem_ptr = reinterpret_cast<volatile uint32_t*>(smem + GRAD_SM_BAR<DP> + (2 * GRAD_MAX_STAGES + 6) * 8);
+    const uint32_t bar_full = sbase + GRAD_SM_BAR<DP, KEYS>, bar_empty = bar_full + GRAD_MAX_STAGES * 8;
+    const uint32_t bar_a = bar_empty + GRAD_MAX_STAGES * 8, bar_s = bar_a + 8, bar_d = bar_s + 16, bar_p = bar_d + 16, bar_done = bar_p + 16;
+    volatile uint32_t* tmem_ptr = reinterpret_cast<volatile uint32_t*>(smem + GRAD_SM_BAR<DP, KEYS> + (2 * GRAD_MAX_STAGES + 8) * 8);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_ptr + 1);
-    const uint32_t ring = sbase + 2 * ABYTES;
+    const uint32_t ring = sbase + RING;
 
     pdl_wait();
     pdl_trigger();
@@ -85,18 +139,17 @@ grad_kernel(const __grid_constant__ CUtensorMap map_a1, const __grid_constant__ 
         return;
     }
     // ---- this CTA's item: a block of 128 rows of A, a range of B's tiles
-    const int64_t blk = blockIdx.x % p.blocks;
-    const int64_t rest = blockIdx.x / p.blocks;
-    const int sp = (int)(rest % p.splits);
-    const int64_t unit = rest / p.splits;
-    const int kvh = (int)(unit % p.kv_heads);
-    const int64_t b = unit / p.kv_heads;
+    const uint32_t rest = blockIdx.x / (uint32_t)p.blocks, blk = blockIdx.x - rest * (uint32_t)p.blocks;
+    const uint32_t unit = rest / (uint32_t)p.splits;
+    const int sp = (int)(rest - unit * p.splits);
+    const int64_t b = unit / (uint32_t)p.kv_heads;
+    const int kvh = (int)(unit - (uint32_t)b * p.kv_heads);
     const int64_t len = p.len.of(b);
-    const int64_t row0 = blk * 128;
+    const int64_t row0 = (int64_t)blk * 128;
     const int64_t tiles = KEYS ? (row0 < len ? p.rt.tiles : 0) : (len + GRAD_ROWS - 1) / GRAD_ROWS;
     const int64_t per = (tiles + p.splits - 1) / p.splits;
-    const int64_t first = min(tiles, per * sp);
-    const int n = (int)(min(tiles, first + per) - first);
+    const int first = (int)min(tiles, per * sp);
+    const int n = (int)min(tiles - first, per);
 
     if (threadIdx.x == 0) {
         *abort_flag = 0;
@@ -107,6 +160,7 @@ grad_kernel(const __grid_constant__ CUtensorMap map_a1, const __grid_constant__ 
         mbar_init(bar_a, 1);
         for (int t = 0; t < 2; t++) {
             mbar_init(bar_s + t * 8, 1);
+            mbar_init(bar_d + t * 8, 1);
             mbar_init(bar_p + t * 8, 4);
         }
         mbar_init(bar_done, 1);
@@ -122,29 +176,50 @@ grad_kernel(const __grid_constant__ CUtensorMap map_a1, const __grid_constant__ 
         // slots that no box fills hold zeros: they are K rows of the products
         const int fill = p.rt.gb * p.rt.bt;
         if (fill < GRAD_ROWS) {
-            for (int s = warp; s < 2 * STAGES; s += GRAD_THREADS / 32)
-                zero_tile_rows(smem + 2 * ABYTES + s * BBYTES, CHUNKS, fill, GRAD_ROWS);
+            for (int s = warp; s < 2 * STAGES; s += GRAD_THREADS / 32) zero_tile_rows(smem + RING + s * BBYTES, CHUNKS, fill, GRAD_ROWS);
         }
-    } else if (n > 0) {
-        // A1 and A2: packed query rows, swizzled as TMA would
-        const int64_t rows = p.queries * p.group;
-        for (int i = threadIdx.x; i < 2 * 128 * (DP / 8); i += GRAD_THREADS) {
-            const int which = i / (128 * (DP / 8)), r = i / (DP / 8) % 128, c = i % (DP / 8);
-            uint4 x = make_uint4(0, 0, 0, 0);
-            if (row0 + r < rows && c * 8 < p.d) {
-                const int64_t t = (row0 + r) / p.group;
-                const int h = kvh * p.group + (int)(row0 + r - t * p.group);
-                x = *reinterpret_cast<const uint4*>((which ? p.g : p.q).at(b, t, h) + c * 8);
-            }
-            *reinterpret_cast<uint4*>(smem + which * ABYTES + (c >> 3) * ATT_CHUNK + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = x;
-        }
-        fence_proxy_async_shared();
     }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_ptr;
     auto wait = [&](uint32_t bar, uint32_t parity) { return mbar_wait(bar, parity, abort_flag, p.status); };
+    auto waits = [&](uint32_t bar, uint32_t parity) { return (bool)__all_sync(0xffffffffu, wait(bar, parity)); };
+    // what a thread of the two groups of four warps owns: a key, or a packed query row
+    const int wg = (warp - 4) >> 2, ew = warp & 3;
+    const uint32_t lanes = (uint32_t)(ew * 32) << 16;
+    const int64_t r = row0 + ew * 32 + lane;
+    const bool live = KEYS ? r < p.len.n : r < (int64_t)p.queries * p.group;
+    int t = 0, g = 0;
+    if (!KEYS && live) {
+        t = (int)((uint32_t)r / (uint32_t)p.group);
+        g = (int)((uint32_t)r - (uint32_t)t * p.group);
+    }
+    if (!KEYS && n > 0) {
+        // A1 and A2 to tensor memory: four warps each, a row a thread
+        if (warp >= 4) {
+            const AttView& src = wg ? p.g : p.q;
+            const uint4* const row = reinterpret_cast<const uint4*>(src.at(b, t, kvh * p.group + g));
+#pragma unroll
+            for (int c = 0; c < DP / 64; c++) {
+                uint32_t x[32];
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    uint4 y = make_uint4(0, 0, 0, 0);
+                    if (live && (8 * c + e) * 8 < p.d) y = __ldg(row + 8 * c + e);
+                    x[4 * e] = y.x;
+                    x[4 * e + 1] = y.y;
+                    x[4 * e + 2] = y.z;
+                    x[4 * e + 3] = y.w;
+                }
+                tc_st32(tmem + (wg ? TG_A2 : TG_A1) + 32 * c + lanes, x);
+            }
+            tc_wait_st();
+            tc_fence_before();
+        }
+        if (warp != 0) asm volatile("bar.sync 1, %0;" ::"n"(GRAD_THREADS - 32) : "memory");
+        tc_fence_after();
+    }
 
     if (warp == 0) {
         if (elect_one() && n > 0) {
@@ -165,22 +240,22 @@ grad_kernel(const __grid_constant__ CUtensorMap map_a1, const __grid_constant__ 
                 if (!ok) break;
                 const uint32_t full = bar_full + slot * 8, b1 = ring + slot * 2 * BBYTES, b2 = b1 + BBYTES;
                 mbar_arrive_expect_tx(full, bytes);
-                const int64_t tile = first + i;
+                const int tile = first + i;
                 if (KEYS) {
-                    const int g0 = (int)(tile % p.rt.gchunks) * p.rt.gb, t0 = (int)(tile / p.rt.gchunks) * p.rt.bt;
+                    const int block = tile / p.rt.gchunks, g0 = (tile - block * p.rt.gchunks) * p.rt.gb, t0 = block * p.rt.bt;
                     for (int c = 0; c < CHUNKS; c++) {
                         tma_load_5d(b1 + c * GRAD_ROWS * 128, &map_b1, full, c * 64, g0, t0, kvh * p.b1m.head_step,
                                     (int)b * p.b1m.batch_step);
                         tma_load_5d(b2 + c * GRAD_ROWS * 128, &map_b2, full, c * 64, g0, t0, kvh * p.b2m.head_step,
                                     (int)b * p.b2m.batch_step);
                     }
-                    bulk_load(sbase + GRAD_SM_STAT<DP> + slot * GRAD_STAT_BYTES, p.stat + (unit * p.rt.tiles + tile) * GRAD_ROWS,
-                              GRAD_STAT_BYTES, full);
+                    bulk_load(sbase + GRAD_SM_STAT<DP, KEYS> + slot * GRAD_STAT_BYTES,
+                              p.stat + ((int64_t)unit * p.rt.tiles + tile) * 2 * GRAD_ROWS, GRAD_STAT_BYTES, full);
                 } else {
                     for (int c = 0; c < CHUNKS; c++) {
-                        tma_load_4d(b1 + c * GRAD_ROWS * 128, &map_b1, full, c * 64, (int)tile * GRAD_ROWS, kvh * p.b1m.head_step,
+                        tma_load_4d(b1 + c * GRAD_ROWS * 128, &map_b1, full, c * 64, tile * GRAD_ROWS, kvh * p.b1m.head_step,
                                     (int)b * p.b1m.batch_step);
-                        tma_load_4d(b2 + c * GRAD_ROWS * 128, &map_b2, full, c * 64, (int)tile * GRAD_ROWS, kvh * p.b2m.head_step,
+                        tma_load_4d(b2 + c * GRAD_ROWS * 128, &map_b2, full, c * 64, tile * GRAD_ROWS, kvh * p.b2m.head_step,
                                     (int)b * p.b2m.batch_step);
                     }
                 }
@@ -197,40 +272,41 @@ grad_kernel(const __grid_constant__ CUtensorMap map_a1, const __grid_constant__ 
         }
         __syncwarp();
     } else if (warp == 1) {
+        // every wait is voted on: control flow stays uniform
         const bool leader = elect_one();
-        bool ok = true;
-        if (KEYS && n > 0) ok = wait(bar_a, 0);
-        const int64_t boundary = !KEYS && len < p.len.n && (len & (GRAD_ROWS - 1)) ? len / GRAD_ROWS : -1;
-        int slot = 0;
+        bool ok = !KEYS || n == 0 || waits(bar_a, 0);
+        const int tail = (int)(len & (GRAD_ROWS - 1));
+        const int boundary = !KEYS && len < p.len.n && tail ? (int)(len / GRAD_ROWS) - first : -1;
+        int slot = 0, used = 0;
         uint32_t phase = 0;
         auto scores = [&](int i) {   // S and P' of the next stage
-            ok = ok && wait(bar_full + slot * 8, phase);
-            if (!KEYS && ok && first + i == boundary) {
-                // keys behind the sequence's end, within the tensor: K rows of the products
-                zero_tile_rows(smem + 2 * ABYTES + slot * 2 * BBYTES, CHUNKS, (int)(len & (GRAD_ROWS - 1)), GRAD_ROWS);
-            }
-            ok = __all_sync(0xffffffffu, ok);
-            const uint32_t b1 = ring + slot * 2 * BBYTES;
-            mma_rows<T, DP, GRAD_ROWS>(leader && ok, tmem + TG_S + 64 * (i & 1), sbase, b1);
-            mma_rows<T, DP, GRAD_ROWS>(leader && ok, tmem + TG_P + 64 * (i & 1), sbase + ABYTES, b1 + BBYTES);
+            if (!waits(bar_full + slot * 8, phase)) return false;
+            // keys behind the sequence's end, within the tensor: K rows of the products
+            if (!KEYS && i == boundary) zero_tile_rows(smem + RING + slot * 2 * BBYTES, CHUNKS, tail, GRAD_ROWS);
+            const uint32_t b1 = ring + slot * 2 * BBYTES, x = 64 * (i & 1);
+            if (KEYS) mma_rows<T, DP, GRAD_ROWS>(leader, tmem + TG_S + x, sbase, b1);
+            else mma_rows_ts<T, DP, GRAD_ROWS>(leader, tmem + TG_S + x, tmem + TG_A1, b1);
             tc_commit_by<false>(leader, bar_s + (i & 1) * 8);
+            if (KEYS) mma_rows<T, DP, GRAD_ROWS>(leader, tmem + TG_P + x, sbase + ABYTES, b1 + BBYTES);
+            else mma_rows_ts<T, DP, GRAD_ROWS>(leader, tmem + TG_P + x, tmem + TG_A2, b1 + BBYTES);
+            tc_commit_by<false>(leader, bar_d + (i & 1) * 8);
             if (++slot == STAGES) {
                 slot = 0;
                 phase ^= 1;
             }
+            return true;
         };
-        if (n > 0) scores(0);
-        if (n > 1) scores(1);
-        int used = 0;
+        ok = ok && (n < 1 || scores(0)) && (n < 2 || scores(1));
         for (int i = 0; i < n && ok; i++) {
-            ok = __all_sync(0xffffffffu, wait(bar_p + (i & 1) * 8, (i >> 1) & 1));
+            ok = waits(bar_p + (i & 1) * 8, (i >> 1) & 1);
+            if (!ok) break;
             tc_fence_after();
-            const uint32_t b1 = ring + used * 2 * BBYTES;
-            mma_weights<T, DP, GRAD_ROWS>(leader && ok, tmem + TG_ACC1, tmem + TG_P + 64 * (i & 1), b1, i > 0);
-            if (KEYS) mma_weights<T, DP, GRAD_ROWS>(leader && ok, tmem + TG_ACC2, tmem + TG_S + 64 * (i & 1), b1 + BBYTES, i > 0);
+            const uint32_t b1 = ring + used * 2 * BBYTES, x = 64 * (i & 1);
+            mma_weights<T, DP, GRAD_ROWS>(leader, tmem + TG_ACC1, tmem + TG_P + x, b1, i > 0);
+            if (KEYS) mma_weights<T, DP, GRAD_ROWS>(leader, tmem + TG_ACC2, tmem + TG_S + x, b1 + BBYTES, i > 0);
             tc_commit_by<false>(leader, bar_empty + used * 8);
             if (++used == STAGES) used = 0;
-            if (i + 2 < n) scores(i + 2);
+            if (i + 2 < n) ok = scores(i + 2);
         }
         if (n > 0) tc_commit_by<false>(leader, bar_done);
         if (!ok) {   // let the MMAs in flight retire before tensor memory goes away
@@ -239,21 +315,14 @@ grad_kernel(const __grid_constant__ CUtensorMap map_a1, const __grid_constant__ 
             }
         }
     } else if (warp >= 4) {
-        const int wg = (warp - 4) >> 2, ew = warp & 3;
-        const uint32_t lanes = (uint32_t)(ew * 32) << 16;
-        const int64_t r = row0 + ew * 32 + lane;   // key, or packed query row
         const float c = p.scale * kLog2e;
         const float factor = HALF ? grad_factor(__ldcg(p.gmax)) : 1.f;
-        float my_lse = 0.f, my_delta = 0.f;
-        bool live = KEYS ? r < p.len.n : r < p.queries * p.group;
-        int64_t t = 0;
-        int g = 0;
+        float mlse = 0.f, mdelta = 0.f;
         if (!KEYS && live) {
-            t = r / p.group;
-            g = (int)(r - t * p.group);
-            const float2 st = __ldcg(p.stat + unit * p.rt.tiles * GRAD_ROWS + p.rt.place((int)t, g));
-            my_lse = st.x;
-            my_delta = st.y * factor;
+            const int64_t place = p.rt.place(t, g);
+            const float* const st = p.stat + ((int64_t)unit * p.rt.tiles + place / GRAD_ROWS) * 2 * GRAD_ROWS + place % GRAD_ROWS;
+            mlse = __ldcg(st);
+            mdelta = __ldcg(st + GRAD_ROWS);
         }
         bool ok = true;
         for (int i = wg; i < n; i += 2) {
@@ -264,50 +333,44 @@ grad_kernel(const __grid_constant__ CUtensorMap map_a1, const __grid_constant__ 
             if (!ok) break;
             tc_fence_after();
             const uint32_t ts = tmem + TG_S + 64 * wg + lanes, tp = tmem + TG_P + 64 * wg + lanes;
-            const uint32_t stat = sbase + GRAD_SM_STAT<DP> + (i % STAGES) * GRAD_STAT_BYTES;
-            const int lim = KEYS ? GRAD_ROWS : (int)min(len - (first + i) * GRAD_ROWS, (int64_t)GRAD_ROWS);
-            uint32_t s[2][32], dp[2][32];
+            const uint32_t stat = sbase + GRAD_SM_STAT<DP, KEYS> + (i % STAGES) * GRAD_STAT_BYTES;
+            const int lim = KEYS ? GRAD_ROWS : (int)(len - (int64_t)(first + i) * GRAD_ROWS);
+            uint32_t s[2][32];
             tc_ld32(ts, s[0]);
-            tc_ld32(tp, dp[0]);
             tc_ld32(ts + 32, s[1]);
+            ok = waits(bar_d + wg * 8, (i >> 1) & 1);
+            if (!ok) break;
+            tc_fence_after();
+            uint32_t dp[2][32];
+            tc_ld32(tp, dp[0]);
+            tc_wait_ld32(s[0]);
+            tc_wait_ld32(s[1]);
+            tc_wait_ld32(dp[0]);
             tc_ld32(tp + 32, dp[1]);
 #pragma unroll
             for (int h = 0; h < 2; h++) {
-                tc_wait_ld32(s[h]);
-                tc_wait_ld32(dp[h]);
-            }
-#pragma unroll
-            for (int h = 0; h < 2; h++) {
                 uint32_t wp[16], ws[16];
+                if (h == 1) tc_wait_ld32(dp[1]);
+                grad32<T, KEYS>(s[h], dp[h], c, factor, stat + 32 * h * 4, mlse, mdelta, wp, ws);
+                if (!KEYS && lim < GRAD_ROWS) {   // keys behind the end
 #pragma unroll
-                for (int e = 0; e < 32; e += 2) {
-                    float l0 = my_lse, l1 = my_lse, d0 = my_delta, d1 = my_delta;
-                    if (KEYS) {
-                        const uint4 x = lds128(stat + (32 * h + e) * 8);
-                        l0 = __uint_as_float(x.x);
-                        d0 = __uint_as_float(x.y) * factor;
-                        l1 = __uint_as_float(x.z);
-                        d1 = __uint_as_float(x.w) * factor;
+                    for (int e = 0; e < 16; e++) {
+                        if (32 * h + 2 * e >= lim) ws[e] = 0;
+                        else if (32 * h + 2 * e + 1 >= lim) ws[e] &= 0xffffu;
                     }
-                    const float p0 = ex2(fmaf(__uint_as_float(s[h][e]), c, -l0)), p1 = ex2(fmaf(__uint_as_float(s[h][e + 1]), c, -l1));
-                    float s0 = p0 * fmaf(__uint_as_float(dp[h][e]), factor, -d0), s1 = p1 * fmaf(__uint_as_float(dp[h][e + 1]), factor, -d1);
-                    if (!KEYS) {
-                        if (32 * h + e >= lim) s0 = 0.f;
-                        if (32 * h + e + 1 >= lim) s1 = 0.f;
-                    }
-                    wp[e >> 1] = pack2<T>(p0, p1);
-                    ws[e >> 1] = pack2<T>(s0, s1);
                 }
                 if (KEYS) tc_st16(ts + 16 * h, wp);
+                // the second half's P' is in registers by now, or on its way to them: the first half's ds overwrites the first quarter
                 tc_st16(tp + 16 * h, ws);
             }
             tc_wait_st();
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(bar_p + wg * 8);
+            mbar_arrive_if(lane == 0, bar_p + wg * 8);
         }
         // ------------------------------ results: KEYS: a group of warps an accumulator, else half of its columns each
-        if (ok && n > 0) ok = __all_sync(0xffffffffu, wait(bar_done, 0));
+        if (ok && n > 0) ok = wait(bar_done, 0);
+        ok = __all_sync(0xffffffffu, ok);
         if (ok) {
             tc_fence_after();
             const bool zero = n == 0 || (KEYS && r >= len);
@@ -315,10 +378,12 @@ grad_kernel(const __grid_constant__ CUtensorMap map_a1, const __grid_constant__ 
             const int64_t at = KEYS ? ((b * p.len.n + r) * p.kv_heads + kvh) * p.d
                                     : ((b * p.queries + t) * p.heads + kvh * p.group + g) * p.d;
             const uint32_t acc = tmem + (KEYS && wg ? TG_ACC2 : TG_ACC1) + lanes;
-            constexpr int NCH = KEYS ? DP / 32 : DP / 64;
+            constexpr int COLS = KEYS ? DP : DP / 2;
+            const int col0 = KEYS ? 0 : wg * COLS;
+            uint8_t* const stage = smem + (warp - 4) * 32 * COLS * 2;   // tiles are done with
 #pragma unroll 1
-            for (int ch = 0; ch < NCH; ch++) {
-                const int col = 32 * (KEYS ? ch : wg * NCH + ch);
+            for (int ch = 0; ch < COLS / 32; ch++) {
+                const int col = col0 + 32 * ch;
                 uint32_t o[32];
                 if (n > 0) {
                     tc_ld32(acc + col, o);
@@ -326,24 +391,21 @@ grad_kernel(const __grid_constant__ CUtensorMap map_a1, const __grid_constant__ 
                 }
 #pragma unroll
                 for (int e = 0; e < 32; e++) o[e] = zero ? 0u : __float_as_uint(__uint_as_float(o[e]) * mul);
-                if (!live) continue;
-                if (p.part) {
+                if (!p.part) {
+                    stage_columns32<T, COLS>(stage, o, 4 * ch);
+                } else if (live) {
                     float* const po = p.part + sp * p.part_stride + (KEYS && wg ? p.part2 : 0) + at;
 #pragma unroll
-                    for (int e = 0; e < 32; e += 4)
-                        if (col + e < p.d) *reinterpret_cast<uint4*>(po + col + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
-                } else {
-                    uint16_t* const po = (KEYS && wg ? p.out2 : p.out1) + at;
-#pragma unroll
                     for (int e = 0; e < 32; e += 8)
-                        if (col + e < p.d)
-                            *reinterpret_cast<uint4*>(po + col + e) =
-                                    make_uint4(pack2<T>(__uint_as_float(o[e]), __uint_as_float(o[e + 1])),
-                                               pack2<T>(__uint_as_float(o[e + 2]), __uint_as_float(o[e + 3])),
-                                               pack2<T>(__uint_as_float(o[e + 4]), __uint_as_float(o[e + 5])),
-                                               pack2<T>(__uint_as_float(o[e + 6]), __uint_as_float(o[e + 7])));
+                        if (col + e < p.d) {
+                            const float v[8] = {__uint_as_float(o[e]),     __uint_as_float(o[e + 1]), __uint_as_float(o[e + 2]),
+                                                __uint_as_float(o[e + 3]), __uint_as_float(o[e + 4]), __uint_as_float(o[e + 5]),
+                                                __uint_as_float(o[e + 6]), __uint_as_float(o[e + 7])};
+                            st_global_v8(po + col + e, v);
+                        }
                 }
             }
+            if (!p.part) store_rows<COLS>(stage, KEYS && wg ? p.out2 : p.out1, live ? at : -1, col0, p.d);
         }
     }
     tc_fence_before();
@@ -355,7 +417,7 @@ grad_kernel(const __grid_constant__ CUtensorMap map_a1, const __grid_constant__ 
 // ---- grad_stat_kernel: what the gradients need of every query row, 16 lanes a slot ----------------------
 template <typename T>
 __global__ void __launch_bounds__(256) grad_stat_kernel(AttView g, const uint16_t* out, const float* lse, RowTiles rt, int64_t units, int heads,
-                                                        int kv_heads, int d, float2* stat, uint32_t* gmax) {
+                                                        int kv_heads, int d, float* stat, uint32_t* gmax) {
     const int sub = threadIdx.x & 15;
     const int64_t i = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
     const bool in = i < units * rt.tiles * rt.slots;
@@ -383,7 +445,9 @@ __global__ void __launch_bounds__(256) grad_stat_kernel(AttView g, const uint16_
     for (int o = 8; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
     if (in && sub == 0) {
         const float l = live ? lse[row] * kLog2e : CUDART_INF_F;
-        stat[i] = make_float2(l == -CUDART_INF_F ? CUDART_INF_F : l, live ? dot : 0.f);
+        float* const st = stat + tile_of * 2 * rt.slots + i % rt.slots;
+        st[0] = l == -CUDART_INF_F ? l : -l;   // -INF either way where nothing is to be seen
+        st[rt.slots] = live ? -dot : 0.f;
     }
     if (gmax) {   // the largest finite one; the order does not matter
         if (top >= 0x7f800000u) top = 0;
@@ -454,10 +518,10 @@ int launch_grad(const CUtensorMap* maps, const GradParams& p, int64_t items, cud
     static bool attr_set[kMaxDevices] = {false};
     const int slot = device_slot();
     if (!attr_set[slot]) {
-        B200F_CUDA_TRY(cudaFuncSetAttribute(grad_kernel<T, DP, KEYS>, cudaFuncAttributeMaxDynamicSharedMemorySize, GRAD_SMEM<DP>));
+        B200F_CUDA_TRY(cudaFuncSetAttribute(grad_kernel<T, DP, KEYS>, cudaFuncAttributeMaxDynamicSharedMemorySize, GRAD_SMEM<DP, KEYS>));
         attr_set[slot] = true;
     }
-    const cudaError_t e = launch_kernel(grad_kernel<T, DP, KEYS>, dim3((unsigned)items), GRAD_THREADS, GRAD_SMEM<DP>, Launch(st), maps[0],
+    const cudaError_t e = launch_kernel(grad_kernel<T, DP, KEYS>, dim3((unsigned)items), GRAD_THREADS, GRAD_SMEM<DP, KEYS>, Launch(st), maps[0],
                                         maps[1], maps[2], maps[3], p);
     if (e != cudaSuccess) {
         (void)cudaGetLastError();
@@ -468,7 +532,7 @@ int launch_grad(const CUtensorMap* maps, const GradParams& p, int64_t items, cud
 }
 
 template <typename T>
-int launch_backward(const B200FAttendBackwardArgs& a, const GradPlan& pl, GradParams p, const uint16_t* out, float2* stat, uint32_t* gmax,
+int launch_backward(const B200FAttendBackwardArgs& a, const GradPlan& pl, GradParams p, const uint16_t* out, float* stat, uint32_t* gmax,
                     float* part, const AttView& k, const AttView& v) {
     const cudaStream_t st = (cudaStream_t)a.stream;
     const bool wide = a.d > 64;
@@ -566,7 +630,7 @@ extern "C" int b200f_attend_backward(const B200FAttendBackwardArgs* a) {
         return B200F_ERR_UNSUPPORTED;
     uint8_t* const scratch = static_cast<uint8_t*>(a->scratch);
     uint32_t* const gmax = a->storage == B200F_STORAGE_F16 ? reinterpret_cast<uint32_t*>(scratch) : nullptr;
-    float2* const stat = reinterpret_cast<float2*>(scratch + 256);
+    float* const stat = reinterpret_cast<float*>(scratch + 256);
     float* const part = reinterpret_cast<float*>(scratch + 256 + pl.stat_bytes);
     GradParams p{};
     p.q = q;

@@ -130,6 +130,20 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
     return d;
 }
 
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n\t"
+        ".reg .b64 a, b, d;\n\t"
+        "mov.b64 a, {%2, %3};\n\t"
+        "mov.b64 b, {%4, %5};\n\t"
+        "mul.rn.f32x2 d, a, b;\n\t"
+        "mov.b64 {%0, %1}, d;\n\t"
+        "}\n"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -226,6 +240,17 @@ __device__ __forceinline__ void mma_rows(bool leader, uint32_t d_tmem, uint32_t 
             tc_mma_f16_by<false>(leader, d_tmem, da + 2 * k, db + 2 * k, att_idesc<T>(N, false), c + k > 0);
     }
 }
+// The same with A [128][DP] in tensor memory.
+template <typename T, int DP, int N>
+__device__ __forceinline__ void mma_rows_ts(bool leader, uint32_t d_tmem, uint32_t a_tmem, uint32_t b_smem) {
+#pragma unroll
+    for (int c = 0; c < DP / 64; c++) {
+        const uint64_t db = make_smem_desc(b_smem + c * (N * 128));
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+            tc_mma_ts_by(leader, d_tmem, a_tmem + 32 * c + 8 * k, db + 2 * k, att_idesc<T>(N, false), c + k > 0);
+    }
+}
 // D[128][DP] (+)= P B over the K rows of the tile B; P [128][K] in tensor memory.
 template <typename T, int DP, int K>
 __device__ __forceinline__ void mma_weights(bool leader, uint32_t d_tmem, uint32_t p_tmem, uint32_t b_smem, bool accumulate) {
@@ -233,6 +258,36 @@ __device__ __forceinline__ void mma_weights(bool leader, uint32_t d_tmem, uint32
 #pragma unroll
     for (int k = 0; k < K / 16; k++)
         tc_mma_ts_by(leader, d_tmem, p_tmem + 8 * k, db + 128 * k, att_idesc<T>(DP, true), accumulate || k > 0);
+}
+
+// 32 rows of COLS 16-bit elements that a warp has put into `stage` (row r's 16-byte piece c at piece c ^ (r & 7)) go to global memory
+// as whole rows: row r to dst + at, its lane r's `at` (negative: nowhere), d elements of it from column col on.
+template <int COLS>
+__device__ __forceinline__ void store_rows(const uint8_t* stage, uint16_t* dst, int64_t at, int col, int d) {
+    constexpr int PER_ROW = COLS / 8;
+    const int lane = threadIdx.x & 31, piece = lane % PER_ROW;
+    __syncwarp();
+#pragma unroll 4
+    for (int r = lane / PER_ROW; r < 32; r += 32 / PER_ROW) {
+        const int64_t to = __shfl_sync(0xffffffffu, at, r);
+        if (to >= 0 && col + piece * 8 < d)
+            *reinterpret_cast<uint4*>(dst + to + col + piece * 8) =
+                    *reinterpret_cast<const uint4*>(stage + r * (COLS * 2) + ((piece ^ (r & (PER_ROW < 8 ? PER_ROW - 1 : 7))) << 4));
+    }
+    __syncwarp();
+}
+// 32 of a lane's columns, from piece c0 on, to that stage
+template <typename T, int COLS>
+__device__ __forceinline__ void stage_columns32(uint8_t* stage, const uint32_t (&o)[32], int c0) {
+    constexpr int PER_ROW = COLS / 8;
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int e = 0; e < 4; e++)
+        *reinterpret_cast<uint4*>(stage + lane * (COLS * 2) + (((c0 + e) ^ (lane & (PER_ROW < 8 ? PER_ROW - 1 : 7))) << 4)) =
+                make_uint4(pack2<T>(__uint_as_float(o[8 * e]), __uint_as_float(o[8 * e + 1])),
+                           pack2<T>(__uint_as_float(o[8 * e + 2]), __uint_as_float(o[8 * e + 3])),
+                           pack2<T>(__uint_as_float(o[8 * e + 4]), __uint_as_float(o[8 * e + 5])),
+                           pack2<T>(__uint_as_float(o[8 * e + 6]), __uint_as_float(o[8 * e + 7])));
 }
 
 // Rows [first, rows) of a tile in shared memory become zero; a warp calls it.
