@@ -44,7 +44,7 @@ constexpr uint32_t TG_S = 0, TG_P = 128, TG_ACC1 = 256, TG_ACC2 = 384;   // S an
 constexpr uint32_t TG_A1 = 384, TG_A2 = 448;                             // not KEYS
 
 struct GradParams {
-    AttMap a1m, a2m, b1m, b2m;
+    AttMap km, vm, qm, gm;
     AttView q, g;            // queries and output gradients (KEYS = false: A1 and A2 are read with plain loads)
     AttLengths len;
     RowTiles rt;             // query rows in tiles of GRAD_ROWS
@@ -116,10 +116,9 @@ __device__ __forceinline__ void grad32(const uint32_t (&s)[32], const uint32_t (
 }
 
 template <typename T, int DP, bool KEYS>
-__global__ void __launch_bounds__(GRAD_THREADS, 1)
-grad_kernel(const __grid_constant__ CUtensorMap map_a1, const __grid_constant__ CUtensorMap map_a2,
-            const __grid_constant__ CUtensorMap map_b1, const __grid_constant__ CUtensorMap map_b2, const GradParams p) {
-    extern __shared__ __align__(1024) uint8_t smem[];
+__device__ __forceinline__ void grad_item(const CUtensorMap& map_k, const CUtensorMap& map_v, const CUtensorMap& map_q, const CUtensorMap& map_g,
+                                          const GradParams& p, uint8_t* smem, uint32_t item) {
+    const CUtensorMap &map_b1 = KEYS ? map_q : map_k, &map_b2 = KEYS ? map_g : map_v;
     constexpr int STAGES = GRAD_STAGES<DP, KEYS>, ABYTES = GRAD_A_BYTES<DP>, BBYTES = GRAD_B_BYTES<DP>, CHUNKS = DP / 64;
     constexpr int RING = GRAD_SM_RING<DP, KEYS>;
     constexpr bool HALF = std::is_same<T, __half>::value;
@@ -132,14 +131,8 @@ grad_kernel(const __grid_constant__ CUtensorMap map_a1, const __grid_constant__ 
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_ptr + 1);
     const uint32_t ring = sbase + RING;
 
-    pdl_wait();
-    pdl_trigger();
-    if ((sbase & 1023u) != 0) {
-        if (threadIdx.x == 0) atomicOr(p.status, kDevErrSmemAlign);
-        return;
-    }
     // ---- this CTA's item: a block of 128 rows of A, a range of B's tiles
-    const uint32_t rest = blockIdx.x / (uint32_t)p.blocks, blk = blockIdx.x - rest * (uint32_t)p.blocks;
+    const uint32_t rest = item / (uint32_t)p.blocks, blk = item - rest * (uint32_t)p.blocks;
     const uint32_t unit = rest / (uint32_t)p.splits;
     const int sp = (int)(rest - unit * p.splits);
     const int64_t b = unit / (uint32_t)p.kv_heads;
@@ -151,6 +144,25 @@ grad_kernel(const __grid_constant__ CUtensorMap map_a1, const __grid_constant__ 
     const int first = (int)min(tiles, per * sp);
     const int n = (int)min(tiles - first, per);
 
+    if (n == 0) {   // nothing is seen: zeros
+        const int vecs = p.d / 8, piece = threadIdx.x % vecs;
+        for (int x = threadIdx.x / vecs; x < 128; x += GRAD_THREADS / vecs) {
+            const int64_t row = row0 + x;
+            if (threadIdx.x >= GRAD_THREADS / vecs * vecs || row >= (KEYS ? p.len.n : (int64_t)p.queries * p.group)) break;
+            const uint32_t t = (uint32_t)row / (uint32_t)p.group, g = (uint32_t)row - t * (uint32_t)p.group;
+            const int64_t at = (KEYS ? ((b * p.len.n + row) * p.kv_heads + kvh) * p.d
+                                     : ((b * p.queries + t) * p.heads + kvh * p.group + g) * p.d) + piece * 8;
+            const float none[8] = {};
+            if (p.part) {
+                st_global_v8(p.part + sp * p.part_stride + at, none);
+                if (KEYS) st_global_v8(p.part + sp * p.part_stride + p.part2 + at, none);
+            } else {
+                *reinterpret_cast<uint4*>(p.out1 + at) = make_uint4(0, 0, 0, 0);
+                if (KEYS) *reinterpret_cast<uint4*>(p.out2 + at) = make_uint4(0, 0, 0, 0);
+            }
+        }
+        return;
+    }
     if (threadIdx.x == 0) {
         *abort_flag = 0;
         for (int s = 0; s < STAGES; s++) {
@@ -195,7 +207,7 @@ grad_kernel(const __grid_constant__ CUtensorMap map_a1, const __grid_constant__ 
         t = (int)((uint32_t)r / (uint32_t)p.group);
         g = (int)((uint32_t)r - (uint32_t)t * p.group);
     }
-    if (!KEYS && n > 0) {
+    if (!KEYS) {
         // A1 and A2 to tensor memory: four warps each, a row a thread
         if (warp >= 4) {
             const AttView& src = wg ? p.g : p.q;
@@ -222,15 +234,17 @@ grad_kernel(const __grid_constant__ CUtensorMap map_a1, const __grid_constant__ 
     }
 
     if (warp == 0) {
-        if (elect_one() && n > 0) {
+        if (elect_one()) {
             bool ok = true;
             if (KEYS) {
                 mbar_arrive_expect_tx(bar_a, 2 * ABYTES);
-                for (int c = 0; c < CHUNKS; c++) {
-                    tma_load_4d(sbase + c * ATT_CHUNK, &map_a1, bar_a, c * 64, (int)row0, kvh * p.a1m.head_step, (int)b * p.a1m.batch_step);
-                    tma_load_4d(sbase + ABYTES + c * ATT_CHUNK, &map_a2, bar_a, c * 64, (int)row0, kvh * p.a2m.head_step,
-                                (int)b * p.a2m.batch_step);
-                }
+                for (int c = 0; c < CHUNKS; c++)
+                    for (int h = 0; h < 128; h += GRAD_ROWS) {
+                        tma_load_4d(sbase + c * ATT_CHUNK + h * 128, &map_k, bar_a, c * 64, (int)row0 + h, kvh * p.km.head_step,
+                                    (int)b * p.km.batch_step);
+                        tma_load_4d(sbase + ABYTES + c * ATT_CHUNK + h * 128, &map_v, bar_a, c * 64, (int)row0 + h, kvh * p.vm.head_step,
+                                    (int)b * p.vm.batch_step);
+                    }
             }
             const uint32_t bytes = KEYS ? 2 * CHUNKS * p.rt.gb * p.rt.bt * 128 + GRAD_STAT_BYTES : 2 * BBYTES;
             int slot = 0;
@@ -244,19 +258,19 @@ grad_kernel(const __grid_constant__ CUtensorMap map_a1, const __grid_constant__ 
                 if (KEYS) {
                     const int block = tile / p.rt.gchunks, g0 = (tile - block * p.rt.gchunks) * p.rt.gb, t0 = block * p.rt.bt;
                     for (int c = 0; c < CHUNKS; c++) {
-                        tma_load_5d(b1 + c * GRAD_ROWS * 128, &map_b1, full, c * 64, g0, t0, kvh * p.b1m.head_step,
-                                    (int)b * p.b1m.batch_step);
-                        tma_load_5d(b2 + c * GRAD_ROWS * 128, &map_b2, full, c * 64, g0, t0, kvh * p.b2m.head_step,
-                                    (int)b * p.b2m.batch_step);
+                        tma_load_5d(b1 + c * GRAD_ROWS * 128, &map_b1, full, c * 64, g0, t0, kvh * p.qm.head_step,
+                                    (int)b * p.qm.batch_step);
+                        tma_load_5d(b2 + c * GRAD_ROWS * 128, &map_b2, full, c * 64, g0, t0, kvh * p.gm.head_step,
+                                    (int)b * p.gm.batch_step);
                     }
                     bulk_load(sbase + GRAD_SM_STAT<DP, KEYS> + slot * GRAD_STAT_BYTES,
                               p.stat + ((int64_t)unit * p.rt.tiles + tile) * 2 * GRAD_ROWS, GRAD_STAT_BYTES, full);
                 } else {
                     for (int c = 0; c < CHUNKS; c++) {
-                        tma_load_4d(b1 + c * GRAD_ROWS * 128, &map_b1, full, c * 64, tile * GRAD_ROWS, kvh * p.b1m.head_step,
-                                    (int)b * p.b1m.batch_step);
-                        tma_load_4d(b2 + c * GRAD_ROWS * 128, &map_b2, full, c * 64, tile * GRAD_ROWS, kvh * p.b2m.head_step,
-                                    (int)b * p.b2m.batch_step);
+                        tma_load_4d(b1 + c * GRAD_ROWS * 128, &map_b1, full, c * 64, tile * GRAD_ROWS, kvh * p.km.head_step,
+                                    (int)b * p.km.batch_step);
+                        tma_load_4d(b2 + c * GRAD_ROWS * 128, &map_b2, full, c * 64, tile * GRAD_ROWS, kvh * p.vm.head_step,
+                                    (int)b * p.vm.batch_step);
                     }
                 }
                 if (++slot == STAGES) {
@@ -274,7 +288,7 @@ grad_kernel(const __grid_constant__ CUtensorMap map_a1, const __grid_constant__ 
     } else if (warp == 1) {
         // every wait is voted on: control flow stays uniform
         const bool leader = elect_one();
-        bool ok = !KEYS || n == 0 || waits(bar_a, 0);
+        bool ok = !KEYS || waits(bar_a, 0);
         const int tail = (int)(len & (GRAD_ROWS - 1));
         const int boundary = !KEYS && len < p.len.n && tail ? (int)(len / GRAD_ROWS) - first : -1;
         int slot = 0, used = 0;
@@ -296,7 +310,7 @@ grad_kernel(const __grid_constant__ CUtensorMap map_a1, const __grid_constant__ 
             }
             return true;
         };
-        ok = ok && (n < 1 || scores(0)) && (n < 2 || scores(1));
+        ok = ok && scores(0) && (n < 2 || scores(1));
         for (int i = 0; i < n && ok; i++) {
             ok = waits(bar_p + (i & 1) * 8, (i >> 1) & 1);
             if (!ok) break;
@@ -308,7 +322,7 @@ grad_kernel(const __grid_constant__ CUtensorMap map_a1, const __grid_constant__ 
             if (++used == STAGES) used = 0;
             if (i + 2 < n) ok = scores(i + 2);
         }
-        if (n > 0) tc_commit_by<false>(leader, bar_done);
+        tc_commit_by<false>(leader, bar_done);
         if (!ok) {   // let the MMAs in flight retire before tensor memory goes away
             const long long t0 = clock64();
             while (clock64() - t0 < 200000LL) {
@@ -369,11 +383,11 @@ grad_kernel(const __grid_constant__ CUtensorMap map_a1, const __grid_constant__ 
             mbar_arrive_if(lane == 0, bar_p + wg * 8);
         }
         // ------------------------------ results: KEYS: a group of warps an accumulator, else half of its columns each
-        if (ok && n > 0) ok = wait(bar_done, 0);
+        if (ok) ok = wait(bar_done, 0);
         ok = __all_sync(0xffffffffu, ok);
         if (ok) {
             tc_fence_after();
-            const bool zero = n == 0 || (KEYS && r >= len);
+            const bool zero = KEYS && r >= len;
             const float mul = (KEYS && wg == 1) ? 1.f : p.scale / factor;
             const int64_t at = KEYS ? ((b * p.len.n + r) * p.kv_heads + kvh) * p.d
                                     : ((b * p.queries + t) * p.heads + kvh * p.group + g) * p.d;
@@ -385,10 +399,8 @@ grad_kernel(const __grid_constant__ CUtensorMap map_a1, const __grid_constant__ 
             for (int ch = 0; ch < COLS / 32; ch++) {
                 const int col = col0 + 32 * ch;
                 uint32_t o[32];
-                if (n > 0) {
-                    tc_ld32(acc + col, o);
-                    tc_wait_ld32(o);
-                }
+                tc_ld32(acc + col, o);
+                tc_wait_ld32(o);
 #pragma unroll
                 for (int e = 0; e < 32; e++) o[e] = zero ? 0u : __float_as_uint(__uint_as_float(o[e]) * mul);
                 if (!p.part) {
@@ -412,6 +424,23 @@ grad_kernel(const __grid_constant__ CUtensorMap map_a1, const __grid_constant__ 
     __syncthreads();
     if (warp == 1)
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS) : "memory");
+}
+
+// Items of the keys first, which take longest, then those of the query rows: one launch, one tail.
+template <typename T, int DP>
+__global__ void __launch_bounds__(GRAD_THREADS, 1)
+grad_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_q,
+            const __grid_constant__ CUtensorMap map_g, const __grid_constant__ GradParams keys, const __grid_constant__ GradParams rows,
+            uint32_t key_items) {
+    extern __shared__ __align__(1024) uint8_t smem[];
+    pdl_wait();
+    pdl_trigger();
+    if ((smem_u32(smem) & 1023u) != 0) {
+        if (threadIdx.x == 0) atomicOr(keys.status, kDevErrSmemAlign);
+        return;
+    }
+    if (blockIdx.x < key_items) grad_item<T, DP, true>(map_k, map_v, map_q, map_g, keys, smem, blockIdx.x);
+    else grad_item<T, DP, false>(map_k, map_v, map_q, map_g, rows, smem, blockIdx.x - key_items);
 }
 
 // ---- grad_stat_kernel: what the gradients need of every query row, 16 lanes a slot ----------------------
@@ -482,7 +511,7 @@ struct GradPlan {
     RowTiles rt;
     int64_t key_blocks, row_blocks;
     int key_splits, row_splits;
-    size_t stat_bytes, part_bytes, scratch;
+    size_t stat_bytes, key_part_bytes, scratch;
 };
 // Ranges of the streamed tiles: as many as fill the SMs once, of at least MIN_TILES tiles of 64 rows.
 constexpr int MIN_TILES = 4;
@@ -493,18 +522,18 @@ GradPlan plan_grad(const B200FAttendBackwardArgs& a) {
     pl.rt = row_tiles(GRAD_ROWS, a.queries, group);
     pl.key_blocks = ceil_div64(a.n, 128);
     pl.row_blocks = ceil_div64(a.queries * group, 128);
-    auto splits = [&](int64_t items, int64_t tiles) {
-        int64_t s = items > 0 ? sm / items : 1;
+    const int64_t both = units * (pl.key_blocks + pl.row_blocks);
+    auto splits = [&](int64_t tiles) {
+        int64_t s = both > 0 ? sm / both : 1;
         if (s > tiles / MIN_TILES) s = tiles / MIN_TILES;
         return (int)(s < 1 ? 1 : s);
     };
-    pl.key_splits = splits(units * pl.key_blocks, pl.rt.tiles);
-    pl.row_splits = splits(units * pl.row_blocks, ceil_div64(a.n, GRAD_ROWS));
+    pl.key_splits = splits(pl.rt.tiles);
+    pl.row_splits = splits(ceil_div64(a.n, GRAD_ROWS));
     pl.stat_bytes = (size_t)round_up64(units * pl.rt.tiles * GRAD_ROWS * 8, 256);
     const int64_t keys = units * a.n * a.d, rows = a.batch * a.queries * a.heads * a.d;
-    size_t kp = pl.key_splits > 1 ? (size_t)pl.key_splits * 2 * keys * 4 : 0, rp = pl.row_splits > 1 ? (size_t)pl.row_splits * rows * 4 : 0;
-    pl.part_bytes = kp > rp ? kp : rp;   // one after the other
-    pl.scratch = 256 + pl.stat_bytes + pl.part_bytes;
+    pl.key_part_bytes = pl.key_splits > 1 ? (size_t)round_up64(pl.key_splits * 2 * keys * 4, 256) : 0;
+    pl.scratch = 256 + pl.stat_bytes + pl.key_part_bytes + (pl.row_splits > 1 ? (size_t)pl.row_splits * rows * 4 : 0);
     return pl;
 }
 
@@ -513,16 +542,17 @@ int check_grad(const B200FAttendBackwardArgs* a) {
     return att_sizes_ok(a->batch, a->queries, a->n, a->heads, a->kv_heads, a->d, a->storage, a->scale);
 }
 
-template <typename T, int DP, bool KEYS>
-int launch_grad(const CUtensorMap* maps, const GradParams& p, int64_t items, cudaStream_t st) {
+template <typename T, int DP>
+int launch_grad(const CUtensorMap* maps, const GradParams& keys, const GradParams& rows, int64_t key_items, int64_t row_items, cudaStream_t st) {
+    constexpr int SMEM = GRAD_SMEM<DP, true> > GRAD_SMEM<DP, false> ? GRAD_SMEM<DP, true> : GRAD_SMEM<DP, false>;
     static bool attr_set[kMaxDevices] = {false};
     const int slot = device_slot();
     if (!attr_set[slot]) {
-        B200F_CUDA_TRY(cudaFuncSetAttribute(grad_kernel<T, DP, KEYS>, cudaFuncAttributeMaxDynamicSharedMemorySize, GRAD_SMEM<DP, KEYS>));
+        B200F_CUDA_TRY(cudaFuncSetAttribute(grad_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM));
         attr_set[slot] = true;
     }
-    const cudaError_t e = launch_kernel(grad_kernel<T, DP, KEYS>, dim3((unsigned)items), GRAD_THREADS, GRAD_SMEM<DP, KEYS>, Launch(st), maps[0],
-                                        maps[1], maps[2], maps[3], p);
+    const cudaError_t e = launch_kernel(grad_kernel<T, DP>, dim3((unsigned)(key_items + row_items)), GRAD_THREADS, SMEM, Launch(st), maps[0],
+                                        maps[1], maps[2], maps[3], keys, rows, (uint32_t)key_items);
     if (e != cudaSuccess) {
         (void)cudaGetLastError();
         return B200F_ERR_CUDA;
@@ -535,19 +565,46 @@ template <typename T>
 int launch_backward(const B200FAttendBackwardArgs& a, const GradPlan& pl, GradParams p, const uint16_t* out, float* stat, uint32_t* gmax,
                     float* part, const AttView& k, const AttView& v) {
     const cudaStream_t st = (cudaStream_t)a.stream;
-    const bool wide = a.d > 64;
-    int rc = B200F_OK;
+    const int64_t units = a.batch * a.kv_heads;
     if (pl.rt.tiles > 0) {
         if (gmax) B200F_CUDA_TRY(cudaMemsetAsync(gmax, 0, 4, st));
-        const int64_t slots = a.batch * a.kv_heads * pl.rt.tiles * GRAD_ROWS;
-        grad_stat_kernel<T><<<(unsigned)ceil_div64(slots, 16), 256, 0, st>>>(p.g, out, a.lse, pl.rt, a.batch * a.kv_heads, a.heads, a.kv_heads,
-                                                                           a.d, stat, gmax);
+        const int64_t slots = units * pl.rt.tiles * GRAD_ROWS;
+        grad_stat_kernel<T><<<(unsigned)ceil_div64(slots, 16), 256, 0, st>>>(p.g, out, a.lse, pl.rt, units, a.heads, a.kv_heads, a.d, stat, gmax);
         count_launch();
         B200F_LAUNCH_CHECK();
     }
-    auto join = [&](int splits, int64_t n1, int64_t n2, void* o1, void* o2) {
-        const cudaError_t e = launch_kernel(grad_join_kernel<T>, dim3((unsigned)ceil_div64((n1 + n2) / 4, 256)), 256, 0, Launch(st, true), part,
-                                            splits, n1 + n2, n1, n2, static_cast<uint16_t*>(o1), static_cast<uint16_t*>(o2));
+    CUtensorMap maps[4] = {};
+    int rc = B200F_OK;
+    if (a.n > 0) {
+        rc = make_rows_map(&maps[0], &p.km, k, a.storage, a.d, a.n, a.kv_heads, a.batch, GRAD_ROWS);
+        if (rc == B200F_OK) rc = make_rows_map(&maps[1], &p.vm, v, a.storage, a.d, a.n, a.kv_heads, a.batch, GRAD_ROWS);
+    }
+    if (rc == B200F_OK && a.queries > 0) {
+        rc = make_queries_map(&maps[2], &p.qm, p.q, a.storage, a.d, pl.rt, a.kv_heads, a.batch);
+        if (rc == B200F_OK) rc = make_queries_map(&maps[3], &p.gm, p.g, a.storage, a.d, pl.rt, a.kv_heads, a.batch);
+    }
+    if (rc != B200F_OK) return rc;
+    const int64_t keys = units * a.n * a.d, rows = a.batch * a.queries * a.heads * a.d;
+    GradParams pk = p, pr = p;
+    pk.splits = pl.key_splits;
+    pk.blocks = pl.key_blocks;
+    pk.out1 = static_cast<uint16_t*>(a.grad_k);
+    pk.out2 = static_cast<uint16_t*>(a.grad_v);
+    pk.part = pl.key_splits > 1 ? part : nullptr;
+    pk.part_stride = 2 * keys;
+    pk.part2 = keys;
+    pr.splits = pl.row_splits;
+    pr.blocks = pl.row_blocks;
+    pr.out1 = static_cast<uint16_t*>(a.grad_q);
+    pr.out2 = nullptr;
+    pr.part = pl.row_splits > 1 ? part + pl.key_part_bytes / 4 : nullptr;
+    pr.part_stride = rows;
+    pr.part2 = 0;
+    rc = a.d > 64 ? launch_grad<T, 128>(maps, pk, pr, units * pl.key_blocks * pl.key_splits, units * pl.row_blocks * pl.row_splits, st)
+                  : launch_grad<T, 64>(maps, pk, pr, units * pl.key_blocks * pl.key_splits, units * pl.row_blocks * pl.row_splits, st);
+    auto join = [&](const GradParams& q, int64_t n1, int64_t n2) {
+        const cudaError_t e = launch_kernel(grad_join_kernel<T>, dim3((unsigned)ceil_div64((n1 + n2) / 4, 256)), 256, 0, Launch(st),
+                                            static_cast<const float*>(q.part), q.splits, n1 + n2, n1, n2, q.out1, q.out2);
         if (e != cudaSuccess) {
             (void)cudaGetLastError();
             return B200F_ERR_CUDA;
@@ -555,46 +612,8 @@ int launch_backward(const B200FAttendBackwardArgs& a, const GradPlan& pl, GradPa
         count_launch();
         return B200F_OK;
     };
-    const int64_t units = a.batch * a.kv_heads;
-    if (a.n > 0) {
-        CUtensorMap maps[4] = {};
-        rc = make_rows_map(&maps[0], &p.a1m, k, a.storage, a.d, a.n, a.kv_heads, a.batch);
-        if (rc == B200F_OK) rc = make_rows_map(&maps[1], &p.a2m, v, a.storage, a.d, a.n, a.kv_heads, a.batch);
-        if (rc == B200F_OK && a.queries > 0) rc = make_queries_map(&maps[2], &p.b1m, p.q, a.storage, a.d, pl.rt, a.kv_heads, a.batch);
-        if (rc == B200F_OK && a.queries > 0) rc = make_queries_map(&maps[3], &p.b2m, p.g, a.storage, a.d, pl.rt, a.kv_heads, a.batch);
-        if (rc != B200F_OK) return rc;
-        const int64_t keys = units * a.n * a.d;
-        p.splits = pl.key_splits;
-        p.blocks = pl.key_blocks;
-        p.out1 = static_cast<uint16_t*>(a.grad_k);
-        p.out2 = static_cast<uint16_t*>(a.grad_v);
-        p.part = pl.key_splits > 1 ? part : nullptr;
-        p.part_stride = 2 * keys;
-        p.part2 = keys;
-        const int64_t items = units * pl.key_blocks * pl.key_splits;
-        rc = wide ? launch_grad<T, 128, true>(maps, p, items, st) : launch_grad<T, 64, true>(maps, p, items, st);
-        if (rc == B200F_OK && p.part) rc = join(p.splits, keys, keys, a.grad_k, a.grad_v);
-        if (rc != B200F_OK) return rc;
-    }
-    if (a.queries > 0) {
-        CUtensorMap maps[4] = {};
-        if (a.n > 0) {
-            rc = make_rows_map(&maps[2], &p.b1m, k, a.storage, a.d, a.n, a.kv_heads, a.batch, GRAD_ROWS);
-            if (rc == B200F_OK) rc = make_rows_map(&maps[3], &p.b2m, v, a.storage, a.d, a.n, a.kv_heads, a.batch, GRAD_ROWS);
-            if (rc != B200F_OK) return rc;
-        }
-        const int64_t rows = a.batch * a.queries * a.heads * a.d;
-        p.splits = pl.row_splits;
-        p.blocks = pl.row_blocks;
-        p.out1 = static_cast<uint16_t*>(a.grad_q);
-        p.out2 = nullptr;
-        p.part = pl.row_splits > 1 ? part : nullptr;
-        p.part_stride = rows;
-        p.part2 = 0;
-        const int64_t items = units * pl.row_blocks * pl.row_splits;
-        rc = wide ? launch_grad<T, 128, false>(maps, p, items, st) : launch_grad<T, 64, false>(maps, p, items, st);
-        if (rc == B200F_OK && p.part) rc = join(p.splits, rows, 0, a.grad_q, nullptr);
-    }
+    if (rc == B200F_OK && pk.part) rc = join(pk, keys, keys);
+    if (rc == B200F_OK && pr.part) rc = join(pr, rows, 0);
     return rc;
 }
 
@@ -625,7 +644,7 @@ extern "C" int b200f_attend_backward(const B200FAttendBackwardArgs* a) {
     const GradPlan pl = plan_grad(*a);
     if (!a->scratch || (reinterpret_cast<uintptr_t>(a->scratch) & 255) != 0 || a->scratch_bytes < pl.scratch) return B200F_ERR_SCRATCH;
     const int64_t units = a->batch * a->kv_heads, lim = 0x7fffffff;
-    if (units * pl.key_blocks * pl.key_splits > lim || units * pl.row_blocks * pl.row_splits > lim ||
+    if (units * pl.key_blocks * pl.key_splits + units * pl.row_blocks * pl.row_splits > lim ||
         units * pl.rt.tiles * GRAD_ROWS / 16 > lim || units * a->n * a->d / 512 > lim)
         return B200F_ERR_UNSUPPORTED;
     uint8_t* const scratch = static_cast<uint8_t*>(a->scratch);
