@@ -177,7 +177,7 @@ def _run(plan, args, addresses: int, unused_scratch: int = 0):
         raise ValueError("%s: operands must lie on 16-byte boundaries" % plan.what)
     if (_status_word or _status())[0]:
         check_attention_status(synchronize=False)
-    if torch.cuda.current_device() != plan.index:
+    if torch._C._cuda_getDevice() != plan.index:
         with torch.cuda.device(plan.index):
             return _run(plan, args, 0, unused_scratch)
     args.stream = torch._C._cuda_getCurrentRawStream(plan.index)
@@ -187,6 +187,25 @@ def _run(plan, args, addresses: int, unused_scratch: int = 0):
     status = plan.fn(ctypes.byref(args))
     if status:
         abi.check_op(status, plan.what)
+
+
+def _dense_strides(shape):
+    out, n = [], 1
+    for s in reversed(shape):
+        out.append(n)
+        n *= max(int(s), 1)
+    return tuple(reversed(out))
+
+
+class _Output:
+    """A dense output of a plan, allocated with as little work as torch asks for."""
+
+    def __init__(self, shape, dtype, device):
+        self.shape, self.strides, self.dtype, self.device = tuple(shape), _dense_strides(shape), dtype, device
+
+    def __call__(self):
+        import torch
+        return torch.empty_strided(self.shape, self.strides, dtype=self.dtype, device=self.device)
 
 
 _NO_SCRATCH = 256   # scratch sizes up to this are not used by attend and attention_mass
@@ -226,9 +245,10 @@ def attend(q, k, v, *, key_lengths=None, scale=None, return_lse=False):
         c.lengths(key_lengths, b)
         _sizes(a, b, t, n, h, hk, d, c.storage, c.scale(scale, d))
         plan = _keep(key, c.plan(a, "b200f_attend"))
+        plan.out, plan.lse = _Output(q.shape, c.dtype, c.device), _Output((b, t, h), torch.float32, c.device)
     a = abi.AttendArgs.from_buffer_copy(plan.proto)
-    out = torch.empty(q.shape, dtype=plan.dtype, device=plan.device)
-    lse = torch.empty(q.shape[:3], dtype=torch.float32, device=plan.device) if return_lse else None
+    out = plan.out()
+    lse = plan.lse() if return_lse else None
     a.q, a.k, a.v, a.out = pq, pk, pv, _ = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()
     a.key_lengths = key_lengths.data_ptr() if key_lengths is not None else None
     a.lse = lse.data_ptr() if return_lse else None
@@ -265,8 +285,9 @@ def attend_backward(grad_out, q, k, v, out, lse, *, key_lengths=None, scale=None
         c.lengths(key_lengths, b)
         _sizes(a, b, t, n, h, hk, d, c.storage, c.scale(scale, d))
         plan = _keep(key, c.plan(a, "b200f_attend_backward"))
+        plan.grads = [_Output(x.shape, c.dtype, c.device) for x in (q, k, v)]
     a = abi.AttendBackwardArgs.from_buffer_copy(plan.proto)
-    gq, gk, gv = (torch.empty(x.shape, dtype=plan.dtype, device=plan.device) for x in (q, k, v))
+    gq, gk, gv = [make() for make in plan.grads]
     a.grad_out, a.q, a.k, a.v, a.out = pg, pq, pk, pv, po = (
         grad_out.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr())
     a.lse, a.grad_q, a.grad_k, a.grad_v = lse.data_ptr(), gq.data_ptr(), gk.data_ptr(), gv.data_ptr()
@@ -306,9 +327,10 @@ def attend_shared(q, shared_k, shared_v, own_k, own_v, own_lengths=None, *, scal
         _sizes(a, b, t, n, h, hk, d, c.storage, c.scale(scale, d))
         a.shared_n, a.causal = p, 1
         plan = _keep(key, c.plan(a, "b200f_attend"))
+        plan.out, plan.lse = _Output(q.shape, c.dtype, c.device), _Output((b, t, h), torch.float32, c.device)
     a = abi.AttendArgs.from_buffer_copy(plan.proto)
-    out = torch.empty(q.shape, dtype=plan.dtype, device=plan.device)
-    lse = torch.empty(q.shape[:3], dtype=torch.float32, device=plan.device) if return_lse else None
+    out = plan.out()
+    lse = plan.lse() if return_lse else None
     a.q, a.shared_k, a.shared_v, a.k, a.v = pq, psk, psv, pk, pv = (
         q.data_ptr(), shared_k.data_ptr(), shared_v.data_ptr(), own_k.data_ptr(), own_v.data_ptr())
     a.out = out.data_ptr()
@@ -345,8 +367,9 @@ def attention_mass(q, k, lse, *, key_lengths=None, scale=None, causal=False, mas
         _sizes(a, b, t, n, h, hk, d, c.storage, c.scale(scale, d))
         a.causal = 1 if causal else 0
         plan = _keep(key, c.plan(a, "b200f_attention_mass"))
+        plan.out = _Output((b, hk, n), torch.float32, c.device)
     a = abi.AttentionMassArgs.from_buffer_copy(plan.proto)
-    out = torch.empty((q.shape[0], k.shape[2], k.shape[1]), dtype=torch.float32, device=plan.device)
+    out = plan.out()
     a.q, a.k, a.lse, a.mass_out = pq, pk, _, _ = q.data_ptr(), k.data_ptr(), lse.data_ptr(), out.data_ptr()
     a.key_lengths = key_lengths.data_ptr() if key_lengths is not None else None
     a.mass_in = mass.data_ptr() if mass is not None else None
@@ -379,14 +402,11 @@ def evict(k, v, mass, key_lengths=None, keep=1, *, recent=0):
         c.lengths(key_lengths, b)
         a.batch, a.n, a.kv_heads, a.d, a.storage, a.keep, a.recent = b, n, hk, d, c.storage, int(keep), int(recent)
         plan = _keep(key, c.plan(a, "b200f_evict", with_scratch=False))
+        plan.outs = [_Output((b, a.keep, hk, d), c.dtype, c.device)] * 2 + [
+            _Output((b, hk, a.keep), torch.float32, c.device), _Output((b, hk, a.keep), torch.int32, c.device),
+            _Output((b,), torch.int32, c.device)]
     a = abi.EvictArgs.from_buffer_copy(plan.proto)
-    b, _, hk, d = k.shape
-    keep = a.keep
-    out_k = torch.empty((b, keep, hk, d), dtype=plan.dtype, device=plan.device)
-    out_v = torch.empty((b, keep, hk, d), dtype=plan.dtype, device=plan.device)
-    out_mass = torch.empty((b, hk, keep), dtype=torch.float32, device=plan.device)
-    out_rows = torch.empty((b, hk, keep), dtype=torch.int32, device=plan.device)
-    out_lengths = torch.empty((b,), dtype=torch.int32, device=plan.device)
+    out_k, out_v, out_mass, out_rows, out_lengths = [make() for make in plan.outs]
     a.k, a.v, a.mass = pk, pv, _ = k.data_ptr(), v.data_ptr(), mass.data_ptr()
     a.key_lengths = key_lengths.data_ptr() if key_lengths is not None else None
     a.out_k, a.out_v, a.out_mass, a.out_rows, a.out_lengths = (
@@ -418,11 +438,12 @@ def attend_index(index, x, values, scale, return_lse):
         a.k_stride[1], a.v_stride[1] = d, vs[0]   # 16-bit rows of an inner-product index lie side by side
         _sizes(a, 1, x.shape[0], n, 1, 1, d, c.storage, c.scale(scale, d))
         plan = _keep(key, c.plan(a, "b200f_attend"))
+        plan.out, plan.lse = _Output(x.shape, c.dtype, c.device), _Output(x.shape[:1], torch.float32, c.device)
     if torch.cuda.is_current_stream_capturing():
         raise ValueError("attend: the rows of an index may move, a graph cannot hold their address")
     a = abi.AttendArgs.from_buffer_copy(plan.proto)
-    out = torch.empty(x.shape, dtype=plan.dtype, device=plan.device)
-    lse = torch.empty(x.shape[:1], dtype=torch.float32, device=plan.device) if return_lse else None
+    out = plan.out()
+    lse = plan.lse() if return_lse else None
     a.q, a.k, a.v, a.out = px, _, pv, _ = x.data_ptr(), index.device_rows(), values.data_ptr(), out.data_ptr()
     a.lse = lse.data_ptr() if return_lse else None
     _run(plan, a, px | pv, _NO_SCRATCH)

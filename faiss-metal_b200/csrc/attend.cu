@@ -458,7 +458,7 @@ attend_tile_kernel(const __grid_constant__ CUtensorMap map_sk, const __grid_cons
 }
 
 // ---- attend_few_kernel ---------------------------------------------------------------------------------
-// At most 16 packed query rows a unit, as when decoding: reading keys and values once is the bound, 3 us of HBM time for every
+// Blocks of 16 packed query rows, at most one a unit as a rule, as when decoding: reading keys and values once is the bound, 3 us of HBM time for every
 // us of tensor work even on mma.sync, whose 16-row tile wastes nothing here (a tcgen05 tile has 128).  Four warps share tiles of
 // 64 keys that TMA streams in, 16 keys a warp, each with a softmax of its own; they are joined once at the end.  Two
 // CTAs an SM, so that one streams while the other starts or ends.
@@ -521,10 +521,11 @@ attend_few_kernel(const __grid_constant__ CUtensorMap map_sk, const __grid_const
     const int shared = p.seg[0].few && (int64_t)blockIdx.x < p.seg[0].items ? 1 : 0;
     const Segment& sg = p.seg[shared ? 0 : 1];
     const int64_t item = (int64_t)blockIdx.x - (shared || !p.seg[0].few ? 0 : p.seg[0].items);
-    const int sp = (int)(item % sg.splits);
-    const int64_t unit = item / sg.splits;
-    const int kvh = (int)(unit % p.kv_heads);
-    const int64_t ub = shared ? 0 : unit / p.kv_heads;
+    const uint32_t x_rb = (uint32_t)item / (uint32_t)sg.row_blocks, row0 = ((uint32_t)item - x_rb * sg.row_blocks) * FEW_ROWS;
+    const uint32_t unit = x_rb / (uint32_t)sg.splits;
+    const int sp = (int)(x_rb - unit * sg.splits);
+    const int64_t ub = shared ? 0 : unit / (uint32_t)p.kv_heads;
+    const int kvh = (int)(shared ? unit : unit - (uint32_t)ub * p.kv_heads);
     const int64_t seq_len = shared ? sg.n : p.len.of(ub);
     const int64_t ntiles = (seq_len + FEW_KEYS - 1) / FEW_KEYS;   // causal ends lie in the last tiles
     const int64_t per = (ntiles + sg.splits - 1) / sg.splits;
@@ -589,7 +590,7 @@ attend_few_kernel(const __grid_constant__ CUtensorMap map_sk, const __grid_const
             for (int e = 0; e < 4; e++) q[i][e] = 0;
 #pragma unroll
         for (int e = 0; e < 2; e++) {
-            const int r = (lane >> 2) + 8 * e;
+            const int r = (int)row0 + (lane >> 2) + 8 * e;
             end[e] = (int64_t)1 << 40;   // rows that do not exist are not masked
             if (r < sg.rows) {
                 const RowAt at = row_at(p, shared, unit, r);
@@ -714,7 +715,8 @@ attend_few_kernel(const __grid_constant__ CUtensorMap map_sk, const __grid_const
         }
         __syncthreads();
         const int part = sg.part0 + sp;
-        for (int i = threadIdx.x; i < sg.rows * (DP / 8); i += FEW_THREADS) {
+        const int live_rows = min(sg.rows - (int)row0, FEW_ROWS);
+        for (int i = threadIdx.x; i < live_rows * (DP / 8); i += FEW_THREADS) {
             const int r = i / (DP / 8), c0 = i % (DP / 8) * 8;
             if (c0 >= p.d) continue;
             float top = -CUDART_INF_F, total = 0.f, acc[8] = {};
@@ -731,7 +733,7 @@ attend_few_kernel(const __grid_constant__ CUtensorMap map_sk, const __grid_const
             }
             const bool none = total == 0.f;
             const float inv = none ? 0.f : 1.f / total;
-            const RowAt at = row_at(p, shared, unit, r);
+            const RowAt at = row_at(p, shared, unit, row0 + r);
             const int64_t grow = (at.b * p.queries + at.t) * p.heads + at.h;
             const float lse2 = none ? -CUDART_INF_F : log2f(total) + (top == -CUDART_INF_F ? 0.f : top);
 #pragma unroll
@@ -830,11 +832,18 @@ struct AttendPlan {
 // rows: about four turns of the two CTAs an SM takes, of at least FEW_MIN_TILES tiles.
 constexpr int MIN_TILES = 2;
 constexpr int FEW_MIN_TILES = 4;
+// Small problems of more rows than a block go to the few-rows kernel too, which starts and ends sooner (5 us against 11 for 1,024 rows and 16
+// keys), block by block, each of which reads the keys again.  us, few / tiles, bf16, d = 128: 2 units of 64 rows and 4,096 keys 10.6 /
+// 15.2, of 128 rows 13.0 / 17.6, of 48 rows and 16,384 keys 21.8 / 18.8; 8 units of 128 rows and 1,024 keys 12.5 / 17.1, of 512 rows
+// and 256 keys 8.5 / 12.6, 512 keys 18.4 / 15.4; 8 units of 1,024 rows and 16 keys 11.1 / 10.9.
+constexpr int64_t FEW_MAX_BLOCKS = 400, FEW_MAX_VISITS = 65536;
 AttendPlan plan_attend(const B200FAttendArgs& a) {
     AttendPlan pl{};
     const int group = a.heads / a.kv_heads;
     const int64_t sm = cached_sm_count();
     int64_t weight[2] = {0, 0}, base[2] = {0, 0}, total = 0;
+    // a join costs what three or four tiles take, one after the other; with keys of both kinds there is one anyway
+    const int64_t alone = a.shared_n > 0 && a.n > 0 ? 1 : 4;
     for (int i = 0; i < 2; i++) {
         Segment& s = pl.seg[i];
         const int64_t units = i == 0 ? a.kv_heads : a.batch * a.kv_heads;
@@ -844,18 +853,20 @@ AttendPlan plan_attend(const B200FAttendArgs& a) {
         s.splits = s.row_blocks = 1;
         // without any keys rows of zeros are written by the own segment
         const bool on = s.n > 0 || (i == 1 && a.shared_n == 0);
-        s.few = rows <= FEW_ROWS;
+        const int64_t blocks = units * ceil_div64(rows, FEW_ROWS);
+        s.few = rows <= FEW_ROWS || (blocks <= FEW_MAX_BLOCKS && blocks * s.n <= FEW_MAX_VISITS);
         if (!on) continue;
         if (s.few) {
             const int64_t tiles = ceil_div64(s.n, FEW_KEYS);
-            int64_t want = 8 * sm / units;
+            s.row_blocks = (int)ceil_div64(rows, FEW_ROWS);
+            int64_t want = 8 * sm / (units * s.row_blocks);
             if (want > tiles / FEW_MIN_TILES) want = tiles / FEW_MIN_TILES;
             s.splits = (int)(want < 1 ? 1 : want);
-            s.items = units * s.splits;
+            s.items = units * s.splits * s.row_blocks;
             continue;
         }
         const int64_t tiles = ceil_div64(s.n, TILE_KEYS);
-        s.split = rows <= 128 && tiles >= 2;
+        s.split = rows <= 128 && tiles > alone;
         s.row_blocks = (int)ceil_div64(rows, s.split ? 128 : 256);
         base[i] = units * s.row_blocks;
         weight[i] = base[i] * tiles;
@@ -867,7 +878,7 @@ AttendPlan plan_attend(const B200FAttendArgs& a) {
         if (base[i] > 0) {
             const int64_t tiles = ceil_div64(s.n, TILE_KEYS);
             const int64_t share = total > 0 ? (int64_t)((double)sm * weight[i] / total / base[i]) : 1;
-            const int64_t most = tiles / (s.split ? 2 * MIN_TILES : MIN_TILES);
+            const int64_t most = tiles <= alone ? 1 : tiles / (s.split ? 2 * MIN_TILES : MIN_TILES);
             s.splits = (int)(share < most ? share : most);
             if (s.splits < 1) s.splits = 1;
             s.items = base[i] * s.splits;
