@@ -18,6 +18,8 @@ namespace {
 // Weights are exp2(c (s - m)) for a reference m that is taken from a row's first tile and moves, with O rescaled, only when a tile's
 // weights add up to 2^15 or more: no maximum is looked for before the exponentials.  Sums stay in fp32.  The weights of the first 96
 // keys go to the tensor cores while those of the others are computed.
+// d <= 64 leaves tensor memory for P beside S (APART): the next scores are computed as soon as these are in registers, and the way
+// round is the softmax alone.
 constexpr int TILE_THREADS = 384;          // TMA, an issuer of MMAs a stream, a spare warp; 2 x 4 softmax warps
 constexpr int TILE_REGS_FEW = 80, TILE_REGS_MANY = 208;   // 128 and 256 threads of the 384 x 168 at launch
 static_assert(128 * TILE_REGS_FEW + 256 * TILE_REGS_MANY <= 384 * 168, "registers of a CTA");
@@ -34,9 +36,13 @@ constexpr int TILE_STAGES = DP == 128 ? 5 : 10;
 template <int DP>
 constexpr int TILE_SM_BAR = 2 * TILE_Q_BYTES<DP> + TILE_STAGES<DP>*TILE_STAGE_BYTES<DP>;
 template <int DP>
-constexpr int TILE_SMEM = TILE_SM_BAR<DP> + (2 * TILE_MAX_STAGES + 10) * 8 + 16;
+constexpr int TILE_SMEM = TILE_SM_BAR<DP> + (2 * TILE_MAX_STAGES + 14) * 8 + 16;
 static_assert(TILE_SMEM<128> <= 232448 && TILE_SMEM<64> <= 232448, "shared memory of a CTA");
-constexpr uint32_t TM_S = 0, TM_O = 256;   // stream t: S at 128 t, O at 256 + 128 t
+constexpr uint32_t TM_S = 0, TM_O = 256;   // stream t: S at 128 t, O at 256 + 128 t; P: see APART
+template <int DP>
+constexpr bool TILE_APART = DP == 64;
+template <int DP>
+constexpr uint32_t TM_P = TILE_APART<DP> ? TM_O + 64 : TM_S;
 
 // A set of keys and the query rows that read them.  Work items: (unit, block of rows, range of keys).
 struct Segment {
@@ -87,11 +93,13 @@ attend_tile_kernel(const __grid_constant__ CUtensorMap map_sk, const __grid_cons
     extern __shared__ __align__(1024) uint8_t smem[];
     constexpr int STAGES = TILE_STAGES<DP>, STAGE = TILE_STAGE_BYTES<DP>, QBYTES = TILE_Q_BYTES<DP>, CHUNKS = DP / 64;
     constexpr int HALF_RING = (STAGES + 1) / 2;
+    constexpr bool APART = TILE_APART<DP>;
     const uint32_t sbase = smem_u32(smem);
     const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0);
     const int lane = threadIdx.x & 31;
     const uint32_t bar_full = sbase + TILE_SM_BAR<DP>, bar_empty = bar_full + TILE_MAX_STAGES * 8;
     const uint32_t bar_s = bar_empty + TILE_MAX_STAGES * 8, bar_p = bar_s + 16, bar_part = bar_p + 32, bar_done = bar_part + 16;   // [stream]; P: [stream][part]
+    const uint32_t bar_free = bar_done + 16, bar_o = bar_free + 16;   // APART: scores read; P V done
     volatile uint32_t* tmem_ptr = reinterpret_cast<volatile uint32_t*>(smem + TILE_SMEM<DP> - 16);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_ptr + 1);
 
@@ -162,6 +170,8 @@ attend_tile_kernel(const __grid_constant__ CUtensorMap map_sk, const __grid_cons
             mbar_init(bar_s + i * 8, 1);
             mbar_init(bar_part + i * 8, 1);
             mbar_init(bar_done + i * 8, 1);
+            mbar_init(bar_free + i * 8, 4);
+            mbar_init(bar_o + i * 8, 1);
         }
         for (int i = 0; i < 4; i++) mbar_init(bar_p + i * 8, 4);
         mbar_fence_init();
@@ -210,11 +220,13 @@ attend_tile_kernel(const __grid_constant__ CUtensorMap map_sk, const __grid_cons
             if (n0 > 0) load(0, mk, sg.km, first0);
             if (sg.split && n1 > 0) load(1, mk, sg.km, first1);
             for (int j = 0; j < n0 && ok; j++) {
+                if (APART && j + 1 < n0) load(0, mk, sg.km, first0 + j + 1);
                 load(0, mv, sg.vm, first0 + j);
-                if (j + 1 < n0) load(0, mk, sg.km, first0 + j + 1);
+                if (!APART && j + 1 < n0) load(0, mk, sg.km, first0 + j + 1);
                 if (sg.split && j < n1) {
+                    if (APART && j + 1 < n1) load(1, mk, sg.km, first1 + j + 1);
                     load(1, mv, sg.vm, first1 + j);
-                    if (j + 1 < n1) load(1, mk, sg.km, first1 + j + 1);
+                    if (!APART && j + 1 < n1) load(1, mk, sg.km, first1 + j + 1);
                 }
             }
             if (!ok) {   // let the copies in flight land before shared memory goes away
@@ -263,8 +275,13 @@ attend_tile_kernel(const __grid_constant__ CUtensorMap map_sk, const __grid_cons
                 if (gives[t]) tc_commit_by<false>(leader, bar_empty + slot[t] * 8);
                 next(t);
             };
-            // P V of tile j and, more, the scores of the next
+            // P V of tile j and, more, the scores of the next: behind it, or APART in front
             auto turn = [&](int t, int j, bool more) __attribute__((always_inline)) {
+                if (APART && more) {
+                    if (!keys_there(t) || !waits(bar_free + t * 8, j & 1)) return false;
+                    tc_fence_after();
+                    scores(t);
+                }
                 if (t == 0 || SPLIT) {
                     if (!waits(bar_full + slot[t] * 8, phase[t])) return false;
                     // rows behind the sequence's end, within the tensor: whatever they hold, 0 * it must be 0
@@ -274,7 +291,7 @@ attend_tile_kernel(const __grid_constant__ CUtensorMap map_sk, const __grid_cons
                 const int s = slot[t];
                 const uint64_t db = dv + (uint64_t)(s * (STAGE >> 4));
                 auto product = [&](int k) __attribute__((always_inline)) {   // 16 keys
-                    tc_mma_ts_by(leader, tmem + TM_O + 128 * t, tmem + TM_S + 128 * t + 8 * k, db + 128 * k, att_idesc<T>(DP, true),
+                    tc_mma_ts_by(leader, tmem + TM_O + 128 * t, tmem + TM_P<DP> + 128 * t + 8 * k, db + 128 * k, att_idesc<T>(DP, true),
                                  k > 0 ? 1u : (uint32_t)(j > 0));
                 };
                 if (!waits(bar_p + 2 * t * 8, j & 1)) return false;
@@ -283,13 +300,14 @@ attend_tile_kernel(const __grid_constant__ CUtensorMap map_sk, const __grid_cons
                 for (int k = 0; k < PART_KEYS / 16; k++) product(k);
                 tc_commit_by<false>(leader, bar_part + t * 8);
                 next(t);
-                if (more && !keys_there(t)) return false;
+                if (!APART && more && !keys_there(t)) return false;
                 if (!waits(bar_p + (2 * t + 1) * 8, j & 1)) return false;
                 tc_fence_after();
 #pragma unroll
                 for (int k = PART_KEYS / 16; k < TILE_KEYS / 16; k++) product(k);
-                if (more) scores(t);
-                else tc_commit_by<false>(leader, bar_done + t * 8);
+                if (!more) tc_commit_by<false>(leader, bar_done + t * 8);
+                else if (APART) tc_commit_by<false>(leader, bar_o + t * 8);
+                else scores(t);
                 if (gives[t]) tc_commit_by<false>(leader, bar_empty + s * 8);
                 return true;
             };
@@ -327,7 +345,7 @@ attend_tile_kernel(const __grid_constant__ CUtensorMap map_sk, const __grid_cons
         // keys this row sees; rows that do not exist are not masked
         const int end = !live ? 0x7ffffff0 : (int)(shared ? seq_len : p.len.seen(seq_len, at.t));
         const uint32_t ts = tmem + TM_S + 128 * t + ((uint32_t)(ew * 32) << 16);
-        const uint32_t to = tmem + TM_O + 128 * t + ((uint32_t)(ew * 32) << 16);
+        const uint32_t to = tmem + TM_O + 128 * t + ((uint32_t)(ew * 32) << 16), tp = tmem + TM_P<DP> + 128 * t + ((uint32_t)(ew * 32) << 16);
         const float c = p.scale * kLog2e;
         float m = -CUDART_INF_F, l = 0.f;
         float mc = CUDART_NAN_F;   // -c m; no reference yet: the first tile's sum fails the test below
@@ -337,7 +355,7 @@ attend_tile_kernel(const __grid_constant__ CUtensorMap map_sk, const __grid_cons
         auto weigh = [&](auto mix, uint32_t (&x)[32], float mc_now, int i) __attribute__((always_inline)) {
             uint32_t w[16];
             const float2 z = weigh32<T, decltype(mix)::value>(x, c, mc_now, w);
-            tc_st16(ts + 16 * i, w);
+            tc_st16(tp + 16 * i, w);
             return z.x + z.y;
         };
         for (int j = 0; j < nt; j++) {
@@ -347,6 +365,11 @@ attend_tile_kernel(const __grid_constant__ CUtensorMap map_sk, const __grid_cons
             const int lim = end - (kt0 + j) * TILE_KEYS;
             const bool masked = __any_sync(0xffffffffu, lim < TILE_KEYS);
             tc_ld32(ts, s[0]);
+            if (APART && j > 0) {   // P and O may be written when the previous product is done
+                ok = __all_sync(0xffffffffu, wait(bar_o + t * 8, (j - 1) & 1));
+                if (!ok) break;
+                tc_fence_after();
+            }
 #pragma unroll
             for (int h = 0; h < 2; h++) {
                 constexpr int PART = PART_KEYS / 32;
@@ -355,6 +378,11 @@ attend_tile_kernel(const __grid_constant__ CUtensorMap map_sk, const __grid_cons
                 for (int i = h ? PART : 0; i < (h ? 4 : PART); i++) {
                     tc_wait_ld32(s[i]);
                     if (i < 3) tc_ld32(ts + 32 * (i + 1), s[i + 1]);   // under the exponentials of this chunk
+                    if (APART && i == 3) {
+                        tc_fence_before();
+                        __syncwarp();
+                        mbar_arrive_if(lane == 0, bar_free + t * 8);
+                    }
                     if (!masked) {
                         sum += weigh(std::true_type(), s[i], mc, i);
                     } else {
@@ -377,7 +405,7 @@ attend_tile_kernel(const __grid_constant__ CUtensorMap map_sk, const __grid_cons
                     m = now;
                     l *= f;
                     mc = m == -CUDART_INF_F ? CUDART_NAN_F : -m * c;
-                    // O holds what came before: the previous tile's product is done, since the scores are there; the first part's
+                    // O holds what came before: the previous tile's product is done (APART: waited for, else since the scores are there); the first part's
                     // may be under way
                     if (moved && h == 1) {
                         ok = __all_sync(0xffffffffu, wait(bar_part + t * 8, j & 1));

@@ -165,11 +165,22 @@ __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
 
 // 2^y of two values on the FMA pipe: y = n + f with n the nearest integer (Cody and Waite's range reduction, the rounding by adding
 // 1.5 * 2^23), 2^f by a polynomial of degree 4 (fitted here to the relative error on [-1/2, 1/2], 2.7e-6 in fp32), n added to the
-// exponent.  Down to 2^-126; for y up to 126.
+// exponent.  2^-126 below that, 2^126 above, and something above 2^126 or NaN for NaN.
+__device__ __forceinline__ float clamp126(float y) {
+    float z;
+    asm("{\n\t"
+        ".reg .f32 t;\n\t"
+        "max.NaN.f32 t, %1, 0fC2FC0000;\n\t"
+        "min.NaN.f32 %0, t, 0f42FC0000;\n\t"
+        "}\n"
+        : "=f"(z)
+        : "f"(y));
+    return z;
+}
 __device__ __forceinline__ float2 ex2_fma(float2 y) {
     constexpr float ROUND = 12582912.f;
-    y.x = fmaxf(y.x, -126.f);
-    y.y = fmaxf(y.y, -126.f);
+    y.x = clamp126(y.x);
+    y.y = clamp126(y.y);
     const float2 r = add2(y, make_float2(ROUND, ROUND));
     const float2 f = add2(y, fma2(r, make_float2(-1.f, -1.f), make_float2(ROUND, ROUND)));
     float2 z = fma2(f, make_float2(0.009570104735915316f, 0.009570104735915316f), make_float2(0.05591786050289549f, 0.05591786050289549f));
@@ -184,7 +195,7 @@ __device__ __forceinline__ float2 ex2_fma(float2 y) {
 // w = exp2(x c + mc) of 32 values, packed; returns their sums.  In groups of eight, and each step for the whole group before the next:
 // the compiler keeps this order, and an exponential's result takes some 40 cycles (a warp alone on its scheduler: 1,090
 // cycles for 64 values step by step, 600 this way; the exponential unit takes 512).
-// MIX: two of eight by ex2_fma, which takes the load off that unit; for finite values only.
+// MIX: two of eight by ex2_fma, which takes the load off that unit; -INF gives 2^-126, +INF and NaN a large sum.
 template <typename T, bool MIX>
 __device__ __forceinline__ float2 weigh32(const uint32_t (&x)[32], float c, float mc, uint32_t* w) {
     const float2 c2 = make_float2(c, c), mc2 = make_float2(mc, mc);

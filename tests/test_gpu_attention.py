@@ -65,9 +65,24 @@ SHAPES = [
     (1, 1000, 1, 2, 2, 128, None),
 ]
 
+# large enough for tiles of 128 rows and keys: pairs of row tiles with one range of keys and with several, one row tile with two streams
+# of keys, rows that end inside a tile, groups that do not divide one
+TILES = [
+    (4, 15, 3000, 8, 2, 128, (3000, 129, 2048, 0)),
+    (4, 15, 3000, 8, 2, 64, (2999, 1, 700, 3000)),
+    (1, 150, 2100, 8, 2, 80, None),
+    (2, 333, 1111, 6, 2, 64, (1111, 1000)),
+    (2, 333, 1111, 6, 2, 128, (515, 1111)),
+    (3, 300, 520, 12, 4, 96, (520, 512, 511)),
+    (3, 257, 500, 14, 2, 64, (500, 384, 0)),
+    (1, 2048, 384, 4, 4, 128, None),
+    (24, 17, 800, 14, 2, 128, None),
+    (2, 40, 9000, 3, 1, 8, (9000, 4000)),
+]
+
 
 @pytest.mark.parametrize("dtype", list(TYPES))
-@pytest.mark.parametrize("shape", SHAPES, ids=str)
+@pytest.mark.parametrize("shape", SHAPES + TILES, ids=str)
 def test_attend(fm, shape, dtype):
     b, lq, lk, h, hk, d, n = shape
     dt = TYPES[dtype]
@@ -94,11 +109,67 @@ def test_attend_large_scores_and_rising_maxima(fm):
         assert ((out.double() - want[0]).abs() <= 1.1 * slack * unit(dt) * (want[0].abs() + 2 * want[2]) + 1e-30).all()
 
 
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("lq", [4, 24, 700])
+def test_one_key_decides(fm, lq, d):
+    """One key's score is far above all others, at every place of a tile in turn, in the first tile and later ones: by less and by more than
+    weights may grow before the reference moves, and by more than fp32 exponents reach."""
+    dt = torch.bfloat16
+    places = torch.arange(0, 600, 1 if lq == 4 else 13, device="cuda")
+    b, lk = len(places), 640
+    q = torch.zeros(b, lq, 2, d, dtype=dt, device="cuda")
+    q[..., 0] = 1
+    for jump in (6.0, 14.0, 40.0, 300.0, 30000.0):
+        k, v = rand(2, dt, b, lk, 1, d) * 0.25, rand(3, dt, b, lk, 1, d)
+        k[torch.arange(b), places, 0, 0] = jump
+        out, lse = fm.attend(q, k, v, scale=math.log(2.0), return_lse=True)     # jump is in powers of two
+        want = R.attend(q, k, v, scale=math.log(2.0))
+        assert ((out.double() - want[0]).abs() <= 2.2 * unit(dt) * want[2] + 1e-6).all(), jump
+        assert ((lse.double() - want[1]).abs() <= 2e-5 + 1e-6 * want[1].abs()).all(), jump
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+@pytest.mark.parametrize("lq", [4, 700])
+def test_nan_in_a_seen_key_comes_through(fm, lq, bad):
+    # a NaN or infinite score, wherever it is, makes the row NaN, as the definition does
+    dt = torch.float16
+    places = torch.arange(0, 300, 7, device="cuda")
+    b, lk, d = len(places), 300, 64
+    q, k, v = rand(1, dt, b, lq, 1, d).abs() + 0.25, rand(2, dt, b, lk, 1, d), rand(3, dt, b, lk, 1, d)
+    k[torch.arange(b), places, 0, 3] = bad
+    out, lse = fm.attend(q, k, v, return_lse=True)
+    assert torch.isnan(out).all()
+    assert (torch.isnan(lse) if math.isnan(bad) else torch.isnan(lse) | (lse == math.inf)).all()
+
+
+@pytest.mark.parametrize("shape", [(4, 15, 3000, 8, 2, 128), (2, 333, 1111, 6, 2, 64), (8, 1, 700, 8, 2, 128), (2, 600, 600, 8, 2, 128)], ids=str)
+def test_results_do_not_depend_on_timing(fm, shape):
+    # the same bits again and again, beside other work on the GPU
+    b, lq, lk, h, hk, d = shape
+    dt = torch.bfloat16
+    q, k, v, grad = rand(1, dt, b, lq, h, d), rand(2, dt, b, lk, hk, d), rand(3, dt, b, lk, hk, d), rand(4, dt, b, lq, h, d)
+    noise, other = torch.randn(2048, 2048, device="cuda"), torch.cuda.Stream()
+
+    def run():
+        out, lse = fm.attend(q, k, v, return_lse=True)
+        return (out, lse, *fm.attend_backward(grad, q, k, v, out, lse), fm.attention_mass(q, k, lse))
+
+    want = run()
+    for i in range(40):
+        with torch.cuda.stream(other):
+            for _ in range(i % 5):
+                noise @ noise
+        assert all(torch.equal(x, y) for x, y in zip(want, run()))
+    torch.cuda.synchronize()
+    fm.check_attention_status()
+
+
 @pytest.mark.parametrize("dtype", list(TYPES))
-def test_attend_masked_rows_have_no_influence(fm, dtype):
+@pytest.mark.parametrize("lq,lk", [(40, 300), (700, 900)])
+def test_attend_masked_rows_have_no_influence(fm, dtype, lq, lk):
     dt = TYPES[dtype]
-    q, k, v = rand(1, dt, 3, 40, 4, 64), rand(2, dt, 3, 300, 2, 64), rand(3, dt, 3, 300, 2, 64)
-    n = lens(131, 0, 299)
+    q, k, v = rand(1, dt, 3, lq, 4, 64), rand(2, dt, 3, lk, 2, 64), rand(3, dt, 3, lk, 2, 64)
+    n = lens(131, 0, lk - 1)
     want = fm.attend(q, k, v, key_lengths=n, return_lse=True)
     bad_k, bad_v = k.clone(), v.clone()
     for i, x in enumerate(n.tolist()):
@@ -107,7 +178,7 @@ def test_attend_masked_rows_have_no_influence(fm, dtype):
     got = fm.attend(q, bad_k, bad_v, key_lengths=n, return_lse=True)
     assert all(torch.equal(a, b) for a, b in zip(want, got))
     assert (got[0][1] == 0).all() and (got[1][1] == -math.inf).all()
-    grad = rand(4, dt, 3, 40, 4, 64)
+    grad = rand(4, dt, 3, lq, 4, 64)
     a = fm.attend_backward(grad, q, k, v, *want, key_lengths=n)
     c = fm.attend_backward(grad, q, bad_k, bad_v, *want, key_lengths=n)
     assert all(torch.equal(x, y) for x, y in zip(a, c))
@@ -164,7 +235,7 @@ def check_grads(got, ref, dtype):
 
 
 @pytest.mark.parametrize("dtype", list(TYPES))
-@pytest.mark.parametrize("shape", [s for s in SHAPES if s[2]], ids=str)
+@pytest.mark.parametrize("shape", [s for s in SHAPES + TILES if s[2]], ids=str)
 def test_attend_backward(fm, shape, dtype):
     b, lq, lk, h, hk, d, n = shape
     dt = TYPES[dtype]
@@ -224,6 +295,12 @@ SHARED = [
     (2, 9, 4097, 600, 4, 4, 128, (600, 8)),
     (3, 150, 200, 400, 4, 2, 64, (400, 150, 140)),
     (2, 1, 20000, 5, 8, 1, 128, None),
+    (40, 3, 3000, 300, 8, 2, 128, None),
+    (40, 3, 3000, 300, 8, 2, 64, tuple(3 + 7 * i for i in range(40))),
+    (2, 150, 3000, 2900, 8, 2, 64, (2900, 151)),
+    (2, 150, 3000, 2900, 8, 2, 128, (1500, 2900)),
+    (3, 200, 1, 1700, 8, 2, 96, (200, 1700, 30)),
+    (64, 1, 4000, 1, 32, 4, 72, None),
 ]
 
 
