@@ -447,6 +447,9 @@ def attend_index(index, x, values, scale, return_lse):
     a.q, a.k, a.v, a.out = px, _, pv, _ = x.data_ptr(), index.device_rows(), values.data_ptr(), out.data_ptr()
     a.lse = lse.data_ptr() if return_lse else None
     _run(plan, a, px | pv, _NO_SCRATCH)
-    # adds and resets run on the index's own stream, and have completed when they return
-    index.resources.wait_stream(torch.cuda.current_stream(plan.device).cuda_stream)
+    # adds and resets run on the index's own stream, and have completed when they return; the next one waits for this read
+    event = index._reads.get(a.stream)
+    if event is None:
+        event = index._reads[a.stream] = torch.cuda.Event()
+    event.record()
     return (out, lse) if return_lse else out

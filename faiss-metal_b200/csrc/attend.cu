@@ -709,8 +709,11 @@ attend_few_kernel(const __grid_constant__ CUtensorMap map_sk, const __grid_const
                 mma16816<T>(o[2 * t], w, b[0], b[1]);
                 mma16816<T>(o[2 * t + 1], w, b[2], b[3]);
             }
+            // The values may still be on their way to registers (the products that take them are under way): the stage is not given to TMA
+            // before they are there.
+            fence_proxy_async_shared();
             __syncwarp();
-            if (lane == 0) mbar_arrive(bar_empty + slot * 8);
+            mbar_arrive_if(lane == 0, bar_empty + slot * 8);
             if (++slot == STAGES) {
                 slot = 0;
                 phase ^= 1;
@@ -783,13 +786,14 @@ attend_few_kernel(const __grid_constant__ CUtensorMap map_sk, const __grid_const
 
 // ---- attend_join_kernel: partial results of a row become its result ------------------
 // W warps a row, each W-th part, so that many parts are on their way at once (1,000 rows of 37 parts: 31 us with a warp a row).
+// 8 warps a CTA, or W = 32.
 template <typename T>
-__global__ void __launch_bounds__(256) attend_join_kernel(const float* part_o, const float* part_lse, int parts, int64_t rows, int d, int W,
+__global__ void __launch_bounds__(1024) attend_join_kernel(const float* part_o, const float* part_lse, int parts, int64_t rows, int d, int W,
                                                           uint16_t* out, float* lse) {
-    __shared__ float4 acc_s[8][32];
-    __shared__ float total_s[8];
+    __shared__ float4 acc_s[32][32];
+    __shared__ float total_s[32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int64_t row = (int64_t)blockIdx.x * (8 / W) + warp / W;
+    const int64_t row = (int64_t)blockIdx.x * ((blockDim.x >> 5) / W) + warp / W;
     pdl_wait();
     pdl_trigger();
     const bool in = row < rows;
@@ -856,61 +860,83 @@ struct AttendPlan {
     size_t scratch;
 };
 
-// Ranges of keys.  Tiles: as many as fill the SMs once, of at least MIN_TILES tiles; a segment's share goes by its tiles.  Few
-// rows: about four turns of the two CTAs an SM takes, of at least FEW_MIN_TILES tiles.
+// How a segment's work is cut: ranges of keys that fill the SMs, of at least MIN_TILES tiles; and by which kernel.  Blocks of more than
+// 16 rows may go to either: the few-rows kernel starts and ends sooner, but reads the keys again for every block.  What is measured
+// (us, bf16, d = 128): a tile CTA 7 and 1.7 a tile of 128 keys, one an SM; a few-rows CTA 3.5 and 0.5 a tile of 64, two an SM; joining parts
+// 4.5.  E.g. few-rows / tiles: 2 units of 64 rows and 4,096 keys 10.6 / 15.2, of 48 rows and 16,384 keys 21.8 / 18.8; 8 units of 512
+// rows and 256 keys 8.5 / 12.6, 512 keys 18.4 / 15.4.
 constexpr int MIN_TILES = 2;
 constexpr int FEW_MIN_TILES = 4;
-// Small problems of more rows than a block go to the few-rows kernel too, which starts and ends sooner (5 us against 11 for 1,024 rows and 16
-// keys), block by block, each of which reads the keys again.  us, few / tiles, bf16, d = 128: 2 units of 64 rows and 4,096 keys 10.6 /
-// 15.2, of 128 rows 13.0 / 17.6, of 48 rows and 16,384 keys 21.8 / 18.8; 8 units of 128 rows and 1,024 keys 12.5 / 17.1, of 512 rows
-// and 256 keys 8.5 / 12.6, 512 keys 18.4 / 15.4; 8 units of 1,024 rows and 16 keys 11.1 / 10.9.
-constexpr int64_t FEW_MAX_BLOCKS = 400, FEW_MAX_VISITS = 65536;
+constexpr double TILE_START_US = 7, TILE_US = 1.7, FEW_START_US = 3.5, FEW_US = 0.5, JOIN_US = 4.5;
+
+// share: CTAs that the segment may fill.  Returns its time.
+double cut_tiles(Segment& s, int64_t units, int64_t rows, double share, bool joined) {
+    const int64_t tiles = ceil_div64(s.n, TILE_KEYS);
+    // a join costs what three or four tiles take, one after the other
+    const int64_t alone = joined ? 1 : 4;
+    s.few = 0;
+    s.split = rows <= 128 && tiles > alone;
+    s.row_blocks = (int)ceil_div64(rows, s.split ? 128 : 256);
+    const int64_t base = units * s.row_blocks, most = tiles <= alone ? 1 : tiles / (s.split ? 2 * MIN_TILES : MIN_TILES);
+    int64_t splits = (int64_t)(share / base);
+    if (splits > most) splits = most;
+    s.splits = (int)(splits < 1 ? 1 : splits);
+    s.items = base * s.splits;
+    const int streams = s.split ? 2 * s.splits : s.splits;
+    const int64_t sm = cached_sm_count();
+    return (double)ceil_div64(s.items, sm) * (TILE_START_US + TILE_US * (double)ceil_div64(tiles, streams)) +
+           (!joined && streams > 1 ? JOIN_US : 0);
+}
+double cut_few(Segment& s, int64_t units, int64_t rows, bool joined) {
+    const int64_t tiles = ceil_div64(s.n, FEW_KEYS), sm = cached_sm_count();
+    s.few = 1;
+    s.split = 0;
+    s.row_blocks = (int)ceil_div64(rows, FEW_ROWS);
+    const int64_t base = units * s.row_blocks;
+    // one turn of the two CTAs an SM takes; with more blocks than SMs about four, since sequences differ in length
+    int64_t want = (base >= sm ? 8 : 2) * sm / base;
+    if (want > tiles / FEW_MIN_TILES) want = tiles / FEW_MIN_TILES;
+    s.splits = (int)(want < 1 ? 1 : want);
+    s.items = base * s.splits;
+    return (double)ceil_div64(s.items, 2 * sm) * (FEW_START_US + FEW_US * (double)ceil_div64(tiles, s.splits)) +
+           (!joined && s.splits > 1 ? JOIN_US : 0);
+}
+
 AttendPlan plan_attend(const B200FAttendArgs& a) {
     AttendPlan pl{};
     const int group = a.heads / a.kv_heads;
-    const int64_t sm = cached_sm_count();
-    int64_t weight[2] = {0, 0}, base[2] = {0, 0}, total = 0;
-    // a join costs what three or four tiles take, one after the other; with keys of both kinds there is one anyway
-    const int64_t alone = a.shared_n > 0 && a.n > 0 ? 1 : 4;
+    const double sm = (double)cached_sm_count();
+    const bool joined = a.shared_n > 0 && a.n > 0;
+    int64_t units[2], rows_of[2];
+    bool on[2];
+    double weight[2] = {0, 0};
     for (int i = 0; i < 2; i++) {
         Segment& s = pl.seg[i];
-        const int64_t units = i == 0 ? a.kv_heads : a.batch * a.kv_heads;
+        units[i] = i == 0 ? a.kv_heads : a.batch * a.kv_heads;
         s.n = i == 0 ? a.shared_n : a.n;
-        const int64_t rows = (i == 0 ? a.batch : 1) * a.queries * group;
-        s.rows = (int)rows;
+        rows_of[i] = (i == 0 ? a.batch : 1) * a.queries * group;
+        s.rows = (int)rows_of[i];
         s.splits = s.row_blocks = 1;
         // without any keys rows of zeros are written by the own segment
-        const bool on = s.n > 0 || (i == 1 && a.shared_n == 0);
-        const int64_t blocks = units * ceil_div64(rows, FEW_ROWS);
-        s.few = rows <= FEW_ROWS || (blocks <= FEW_MAX_BLOCKS && blocks * s.n <= FEW_MAX_VISITS);
-        if (!on) continue;
-        if (s.few) {
-            const int64_t tiles = ceil_div64(s.n, FEW_KEYS);
-            s.row_blocks = (int)ceil_div64(rows, FEW_ROWS);
-            int64_t want = 8 * sm / (units * s.row_blocks);
-            if (want > tiles / FEW_MIN_TILES) want = tiles / FEW_MIN_TILES;
-            s.splits = (int)(want < 1 ? 1 : want);
-            s.items = units * s.splits * s.row_blocks;
+        on[i] = s.n > 0 || (i == 1 && a.shared_n == 0);
+        if (!on[i]) {
+            s.few = 1;   // no CTAs of either kernel
             continue;
         }
-        const int64_t tiles = ceil_div64(s.n, TILE_KEYS);
-        s.split = rows <= 128 && tiles > alone;
-        s.row_blocks = (int)ceil_div64(rows, s.split ? 128 : 256);
-        base[i] = units * s.row_blocks;
-        weight[i] = base[i] * tiles;
-        total += weight[i];
+        Segment tile = s;
+        const double few_us = cut_few(s, units[i], rows_of[i], joined);
+        if (rows_of[i] <= FEW_ROWS) continue;
+        if (cut_tiles(tile, units[i], rows_of[i], sm, joined) < few_us) {
+            s = tile;
+            weight[i] = (double)units[i] * s.row_blocks * (double)ceil_div64(s.n, TILE_KEYS);
+        }
     }
+    // both by tiles: each gets the SMs that its tiles ask for
+    if (weight[0] > 0 && weight[1] > 0)
+        for (int i = 0; i < 2; i++) (void)cut_tiles(pl.seg[i], units[i], rows_of[i], sm * weight[i] / (weight[0] + weight[1]), joined);
     for (int i = 0; i < 2; i++) {
         Segment& s = pl.seg[i];
         s.part0 = pl.parts;
-        if (base[i] > 0) {
-            const int64_t tiles = ceil_div64(s.n, TILE_KEYS);
-            const int64_t share = total > 0 ? (int64_t)((double)sm * weight[i] / total / base[i]) : 1;
-            const int64_t most = tiles <= alone ? 1 : tiles / (s.split ? 2 * MIN_TILES : MIN_TILES);
-            s.splits = (int)(share < most ? share : most);
-            if (s.splits < 1) s.splits = 1;
-            s.items = base[i] * s.splits;
-        }
         pl.items[s.few] += s.items;
         if (s.items > 0) pl.parts += s.split ? 2 * s.splits : s.splits;
     }
@@ -949,8 +975,8 @@ int launch_attend(const CUtensorMap* maps, const TileParams& p, const AttendPlan
         count_launch();
     }
     if (e == cudaSuccess && pl.parts > 1) {
-        const int W = pl.parts > 16 ? 8 : pl.parts > 8 ? 4 : pl.parts > 4 ? 2 : 1;
-        e = launch_kernel(attend_join_kernel<T>, dim3((unsigned)ceil_div64(p.rows_total, 8 / W)), 256, 0, Launch(st, true),
+        const int W = pl.parts > 64 ? 32 : pl.parts > 16 ? 8 : pl.parts > 8 ? 4 : pl.parts > 4 ? 2 : 1, warps = W > 8 ? W : 8;
+        e = launch_kernel(attend_join_kernel<T>, dim3((unsigned)ceil_div64(p.rows_total, warps / W)), 32 * warps, 0, Launch(st, true),
                           static_cast<const float*>(p.part_o), static_cast<const float*>(p.part_lse), pl.parts, p.rows_total, p.d, W, p.out,
                           p.lse);
         count_launch();

@@ -513,8 +513,9 @@ struct GradPlan {
     int key_splits, row_splits;
     size_t stat_bytes, key_part_bytes, scratch;
 };
-// Ranges of the streamed tiles: as many as fill the SMs once, of at least MIN_TILES tiles of 64 rows.
-constexpr int MIN_TILES = 4;
+// Ranges of the streamed tiles: where an item would take more than twice an SM's share of the work, as many as bring it down to that, of
+// at least MIN_TILES tiles of 64 rows.
+constexpr int MIN_TILES = 8;
 GradPlan plan_grad(const B200FAttendBackwardArgs& a) {
     GradPlan pl{};
     const int group = a.heads / a.kv_heads;
@@ -522,14 +523,15 @@ GradPlan plan_grad(const B200FAttendBackwardArgs& a) {
     pl.rt = row_tiles(GRAD_ROWS, a.queries, group);
     pl.key_blocks = ceil_div64(a.n, 128);
     pl.row_blocks = ceil_div64(a.queries * group, 128);
-    const int64_t both = units * (pl.key_blocks + pl.row_blocks);
-    auto splits = [&](int64_t tiles) {
-        int64_t s = both > 0 ? sm / both : 1;
-        if (s > tiles / MIN_TILES) s = tiles / MIN_TILES;
-        return (int)(s < 1 ? 1 : s);
+    // what an SM has to do, in tiles (a tile of the keys takes 1.4 of the rows')
+    const int64_t row_tiles = ceil_div64(a.n, GRAD_ROWS);
+    const int64_t share = (units * pl.key_blocks * pl.rt.tiles * 7 / 5 + units * pl.row_blocks * row_tiles) / sm;
+    auto splits = [&](int64_t tiles, int64_t most) {
+        if (most < MIN_TILES) most = MIN_TILES;
+        return (int)(tiles > 2 * most ? ceil_div64(tiles, most) : 1);
     };
-    pl.key_splits = splits(pl.rt.tiles);
-    pl.row_splits = splits(ceil_div64(a.n, GRAD_ROWS));
+    pl.key_splits = splits(pl.rt.tiles, share * 5 / 7);
+    pl.row_splits = splits(row_tiles, share);
     pl.stat_bytes = (size_t)round_up64(units * pl.rt.tiles * GRAD_ROWS * 8, 256);
     const int64_t keys = units * a.n * a.d, rows = a.batch * a.queries * a.heads * a.d;
     pl.key_part_bytes = pl.key_splits > 1 ? (size_t)round_up64(pl.key_splits * 2 * keys * 4, 256) : 0;

@@ -150,6 +150,13 @@ class B200IndexFlat:
         self.metric_type = metric
         self.storage = storage
         self.is_trained = True
+        self._reads = {}   # of attend(), by stream: the last one's event
+
+    def _finish_reads(self):
+        """Rows do not move or go while attend() reads them on another stream than the index's own."""
+        for event in self._reads.values():
+            event.synchronize()
+        self._reads.clear()
 
     # -- faiss::Index surface ---------------------------------------------------------
     @property
@@ -162,9 +169,11 @@ class B200IndexFlat:
         n = int(x.shape[0])
         _check(x, "add: x", "float32", (n, self.d))
         self.resources._order_after_torch(x)
+        self._finish_reads()
         abi.check(abi.lib().b200f_index_add(self._h, n, _ptr(x) if n else None), "add")
 
     def reserve(self, n: int):
+        self._finish_reads()
         abi.check(abi.lib().b200f_index_reserve(self._h, int(n)), "reserve")
 
     def search(self, x, k: int, distances=None, labels=None):
@@ -225,14 +234,15 @@ class B200IndexFlat:
 
         Inner-product indexes with FP16 or BF16 storage and d a multiple of 8 up to 128.  x [n, d] and values [ntotal, d]: torch
         CUDA tensors of the storage's type on the index's device.  scale: 1 / sqrt(d) by default.  Returns [n, d] and, with
-        return_lse, the log-sums, float32 [n].  Queued on torch's current stream; later calls of the index wait for it.  Not
-        while that stream is captured."""
+        return_lse, the log-sums, float32 [n].  Queued on torch's current stream; add(), reset() and close() wait for it.  Not while that
+        stream is captured."""
         from . import attention
         return attention.attend_index(self, x, values, scale, return_lse)
 
     def reset(self):
         """Removes all rows.  Their device memory stays mapped for the next add(), up to 8 GiB a device;
         StandardB200Resources.release_retained() gives it back."""
+        self._finish_reads()
         abi.check(abi.lib().b200f_index_reset(self._h), "reset")
 
     def reconstruct(self, key: int) -> np.ndarray:
@@ -280,6 +290,7 @@ class B200IndexFlat:
 
     def close(self):
         if getattr(self, "_h", None):
+            self._finish_reads()
             abi.lib().b200f_index_destroy(self._h)
             self._h = None
 

@@ -142,7 +142,8 @@ def test_nan_in_a_seen_key_comes_through(fm, lq, bad):
     assert (torch.isnan(lse) if math.isnan(bad) else torch.isnan(lse) | (lse == math.inf)).all()
 
 
-@pytest.mark.parametrize("shape", [(4, 15, 3000, 8, 2, 128), (2, 333, 1111, 6, 2, 64), (8, 1, 700, 8, 2, 128), (2, 600, 600, 8, 2, 128)], ids=str)
+@pytest.mark.parametrize("shape", [(4, 15, 3000, 8, 2, 128), (4, 15, 3000, 8, 2, 64), (2, 333, 1111, 6, 2, 64), (8, 1, 700, 8, 2, 128), (2, 600, 600, 8, 2, 128),
+                                   (1, 60, 3000, 2, 2, 128), (24, 40, 800, 14, 2, 128)], ids=str)
 def test_results_do_not_depend_on_timing(fm, shape):
     # the same bits again and again, beside other work on the GPU
     b, lq, lk, h, hk, d = shape
@@ -159,7 +160,14 @@ def test_results_do_not_depend_on_timing(fm, shape):
         with torch.cuda.stream(other):
             for _ in range(i % 5):
                 noise @ noise
-        assert all(torch.equal(x, y) for x, y in zip(want, run()))
+        for name, x, y in zip(("out", "lse", "grad_q", "grad_k", "grad_v", "mass"), want, run()):
+            assert torch.equal(x, y), (name, i)
+    # the forward pass alone, many times: tiles that come out of the L2 cache are refilled soon after they are given back
+    for i in range(400):
+        if i % 3 == 0:
+            with torch.cuda.stream(other):
+                noise @ noise
+        assert torch.equal(want[0], fm.attend(q, k, v)), i
     torch.cuda.synchronize()
     fm.check_attention_status()
 
