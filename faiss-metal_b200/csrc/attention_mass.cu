@@ -264,13 +264,9 @@ mass_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ C
                                         make_float2(c, c), make_float2(__uint_as_float(l.z), __uint_as_float(l.w)));
                     }
 #pragma unroll
-                    for (int e = 0; e < (FEW ? 4 : 2); e++) {
+                    for (int e = 0; e < 4; e++) {
                         y[e].x = ex2(y[e].x);
                         y[e].y = ex2(y[e].y);
-                    }
-                    if (!FEW) {   // half of them: the exponential unit bounds this loop
-                        y[2] = ex2_fma(y[2]);
-                        y[3] = ex2_fma(y[3]);
                     }
                     if (masked) {
 #pragma unroll

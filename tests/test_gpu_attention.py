@@ -78,6 +78,10 @@ TILES = [
     (1, 2048, 384, 4, 4, 128, None),
     (24, 17, 800, 14, 2, 128, None),
     (2, 40, 9000, 3, 1, 8, (9000, 4000)),
+    (24, 17, 900, 14, 2, 64, tuple(40 * i for i in range(23)) + (900,)),
+    (40, 30, 700, 4, 2, 128, tuple(17 * i for i in range(40))),
+    (4, 32, 6000, 8, 2, 64, (6000, 5999, 129, 3000)),
+    (4, 32, 6000, 8, 2, 128, (6000, 0, 4481, 3000)),
 ]
 
 
@@ -309,6 +313,8 @@ SHARED = [
     (2, 150, 3000, 2900, 8, 2, 128, (1500, 2900)),
     (3, 200, 1, 1700, 8, 2, 96, (200, 1700, 30)),
     (64, 1, 4000, 1, 32, 4, 72, None),
+    (8, 2, 30000, 100, 16, 4, 128, (100, 2, 3, 50, 64, 65, 99, 7)),
+    (8, 2, 30000, 100, 16, 4, 64, None),
 ]
 
 
