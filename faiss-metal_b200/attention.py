@@ -28,6 +28,7 @@ from . import abi
 _STORAGE = {"float16": abi.STORAGE_F16, "bfloat16": abi.STORAGE_BF16}
 MAX_WIDTH = 128
 MAX_GROUP = 128
+MAX_SCALE = 2e38
 
 
 def check_attention_status(synchronize: bool = True) -> None:
@@ -120,9 +121,9 @@ class _Check:
             raise ValueError("%s: %s: query heads of one key head must not repeat" % (self.what, name))
 
     def scale(self, scale, d: int) -> float:
-        s = 1.0 / math.sqrt(d) if scale is None else float(scale)
-        if not (0.0 < s < 3.0e38):
-            raise ValueError("%s: scale must be positive and finite" % self.what)
+        s = 1.0 / math.sqrt(d) if scale is None else scale
+        if not (0.0 < s <= MAX_SCALE):
+            raise ValueError("%s: scale must be positive and at most %g" % (self.what, MAX_SCALE))
         return s
 
     def plan(self, args, fn: str, with_scratch: bool = True):
@@ -150,6 +151,11 @@ def _keep(key, plan):
         _plans.clear()
     _plans[key] = plan
     return plan
+
+
+def _number(x):
+    """An option as a plain number, as it is now: it goes into a plan's key."""
+    return None if x is None else float(x)
 
 
 def _look(what: str, *tensors):
@@ -229,6 +235,7 @@ def attend(q, k, v, *, key_lengths=None, scale=None, return_lse=False):
     return_lse also the log of each row's sum of exponentials, float32 [batch, queries, heads].  A sequence that sees no
     key has output 0 and log-sum -inf."""
     import torch
+    scale = _number(scale)
     key = tuple(_look("attend", q, k, v, key_lengths) + [scale])
     plan = _plans.get(key)
     if plan is None:
@@ -263,6 +270,7 @@ def attend_backward(grad_out, q, k, v, out, lse, *, key_lengths=None, scale=None
     Keys that no query sees get 0.  Where k or v repeat sequences or heads (stride 0), their gradients come
     for every repetition; add them up."""
     import torch
+    scale = _number(scale)
     key = tuple(_look("attend_backward", grad_out, q, k, v, out, lse, key_lengths) + [scale])
     plan = _plans.get(key)
     if plan is None:
@@ -305,6 +313,7 @@ def attend_shared(q, shared_k, shared_v, own_k, own_v, own_lengths=None, *, scal
     the whole prefix and the own rows j < own_lengths[b] - new + 1 + t.  Returns the output, like q, and with return_lse the log-sums
     over both parts, float32 [batch, new, heads]."""
     import torch
+    scale = _number(scale)
     key = tuple(_look("attend_shared", q, shared_k, shared_v, own_k, own_v, own_lengths) + [scale])
     plan = _plans.get(key)
     if plan is None:
@@ -348,6 +357,7 @@ def attention_mass(q, k, lse, *, key_lengths=None, scale=None, causal=False, mas
     k are the own rows and causal is True (query t sees j < key_lengths[b] - queries + 1 + t), or the prefix, as one
     sequence."""
     import torch
+    scale = _number(scale)
     key = tuple(_look("attention_mass", q, k, lse, key_lengths, mass) + [scale, bool(causal)])
     plan = _plans.get(key)
     if plan is None:
@@ -385,6 +395,7 @@ def evict(k, v, mass, key_lengths=None, keep=1, *, recent=0):
     (k, v, mass, rows, lengths): caches of `keep` rows in the old order, zero behind the last one, their mass [batch, key heads,
     keep], the row each slot was (int32, -1 behind the last one) and the new lengths (int32 [batch])."""
     import torch
+    keep, recent = int(keep), int(recent)
     key = tuple(_look("evict", k, v, mass, key_lengths) + [keep, recent])
     plan = _plans.get(key)
     if plan is None:
@@ -396,11 +407,11 @@ def evict(k, v, mass, key_lengths=None, keep=1, *, recent=0):
         c.shape(v, "v", (b, n, hk, d))
         if hk < 1 or d < 8 or d > 1024 or d % 8:
             raise ValueError("evict: width %d of %d key heads: expected a multiple of 8 up to 1024, and a head" % (d, hk))
-        if int(keep) < 1 or int(recent) < 0 or int(recent) > int(keep):
+        if keep < 1 or recent < 0 or recent > keep:
             raise ValueError("evict: expected keep >= 1 and 0 <= recent <= keep, got %d and %d" % (keep, recent))
         c.dense(mass, "mass", (b, hk, n), torch.float32)
         c.lengths(key_lengths, b)
-        a.batch, a.n, a.kv_heads, a.d, a.storage, a.keep, a.recent = b, n, hk, d, c.storage, int(keep), int(recent)
+        a.batch, a.n, a.kv_heads, a.d, a.storage, a.keep, a.recent = b, n, hk, d, c.storage, keep, recent
         plan = _keep(key, c.plan(a, "b200f_evict", with_scratch=False))
         plan.outs = [_Output((b, a.keep, hk, d), c.dtype, c.device)] * 2 + [
             _Output((b, hk, a.keep), torch.float32, c.device), _Output((b, hk, a.keep), torch.int32, c.device),
@@ -418,6 +429,7 @@ def evict(k, v, mass, key_lengths=None, keep=1, *, recent=0):
 def attend_index(index, x, values, scale, return_lse):
     """B200IndexFlat.attend()."""
     import torch
+    scale = _number(scale)
     n, d = index.ntotal, index.d
     key = tuple(_look("attend", x, values) + [scale, n, d, index.storage, index.metric_type, index.resources.device])
     plan = _plans.get(key)
@@ -439,6 +451,9 @@ def attend_index(index, x, values, scale, return_lse):
         _sizes(a, 1, x.shape[0], n, 1, 1, d, c.storage, c.scale(scale, d))
         plan = _keep(key, c.plan(a, "b200f_attend"))
         plan.out, plan.lse = _Output(x.shape, c.dtype, c.device), _Output(x.shape[:1], torch.float32, c.device)
+    if torch._C._cuda_getDevice() != plan.index:   # streams, captures and events below are those of the index's device
+        with torch.cuda.device(plan.index):
+            return attend_index(index, x, values, scale, return_lse)
     if torch.cuda.is_current_stream_capturing():
         raise ValueError("attend: the rows of an index may move, a graph cannot hold their address")
     a = abi.AttendArgs.from_buffer_copy(plan.proto)

@@ -632,7 +632,7 @@ extern "C" size_t b200f_attend_backward_scratch_bytes(const B200FAttendBackwardA
 extern "C" int b200f_attend_backward(const B200FAttendBackwardArgs* a) {
     const int rc = check_grad(a);
     if (rc != B200F_OK) return rc;
-    if (a->batch == 0) return B200F_OK;
+    if (a->batch == 0 || (a->queries == 0 && a->n == 0)) return B200F_OK;
     const AttView g = att_view(a->grad_out, a->grad_out_stride), q = att_view(a->q, a->q_stride);
     const AttView k = att_view(a->k, a->k_stride), v = att_view(a->v, a->v_stride);
     auto aligned = [](const void* x) { return x && (reinterpret_cast<uintptr_t>(x) & 15) == 0; };

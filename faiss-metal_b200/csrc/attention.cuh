@@ -7,6 +7,7 @@ namespace b200f {
 
 constexpr int ATT_MAX_D = 128;
 constexpr int ATT_MAX_GROUP = 128;   // query heads a key head
+constexpr float ATT_MAX_SCALE = 2e38f;   // scale * log2(e) is finite
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
@@ -32,7 +33,7 @@ inline bool att_view_ok(const AttView& v, int64_t batch, int64_t rows, int64_t h
 inline int att_sizes_ok(int64_t batch, int64_t queries, int64_t n, int heads, int kv_heads, int d, int storage, float scale) {
     if (storage != B200F_STORAGE_F16 && storage != B200F_STORAGE_BF16) return B200F_ERR_BAD_ARG;
     if (batch < 0 || queries < 0 || n < 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads != 0 ||
-        heads / kv_heads > ATT_MAX_GROUP || d < 8 || d > ATT_MAX_D || d % 8 != 0 || !(scale > 0.f) || scale > 3.0e38f)
+        heads / kv_heads > ATT_MAX_GROUP || d < 8 || d > ATT_MAX_D || d % 8 != 0 || !(scale > 0.f) || scale > ATT_MAX_SCALE)
         return B200F_ERR_BAD_ARG;
     const int64_t lim = ((int64_t)1 << 31) - 1;
     if (n > lim - 1024 || batch > lim || queries > lim || kv_heads > 65535 || (batch > 0 && queries > lim / batch) ||

@@ -367,7 +367,7 @@ typedef struct B200FAttendArgs {
     int64_t batch, queries;
     int32_t heads, kv_heads, d, storage;
     int32_t causal;             /* of the own keys */
-    float scale;                /* > 0 */
+    float scale;                /* > 0, up to 2e38 */
 } B200FAttendArgs;
 size_t b200f_attend_scratch_bytes(const B200FAttendArgs* args);   /* pointers are not looked at; 0 also on bad arguments */
 /* out = softmax(scale * q k^T) v over the shared and the own keys together. */

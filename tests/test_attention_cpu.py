@@ -136,3 +136,57 @@ def test_definitions_against_autograd():
     # weights of a query sum to one over the keys
     m = R.mass(q.detach(), k.detach(), lse.detach(), n)
     assert torch.allclose(m.sum(-1), torch.full((2, 2), 10.0, dtype=torch.float64))
+
+
+def test_scale_that_overflows_in_base_2(fm):
+    L = fm.lib()
+    a = attend_args(fm, scale=2.5e38)
+    assert L.b200f_attend_scratch_bytes(ctypes.byref(a)) == 0
+    assert L.b200f_attend(ctypes.byref(a)) == fm.abi.ERR_BAD_ARG
+
+
+def test_gradient_of_neither_queries_nor_keys(fm):
+    b = fm.abi.AttendBackwardArgs()
+    for name, x in dict(status=64, batch=2, heads=4, kv_heads=2, d=64, storage=2, scale=0.125, scratch=4096, scratch_bytes=1 << 20).items():
+        setattr(b, name, x)
+    assert fm.lib().b200f_attend_backward(ctypes.byref(b)) == 0
+
+
+def test_index_reads_belong_to_the_index_device(fm, monkeypatch):
+    # current device 0, index on device 1: the call goes on under the index's device, before it looks at captures, streams and events
+    from importlib import import_module
+    A = import_module(fm.__name__ + ".attention")
+    where = [0]
+
+    class device:
+        def __init__(self, i):
+            self.i = i
+
+        def __enter__(self):
+            self.old, where[0] = where[0], self.i
+
+        def __exit__(self, *_):
+            where[0] = self.old
+
+    class event:
+        def record(self):
+            seen.append(("event", where[0]))
+
+    seen = []
+    plan = type("plan", (), dict(index=1, proto=bytes(fm.abi.AttendArgs()), out=staticmethod(lambda: x), lse=None, what="attend"))
+    x = torch.zeros(2, 64, dtype=torch.float16)
+    index = type("index", (), dict(ntotal=2, d=64, storage=1, metric_type=0, _reads={}, device_rows=lambda self: 64,
+                                   resources=type("r", (), dict(device=1))))()
+
+    class plans(dict):
+        def get(self, key):
+            return plan
+
+    monkeypatch.setattr(A, "_plans", plans())
+    monkeypatch.setattr(A, "_run", lambda *_: seen.append(("run", where[0])))
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: where[0], raising=False)
+    monkeypatch.setattr(torch.cuda, "device", device)
+    monkeypatch.setattr(torch.cuda, "Event", event)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: seen.append(("capture", where[0])))
+    A.attend_index(index, x, x, None, False)
+    assert seen == [("capture", 1), ("run", 1), ("event", 1)]

@@ -614,3 +614,33 @@ def test_nothing_to_do(fm):
     assert fm.attention_mass(q, k, lse).shape == (2, 2, 0)
     nk, nv, nm, rows, n = fm.evict(k, k, e(2, 2, 0, device="cuda"), None, 4)
     assert (nk == 0).all() and (rows == -1).all() and (n == 0).all() and (nm == 0).all()
+
+
+def test_neither_queries_nor_keys(fm):
+    q, k = (torch.empty(2, 0, 2, 64, dtype=torch.float16, device="cuda") for _ in range(2))
+    out, lse = fm.attend(q, k, k, return_lse=True)
+    assert [x.shape for x in fm.attend_backward(q, q, k, k, out, lse)] == [q.shape, k.shape, k.shape]
+    assert fm.attention_mass(q, k, lse).shape == (2, 2, 0)
+
+
+def test_options_given_as_tensors_are_read_at_every_call(fm):
+    dt = torch.float16
+    q, k, v = rand(1, dt, 1, 5, 2, 64), rand(2, dt, 1, 40, 2, 64), rand(3, dt, 1, 40, 2, 64)
+    m = rand(4, torch.float32, 1, 2, 40)
+    scale, keep = torch.tensor(0.5), torch.tensor(8)
+    for s, n in ((0.5, 8), (0.125, 5)):
+        scale.fill_(s)
+        keep.fill_(n)
+        assert torch.equal(fm.attend(q, k, v, scale=scale), fm.attend(q, k, v, scale=s))
+        assert fm.evict(k, v, m, None, keep)[0].shape[1] == n
+
+
+def test_scales_up_to_the_largest(fm):
+    dt = torch.float16
+    q = torch.zeros(1, 20, 1, 64, dtype=dt, device="cuda")
+    v = rand(3, dt, 1, 300, 1, 64)
+    for n in (20, 300):                                     # scores of 0, whatever the scale
+        out = fm.attend(q, torch.ones_like(v[:, :n]), v[:, :n], scale=2e38)
+        assert torch.equal(out, fm.attend(q, torch.ones_like(v[:, :n]), v[:, :n], scale=1.0))
+    with pytest.raises(ValueError):
+        fm.attend(q, v, v, scale=2.5e38)
