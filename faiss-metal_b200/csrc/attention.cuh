@@ -48,13 +48,6 @@ template <>
 __device__ __forceinline__ float to_f32<__half>(uint16_t u) { return __half2float(__ushort_as_half(u)); }
 template <>
 __device__ __forceinline__ float to_f32<__nv_bfloat16>(uint16_t u) { return __bfloat162float(__ushort_as_bfloat16(u)); }
-template <typename T>
-__device__ __forceinline__ uint16_t from_f32(float f);
-template <>
-__device__ __forceinline__ uint16_t from_f32<__half>(float f) { return __half_as_ushort(__float2half_rn(f)); }
-template <>
-__device__ __forceinline__ uint16_t from_f32<__nv_bfloat16>(float f) { return __bfloat16_as_ushort(__float2bfloat16_rn(f)); }
-
 // Keys that query t of sequence b sees: its length, clamped, and the causal end.
 struct AttLengths {
     const int32_t* lengths;   // null: all n

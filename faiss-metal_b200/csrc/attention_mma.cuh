@@ -78,23 +78,6 @@ __device__ __forceinline__ void tc_st16(uint32_t taddr, const uint32_t* r) {
               "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
             : "memory");
 }
-// 32 lanes x 16 consecutive columns, and the wait tied to the registers of one load
-__device__ __forceinline__ void tc_ld16(uint32_t taddr, uint32_t (&r)[16]) {
-    asm volatile(
-            "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
-            "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-            : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-              "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-            : "r"(taddr)
-            : "memory");
-}
-__device__ __forceinline__ void tc_wait_ld16(uint32_t (&r)[16]) {
-    asm volatile("tcgen05.wait::ld.sync.aligned;"
-                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
-                   "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
-                 :
-                 : "memory");
-}
 // 32 lanes x 16 consecutive columns, complete on return
 __device__ __forceinline__ void tc_ld16_wait(uint32_t taddr, uint32_t (&r)[16]) {
     asm volatile(
@@ -107,16 +90,6 @@ __device__ __forceinline__ void tc_ld16_wait(uint32_t taddr, uint32_t (&r)[16]) 
             : "memory");
 }
 __device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-
-// 32 lanes x 64 consecutive columns, complete on return
-__device__ __forceinline__ void tc_ld64_wait(uint32_t taddr, uint32_t (&r)[64]) {
-    uint32_t (&a)[32] = *reinterpret_cast<uint32_t (*)[32]>(&r[0]);
-    uint32_t (&b)[32] = *reinterpret_cast<uint32_t (*)[32]>(&r[32]);
-    tc_ld32(taddr, a);
-    tc_ld32(taddr + 32, b);
-    tc_wait_ld32(a);
-    tc_wait_ld32(b);
-}
 
 // two at once
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {

