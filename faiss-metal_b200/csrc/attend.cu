@@ -545,8 +545,9 @@ attend_few_kernel(const __grid_constant__ CUtensorMap map_sk, const __grid_const
     const uint32_t bar_full = sbase + FEW_SM_BAR<DP>, bar_empty = bar_full + STAGES * 8;
     volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + FEW_SM_BAR<DP> + 2 * STAGES * 8);
 
-    // Launched behind the tile kernel of the same call, whose inputs are complete and whose results it does not read: it waits for
-    // that kernel only when it ends, so that whoever waits for it has both.
+    // Launched behind the tile kernel of the same call, whose inputs are complete and whose results it does not read: it runs on the SMs
+    // that this one leaves free, and its last CTA waits for it at its end, so that whoever waits for this grid has both.  (All CTAs
+    // waiting would keep those SMs from taking the next.)
     pdl_trigger();
     if ((sbase & 1023u) != 0) {
         if (threadIdx.x == 0) atomicOr(p.status, kDevErrSmemAlign);
@@ -787,7 +788,7 @@ attend_few_kernel(const __grid_constant__ CUtensorMap map_sk, const __grid_const
             }
         }
     }
-    pdl_wait();
+    if (blockIdx.x == gridDim.x - 1) pdl_wait();
 }
 
 // ---- attend_join_kernel: partial results of a row become its result ------------------
@@ -908,6 +909,28 @@ double cut_few(Segment& s, int64_t units, int64_t rows, bool joined) {
            (!joined && s.splits > 1 ? JOIN_US : 0);
 }
 
+// Tiles beside blocks of 16 rows, which take few_us on all SMs: as many SMs for the tiles as make both end soonest.  64 tokens, 32 heads on 8, behind
+// 32,768 shared and up to 1,024 own rows: 80 us with 0.6 - 0.7 of the SMs, 90 us with all, one kernel after the other; 128 tokens, 16
+// heads on 2, behind 4,096 and up to 512: 33 - 36 us against 43; with all but 5 us the tiles' work all is best (32 x 2 tokens behind 65,536 rows: 73 us
+// against 78 with 0.8).
+void leave_sms(Segment& s, int64_t units, int64_t rows, double few_us) {
+    const double sm = (double)cached_sm_count();
+    const int64_t base = units * s.row_blocks;
+    Segment best = s;
+    double least = 1e30;
+    for (int64_t splits = s.splits; splits >= 1; splits--) {
+        Segment t = s;
+        const double us = cut_tiles(t, units, rows, (double)(base * splits), true), left = sm - (double)t.items;
+        if (left < 0) continue;
+        const double total = left * us >= few_us * sm ? us : (us * (double)t.items + few_us * sm) / sm;
+        if (total < least) {
+            least = total;
+            best = t;
+        }
+    }
+    s = best;
+}
+
 AttendPlan plan_attend(const B200FAttendArgs& a) {
     AttendPlan pl{};
     const int group = a.heads / a.kv_heads;
@@ -915,7 +938,7 @@ AttendPlan plan_attend(const B200FAttendArgs& a) {
     const bool joined = a.shared_n > 0 && a.n > 0;
     int64_t units[2], rows_of[2];
     bool on[2];
-    double weight[2] = {0, 0};
+    double weight[2] = {0, 0}, few_us[2] = {0, 0};
     for (int i = 0; i < 2; i++) {
         Segment& s = pl.seg[i];
         units[i] = i == 0 ? a.kv_heads : a.batch * a.kv_heads;
@@ -930,16 +953,18 @@ AttendPlan plan_attend(const B200FAttendArgs& a) {
             continue;
         }
         Segment tile = s;
-        const double few_us = cut_few(s, units[i], rows_of[i], joined);
+        few_us[i] = cut_few(s, units[i], rows_of[i], joined);
         if (rows_of[i] <= FEW_ROWS) continue;
-        if (cut_tiles(tile, units[i], rows_of[i], sm, joined) < few_us) {
+        if (cut_tiles(tile, units[i], rows_of[i], sm, joined) < few_us[i]) {
             s = tile;
             weight[i] = (double)units[i] * s.row_blocks * (double)ceil_div64(s.n, TILE_KEYS);
         }
     }
-    // both by tiles: each gets the SMs that its tiles ask for
+    // both by tiles: each gets the SMs that its tiles ask for; one: it leaves some to the other kernel
     if (weight[0] > 0 && weight[1] > 0)
         for (int i = 0; i < 2; i++) (void)cut_tiles(pl.seg[i], units[i], rows_of[i], sm * weight[i] / (weight[0] + weight[1]), joined);
+    for (int i = 0; i < 2; i++)
+        if (weight[i] > 0 && on[1 - i] && pl.seg[1 - i].few) leave_sms(pl.seg[i], units[i], rows_of[i], few_us[1 - i]);
     for (int i = 0; i < 2; i++) {
         Segment& s = pl.seg[i];
         s.part0 = pl.parts;

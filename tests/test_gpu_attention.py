@@ -644,3 +644,22 @@ def test_scales_up_to_the_largest(fm):
         assert torch.equal(out, fm.attend(q, torch.ones_like(v[:, :n]), v[:, :n], scale=1.0))
     with pytest.raises(ValueError):
         fm.attend(q, v, v, scale=2.5e38)
+
+
+@pytest.mark.parametrize("shape", [(64, 1, 5000, 700, 32, 8, 128), (128, 1, 4096, 512, 16, 2, 64), (33, 2, 9000, 60, 8, 2, 96)], ids=str)
+def test_prefix_and_own_rows_at_the_same_time(fm, shape):
+    b, t, p, n, h, hk, d = shape
+    dt = torch.bfloat16
+    q, pk, pv = rand(1, dt, b, t, h, d, scale=1.5), rand(2, dt, p, hk, d), rand(3, dt, p, hk, d)
+    k, v = rand(4, dt, b, n, hk, d), rand(5, dt, b, n, hk, d)
+    length = torch.randint(0, n + 1, (b,), generator=torch.Generator().manual_seed(6)).int().cuda()
+    out, lse = fm.attend_shared(q, pk, pv, k, v, length, return_lse=True)
+    check_out(out, lse, R.attend(q, k, v, length, causal=True, shared=(pk, pv)), dt, p + n)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        captured = fm.attend_shared(q, pk, pv, k, v, length) + 0       # read at once by a kernel that is launched plainly
+    for _ in range(100):
+        assert torch.equal(fm.attend_shared(q, pk, pv, k, v, length), out)
+        g.replay()
+        assert torch.equal(captured, out)
+    fm.check_attention_status()
