@@ -347,7 +347,9 @@ MassPlan plan_mass(const B200FAttentionMassArgs& a) {
     } else {
         pl.blocks = (int)tiles;
         int64_t s = units * tiles > 0 ? 4 * sm / (units * tiles) : 1;
-        if (s > pl.rt.tiles / 2) s = pl.rt.tiles / 2;
+        // at least four row tiles a range: joining costs 3 us, as much as four take (8 heads of 4 x 512 queries and keys, d = 64: 8.8 us in one
+        // range, 10.2 in two; 12 heads of 3 x 700 over 300: 10.2 and 13.2 in three; 4 key heads, 4,444 rows over 2,049: 40 and 22 in eight)
+        if (s > pl.rt.tiles / 4) s = pl.rt.tiles / 4;
         pl.splits = (int)(s < 1 ? 1 : s);
     }
     pl.scratch = 256 + (pl.splits > 1 ? (size_t)pl.splits * units * a.n * 4 : 0);
