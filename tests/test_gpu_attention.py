@@ -663,3 +663,33 @@ def test_prefix_and_own_rows_at_the_same_time(fm, shape):
         g.replay()
         assert torch.equal(captured, out)
     fm.check_attention_status()
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_a_reader_is_trained(fm, dtype):
+    """attend and attend_backward as the two halves of an autograd function, under eager calls and side streams."""
+    dt = TYPES[dtype]
+
+    class Read(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, q, k, v, n):
+            out, lse = fm.attend(q, k, v, key_lengths=n, return_lse=True)
+            ctx.save_for_backward(q, k, v, n, out, lse)
+            return out
+
+        @staticmethod
+        def backward(ctx, grad):
+            q, k, v, n, out, lse = ctx.saved_tensors
+            return (*fm.attend_backward(grad.contiguous(), q, k, v, out, lse, key_lengths=n), None)
+
+    q, k, v = (rand(i, dt, *s).requires_grad_() for i, s in ((1, (2, 140, 4, 64)), (2, (2, 333, 2, 64)), (3, (2, 333, 2, 64))))
+    n, w = lens(333, 65), rand(4, dt, 2, 140, 4, 64)
+    for stream in (torch.cuda.current_stream(), torch.cuda.Stream()):
+        stream.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(stream):
+            (Read.apply(q, k, v, n) * w).sum().backward()
+        torch.cuda.current_stream().wait_stream(stream)
+        check_grads([x.grad for x in (q, k, v)], R.backward(w, q.detach(), k.detach(), v.detach(), n), dt)
+        for x in (q, k, v):
+            x.grad = None
+    fm.check_attention_status()
