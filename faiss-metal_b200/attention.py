@@ -310,7 +310,8 @@ def attend_shared(q, shared_k, shared_v, own_k, own_v, own_lengths=None, *, scal
     q [batch, new, heads, width]: the last `new` tokens of every sequence, one when decoding; shared_k, shared_v [prefix,
     key heads, width]; own_k, own_v [batch, rows, key heads, width], with the new tokens' rows already in them;
     own_lengths (int32 [batch], on the device): rows of each sequence, the new ones included (default: all).  Query t sees
-    the whole prefix and the own rows j < own_lengths[b] - new + 1 + t.  Returns the output, like q, and with return_lse the log-sums
+    the whole prefix and the own rows j < own_lengths[b] - new + 1 + t (a value that is infinite or NaN in a row that only later queries see may
+    reach it all the same).  Returns the output, like q, and with return_lse the log-sums
     over both parts, float32 [batch, new, heads]."""
     import torch
     scale = _number(scale)
