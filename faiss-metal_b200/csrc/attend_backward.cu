@@ -532,8 +532,9 @@ GradPlan plan_grad(const B200FAttendBackwardArgs& a) {
         if (most < MIN_TILES) most = MIN_TILES;
         return (int)(tiles > 2 * most ? ceil_div64(tiles, most) : 1);
     };
-    pl.key_splits = splits(pl.rt.tiles, share * 5 / 7);
-    pl.row_splits = splits(row_tiles, share);
+    // with nothing on one side there are no sums on the other to cut
+    pl.key_splits = a.n > 0 ? splits(pl.rt.tiles, share * 5 / 7) : 1;
+    pl.row_splits = a.queries > 0 ? splits(row_tiles, share) : 1;
     pl.stat_bytes = (size_t)round_up64(units * pl.rt.tiles * GRAD_ROWS * 8, 256);
     const int64_t keys = units * a.n * a.d, rows = a.batch * a.queries * a.heads * a.d;
     pl.key_part_bytes = pl.key_splits > 1 ? (size_t)round_up64(pl.key_splits * 2 * keys * 4, 256) : 0;
