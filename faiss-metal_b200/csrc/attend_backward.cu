@@ -29,7 +29,14 @@ template <int DP>
 constexpr int GRAD_A_BYTES = DP / 64 * ATT_CHUNK;
 template <int DP>
 constexpr int GRAD_B_BYTES = DP / 64 * GRAD_ROWS * 128;
-constexpr int GRAD_STAT_BYTES = GRAD_ROWS * 8;
+// Statistics of a streamed tile (see grad_stat_kernel), GRAD_ROWS of each: bf16 two floats; fp16 two floats and a 16-bit word, which the keys'
+// pass takes, and two more floats.
+template <typename T>
+constexpr int GRAD_STATS = (std::is_same<T, __half>::value ? 18 : 8) * GRAD_ROWS / 4;   // floats
+template <typename T>
+constexpr int GRAD_KEY_STAT_BYTES = (std::is_same<T, __half>::value ? 10 : 8) * GRAD_ROWS;
+constexpr int GRAD_STAT_BYTES = GRAD_KEY_STAT_BYTES<__half>;   // room for them in a stage
+constexpr int STAT_DELTA = GRAD_ROWS, STAT_MOVED = 2 * GRAD_ROWS, STAT_ALONE = 5 * GRAD_ROWS / 2, STAT_FACTOR = 7 * GRAD_ROWS / 2;
 template <int DP, bool KEYS>
 constexpr int GRAD_STAGES = DP == 64 ? 8 : KEYS ? 4 : 6;
 template <int DP, bool KEYS>
@@ -50,8 +57,9 @@ struct GradParams {
     AttView q, g;            // queries and output gradients (KEYS = false: A1 and A2 are read with plain loads)
     AttLengths len;
     RowTiles rt;             // query rows in tiles of GRAD_ROWS
-    const float* stat;       // [unit][tile]: of every slot minus the lse in base 2 (-INF: no row), then minus delta
-    const uint32_t* gmax;    // fp16: bit pattern of the largest |do|
+    const float* stat;       // [unit][tile][GRAD_STATS]
+    const uint32_t* range;   // fp16: [2][unit], see UnitRange
+    int64_t units;
     int64_t queries;
     int heads, kv_heads, group, d;
     float scale;
@@ -64,48 +72,99 @@ struct GradParams {
     int32_t* status;
 };
 
-// fp16 score gradients are multiplied by a power of two that brings the largest element of do into [2^-3, 2^-2): they stay clear of fp16's
-// subnormals.  |ds| <= |do| |v - o| <= 2^-2 sqrt(128) * 2 max |v|, below 65504 while a value row's norm is below 11,500.
-__device__ __forceinline__ float grad_factor(uint32_t max_bits) {
-    const int e = (int)(max_bits >> 23) - 127;
-    return max_bits == 0 || e > 126 ? 1.f : exp2f((float)min(max(-3 - e, -100), 100));
+// fp16: powers of two keep what is rounded to 16 bits clear of subnormals and of overflow.
+// Weights are held 2^12 up: n of them, each 1 / n, are normal numbers up to n = 2^26.
+// A row's score gradients are at most |do| |v - o| <= 2 |do| max |v|, over the values that its sequence sees.  With |do| < 2^ld, |v| < 2^lv and
+// |q| < 2^lq (the largest entry) the factor 2^(13 - lv - ld) brings that bound to [2^12, 2^14), whatever other rows hold.  dq takes
+// it as it is: a row is a thread's own.  dk adds up rows of different factors 2^e, so that the rows of q take the rest 2^x of a common 2^E, e + x = E
+// (grad_stat_kernel writes them, exactly but for entries below 2^-22 of the row's largest): E is the largest for which no row of the unit passes
+// 2^15 with x, and a row's own factor is kept unless |do| |q| is below 2^-17 of the unit's largest (the largest entry of 2^x q stays at 2^-3
+// or more).  One factor for the call, from the largest |do|, lost rows 2^10 below it to subnormals (grad_q 12 % off at 4,096 keys).
+// Terms below 2^-26 of their row's bound lose bits still: weights of 2^-22 and less where a value row is much longer than those that count.
+constexpr int WEIGHT_BITS = 12, DS_BITS = 13, Q_BITS = 15, Q_LEAST_BITS = -2;
+__device__ __forceinline__ float power_of_2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }   // |e| <= 126
+// |x| < 2^(this), at least half of that
+__device__ __forceinline__ int bits_above(float x) { return (int)((__float_as_uint(x) >> 23) & 255u) - 126; }
+// of a norm, from its square
+__device__ __forceinline__ int norm_bits(float square) { return (bits_above(square) + 1) >> 1; }
+__device__ __forceinline__ bool usable(float largest) { return largest > 0.f && largest < CUDART_INF_F; }
+// 8 entries of an fp16 row: their squares added, their largest magnitude (INF where one is not finite)
+__device__ __forceinline__ void add_square(const uint4& x, float* square) {
+    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        const float a = to_f32<__half>((uint16_t)w[e]), b = to_f32<__half>((uint16_t)(w[e] >> 16));
+        *square = fmaf(a, a, fmaf(b, b, *square));
+    }
+}
+__device__ __forceinline__ void add_largest(const uint4& x, float* top) {
+    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        const float a = fabsf(to_f32<__half>((uint16_t)w[e])), b = fabsf(to_f32<__half>((uint16_t)(w[e] >> 16)));
+        *top = a + b != a + b ? CUDART_INF_F : fmaxf(*top, fmaxf(a, b));
+    }
 }
 
-// Score gradients of 32 columns, ds = p (dp - delta), and the weights p; mstat = minus log-sums and deltas, of the columns (KEYS; an
-// address in shared memory, the deltas behind the log-sums) or the row's.  Steps by groups, as in weigh32.
+// Of the finite rows of a (sequence, key head): the largest ld + lq, and the largest lv.  Held 256 up, 0: none.
+struct UnitRange {
+    int row, value;
+    __device__ __forceinline__ int common() const { return DS_BITS + Q_BITS - value - row; }   // E
+};
+__device__ __forceinline__ UnitRange unit_range(const uint32_t* range, int64_t units, int64_t unit) {
+    const int row = (int)__ldcg(range + unit), value = (int)__ldcg(range + units + unit);
+    return UnitRange{row ? row - 256 : 0, value ? value - 256 : 0};
+}
+
+// Score gradients of 32 columns from `col` on, ds = p (dp - delta), and the weights p.  KEYS: the columns' statistics lie at `mstat` in shared
+// memory, minus log-sums, minus deltas and, fp16, what undoes the move of the query row, 2^-x: c and `factor` are of rows that were not
+// moved, the deltas hold their factor already (16 bits are enough for a power of two, and the products leave shared memory little time: fp16,
+// the case measured above, 1,610 us with both factors read as floats, 1,570 so, 1,475 without any).  Else the row's own.  Steps by groups, as in weigh32.
 template <typename T, bool KEYS>
-__device__ __forceinline__ void grad32(const uint32_t (&s)[32], const uint32_t (&dp)[32], float c, float factor, uint32_t mstat, float mlse,
-                                       float mdelta, uint32_t (&wp)[16], uint32_t (&ws)[16]) {
+__device__ __forceinline__ void grad32(const uint32_t (&s)[32], const uint32_t (&dp)[32], float c, float factor, uint32_t mstat, int col,
+                                       float mlse, float mdelta, uint32_t (&wp)[16], uint32_t (&ws)[16]) {
     constexpr bool HALF = std::is_same<T, __half>::value;
-    const float2 c2 = make_float2(c, c), f2 = make_float2(factor, factor);
 #pragma unroll
     for (int g = 0; g < 16; g += 4) {
-        float2 l[4], d[4], y[4];
-#pragma unroll
-        for (int e = 0; e < 4; e++) l[e] = make_float2(mlse, mlse), d[e] = make_float2(mdelta, mdelta);
-        if (KEYS) {
+        float2 l[4], d[4], y[4], c2[4], f2[4];
+        auto columns = [&](int at, float2 (&x)[4]) __attribute__((always_inline)) {
 #pragma unroll
             for (int e = 0; e < 4; e += 2) {
-                const uint4 a = lds128(mstat + (2 * (g + e)) * 4), b = lds128(mstat + GRAD_ROWS * 4 + (2 * (g + e)) * 4);
-                l[e] = make_float2(__uint_as_float(a.x), __uint_as_float(a.y));
-                l[e + 1] = make_float2(__uint_as_float(a.z), __uint_as_float(a.w));
-                d[e] = make_float2(__uint_as_float(b.x), __uint_as_float(b.y));
-                d[e + 1] = make_float2(__uint_as_float(b.z), __uint_as_float(b.w));
+                const uint4 a = lds128(mstat + (at + col + 2 * (g + e)) * 4);
+                x[e] = make_float2(__uint_as_float(a.x), __uint_as_float(a.y));
+                x[e + 1] = make_float2(__uint_as_float(a.z), __uint_as_float(a.w));
+            }
+        };
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            l[e] = make_float2(mlse, mlse), d[e] = make_float2(mdelta, mdelta), c2[e] = make_float2(c, c), f2[e] = make_float2(factor, factor);
+        if (KEYS) {
+            columns(0, l);
+            columns(STAT_DELTA, d);
+            if (HALF) {
+                const uint4 a = lds128(mstat + STAT_MOVED * 4 + (col + 2 * g) * 2);
+                const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const float2 m = make_float2(__uint_as_float(w[e] << 16), __uint_as_float(w[e] & 0xffff0000u));
+                    c2[e] = mul2(c2[e], m);
+                    f2[e] = mul2(f2[e], m);
+                }
             }
         }
 #pragma unroll
         for (int e = 0; e < 4; e++)
-            y[e] = fma2(make_float2(__uint_as_float(s[2 * (g + e)]), __uint_as_float(s[2 * (g + e) + 1])), c2, l[e]);
+            y[e] = fma2(make_float2(__uint_as_float(s[2 * (g + e)]), __uint_as_float(s[2 * (g + e) + 1])), c2[e], l[e]);
 #pragma unroll
         for (int e = 0; e < 4; e++) {
             y[e].x = ex2(y[e].x);
             y[e].y = ex2(y[e].y);
         }
 #pragma unroll
-        for (int e = 0; e < 4; e++) d[e] = add2(make_float2(__uint_as_float(dp[2 * (g + e)]), __uint_as_float(dp[2 * (g + e) + 1])), d[e]);
-        if (HALF) {
-#pragma unroll
-            for (int e = 0; e < 4; e++) d[e] = mul2(d[e], f2);
+        for (int e = 0; e < 4; e++) {
+            const float2 x = make_float2(__uint_as_float(dp[2 * (g + e)]), __uint_as_float(dp[2 * (g + e) + 1]));
+            if (!HALF) d[e] = add2(x, d[e]);
+            else d[e] = KEYS ? fma2(x, f2[e], d[e]) : mul2(add2(x, d[e]), f2[e]);
         }
 #pragma unroll
         for (int e = 0; e < 4; e++) {
@@ -248,7 +307,7 @@ __device__ __forceinline__ void grad_item(const CUtensorMap& map_k, const CUtens
                                     (int)b * p.vm.batch_step);
                     }
             }
-            const uint32_t bytes = KEYS ? 2 * CHUNKS * p.rt.gb * p.rt.bt * 128 + GRAD_STAT_BYTES : 2 * BBYTES;
+            const uint32_t bytes = KEYS ? 2 * CHUNKS * p.rt.gb * p.rt.bt * 128 + GRAD_KEY_STAT_BYTES<T> : 2 * BBYTES;
             int slot = 0;
             uint32_t phase = 0;
             for (int i = 0; i < n && ok; i++) {
@@ -266,7 +325,7 @@ __device__ __forceinline__ void grad_item(const CUtensorMap& map_k, const CUtens
                                     (int)b * p.gm.batch_step);
                     }
                     bulk_load(sbase + GRAD_SM_STAT<DP, KEYS> + slot * GRAD_STAT_BYTES,
-                              p.stat + ((int64_t)unit * p.rt.tiles + tile) * 2 * GRAD_ROWS, GRAD_STAT_BYTES, full);
+                              p.stat + ((int64_t)unit * p.rt.tiles + tile) * GRAD_STATS<T>, GRAD_KEY_STAT_BYTES<T>, full);
                 } else {
                     for (int c = 0; c < CHUNKS; c++) {
                         tma_load_4d(b1 + c * GRAD_ROWS * 128, &map_b1, full, c * 64, tile * GRAD_ROWS, kvh * p.km.head_step,
@@ -332,14 +391,15 @@ __device__ __forceinline__ void grad_item(const CUtensorMap& map_k, const CUtens
         }
     } else if (warp >= 4) {
         const float c = p.scale * kLog2e;
-        const float factor = HALF ? grad_factor(__ldcg(p.gmax)) : 1.f;
-        float mlse = 0.f, mdelta = 0.f;
+        float mlse = 0.f, mdelta = 0.f, factor = 1.f;
         if (!KEYS && live) {
             const int64_t place = p.rt.place(t, g);
-            const float* const st = p.stat + ((int64_t)unit * p.rt.tiles + place / GRAD_ROWS) * 2 * GRAD_ROWS + place % GRAD_ROWS;
+            const float* const st = p.stat + ((int64_t)unit * p.rt.tiles + place / GRAD_ROWS) * GRAD_STATS<T> + place % GRAD_ROWS;
             mlse = __ldcg(st);
-            mdelta = __ldcg(st + GRAD_ROWS);
+            mdelta = __ldcg(st + (HALF ? STAT_ALONE : STAT_DELTA));
+            if (HALF) factor = __ldcg(st + STAT_FACTOR);
         }
+        if (KEYS && HALF) factor = power_of_2(unit_range(p.range, p.units, unit).common() - WEIGHT_BITS);
         bool ok = true;
         for (int i = wg; i < n; i += 2) {
             ok = wait(bar_s + wg * 8, (i >> 1) & 1);
@@ -367,7 +427,7 @@ __device__ __forceinline__ void grad_item(const CUtensorMap& map_k, const CUtens
             for (int h = 0; h < 2; h++) {
                 uint32_t wp[16], ws[16];
                 if (h == 1) tc_wait_ld32(dp[1]);
-                grad32<T, KEYS>(s[h], dp[h], c, factor, stat + 32 * h * 4, mlse, mdelta, wp, ws);
+                grad32<T, KEYS>(s[h], dp[h], c, factor, stat, 32 * h, mlse, mdelta, wp, ws);
                 if (!KEYS && lim < GRAD_ROWS) {   // keys behind the end
 #pragma unroll
                     for (int e = 0; e < 16; e++) {
@@ -390,7 +450,9 @@ __device__ __forceinline__ void grad_item(const CUtensorMap& map_k, const CUtens
         if (ok) {
             tc_fence_after();
             const bool zero = KEYS && r >= len;
-            const float mul = (KEYS && wg == 1) ? 1.f : p.scale / factor;
+            const float mul = (KEYS && wg == 1) ? 1.f : p.scale;
+            float undo = 1.f;   // of the powers of two
+            if (HALF) undo = KEYS && wg ? power_of_2(-WEIGHT_BITS) : power_of_2(-WEIGHT_BITS) / factor;
             const int64_t at = KEYS ? ((b * p.len.n + r) * p.kv_heads + kvh) * p.d
                                     : ((b * p.queries + t) * p.heads + kvh * p.group + g) * p.d;
             const uint32_t acc = tmem + (KEYS && wg ? TG_ACC2 : TG_ACC1) + lanes;
@@ -404,7 +466,7 @@ __device__ __forceinline__ void grad_item(const CUtensorMap& map_k, const CUtens
                 tc_ld32(acc + col, o);
                 tc_wait_ld32(o);
 #pragma unroll
-                for (int e = 0; e < 32; e++) o[e] = zero ? 0u : __float_as_uint(__uint_as_float(o[e]) * mul);
+                for (int e = 0; e < 32; e++) o[e] = zero ? 0u : __float_as_uint(__uint_as_float(o[e]) * undo * mul);
                 if (!p.part) {
                     stage_columns32<T, COLS>(stage, o, 4 * ch);
                 } else if (live) {
@@ -445,45 +507,133 @@ grad_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ C
     else grad_item<T, DP, false>(map_k, map_v, map_q, map_g, rows, smem, blockIdx.x - key_items);
 }
 
-// ---- grad_stat_kernel: what the gradients need of every query row, 16 lanes a slot ----------------------
-template <typename T>
-__global__ void __launch_bounds__(256) grad_stat_kernel(AttView g, const uint16_t* out, const float* lse, RowTiles rt, int64_t units, int heads,
-                                                        int kv_heads, int d, float* stat, uint32_t* gmax) {
-    const int sub = threadIdx.x & 15;
-    const int64_t i = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
-    const bool in = i < units * rt.tiles * rt.slots;
-    const int64_t tile_of = in ? i / rt.slots : 0, unit = tile_of / rt.tiles;
+// ---- fp16: grad_range_kernel: the units' largest rows (UnitRange) --------------------------------
+// A CTA takes rows of a unit, of do and q or of v, LANES lanes a row and four rows a lane.  A maximum does not depend on the order.  Rows that are
+// not finite, or zero, do not count: their terms are NaN, or 0, whatever the factors.
+template <int LANES>
+constexpr int RANGE_ROWS = 4 * 256 / LANES;
+template <int LANES>
+__global__ void __launch_bounds__(256, 5) grad_range_kernel(AttView g, AttView q, AttView v, AttLengths len, uint32_t units, uint32_t kv_heads,
+                                                            uint32_t group, int d, uint32_t* range) {
+    constexpr int ROWS = RANGE_ROWS<LANES>;
+    const int sub = threadIdx.x % LANES, slot = threadIdx.x / LANES;
+    const uint32_t rows = (uint32_t)len.queries * group;
+    const uint32_t row_blocks = (rows + ROWS - 1) / ROWS, blocks = row_blocks + (uint32_t)((len.n + ROWS - 1) / ROWS);
+    for (uint32_t item = blockIdx.x; item < units * blocks; item += gridDim.x) {   // below 2^31: b200f_attend_backward sees to it
+        const uint32_t unit = item / blocks, block = item - unit * blocks, b = unit / kv_heads, kvh = unit - b * kv_heads;
+        uint32_t most = 0;
+        auto take = [&](bool query, uint32_t row0, uint32_t end) __attribute__((always_inline)) {
+            uint4 x[4], y[4];
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const uint32_t r = row0 + 256 / LANES * k + slot;
+                x[k] = y[k] = make_uint4(0, 0, 0, 0);
+                if (r < end && sub * 8 < d) {
+                    const uint32_t t = query ? r / group : r, h = query ? kvh * group + (r - t * group) : kvh;
+                    x[k] = *reinterpret_cast<const uint4*>((query ? g : v).at(b, t, h) + sub * 8);
+                    if (query) y[k] = *reinterpret_cast<const uint4*>(q.at(b, t, h) + sub * 8);
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                float square = 0.f, top = 1.f;
+                add_square(x[k], &square);
+                if (query) top = 0.f, add_largest(y[k], &top);
+#pragma unroll
+                for (int o = LANES / 2; o > 0; o >>= 1) {
+                    square += __shfl_xor_sync(0xffffffffu, square, o);
+                    if (query) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                }
+                if (usable(square) && usable(top)) most = max(most, 256u + norm_bits(square) + (query ? bits_above(top) : 0));
+            }
+        };
+        if (block < row_blocks) {
+            take(true, block * ROWS, rows);
+        } else {
+            const uint32_t row0 = (block - row_blocks) * ROWS, end = (uint32_t)len.of(b);
+            if (row0 >= end) continue;
+            take(false, row0, end);
+        }
+        most = __reduce_max_sync(0xffffffffu, most);
+        uint32_t* const to = range + (block < row_blocks ? 0 : units) + unit;
+        if ((threadIdx.x & 31) == 0 && most > __ldcg(to)) atomicMax(to, most);
+    }
+}
+
+// ---- grad_stat_kernel: what the gradients need of every query row, LANES lanes a slot ----------------------
+// Of every slot minus the log-sum in base 2 (-INF: no row, or nothing to be seen) and minus delta.  fp16: the log-sum's weight is 2^WEIGHT_BITS up and
+// delta is multiplied by the factor 2^(e - WEIGHT_BITS) of the keys' pass; then 2^-x (as bf16), minus delta as it is, the factor of dq; and the query
+// rows 2^x q, dense, go to moved_q.
+template <typename T, int LANES>
+__global__ void __launch_bounds__(256) grad_stat_kernel(AttView g, AttView q, const uint16_t* out, const float* lse, RowTiles rt, uint32_t units,
+                                                        int heads, int kv_heads, int d, float c, float* stat, const uint32_t* range,
+                                                        uint16_t* moved_q) {
+    constexpr bool HALF = std::is_same<T, __half>::value;
+    constexpr int SLOTS = 256 / LANES;   // of a CTA, all of one tile
+    const int sub = threadIdx.x % LANES;
+    const uint32_t tile_of = blockIdx.x / (GRAD_ROWS / SLOTS), unit = tile_of / (uint32_t)rt.tiles;
+    const int slot = (int)(blockIdx.x % (GRAD_ROWS / SLOTS)) * SLOTS + threadIdx.x / LANES;
     int t, gg;
-    const bool live = in && rt.at((int)(tile_of - unit * rt.tiles), (int)(i % rt.slots), &t, &gg);
-    float dot = 0.f;
-    uint32_t top = 0;
-    const int h = (int)(unit % kv_heads) * rt.group + (live ? gg : 0);
-    const int64_t b = unit / kv_heads;
-    const int64_t row = live ? (b * rt.queries + t) * heads + h : 0;
-    if (live && sub * 8 < d) {
+    const bool live = rt.at((int)(tile_of - unit * rt.tiles), slot, &t, &gg);
+    float dot = 0.f, square = 0.f, top = 0.f;
+    const uint32_t b = unit / (uint32_t)kv_heads;
+    const int h = (int)(unit - b * kv_heads) * rt.group + (live ? gg : 0);
+    const int64_t row = live ? ((int64_t)b * rt.queries + t) * heads + h : 0;
+    const bool mine = live && sub * 8 < d;
+    uint4 z = make_uint4(0, 0, 0, 0);
+    if (mine) {
         const uint4 x = *reinterpret_cast<const uint4*>(g.at(b, t, h) + sub * 8);
         const uint4 y = *reinterpret_cast<const uint4*>(out + row * d + sub * 8);
+        if (HALF) z = *reinterpret_cast<const uint4*>(q.at(b, t, h) + sub * 8);
         const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-            const float a = to_f32<T>((uint16_t)xs[e]), c = to_f32<T>((uint16_t)(xs[e] >> 16));
-            dot = fmaf(a, to_f32<T>((uint16_t)ys[e]), dot);
-            dot = fmaf(c, to_f32<T>((uint16_t)(ys[e] >> 16)), dot);
-            top = max(top, max(__float_as_uint(a) & 0x7fffffffu, __float_as_uint(c) & 0x7fffffffu));
+            dot = fmaf(to_f32<T>((uint16_t)xs[e]), to_f32<T>((uint16_t)ys[e]), dot);
+            dot = fmaf(to_f32<T>((uint16_t)(xs[e] >> 16)), to_f32<T>((uint16_t)(ys[e] >> 16)), dot);
+        }
+        if (HALF) {
+            add_square(x, &square);
+            add_largest(z, &top);
         }
     }
 #pragma unroll
-    for (int o = 8; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
-    if (in && sub == 0) {
-        const float l = live ? lse[row] * kLog2e : CUDART_INF_F;
-        float* const st = stat + tile_of * 2 * rt.slots + i % rt.slots;
-        st[0] = l == -CUDART_INF_F ? l : -l;   // -INF either way where nothing is to be seen
-        st[rt.slots] = live ? -dot : 0.f;
+    for (int o = LANES / 2; o > 0; o >>= 1) {
+        dot += __shfl_xor_sync(0xffffffffu, dot, o);
+        if (HALF) {
+            square += __shfl_xor_sync(0xffffffffu, square, o);
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        }
     }
-    if (gmax) {   // the largest finite one; the order does not matter
-        if (top >= 0x7f800000u) top = 0;
-        top = __reduce_max_sync(0xffffffffu, top);
-        if ((threadIdx.x & 31) == 0 && top > __ldcg(gmax)) atomicMax(gmax, top);
+    // exponents: the query row's move x, with which its score gradients have e = common - x (at most `alone`), and those for dq
+    int x = 0, e = 0, alone = 0;
+    if (HALF && live) {
+        const UnitRange u = unit_range(range, units, unit);
+        if (usable(square)) {
+            alone = DS_BITS - u.value - norm_bits(square);
+            x = u.common() - alone;
+            if (!usable(top)) x = max(x, 0);   // zeros do not mind
+            else if (c <= 1e30f) x = max(x, Q_LEAST_BITS - bits_above(top));
+            else x = min(max(x, 0), Q_BITS - bits_above(top));   // c 2^-x stays finite
+        }
+        e = u.common() - x;
+    }
+    if (sub == 0) {
+        const float l = live ? lse[row] * kLog2e : CUDART_INF_F;
+        float* const st = stat + (int64_t)tile_of * GRAD_STATS<T> + slot;
+        // -INF either way where nothing is to be seen
+        st[0] = l == -CUDART_INF_F ? l : (HALF ? (float)WEIGHT_BITS - l : -l);
+        const float delta = live ? -dot : 0.f;
+        st[STAT_DELTA] = HALF ? delta * power_of_2(e - WEIGHT_BITS) : delta;
+        if (HALF) {
+            reinterpret_cast<uint16_t*>(st - slot + STAT_MOVED)[slot] = (uint16_t)(__float_as_uint(power_of_2(-x)) >> 16);
+            st[STAT_ALONE] = delta;
+            st[STAT_FACTOR] = power_of_2(alone - WEIGHT_BITS);
+        }
+    }
+    if (HALF && mine) {
+        const float f = power_of_2(x);
+        auto moved = [&](uint32_t w) { return pack2<T>(to_f32<T>((uint16_t)w) * f, to_f32<T>((uint16_t)(w >> 16)) * f); };
+        *reinterpret_cast<uint4*>(moved_q + row * d + sub * 8) = make_uint4(moved(z.x), moved(z.y), moved(z.z), moved(z.w));
     }
 }
 
@@ -513,7 +663,7 @@ struct GradPlan {
     RowTiles rt;
     int64_t key_blocks, row_blocks;
     int key_splits, row_splits;
-    size_t stat_bytes, key_part_bytes, scratch;
+    size_t range_bytes, stat_bytes, moved_bytes, key_part_bytes, scratch;
 };
 // Ranges of the streamed tiles: where an item would take more than twice an SM's share of the work, as many as bring it down to that, of
 // at least MIN_TILES tiles of 64 rows.
@@ -535,10 +685,13 @@ GradPlan plan_grad(const B200FAttendBackwardArgs& a) {
     // with nothing on one side there are no sums on the other to cut
     pl.key_splits = a.n > 0 ? splits(pl.rt.tiles, share * 5 / 7) : 1;
     pl.row_splits = a.queries > 0 ? splits(row_tiles, share) : 1;
-    pl.stat_bytes = (size_t)round_up64(units * pl.rt.tiles * GRAD_ROWS * 8, 256);
+    const bool half = a.storage == B200F_STORAGE_F16;
     const int64_t keys = units * a.n * a.d, rows = a.batch * a.queries * a.heads * a.d;
+    pl.range_bytes = half ? (size_t)round_up64(2 * units * 4, 256) : 0;
+    pl.stat_bytes = (size_t)round_up64(units * pl.rt.tiles * 4 * (half ? GRAD_STATS<__half> : GRAD_STATS<__nv_bfloat16>), 256);
+    pl.moved_bytes = half ? (size_t)round_up64(rows * 2, 256) : 0;
     pl.key_part_bytes = pl.key_splits > 1 ? (size_t)round_up64(pl.key_splits * 2 * keys * 4, 256) : 0;
-    pl.scratch = 256 + pl.stat_bytes + pl.key_part_bytes + (pl.row_splits > 1 ? (size_t)pl.row_splits * rows * 4 : 0);
+    pl.scratch = 256 + pl.range_bytes + pl.stat_bytes + pl.moved_bytes + pl.key_part_bytes + (pl.row_splits > 1 ? (size_t)pl.row_splits * rows * 4 : 0);
     return pl;
 }
 
@@ -567,14 +720,32 @@ int launch_grad(const CUtensorMap* maps, const GradParams& keys, const GradParam
 }
 
 template <typename T>
-int launch_backward(const B200FAttendBackwardArgs& a, const GradPlan& pl, GradParams p, const uint16_t* out, float* stat, uint32_t* gmax,
-                    float* part, const AttView& k, const AttView& v) {
+int launch_backward(const B200FAttendBackwardArgs& a, const GradPlan& pl, GradParams p, const uint16_t* out, uint8_t* scratch, const AttView& k,
+                    const AttView& v) {
+    constexpr bool HALF = std::is_same<T, __half>::value;
+    uint32_t* const range = reinterpret_cast<uint32_t*>(scratch);
+    float* const stat = reinterpret_cast<float*>(scratch + pl.range_bytes);
+    uint16_t* const moved_q = reinterpret_cast<uint16_t*>(scratch + pl.range_bytes + pl.stat_bytes);
+    float* const part = reinterpret_cast<float*>(scratch + pl.range_bytes + pl.stat_bytes + pl.moved_bytes);
+    p.stat = stat;
+    p.range = range;
     const cudaStream_t st = (cudaStream_t)a.stream;
     const int64_t units = a.batch * a.kv_heads;
     if (pl.rt.tiles > 0) {
-        if (gmax) B200F_CUDA_TRY(cudaMemsetAsync(gmax, 0, 4, st));
-        const int64_t slots = units * pl.rt.tiles * GRAD_ROWS;
-        grad_stat_kernel<T><<<(unsigned)ceil_div64(slots, 16), 256, 0, st>>>(p.g, out, a.lse, pl.rt, units, a.heads, a.kv_heads, a.d, stat, gmax);
+        if (HALF) {
+            B200F_CUDA_TRY(cudaMemsetAsync(range, 0, 2 * units * 4, st));
+            const int64_t per = a.d <= 64 ? RANGE_ROWS<8> : RANGE_ROWS<16>, most = (int64_t)cached_sm_count() * 24;
+            const int64_t items = units * (ceil_div64(a.queries * pl.rt.group, per) + ceil_div64(a.n, per));
+            auto* const kernel = a.d <= 64 ? grad_range_kernel<8> : grad_range_kernel<16>;
+            kernel<<<(unsigned)(items < most ? items : most), 256, 0, st>>>(p.g, p.q, v, p.len, (uint32_t)units, (uint32_t)a.kv_heads,
+                                                                            (uint32_t)pl.rt.group, a.d, range);
+            count_launch();
+            B200F_LAUNCH_CHECK();
+        }
+        auto* const kernel = a.d <= 64 ? grad_stat_kernel<T, 8> : grad_stat_kernel<T, 16>;
+        const int64_t blocks = units * pl.rt.tiles * (GRAD_ROWS * (a.d <= 64 ? 8 : 16) / 256);
+        kernel<<<(unsigned)blocks, 256, 0, st>>>(p.g, p.q, out, a.lse, pl.rt, (uint32_t)units, a.heads, a.kv_heads, a.d, a.scale * kLog2e, stat, range,
+                                                 moved_q);
         count_launch();
         B200F_LAUNCH_CHECK();
     }
@@ -585,7 +756,8 @@ int launch_backward(const B200FAttendBackwardArgs& a, const GradPlan& pl, GradPa
         if (rc == B200F_OK) rc = make_rows_map(&maps[1], &p.vm, v, a.storage, a.d, a.n, a.kv_heads, a.batch, GRAD_ROWS);
     }
     if (rc == B200F_OK && a.queries > 0) {
-        rc = make_queries_map(&maps[2], &p.qm, p.q, a.storage, a.d, pl.rt, a.kv_heads, a.batch);
+        const AttView moved{moved_q, a.queries * a.heads * a.d, (int64_t)a.heads * a.d, a.d};
+        rc = make_queries_map(&maps[2], &p.qm, HALF ? moved : p.q, a.storage, a.d, pl.rt, a.kv_heads, a.batch);
         if (rc == B200F_OK) rc = make_queries_map(&maps[3], &p.gm, p.g, a.storage, a.d, pl.rt, a.kv_heads, a.batch);
     }
     if (rc != B200F_OK) return rc;
@@ -649,20 +821,15 @@ extern "C" int b200f_attend_backward(const B200FAttendBackwardArgs* a) {
     const GradPlan pl = plan_grad(*a);
     if (!a->scratch || (reinterpret_cast<uintptr_t>(a->scratch) & 255) != 0 || a->scratch_bytes < pl.scratch) return B200F_ERR_SCRATCH;
     const int64_t units = a->batch * a->kv_heads, lim = 0x7fffffff;
-    if (units * pl.key_blocks * pl.key_splits + units * pl.row_blocks * pl.row_splits > lim ||
+    if (units * pl.key_blocks * pl.key_splits + units * pl.row_blocks * pl.row_splits > lim / 2 ||
         units * pl.rt.tiles * GRAD_ROWS / 16 > lim || units * a->n * a->d / 512 > lim)
         return B200F_ERR_UNSUPPORTED;
-    uint8_t* const scratch = static_cast<uint8_t*>(a->scratch);
-    uint32_t* const gmax = a->storage == B200F_STORAGE_F16 ? reinterpret_cast<uint32_t*>(scratch) : nullptr;
-    float* const stat = reinterpret_cast<float*>(scratch + 256);
-    float* const part = reinterpret_cast<float*>(scratch + 256 + pl.stat_bytes);
     GradParams p{};
     p.q = q;
     p.g = g;
     p.len = AttLengths{a->key_lengths, a->n, a->queries, 0};
     p.rt = pl.rt;
-    p.stat = stat;
-    p.gmax = gmax;
+    p.units = units;
     p.queries = a->queries;
     p.heads = a->heads;
     p.kv_heads = a->kv_heads;
@@ -671,6 +838,7 @@ extern "C" int b200f_attend_backward(const B200FAttendBackwardArgs* a) {
     p.scale = a->scale;
     p.status = a->status;
     const uint16_t* const out = static_cast<const uint16_t*>(a->out);
-    return gmax ? launch_backward<__half>(*a, pl, p, out, stat, gmax, part, k, v)
-                : launch_backward<__nv_bfloat16>(*a, pl, p, out, stat, gmax, part, k, v);
+    uint8_t* const scratch = static_cast<uint8_t*>(a->scratch);
+    return a->storage == B200F_STORAGE_F16 ? launch_backward<__half>(*a, pl, p, out, scratch, k, v)
+                                           : launch_backward<__nv_bfloat16>(*a, pl, p, out, scratch, k, v);
 }

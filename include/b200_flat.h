@@ -343,7 +343,10 @@ int b200f_remap_labels_block_cyclic(int64_t* labels, int64_t count, int64_t bloc
  * gradients are rounded to the operands' type before they are multiplied; sums, log-sums and normalisation
  * are fp32; outputs are rounded once.  Exponentials are the hardware's approximation or a polynomial (2.7e-6 relative).  The
  * backward pass takes rowsum(grad_out * out) from the rounded output, which adds up to half a step of it to every score
- * gradient; in FP16 it is meant for value rows of a norm below 11,500 (larger ones may overflow score gradients).
+ * gradient.  In FP16 every query row's score gradients are rounded with a power of two of their own, from its bound 2 |grad_out| |v|
+ * (|v|: the longest value row that its sequence sees), so that neither other rows nor many keys push them out of the type's normal
+ * range: those below 2^-26 of the bound lose bits; for grad_k also those of rows whose |grad_out| |q| lies more than 2^17 below the
+ * largest of their sequence and key head, bit by bit.
  * No result depends on the order in which CTAs run.
  *
  * status: as for b200f_search (int32[4], [0] != 0: a bounded wait ran out), but never cleared here. */

@@ -1,7 +1,10 @@
-"""Soft reads at the edges of their ranges."""
+"""Soft reads at the edges of their ranges.  u is half a step of the operands' type relative to the value."""
+import math
+
 import pytest
 
-from test_gpu_attention import TYPES
+import attention_ref as R
+from test_gpu_attention import TYPES, lens, rand, unit
 
 pytestmark = pytest.mark.gpu
 
@@ -21,3 +24,160 @@ def test_gradient_of_a_call_with_an_empty_side(fm, lq, lk, dtype):
     assert gq.shape == q.shape and gk.shape == k.shape and gv.shape == v.shape
     assert (gq == 0).all() and (gk == 0).all() and (gv == 0).all()
     fm.check_attention_status()
+
+
+# ---- fp16 gradients far below the largest --------------------------------------------------------
+
+
+def far_from_rows(got, grad, q, k, v, n=None, scale=None):
+    """How far fp16 gradients are beyond their bounds, entry by entry (at most 0 when within), every entry judged by its own terms.
+
+    A term's score gradient (or weight) is rounded once: u of it, uniform at worst, u / sqrt(3) in the mean square; with independent
+    signs a sum of such errors stays within 4.5 u (almost eight standard deviations) of the root of the terms' squares.  delta comes from the rounded
+    output: u of sum |do| |o|.  The result is rounded once: u, at least 2^-25.  A multiplication by a power of two leaves the bound 2 |do| max |v| of a row's score gradients
+    between 2^12 and 2^14 (and a weight of 1 at 2^12): what lies below fp16's normal range then errs by 2^-25 / 2^12 of that bound.  For
+    grad_k a row's query entries take the inverse factors, the largest of them kept at 2^-3 or more, which lets the smallest err by 2^-22 of it; rows so far below the call's largest that this
+    limit holds them err by 2^-53 of that.  fp32 sums: 2^-23 of their running value a step of 16 terms, in ranges of 16,384 at most."""
+    b, lq, h, d = q.shape
+    lk, hk = k.shape[1], k.shape[2]
+    scale = 1.0 / math.sqrt(d) if scale is None else scale
+    seen = R.visible(n, b, lq, lk, False, q.device).any(1)
+    k, v = R.live(k, seen), R.live(v, seen)
+    p, _ = R.softmax(R.scores(q, k, n, scale, False))
+    g, qq, kk, vv = (R.heads_first(x, h) for x in (grad, q, k, v))                     # [b, h, rows, d]
+    o = p @ vv
+    ds = p * (g @ vv.transpose(-1, -2) - (g * o).sum(-1, keepdim=True)) * scale
+    dabs = (g.abs() * o.abs()).sum(-1, keepdim=True) * scale
+    bound = 2 * g.norm(dim=-1, keepdim=True) * vv.norm(dim=-1).amax(-1).view(b, h, 1, 1) * scale
+    qmax, kmax = qq.abs().amax(-1, keepdim=True), kk.abs().amax((-1, -2), keepdim=True)
+    largest = (bound * qmax).view(b, hk, -1).amax(-1)
+
+    def keys(x):                                                                       # sums over a group
+        return x.view(b, hk, h // hk, lk, -1).sum(2).permute(0, 2, 1, 3)
+
+    def turned(x):
+        return x.transpose(-1, -2)
+
+    u, rows = unit(torch.float16), lq * h // hk
+    want = ((ds @ kk).permute(0, 2, 1, 3), keys(turned(ds) @ qq), keys(turned(p) @ g))
+    sig = ((ds.square() @ kk.square()).sqrt().permute(0, 2, 1, 3), keys(turned(ds.square()) @ qq.square()).sqrt(),
+           keys(turned(p.square()) @ g.square()).sqrt())
+    extra = ((u * dabs * (p @ kk).abs() + 4.5 * lk ** 0.5 * 2.0 ** -37 * bound * kmax).permute(0, 2, 1, 3),
+             4.5 * u * keys(turned((p * dabs).square()) @ qq.square()).sqrt()
+             + 4.5 * 2.0 ** -37 * (bound * qmax).square().view(b, hk, -1).sum(-1).sqrt().view(b, 1, hk, 1)
+             + rows * 2.0 ** -53 * largest.view(b, 1, hk, 1) + 2.0 ** -22 * keys(turned(ds.abs()) @ qmax),
+             4.5 * 2.0 ** -37 * g.square().amax(-1).view(b, hk, -1).sum(-1).sqrt().view(b, 1, hk, 1))
+    far = []
+    for x, w, s, e, terms in zip(got, want, sig, extra, (lk, rows, rows)):
+        assert not torch.isnan(x).any()
+        far.append(((x.double() - w).abs() - (u * w.abs() + 4.5 * u * s + e + 2.0 ** -25
+                                              + min(terms, 16384) / 16 * 2.0 ** -23 * (w.abs() + 4.5 * s))).max().item())
+    return far
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("lq,lk", [(256, 4096), (100, 1531)])
+@pytest.mark.parametrize("low,high", [(0, 8), (0, 12), (-4, 14), (-10, 5), (-14, 14)])
+def test_rows_of_small_and_large_gradients_together(fm, lq, lk, d, low, high):
+    """One row's output gradient is 2^(high - low) times the others'.  It reads one key alone, so that the other keys' gradients
+    come from the other rows only."""
+    dt = torch.float16
+    q, k, v = rand(1, dt, 1, lq, 2, d), rand(2, dt, 1, lk, 2, d), rand(3, dt, 1, lk, 2, d)
+    grad = (rand(4, torch.float32, 1, lq, 2, d) * 2.0 ** low).to(dt)
+    grad[0, 17] = 0
+    grad[0, 17, :, 5] = 2.0 ** high
+    q[0, 17], k[0, 40] = 0, 0
+    q[0, 17, :, 3], k[0, 40, :, 3] = 64, 8 * math.sqrt(d) / 4       # score 128 at key 40; the others' are below 32
+    k[0, :40, :, 3].clamp_(max=1)
+    k[0, 41:, :, 3].clamp_(max=1)
+    out, lse = fm.attend(q, k, v, return_lse=True)
+    got = fm.attend_backward(grad, q, k, v, out, lse)
+    far = far_from_rows(got, grad, q, k, v)
+    assert max(far) <= 0, far
+    fm.check_attention_status()
+
+
+@pytest.mark.parametrize("lq,lk,h,hk", [(64, 1000, 4, 2), (300, 3000, 6, 2), (5, 1500, 96, 1)])
+def test_rows_of_every_magnitude(fm, lq, lk, h, hk):
+    # output gradients and queries over 2^20 and 2^12, in turn
+    dt = torch.float16
+    q, k, v = rand(1, torch.float32, 2, lq, h, 64), rand(2, dt, 2, lk, hk, 64), rand(3, dt, 2, lk, hk, 64)
+    grad = rand(4, torch.float32, 2, lq, h, 64)
+    r = torch.arange(2 * lq * h, device="cuda").view(2, lq, h, 1)
+    q = (q * 2.0 ** (-(r * 7 % 13).float())).to(dt)
+    grad = (grad * 2.0 ** ((r * 11 % 21).float() - 10)).to(dt)
+    n = lens(lk, lk // 3)
+    out, lse = fm.attend(q, k, v, key_lengths=n, return_lse=True)
+    far = far_from_rows(fm.attend_backward(grad, q, k, v, out, lse, key_lengths=n), grad, q, k, v, n)
+    assert max(far) <= 0, far
+
+
+@pytest.mark.parametrize("lq,lk", [(32, 1_000_000), (200, 100_000)])
+def test_fp16_gradients_over_many_keys(fm, lq, lk):
+    # a weight is about 1 / keys
+    dt = torch.float16
+    q, k, v, grad = rand(1, dt, 1, lq, 1, 64), rand(2, dt, 1, lk, 1, 64), rand(3, dt, 1, lk, 1, 64), rand(4, dt, 1, lq, 1, 64)
+    grad = grad * 16
+    out, lse = fm.attend(q, k, v, return_lse=True)
+    far = far_from_rows(fm.attend_backward(grad, q, k, v, out, lse), grad, q, k, v)
+    assert max(far) <= 0, far
+
+
+def test_fp16_gradients_of_large_values(fm):
+    # value rows of a norm up to 160,000, all in line with the output gradient
+    dt = torch.float16
+    q, k = rand(1, dt, 1, 150, 2, 64) * 0.125, rand(2, dt, 1, 200, 2, 64) * 0.125
+    v = torch.where(torch.arange(200, device="cuda").view(1, 200, 1, 1) % 2 == 0, 20000.0, -20000.0).expand(1, 200, 2, 64).to(dt).contiguous()
+    grad = torch.full((1, 150, 2, 64), 2.0 ** -7, dtype=dt, device="cuda")
+    for n in (None, lens(2)):
+        out, lse = fm.attend(q, k, v, key_lengths=n, return_lse=True)
+        far = far_from_rows(fm.attend_backward(grad, q, k, v, out, lse, key_lengths=n), grad, q, k, v, n)
+        assert max(far) <= 0, far
+
+
+def test_fp16_gradients_keep_to_their_sequence_and_key_head(fm):
+    # what other sequences and key heads hold changes no bit, nor do rows behind the end
+    dt = torch.float16
+    q, k, v, grad = rand(1, dt, 2, 90, 4, 64), rand(2, dt, 2, 400, 2, 64), rand(3, dt, 2, 400, 2, 64), rand(4, dt, 2, 90, 4, 64)
+    n = lens(400, 333)
+
+    def run(q, k, v, grad):
+        out, lse = fm.attend(q, k, v, key_lengths=n, return_lse=True)
+        return fm.attend_backward(grad, q, k, v, out, lse, key_lengths=n)
+
+    want = run(q, k, v, grad)
+    other = [x.clone() for x in (q, k, v, grad)]
+    other[3][0] *= 2.0 ** 11
+    other[2][0] *= 2.0 ** 9
+    other[0][0] *= 2.0 ** 3
+    other[1][1, 333:], other[2][1, 333:] = math.nan, 60000.0
+    got = run(*other)
+    assert all(torch.equal(x[1], y[1]) for x, y in zip(want, got))
+    other = [x.clone() for x in (q, k, v, grad)]
+    other[3][:, :, :2] *= 2.0 ** 11
+    other[2][:, :, 0] = math.inf
+    got = run(*other)
+    assert torch.equal(want[0][:, :, 2:], got[0][:, :, 2:])
+    assert all(torch.equal(want[i][:, :, 1], got[i][:, :, 1]) for i in (1, 2))
+
+
+def test_fp16_gradients_of_zero_and_of_rows_that_are_not_finite(fm):
+    dt = torch.float16
+    q, k, v, grad = rand(1, dt, 1, 90, 2, 64), rand(2, dt, 1, 400, 2, 64), rand(3, dt, 1, 400, 2, 64), rand(4, dt, 1, 90, 2, 64)
+    q[0, 3], grad[0, 5] = 0, 0
+    out, lse = fm.attend(q, k, v, return_lse=True)
+    got = fm.attend_backward(grad, q, k, v, out, lse)
+    assert max(far_from_rows(got, grad, q, k, v)) <= 0 and (got[0][0, 5] == 0).all()
+    zero = fm.attend_backward(torch.zeros_like(grad), q, k, v, out, lse)
+    assert all((x == 0).all() for x in zero)
+    bad = grad.clone()
+    bad[0, 7, 1, 2] = math.inf
+    gq, gk, gv = fm.attend_backward(bad, q, k, v, out, lse)
+    assert torch.isnan(gq[0, 7, 1]).any() and torch.isnan(gk[:, :, 1]).any() and (torch.isnan(gv[:, :, 1, 2]) | (gv[:, :, 1, 2] == math.inf)).all()
+    keep = torch.arange(90, device="cuda") != 7
+    far = far_from_rows((gq[:, keep][:, :, 0:1].contiguous(), got[1][:, :, :1], got[2][:, :, :1]), grad[:, keep][:, :, :1], q[:, keep][:, :, :1], k[:, :, :1], v[:, :, :1])
+    assert far[0] <= 0
+    assert torch.equal(gk[:, :, 0], got[1][:, :, 0]) and torch.equal(gv[:, :, 0], got[2][:, :, 0])
+    # the row's NaN does not reach other rows' query gradients
+    far = far_from_rows((gq[:, keep][:, :, 1:].contiguous(), got[1][:, :, 1:], got[2][:, :, 1:]), grad[:, keep][:, :, 1:], q[:, keep][:, :, 1:], k[:, :, 1:], v[:, :, 1:])
+    assert far[0] <= 0
