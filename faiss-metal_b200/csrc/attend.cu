@@ -30,6 +30,10 @@ static_assert(128 * TILE_REGS_FEW + 256 * TILE_REGS_MANY <= 384 * 168, "register
 constexpr int PART_KEYS = 96;             // keys whose weights are handed on first
 constexpr float WEIGHTS_MAX = 32768.f;     // fp16 weights end at 65504
 constexpr int TILE_KEYS = 128;
+// A product is added to the sum in tensor memory with some two bits below that sum's last place, the rest cut off: a term loses 2^-26 of the sum
+// on average, and 1,000,000 keys behind one that outweighs them lost 30 % of their share.  After so many tiles (2^15 keys, 2^-11 of the sum)
+// a row's sums go to memory, where they are added up in fp32, and start from 0 again.
+constexpr int SUM_TILES = 256;
 constexpr int TILE_MAX_STAGES = 10;
 template <int DP>
 constexpr int TILE_Q_BYTES = DP / 64 * ATT_CHUNK;
@@ -72,6 +76,7 @@ struct TileParams {
     float* lse;
     float* part_o;         // [parts][rows_total][d], null: the one part is the result
     float* part_lse;       // [parts][rows_total], base 2
+    float* sums;           // [rows_total][d]: of streams of more than SUM_TILES tiles, where there is one part (others have part_o's rows)
     int32_t* status;
 };
 
@@ -296,7 +301,7 @@ attend_tile_kernel(const __grid_constant__ CUtensorMap map_sk, const __grid_cons
                 const uint64_t db = dv + (uint64_t)(s * (STAGE >> 4));
                 auto product = [&](int k) __attribute__((always_inline)) {   // 16 keys
                     tc_mma_ts_by(leader, tmem + TM_O + 128 * t, tmem + TM_P<DP> + 128 * t + 8 * k, db + 128 * k, att_idesc<T>(DP, true),
-                                 k > 0 ? 1u : (uint32_t)(j > 0));
+                                 k > 0 ? 1u : (uint32_t)(j % SUM_TILES != 0));
                 };
                 if (!waits(bar_p + 2 * t * 8, j & 1)) return false;
                 tc_fence_after();
@@ -354,6 +359,31 @@ attend_tile_kernel(const __grid_constant__ CUtensorMap map_sk, const __grid_cons
         float m = -CUDART_INF_F, l = 0.f;
         float mc = CUDART_NAN_F;   // -c m; no reference yet: the first tile's sum fails the test below
         bool ok = true;
+        const bool whole = p.part_o == nullptr;
+        const int part = sg.part0 + (sg.split ? 2 * sp + t : sp);
+        auto row_index = [&] { return (at.b * p.queries + at.t) * p.heads + at.h; };
+        // where this row's sums are kept, in units of the reference m_kept
+        auto kept_row = [&] { return whole ? p.sums + row_index() * p.d : p.part_o + (part * p.rows_total + row_index()) * p.d; };
+        float m_kept = -CUDART_INF_F;
+        auto keep_sums = [&](bool first) __attribute__((always_inline)) {
+            float* const kept = kept_row();
+            const float f = m_kept == m ? 1.f : ex2((m_kept - m) * c);
+            m_kept = m;
+#pragma unroll 1
+            for (int i = 0; i < DP / 16; i++) {
+                uint32_t o[16];
+                tc_ld16_wait(to + 16 * i, o);
+#pragma unroll
+                for (int e = 0; e < 16; e += 4)
+                    if (live && 16 * i + e < p.d) {
+                        float4* const x = reinterpret_cast<float4*>(kept + 16 * i + e);
+                        float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+                        if (!first) y = *x;
+                        *x = make_float4(fmaf(y.x, f, __uint_as_float(o[e])), fmaf(y.y, f, __uint_as_float(o[e + 1])),
+                                         fmaf(y.z, f, __uint_as_float(o[e + 2])), fmaf(y.w, f, __uint_as_float(o[e + 3])));
+                    }
+            }
+        };
         uint32_t s[4][32];
         // weights of 32 keys to tensor memory; returns their sum
         auto weigh = [&](auto mix, uint32_t (&x)[32], float mc_now, int i) __attribute__((always_inline)) {
@@ -374,6 +404,7 @@ attend_tile_kernel(const __grid_constant__ CUtensorMap map_sk, const __grid_cons
                 if (!ok) break;
                 tc_fence_after();
             }
+            if (j > 0 && j % SUM_TILES == 0) keep_sums(j == SUM_TILES);   // the previous product is done (APART: waited for, else since the scores are there)
 #pragma unroll
             for (int h = 0; h < 2; h++) {
                 constexpr int PART = PART_KEYS / 32;
@@ -443,11 +474,11 @@ attend_tile_kernel(const __grid_constant__ CUtensorMap map_sk, const __grid_cons
         if (ok && warp_live) {
             tc_fence_after();
             const bool none = nt == 0;
-            const int64_t grow = (at.b * p.queries + at.t) * p.heads + at.h;
+            const int64_t grow = row_index();
             const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
             const float lse2 = l > 0.f || l != l ? log2f(l) + (m == -CUDART_INF_F ? 0.f : m * c) : -CUDART_INF_F;
-            const bool whole = p.part_o == nullptr;
-            const int part = sg.part0 + (sg.split ? 2 * sp + t : sp);
+            float* const kept = kept_row();
+            if (nt > SUM_TILES) keep_sums(false);
             if (live) {
                 if (whole) {
                     if (p.lse) p.lse[grow] = lse2 * kLn2;
@@ -460,7 +491,17 @@ attend_tile_kernel(const __grid_constant__ CUtensorMap map_sk, const __grid_cons
 #pragma unroll 1
             for (int i = 0; i < DP / 32; i++) {
                 uint32_t o[32];
-                if (!none) {
+                if (nt > SUM_TILES) {
+#pragma unroll
+                    for (int e = 0; e < 32; e += 4) {
+                        float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+                        if (live && 32 * i + e < p.d) y = *reinterpret_cast<const float4*>(kept + 32 * i + e);
+                        o[e] = __float_as_uint(y.x);
+                        o[e + 1] = __float_as_uint(y.y);
+                        o[e + 2] = __float_as_uint(y.z);
+                        o[e + 3] = __float_as_uint(y.w);
+                    }
+                } else if (!none) {
                     tc_ld32(to + 32 * i, o);
                     tc_wait_ld32(o);
                 }
@@ -469,7 +510,7 @@ attend_tile_kernel(const __grid_constant__ CUtensorMap map_sk, const __grid_cons
                 if (whole) {
                     stage_columns32<T, DP>(stage, o, 4 * i);
                 } else if (live && !none) {
-                    float* const po = p.part_o + (part * p.rows_total + grow) * p.d;
+                    float* const po = kept;
 #pragma unroll
                     for (int e = 0; e < 32; e += 8)
                         if (32 * i + e < p.d) {
@@ -499,6 +540,7 @@ attend_tile_kernel(const __grid_constant__ CUtensorMap map_sk, const __grid_cons
 constexpr int FEW_ROWS = 16;
 constexpr int FEW_KEYS = 64;            // keys of a tile
 constexpr int FEW_THREADS = 160;        // four warps, TMA
+constexpr int FEW_SUM_TILES = 2048;     // longest range: a warp's share of it is 2^15 keys (see SUM_TILES)
 template <int DP>
 constexpr int FEW_TILE = DP / 64 * FEW_KEYS * 128;
 template <int DP>
@@ -864,6 +906,7 @@ struct AttendPlan {
     Segment seg[2];
     int64_t items[2];   // CTAs of the tile kernel, of the few-rows kernel
     int parts;
+    bool sums;          // TileParams::sums is wanted
     size_t scratch;
 };
 
@@ -903,6 +946,7 @@ double cut_few(Segment& s, int64_t units, int64_t rows, bool joined) {
     // one turn of the two CTAs an SM takes; with more blocks than SMs about four, since sequences differ in length
     int64_t want = (base >= sm ? 8 : 2) * sm / base;
     if (want > tiles / FEW_MIN_TILES) want = tiles / FEW_MIN_TILES;
+    if (want < ceil_div64(tiles, FEW_SUM_TILES)) want = ceil_div64(tiles, FEW_SUM_TILES);
     s.splits = (int)(want < 1 ? 1 : want);
     s.items = base * s.splits;
     return (double)ceil_div64(s.items, 2 * sm) * (FEW_START_US + FEW_US * (double)ceil_div64(tiles, s.splits)) +
@@ -969,10 +1013,14 @@ AttendPlan plan_attend(const B200FAttendArgs& a) {
         Segment& s = pl.seg[i];
         s.part0 = pl.parts;
         pl.items[s.few] += s.items;
-        if (s.items > 0) pl.parts += s.split ? 2 * s.splits : s.splits;
+        const int streams = s.split ? 2 * s.splits : s.splits;
+        if (s.items > 0) pl.parts += streams;
+        if (!s.few && ceil_div64(ceil_div64(s.n, TILE_KEYS), streams) > SUM_TILES) pl.sums = true;
     }
+    if (pl.parts > 1) pl.sums = false;
     const int64_t rows = a.batch * a.queries * a.heads;
     pl.scratch = 256;
+    if (pl.sums) pl.scratch = (size_t)(256 + rows * a.d * 4);
     if (pl.parts > 1) pl.scratch = (size_t)(round_up64(pl.parts * rows * 4, 256) + pl.parts * rows * a.d * 4);
     return pl;
 }
@@ -1042,7 +1090,7 @@ extern "C" int b200f_attend(const B200FAttendArgs* a) {
         (a->shared_n > 0 && (!att_view_ok(sk, 1, a->shared_n, a->kv_heads) || !att_view_ok(sv, 1, a->shared_n, a->kv_heads))))
         return B200F_ERR_BAD_ARG;
     AttendPlan pl = plan_attend(*a);
-    if (pl.parts > 1 && (!a->scratch || (reinterpret_cast<uintptr_t>(a->scratch) & 255) != 0 || a->scratch_bytes < pl.scratch))
+    if ((pl.parts > 1 || pl.sums) && (!a->scratch || (reinterpret_cast<uintptr_t>(a->scratch) & 255) != 0 || a->scratch_bytes < pl.scratch))
         return B200F_ERR_SCRATCH;
     if (pl.items[0] > 0x7fffffff || pl.items[1] > 0x7fffffff) return B200F_ERR_UNSUPPORTED;
     CUtensorMap maps[4] = {};
@@ -1074,6 +1122,7 @@ extern "C" int b200f_attend(const B200FAttendArgs* a) {
         p.part_lse = static_cast<float*>(a->scratch);
         p.part_o = p.part_lse + round_up64(pl.parts * p.rows_total, 64);
     }
+    if (pl.sums) p.sums = static_cast<float*>(a->scratch);
     const cudaStream_t st = (cudaStream_t)a->stream;
     if (a->storage == B200F_STORAGE_F16)
         return a->d > 64 ? launch_attend<__half, 128>(maps, p, pl, st) : launch_attend<__half, 64>(maps, p, pl, st);

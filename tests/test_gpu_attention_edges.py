@@ -4,7 +4,7 @@ import math
 import pytest
 
 import attention_ref as R
-from test_gpu_attention import TYPES, lens, rand, unit
+from test_gpu_attention import TYPES, check_out, lens, rand, unit
 
 pytestmark = pytest.mark.gpu
 
@@ -181,3 +181,53 @@ def test_fp16_gradients_of_zero_and_of_rows_that_are_not_finite(fm):
     # the row's NaN does not reach other rows' query gradients
     far = far_from_rows((gq[:, keep][:, :, 1:].contiguous(), got[1][:, :, 1:], got[2][:, :, 1:]), grad[:, keep][:, :, 1:], q[:, keep][:, :, 1:], k[:, :, 1:], v[:, :, 1:])
     assert far[0] <= 0
+
+
+# ---- weights far below a row's largest -------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", ["bf16"])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("b,lq,lk", [(75, 256, 1_000_000), (1200, 1, 300_000)])
+def test_a_long_tail_of_small_weights(fm, b, lq, lk, d, dtype):
+    """One key's score lies 18 above all others': each of these weighs 2^-26 of it, all together 0.5 % to 1.5 %, and the sequences are so many that
+    a row's keys are one range.  In fp16 the largest weight is held at 2^7 or more and a weight below the type's normal range errs by 2^-25 at
+    most, a key 2^-32 of the largest value."""
+    dt = TYPES[dtype]
+    q = torch.zeros(b, lq, 1, d, dtype=dt, device="cuda")
+    q[..., 0] = 1
+    k = torch.zeros(1, lk, 1, d, dtype=dt, device="cuda")
+    v = rand(3, dt, 1, lk, 1, d) * 0.25 + 1
+    top = 12_345
+    k[0, top, 0, 0] = 18
+    v[0, top] = 0.25
+    out, lse = fm.attend(q, k.expand(b, -1, -1, -1), v.expand(b, -1, -1, -1), scale=1.0, return_lse=True)
+    w = torch.full((lk, 1), math.exp(-18.0), dtype=torch.float64, device="cuda")
+    w[top] = 1
+    total = w.sum()
+    vv = v[0, :, 0].double()
+    want, size = (w * vv).sum(0) / total, (w * vv.abs()).sum(0) / total
+    tol = unit(dt) * want.abs() + 1.1 * unit(dt) * size + lk * 2.0 ** -32 * vv.abs().max()
+    # sums in the tensor cores are of 2^15 terms, each of which loses 2^-25 of the sum at most
+    tol = tol + 2.0 ** -10 * size
+    assert ((out.double() - want).abs() <= tol).all(), ((out.double() - want).abs() / want.abs()).max().item()
+    assert ((lse.double() - (18 + torch.log(total))).abs() <= 1e-4 + lk / 32 * 2.0 ** -24).all()
+    fm.check_attention_status()
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("b,lq,lk,d", [(80, 130, 70_000, 64), (80, 130, 70_000, 128), (80, 300, 40_000, 72), (74, 100, 140_000, 64), (74, 60, 140_000, 128)])
+def test_sums_of_long_ranges(fm, b, lq, lk, d, dtype):
+    # more keys a range than are summed up in one go; the largest score rises all the way; ends at and beside the borders
+    dt = TYPES[dtype]
+    q, v = rand(1, dt, b, lq, 1, d), rand(3, dt, 1, lk, 1, d)
+    k = rand(2, dt, 1, lk, 1, d) * 0.5
+    q[..., 0] = 1
+    k[0, :, 0, 0] = torch.linspace(-6, 6, lk, device="cuda") * math.sqrt(d)
+    ends = [lk, 32768, 32769, 65536, 0, 32767, 65537, lk - 1]
+    n = torch.tensor([min(lk, ends[i % len(ends)]) for i in range(b)], dtype=torch.int32, device="cuda")
+    out, lse = fm.attend(q, k.expand(b, -1, -1, -1), v.expand(b, -1, -1, -1), key_lengths=n, return_lse=True)
+    for i in range(8):
+        check_out(out[i:i + 1], lse[i:i + 1], R.attend(q[i:i + 1], k, v, n[i:i + 1]), dt, lk)
+    assert torch.equal(out[8:16, :5], fm.attend(q, k.expand(b, -1, -1, -1), v.expand(b, -1, -1, -1), key_lengths=n)[8:16, :5])
+    fm.check_attention_status()
