@@ -15,7 +15,7 @@ namespace {
 // of tensor memory; one warp issues the products of both: S (128 columns, whose first half then holds the weights P) and O.  PAIR: two row tiles
 // over the same keys, each key tile fetched once for both.  SPLIT (no more than 128 rows): one row tile, the streams have
 // different keys.  While one stream exponentiates, the tensor cores work for the other.
-// Weights are exp2(c (s - m)) for a reference m that is taken from a row's first tile and moves, with O rescaled, only when a tile's
+// Weights are exp2(c (s - m)), times a constant, for a reference m that is taken from a row's first tile and moves, with O rescaled, only when a tile's
 // weights add up to 2^15 or more: no maximum is looked for before the exponentials.  Sums stay in fp32.  The weights of the first 96
 // keys go to the tensor cores while those of the others are computed.
 // d <= 64 leaves tensor memory for P beside S (APART): the next scores are computed as soon as these are in registers, and the way
@@ -29,6 +29,13 @@ constexpr int TILE_REGS_FEW = 80, TILE_REGS_MANY = 208;   // 128 and 256 threads
 static_assert(128 * TILE_REGS_FEW + 256 * TILE_REGS_MANY <= 384 * 168, "registers of a CTA");
 constexpr int PART_KEYS = 96;             // keys whose weights are handed on first
 constexpr float WEIGHTS_MAX = 32768.f;     // fp16 weights end at 65504
+// The reference's own weight is 2^(this): fp16 weights down to 2^-22 of it are normal numbers and 2^-33 still counts, where a weight of 1 lost
+// what lies below 2^-25, with 1,000,000 such keys 1.5 % of a row.  96 weights of 2^8 add up to less than WEIGHTS_MAX.
+template <typename T>
+constexpr int TILE_WEIGHT_BITS = std::is_same<T, __half>::value ? 8 : 0;
+// ends of sequences are weighed with the reference as it is up to this power of two
+template <typename T>
+constexpr float TILE_MASKED_BITS = std::is_same<T, __half>::value ? 12.f : 8.f;
 constexpr int TILE_KEYS = 128;
 // A product is added to the sum in tensor memory with some two bits below that sum's last place, the rest cut off: a term loses 2^-26 of the sum
 // on average, and 1,000,000 keys behind one that outweighs them lost 30 % of their share.  After so many tiles (2^15 keys, 2^-11 of the sum)
@@ -357,7 +364,7 @@ attend_tile_kernel(const __grid_constant__ CUtensorMap map_sk, const __grid_cons
         const uint32_t to = tmem + TM_O + 128 * t + ((uint32_t)(ew * 32) << 16), tp = tmem + TM_P<DP> + 128 * t + ((uint32_t)(ew * 32) << 16);
         const float c = p.scale * kLog2e;
         float m = -CUDART_INF_F, l = 0.f;
-        float mc = CUDART_NAN_F;   // -c m; no reference yet: the first tile's sum fails the test below
+        float mc = CUDART_NAN_F;   // TILE_WEIGHT_BITS - c m; no reference yet: the first tile's sum fails the test below
         bool ok = true;
         const bool whole = p.part_o == nullptr;
         const int part = sg.part0 + (sg.split ? 2 * sp + t : sp);
@@ -433,13 +440,13 @@ attend_tile_kernel(const __grid_constant__ CUtensorMap map_sk, const __grid_cons
                     for (int i = h ? PART : 0; i < (h ? 4 : PART); i++)
 #pragma unroll
                         for (int e = 0; e < 32; e += 2) top = max3(top, __uint_as_float(s[i][e]), __uint_as_float(s[i][e + 1]));
-                    const bool grown = masked ? !(fmaf(top, c, mc) <= 8.f) : !(sum < WEIGHTS_MAX);
+                    const bool grown = masked ? !(fmaf(top, c, mc) <= TILE_MASKED_BITS<T>) : !(sum < WEIGHTS_MAX);
                     const float now = grown ? fmaxf(top, m) : m;
                     const bool moved = __any_sync(0xffffffffu, now != m);
                     const float f = now == m ? 1.f : ex2((m - now) * c);   // 0 where nothing was seen before
                     m = now;
                     l *= f;
-                    mc = m == -CUDART_INF_F ? CUDART_NAN_F : -m * c;
+                    mc = m == -CUDART_INF_F ? CUDART_NAN_F : (float)TILE_WEIGHT_BITS<T> - m * c;
                     // O holds what came before: the previous tile's product is done (APART: waited for, else since the scores are there); the first part's
                     // may be under way
                     if (moved && h == 1) {
@@ -476,7 +483,7 @@ attend_tile_kernel(const __grid_constant__ CUtensorMap map_sk, const __grid_cons
             const bool none = nt == 0;
             const int64_t grow = row_index();
             const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
-            const float lse2 = l > 0.f || l != l ? log2f(l) + (m == -CUDART_INF_F ? 0.f : m * c) : -CUDART_INF_F;
+            const float lse2 = l > 0.f || l != l ? log2f(l) - (float)TILE_WEIGHT_BITS<T> + (m == -CUDART_INF_F ? 0.f : m * c) : -CUDART_INF_F;
             float* const kept = kept_row();
             if (nt > SUM_TILES) keep_sums(false);
             if (live) {
@@ -540,6 +547,10 @@ attend_tile_kernel(const __grid_constant__ CUtensorMap map_sk, const __grid_cons
 constexpr int FEW_ROWS = 16;
 constexpr int FEW_KEYS = 64;            // keys of a tile
 constexpr int FEW_THREADS = 160;        // four warps, TMA
+// The reference's own weight is 2^(this), as in the tiles; a row's largest may be 2^FEW_SLACK_BITS above it: 2^15, below fp16's end.
+template <typename T>
+constexpr int FEW_WEIGHT_BITS = std::is_same<T, __half>::value ? 7 : 0;
+constexpr int FEW_SLACK_BITS = 8;
 constexpr int FEW_SUM_TILES = 2048;     // longest range: a warp's share of it is 2^15 keys (see SUM_TILES)
 template <int DP>
 constexpr int FEW_TILE = DP / 64 * FEW_KEYS * 128;
@@ -681,7 +692,7 @@ attend_few_kernel(const __grid_constant__ CUtensorMap map_sk, const __grid_const
             }
         }
         const float c = p.scale * kLog2e;
-        const float slack = fminf(8.f / c, 1e30f);
+        const float slack = fminf((float)FEW_SLACK_BITS / c, 1e30f);
         // this lane's row address in ldmatrix: matrix lane / 8, row lane % 8 of the warp's 16 keys
         const int mi = lane >> 3, mr = lane & 7;
         const int krow = warp * 16 + (mi >> 1) * 8 + mr, kpiece = mi & 1;   // keys: (0-7, d 0-7), (0-7, d 8-15), (8-15, ..)
@@ -746,7 +757,7 @@ attend_few_kernel(const __grid_constant__ CUtensorMap map_sk, const __grid_const
             for (int h = 0; h < 2; h++)
 #pragma unroll
                 for (int e = 0; e < 2; e++) {
-                    const float mc = m[e] == -CUDART_INF_F ? 0.f : -m[e] * c;
+                    const float mc = m[e] == -CUDART_INF_F ? 0.f : (float)FEW_WEIGHT_BITS<T> - m[e] * c;
                     const float x = ex2(fmaf(s[h][2 * e], c, mc)), y = ex2(fmaf(s[h][2 * e + 1], c, mc));
                     l[e] += x + y;
                     w[2 * h + e] = pack2<T>(x, y);
@@ -815,7 +826,7 @@ attend_few_kernel(const __grid_constant__ CUtensorMap map_sk, const __grid_const
             const float inv = none ? 0.f : 1.f / total;
             const RowAt at = row_at(p, shared, unit, row0 + r);
             const int64_t grow = (at.b * p.queries + at.t) * p.heads + at.h;
-            const float lse2 = none ? -CUDART_INF_F : log2f(total) + (top == -CUDART_INF_F ? 0.f : top);
+            const float lse2 = none ? -CUDART_INF_F : log2f(total) - (float)FEW_WEIGHT_BITS<T> + (top == -CUDART_INF_F ? 0.f : top);
 #pragma unroll
             for (int e = 0; e < 8; e++) acc[e] = none ? 0.f : acc[e] * inv;
             if (!p.part_o) {

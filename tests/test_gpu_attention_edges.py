@@ -186,7 +186,7 @@ def test_fp16_gradients_of_zero_and_of_rows_that_are_not_finite(fm):
 # ---- weights far below a row's largest -------------------------------------------------------------
 
 
-@pytest.mark.parametrize("dtype", ["bf16"])
+@pytest.mark.parametrize("dtype", list(TYPES))
 @pytest.mark.parametrize("d", [64, 128])
 @pytest.mark.parametrize("b,lq,lk", [(75, 256, 1_000_000), (1200, 1, 300_000)])
 def test_a_long_tail_of_small_weights(fm, b, lq, lk, d, dtype):
