@@ -446,7 +446,9 @@ attend_tile_kernel(const __grid_constant__ CUtensorMap map_sk, const __grid_cons
                     const float f = now == m ? 1.f : ex2((m - now) * c);   // 0 where nothing was seen before
                     m = now;
                     l *= f;
-                    mc = m == -CUDART_INF_F ? CUDART_NAN_F : (float)TILE_WEIGHT_BITS<T> - m * c;
+                    // scaled scores beyond fp32's range count as infinite: +INF makes the row NaN, -INF weighs nothing
+                    const float m2 = m * c;
+                    mc = fabsf(m2) == CUDART_INF_F ? CUDART_NAN_F : (float)TILE_WEIGHT_BITS<T> - m2;
                     // O holds what came before: the previous tile's product is done (APART: waited for, else since the scores are there); the first part's
                     // may be under way
                     if (moved && h == 1) {
@@ -466,7 +468,7 @@ attend_tile_kernel(const __grid_constant__ CUtensorMap map_sk, const __grid_cons
                     sum = 0.f;
 #pragma unroll
                     for (int i = h ? PART : 0; i < (h ? 4 : PART); i++)
-                        sum += weigh(std::false_type(), s[i], m == -CUDART_INF_F ? 0.f : mc, i);
+                        sum += weigh(std::false_type(), s[i], m2 == -CUDART_INF_F ? 0.f : mc, i);
                 }
                 l += sum;
                 tc_wait_st();
@@ -757,7 +759,9 @@ attend_few_kernel(const __grid_constant__ CUtensorMap map_sk, const __grid_const
             for (int h = 0; h < 2; h++)
 #pragma unroll
                 for (int e = 0; e < 2; e++) {
-                    const float mc = m[e] == -CUDART_INF_F ? 0.f : (float)FEW_WEIGHT_BITS<T> - m[e] * c;
+                    // scaled scores beyond fp32's range count as infinite, as in the tiles
+                    const float m2 = m[e] * c;
+                    const float mc = m2 == -CUDART_INF_F ? 0.f : m2 == CUDART_INF_F ? CUDART_NAN_F : (float)FEW_WEIGHT_BITS<T> - m2;
                     const float x = ex2(fmaf(s[h][2 * e], c, mc)), y = ex2(fmaf(s[h][2 * e + 1], c, mc));
                     l[e] += x + y;
                     w[2 * h + e] = pack2<T>(x, y);

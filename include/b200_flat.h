@@ -337,7 +337,8 @@ int b200f_remap_labels_block_cyclic(int64_t* labels, int64_t count, int64_t bloc
  * 0..n); what lies behind them is never read into a result, NaN included.  causal: query t of T
  * sees only the keys j < key_lengths[b] - T + 1 + t, as when the T queries belong to the sequence's last T rows.
  * A query that sees nothing has output 0 and log-sum -INF.  A value within its sequence's length that is infinite or NaN may reach
- * any query of the sequence, those before it included: their weight is 0, and 0 * NaN is NaN.
+ * any query of the sequence, those before it included: their weight is 0, and 0 * NaN is NaN.  A score that leaves fp32's range when it is
+ * multiplied by scale * log2(e) counts as infinite: +INF makes its row NaN, a key of -INF weighs nothing.
  *
  * Arithmetic: products of 16-bit operands, fp32 accumulation; weights and, in the backward pass, score
  * gradients are rounded to the operands' type before they are multiplied; sums, log-sums and normalisation

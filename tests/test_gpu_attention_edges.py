@@ -231,3 +231,53 @@ def test_sums_of_long_ranges(fm, b, lq, lk, d, dtype):
         check_out(out[i:i + 1], lse[i:i + 1], R.attend(q[i:i + 1], k, v, n[i:i + 1]), dt, lk)
     assert torch.equal(out[8:16, :5], fm.attend(q, k.expand(b, -1, -1, -1), v.expand(b, -1, -1, -1), key_lengths=n)[8:16, :5])
     fm.check_attention_status()
+
+
+# ---- scales near the end of fp32's range -----------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("place", [5, 200])
+@pytest.mark.parametrize("lq,lk", [(4, 300), (700, 300), (700, 1200)])
+def test_scores_near_the_end_of_fp32(fm, lq, lk, place, dtype):
+    """Scores that leave fp32's range when they are scaled count as infinite: a row with a positive one is NaN, negative ones weigh nothing.
+    Those that stay inside give the row that the definition gives."""
+    dt = TYPES[dtype]
+    q = torch.zeros(1, lq, 1, 64, dtype=dt, device="cuda")
+    k, v = torch.zeros(1, lk, 1, 64, dtype=dt, device="cuda"), rand(3, dt, 1, lk, 1, 64)
+    k[0, place, 0, 0] = 2
+    for i, x in enumerate((0.0, 1.0, -1.0, 0.5)):            # scores of 0, 4e38, -4e38 and 2e38 at that key, of 0 elsewhere
+        q[0, i::4, 0, 0] = x
+    out, lse = fm.attend(q, k, v, scale=2e38, return_lse=True)
+    vv = v[0, :, 0].double()
+    rest = torch.arange(lk, device="cuda") != place
+    u = unit(dt)
+
+    def near(x, want, values):
+        # equal weights that are powers of two at most: products and sums are exact but for fp32's rounding, the output is rounded once
+        return ((x.double() - want).abs() <= u * want.abs() + lk * 2.0 ** -23 * values.abs().mean(0) + 2.0 ** -25).all()
+
+    assert near(out[0, 0::4, 0], vv.mean(0), vv)
+    assert ((lse[0, 0::4] - math.log(lk)).abs() < 1e-4).all()
+    assert torch.isnan(out[0, 1::4]).all()
+    assert (torch.isnan(lse[0, 1::4]) | (lse[0, 1::4] == math.inf)).all()
+    assert near(out[0, 2::4, 0], vv[rest].mean(0), vv)
+    assert ((lse[0, 2::4] - math.log(lk - 1)).abs() < 1e-4).all()
+    assert near(out[0, 3::4, 0], vv[place], vv[place:place + 1])
+    assert ((lse[0, 3::4] / 2e38 - 1).abs() < 1e-5).all()
+    fm.check_attention_status()
+
+
+@pytest.mark.parametrize("lq", [4, 700])
+def test_keys_whose_scores_are_minus_infinity(fm, lq):
+    # every score of the first row is -4e38, of the second -4e38 up to the last key, whose score is 0
+    dt = torch.bfloat16
+    q = torch.zeros(1, lq, 1, 64, dtype=dt, device="cuda")
+    q[0, 0::2, 0, 0], q[0, 1::2, 0, 1] = -1, -1
+    k, v = torch.zeros(1, 500, 1, 64, dtype=dt, device="cuda"), rand(3, dt, 1, 500, 1, 64)
+    k[..., :2] = 2
+    k[0, -1, 0, 1] = 0
+    out, lse = fm.attend(q, k, v, scale=2e38, return_lse=True)
+    assert (out[0, 0::2] == 0).all() and (lse[0, 0::2] == -math.inf).all()
+    assert (out[0, 1::2, 0] == v[0, -1, 0]).all() and (lse[0, 1::2].abs() < 1e-5).all()
+    fm.check_attention_status()
