@@ -186,14 +186,13 @@ mass_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ C
         __syncwarp();
     } else if (warp == 1) {
         const bool leader = elect_one();
-        bool ok = n == 0 || wait(bar_a, 0);
+        // waits are voted on: control flow stays uniform, and one that ran out ends the loop of all lanes, with nothing committed
+        bool ok = n == 0 || __all_sync(0xffffffffu, wait(bar_a, 0));
         int slot = 0;
         uint32_t phase = 0;
         const uint32_t idesc = att_idesc<T>(16, false) - (2u << 17) + ((uint32_t)(p.cols >> 3) << 17);
         for (int i = 0; i < n && ok; i++) {
-            ok = wait(bar_full + slot * 8, phase);
-            ok = ok && wait(bar_free + (i & 1) * 8, ((i >> 1) & 1) ^ 1);
-            ok = __all_sync(0xffffffffu, ok);
+            ok = __all_sync(0xffffffffu, wait(bar_full + slot * 8, phase) && wait(bar_free + (i & 1) * 8, ((i >> 1) & 1) ^ 1));
             tc_fence_after();
             const uint32_t s = sbase + p.ring_off + slot * p.stage, a = sbase + p.a_off;
             const uint32_t ka = FEW ? s : a, qa = FEW ? a : s;
@@ -204,8 +203,8 @@ mass_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ C
                 for (int k = 0; k < 4; k++)
                     tc_mma_f16_by<false>(leader && ok, tmem + p.cols * (i & 1), da + 2 * k, db + 2 * k, idesc, c + k > 0);
             }
-            tc_commit_by<false>(leader, bar_s + (i & 1) * 8);
-            tc_commit_by<false>(leader, bar_empty + slot * 8);
+            tc_commit_by<false>(leader && ok, bar_s + (i & 1) * 8);
+            tc_commit_by<false>(leader && ok, bar_empty + slot * 8);
             if (++slot == p.ring) {
                 slot = 0;
                 phase ^= 1;
