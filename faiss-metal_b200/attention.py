@@ -15,7 +15,8 @@ The work is queued on torch's current stream of that device; nothing waits for i
 out) is raised by the next call after it happened, or by ``check_attention_status()``.
 
 The functions do not record gradients: inputs that require them are refused unless gradients are off
-(``torch.no_grad()``); ``attend_backward`` is the gradient.
+(``torch.no_grad()``); ``attend_backward`` is the gradient.  Forward-mode tangents and tensors inside a transform of
+``torch.func`` (``vmap``, ``grad``, ``jvp``) are refused.
 """
 from __future__ import annotations
 
@@ -161,7 +162,12 @@ def _number(x):
 def _look(what: str, *tensors):
     """The part of a plan's key that comes from tensors (None: not given)."""
     import torch
+    forward_ad = torch.autograd.forward_ad
     grad = torch.is_grad_enabled()
+    if torch._C._functorch.peek_interpreter_stack() is not None and any(
+            isinstance(x, torch.Tensor) and torch._C._functorch.is_functorch_wrapped_tensor(x) for x in tensors):
+        raise ValueError("%s: has no form inside torch.func transforms (vmap, grad, jvp)" % what)
+    dual = forward_ad._current_level >= 0 and torch._C._is_fwd_grad_enabled()
     key = [what]
     for x in tensors:
         if x is None:
@@ -172,6 +178,8 @@ def _look(what: str, *tensors):
         if grad and x.requires_grad:
             raise ValueError("%s: a tensor requires a gradient, which is not recorded; use torch.no_grad() and attend_backward"
                              % what)
+        if dual and forward_ad.unpack_dual(x).tangent is not None:
+            raise ValueError("%s: a tensor carries a forward-mode tangent, which is not propagated" % what)
         key.append((x.dtype, x.shape, x.stride(), x.device))
     return key
 
