@@ -25,6 +25,9 @@ namespace {
 constexpr int GRAD_THREADS = 384;   // TMA, MMA, two spare warps; 2 x 4 warps
 constexpr int GRAD_ROWS = 64;       // rows of a streamed tile
 constexpr int GRAD_MAX_STAGES = 8;
+// Tiles whose products are summed up in tensor memory, 2^15 rows; then the sums go to memory and start from 0 (see SUM_TILES in attend.cu).  Even:
+// the same group of warps does it every time.
+constexpr int GRAD_SUM_TILES = 512;
 template <int DP>
 constexpr int GRAD_A_BYTES = DP / 64 * ATT_CHUNK;
 template <int DP>
@@ -68,6 +71,7 @@ struct GradParams {
     uint16_t* out1;          // dk or dq; dense
     uint16_t* out2;          // dv
     float* part;             // splits > 1: [split][out1 | out2] in fp32
+    float* sums;             // one range of more than GRAD_SUM_TILES tiles: [out1 | out2] in fp32
     int64_t part_stride, part2;
     int32_t* status;
 };
@@ -377,8 +381,9 @@ __device__ __forceinline__ void grad_item(const CUtensorMap& map_k, const CUtens
             if (!ok) break;
             tc_fence_after();
             const uint32_t b1 = ring + used * 2 * BBYTES, x = 64 * (i & 1);
-            mma_weights<T, DP, GRAD_ROWS>(leader, tmem + TG_ACC1, tmem + TG_P + x, b1, i > 0);
-            if (KEYS) mma_weights<T, DP, GRAD_ROWS>(leader, tmem + TG_ACC2, tmem + TG_S + x, b1 + BBYTES, i > 0);
+            const bool add = i % GRAD_SUM_TILES != 0;
+            mma_weights<T, DP, GRAD_ROWS>(leader, tmem + TG_ACC1, tmem + TG_P + x, b1, add);
+            if (KEYS) mma_weights<T, DP, GRAD_ROWS>(leader, tmem + TG_ACC2, tmem + TG_S + x, b1 + BBYTES, add);
             tc_commit_by<false>(leader, bar_empty + used * 8);
             if (++used == STAGES) used = 0;
             if (i + 2 < n) ok = scores(i + 2);
@@ -401,6 +406,9 @@ __device__ __forceinline__ void grad_item(const CUtensorMap& map_k, const CUtens
         }
         if (KEYS && HALF) factor = power_of_2(unit_range(p.range, p.units, unit).common() - WEIGHT_BITS);
         bool ok = true;
+        const int64_t at = KEYS ? ((b * p.len.n + r) * p.kv_heads + kvh) * p.d : ((b * p.queries + t) * p.heads + kvh * p.group + g) * p.d;
+        // where this row's sums are kept
+        auto kept = [&](bool second) { return (p.part ? p.part + sp * p.part_stride : p.sums) + (second ? p.part2 : 0) + at; };
         for (int i = wg; i < n; i += 2) {
             ok = wait(bar_s + wg * 8, (i >> 1) & 1);
             // the stage's statistics: complete since the scores are there, and not refilled before this tile's products
@@ -440,10 +448,33 @@ __device__ __forceinline__ void grad_item(const CUtensorMap& map_k, const CUtens
                 tc_st16(tp + 16 * h, ws);
             }
             tc_wait_st();
+            if (i > 0 && i % GRAD_SUM_TILES == 0) {
+                // once the previous tile's products are done, which give their stage back: this tile's wait for bar_p, so that it is not given back again
+                ok = waits(bar_empty + ((i - 1) % STAGES) * 8, ((i - 1) / STAGES) & 1);
+                if (!ok) break;
+                tc_fence_after();
+#pragma unroll 1
+                for (int ch = 0; ch < (KEYS ? 2 : 1) * DP / 16; ch++) {
+                    const bool second = ch >= DP / 16;
+                    const int col = (ch - (second ? DP / 16 : 0)) * 16;
+                    uint32_t o[16];
+                    tc_ld16_wait(tmem + (second ? TG_ACC2 : TG_ACC1) + lanes + col, o);
+#pragma unroll
+                    for (int e = 0; e < 16; e += 4)
+                        if (live && col + e < p.d) {
+                            float4* const x = reinterpret_cast<float4*>(kept(second) + col + e);
+                            float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+                            if (i > GRAD_SUM_TILES) y = *x;
+                            *x = make_float4(y.x + __uint_as_float(o[e]), y.y + __uint_as_float(o[e + 1]), y.z + __uint_as_float(o[e + 2]),
+                                             y.w + __uint_as_float(o[e + 3]));
+                        }
+                }
+            }
             tc_fence_before();
             __syncwarp();
             mbar_arrive_if(lane == 0, bar_p + wg * 8);
         }
+        if (n > GRAD_SUM_TILES) asm volatile("bar.sync 2, 256;" ::: "memory");   // one group's sums, read by both
         // ------------------------------ results: KEYS: a group of warps an accumulator, else half of its columns each
         if (ok) ok = wait(bar_done, 0);
         ok = __all_sync(0xffffffffu, ok);
@@ -453,8 +484,6 @@ __device__ __forceinline__ void grad_item(const CUtensorMap& map_k, const CUtens
             const float mul = (KEYS && wg == 1) ? 1.f : p.scale;
             float undo = 1.f;   // of the powers of two
             if (HALF) undo = KEYS && wg ? power_of_2(-WEIGHT_BITS) : power_of_2(-WEIGHT_BITS) / factor;
-            const int64_t at = KEYS ? ((b * p.len.n + r) * p.kv_heads + kvh) * p.d
-                                    : ((b * p.queries + t) * p.heads + kvh * p.group + g) * p.d;
             const uint32_t acc = tmem + (KEYS && wg ? TG_ACC2 : TG_ACC1) + lanes;
             constexpr int COLS = KEYS ? DP : DP / 2;
             const int col0 = KEYS ? 0 : wg * COLS;
@@ -465,6 +494,17 @@ __device__ __forceinline__ void grad_item(const CUtensorMap& map_k, const CUtens
                 uint32_t o[32];
                 tc_ld32(acc + col, o);
                 tc_wait_ld32(o);
+                if (n > GRAD_SUM_TILES && live) {
+#pragma unroll
+                    for (int e = 0; e < 32; e += 4)
+                        if (col + e < p.d) {
+                            const float4 y = *reinterpret_cast<const float4*>(kept(KEYS && wg) + col + e);
+                            o[e] = __float_as_uint(__uint_as_float(o[e]) + y.x);
+                            o[e + 1] = __float_as_uint(__uint_as_float(o[e + 1]) + y.y);
+                            o[e + 2] = __float_as_uint(__uint_as_float(o[e + 2]) + y.z);
+                            o[e + 3] = __float_as_uint(__uint_as_float(o[e + 3]) + y.w);
+                        }
+                }
 #pragma unroll
                 for (int e = 0; e < 32; e++) o[e] = zero ? 0u : __float_as_uint(__uint_as_float(o[e]) * undo * mul);
                 if (!p.part) {
@@ -663,6 +703,7 @@ struct GradPlan {
     RowTiles rt;
     int64_t key_blocks, row_blocks;
     int key_splits, row_splits;
+    bool key_sums, row_sums;   // one range, whose sums are moved
     size_t range_bytes, stat_bytes, moved_bytes, key_part_bytes, scratch;
 };
 // Ranges of the streamed tiles: where an item would take more than twice an SM's share of the work, as many as bring it down to that, of
@@ -690,8 +731,10 @@ GradPlan plan_grad(const B200FAttendBackwardArgs& a) {
     pl.range_bytes = half ? (size_t)round_up64(2 * units * 4, 256) : 0;
     pl.stat_bytes = (size_t)round_up64(units * pl.rt.tiles * 4 * (half ? GRAD_STATS<__half> : GRAD_STATS<__nv_bfloat16>), 256);
     pl.moved_bytes = half ? (size_t)round_up64(rows * 2, 256) : 0;
-    pl.key_part_bytes = pl.key_splits > 1 ? (size_t)round_up64(pl.key_splits * 2 * keys * 4, 256) : 0;
-    pl.scratch = 256 + pl.range_bytes + pl.stat_bytes + pl.moved_bytes + pl.key_part_bytes + (pl.row_splits > 1 ? (size_t)pl.row_splits * rows * 4 : 0);
+    pl.key_sums = a.n > 0 && pl.key_splits == 1 && pl.rt.tiles > GRAD_SUM_TILES;
+    pl.row_sums = a.queries > 0 && pl.row_splits == 1 && row_tiles > GRAD_SUM_TILES;
+    pl.key_part_bytes = pl.key_splits > 1 || pl.key_sums ? (size_t)round_up64(pl.key_splits * 2 * keys * 4, 256) : 0;
+    pl.scratch = 256 + pl.range_bytes + pl.stat_bytes + pl.moved_bytes + pl.key_part_bytes + (pl.row_splits > 1 || pl.row_sums ? (size_t)pl.row_splits * rows * 4 : 0);
     return pl;
 }
 
@@ -768,6 +811,7 @@ int launch_backward(const B200FAttendBackwardArgs& a, const GradPlan& pl, GradPa
     pk.out1 = static_cast<uint16_t*>(a.grad_k);
     pk.out2 = static_cast<uint16_t*>(a.grad_v);
     pk.part = pl.key_splits > 1 ? part : nullptr;
+    pk.sums = pl.key_sums ? part : nullptr;
     pk.part_stride = 2 * keys;
     pk.part2 = keys;
     pr.splits = pl.row_splits;
@@ -775,6 +819,7 @@ int launch_backward(const B200FAttendBackwardArgs& a, const GradPlan& pl, GradPa
     pr.out1 = static_cast<uint16_t*>(a.grad_q);
     pr.out2 = nullptr;
     pr.part = pl.row_splits > 1 ? part + pl.key_part_bytes / 4 : nullptr;
+    pr.sums = pl.row_sums ? part + pl.key_part_bytes / 4 : nullptr;
     pr.part_stride = rows;
     pr.part2 = 0;
     rc = a.d > 64 ? launch_grad<T, 128>(maps, pk, pr, units * pl.key_blocks * pl.key_splits, units * pl.row_blocks * pl.row_splits, st)

@@ -4,7 +4,7 @@ import math
 import pytest
 
 import attention_ref as R
-from test_gpu_attention import TYPES, check_out, lens, rand, unit
+from test_gpu_attention import TYPES, check_grads, check_out, lens, rand, unit
 
 pytestmark = pytest.mark.gpu
 
@@ -280,4 +280,75 @@ def test_keys_whose_scores_are_minus_infinity(fm, lq):
     out, lse = fm.attend(q, k, v, scale=2e38, return_lse=True)
     assert (out[0, 0::2] == 0).all() and (lse[0, 0::2] == -math.inf).all()
     assert (out[0, 1::2, 0] == v[0, -1, 0]).all() and (lse[0, 1::2].abs() < 1e-5).all()
+    fm.check_attention_status()
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_sums_of_many_queries_in_the_gradient(fm, dtype):
+    """One query's weight times its output gradient is 64 at key 0; 500,000 others give 1.8e-6 each, 0.9 together: just below 2^-25 of the sum."""
+    dt = TYPES[dtype]
+    b, lq, lk, d = 110, 500_000, 128, 64                     # so many sequences that the queries are one range
+    q = torch.zeros(1, lq, 1, d, dtype=dt, device="cuda")
+    q[..., 0] = 1
+    q[0, 0, 0, 0] = -8
+    k, v = torch.zeros(1, lk, 1, d, dtype=dt, device="cuda"), rand(3, dt, 1, lk, 1, d)
+    k[0, 0, 0, 0] = -8.375
+    grad = torch.ones(1, lq, 1, d, dtype=dt, device="cuda")
+    grad[0, 0] = 64
+    many = (lambda x: x.expand(b, -1, -1, -1))
+    out, lse = fm.attend(many(q), many(k), many(v), scale=1.0, return_lse=True)
+    gv = fm.attend_backward(many(grad), many(q), many(k), many(v), out, lse, scale=1.0)[2]
+    p0 = 1 / (1 + 127 * math.exp(-67))
+    want = 64 * p0 + (lq - 1) * math.exp(-8.375) / (127 + math.exp(-8.375))
+    # weights and the result are rounded once, sums of 2^15 terms lose 2^-25 a term
+    assert ((gv[:, 0].double() / want - 1).abs() <= 2.2 * unit(dt) + 2.0 ** -10).all(), (gv[0, 0, 0, 0].item(), want)
+    assert (gv == gv[:1]).all()
+    fm.check_attention_status()
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("lq", [128, 100])
+def test_sums_of_many_keys_in_the_gradient(fm, lq, dtype):
+    """Key 0 has half of a row's weight, 2^19 others the rest: their score gradients, -1 / 2^19 of its own each, meet key entries of 7/16
+    where it has 64, and are less than 2^-25 of the sum."""
+    dt = TYPES[dtype]
+    b, lk, d = 110, 2 ** 19 + 1, 64
+    q = torch.zeros(b, lq, 1, d, dtype=dt, device="cuda")
+    q[..., 0] = 1
+    k, v = torch.full((1, lk, 1, d), 0.4375, dtype=dt, device="cuda"), torch.zeros(1, lk, 1, d, dtype=dt, device="cuda")
+    k[..., 0] = 0
+    k[0, 0] = 64
+    k[0, 0, 0, 0] = 13.1875                                  # ln 2^19 = 13.17
+    v[0, 0] = 1
+    many = (lambda x: x.expand(b, -1, -1, -1))
+    top = k[0, 0, 0, 0].item()
+    grad = torch.ones_like(q)
+    out, lse = fm.attend(q, many(k), many(v), scale=1.0, return_lse=True)
+    gq = fm.attend_backward(grad, q, many(k), many(v), out, lse, scale=1.0)[0]
+    p0 = math.exp(top) / (math.exp(top) + lk - 1)
+    ds = p0 * (1 - p0) * d
+    want = ds * (64 - 0.4375)
+    # score gradients are rounded once, delta comes from the rounded output: u p0 d, of which key 0 and all others take their weights; the
+    # result is rounded once; sums of 2^15 terms lose 2^-25 a term
+    u = unit(dt)
+    tol = u * want + 1.1 * u * ds * 64.4375 + u * p0 * d * (p0 * 64 + (1 - p0) * 0.4375) + 2.0 ** -10 * ds * 64
+    assert ((gq[..., 1:].double() - want).abs() <= tol).all(), (gq[0, 0, 0, 1].item(), want, tol)
+    fm.check_attention_status()
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("b,lq,lk,h,d", [(40, 33_000, 200, 3, 64), (3, 100, 70_000, 8, 72), (40, 40, 70_000, 3, 128), (1, 70_000, 100, 2, 128)])
+def test_gradients_of_long_ranges(fm, b, lq, lk, h, d, dtype):
+    # sums that are moved to memory on the way, in one range and in several, against the definition
+    dt = TYPES[dtype]
+    q, k, v = rand(1, dt, b, lq, h, d, scale=1.5), rand(2, dt, b, lk, 1, d), rand(3, dt, b, lk, 1, d)
+    grad = rand(4, dt, b, lq, h, d)
+    n = torch.tensor([max(lk - 1000 * (i % 3), lk // 2) for i in range(b)], dtype=torch.int32, device="cuda")
+    out, lse = fm.attend(q, k, v, key_lengths=n, return_lse=True)
+    got = fm.attend_backward(grad, q, k, v, out, lse, key_lengths=n)
+    for i in {0, 1 % b, b - 1}:
+        one = slice(i, i + 1)
+        check_grads([x[one] for x in got], R.backward(grad[one], q[one], k[one], v[one], n[one]), dt)
+    again = fm.attend_backward(grad, q, k, v, out, lse, key_lengths=n)
+    assert all(torch.equal(x, y) for x, y in zip(got, again))
     fm.check_attention_status()
