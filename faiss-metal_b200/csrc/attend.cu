@@ -39,7 +39,8 @@ constexpr float TILE_MASKED_BITS = std::is_same<T, __half>::value ? 12.f : 8.f;
 constexpr int TILE_KEYS = 128;
 // A product is added to the sum in tensor memory with some two bits below that sum's last place, the rest cut off: a term loses 2^-26 of the sum
 // on average, and 1,000,000 keys behind one that outweighs them lost 30 % of their share.  After so many tiles (2^15 keys, 2^-11 of the sum)
-// a row's sums go to memory, where they are added up in fp32, and start from 0 again.
+// a row's sums go to memory, where they are added up in fp32, and start from 0 again; so does the sum of its weights, whose small terms round the same way
+// one after the other.
 constexpr int SUM_TILES = 256;
 constexpr int TILE_MAX_STAGES = 10;
 template <int DP>
@@ -371,11 +372,13 @@ attend_tile_kernel(const __grid_constant__ CUtensorMap map_sk, const __grid_cons
         auto row_index = [&] { return (at.b * p.queries + at.t) * p.heads + at.h; };
         // where this row's sums are kept, in units of the reference m_kept
         auto kept_row = [&] { return whole ? p.sums + row_index() * p.d : p.part_o + (part * p.rows_total + row_index()) * p.d; };
-        float m_kept = -CUDART_INF_F;
+        float m_kept = -CUDART_INF_F, l_kept = 0.f;
         auto keep_sums = [&](bool first) __attribute__((always_inline)) {
             float* const kept = kept_row();
             const float f = m_kept == m ? 1.f : ex2((m_kept - m) * c);
             m_kept = m;
+            l_kept = fmaf(l_kept, f, l);
+            l = 0.f;
 #pragma unroll 1
             for (int i = 0; i < DP / 16; i++) {
                 uint32_t o[16];
@@ -483,11 +486,14 @@ attend_tile_kernel(const __grid_constant__ CUtensorMap map_sk, const __grid_cons
         if (ok && warp_live) {
             tc_fence_after();
             const bool none = nt == 0;
+            float* const kept = kept_row();
+            if (nt > SUM_TILES) {
+                keep_sums(false);
+                l = l_kept;
+            }
             const int64_t grow = row_index();
             const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
             const float lse2 = l > 0.f || l != l ? log2f(l) - (float)TILE_WEIGHT_BITS<T> + (m == -CUDART_INF_F ? 0.f : m * c) : -CUDART_INF_F;
-            float* const kept = kept_row();
-            if (nt > SUM_TILES) keep_sums(false);
             if (live) {
                 if (whole) {
                     if (p.lse) p.lse[grow] = lse2 * kLn2;

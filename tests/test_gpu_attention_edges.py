@@ -352,3 +352,20 @@ def test_gradients_of_long_ranges(fm, b, lq, lk, h, d, dtype):
     again = fm.attend_backward(grad, q, k, v, out, lse, key_lengths=n)
     assert all(torch.equal(x, y) for x, y in zip(got, again))
     fm.check_attention_status()
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_log_sums_of_a_million_keys(fm, dtype):
+    """The weights of 1,000,000 equal keys, 1.5 % of the first one's all together, are added up with fp32's rounding: 96 or 32 at once, in chains of
+    2^15 keys (half a step of 2^-23 each, 512 of them) that are then added up (31), and exponentials are good to 2.7e-6."""
+    dt = TYPES[dtype]
+    b, lk = 75, 1_000_000
+    q = torch.zeros(b, 256, 1, 64, dtype=dt, device="cuda")
+    q[..., 0] = 1
+    k = torch.zeros(1, lk, 1, 64, dtype=dt, device="cuda")
+    k[0, 0, 0, 0] = 18
+    many = (lambda x: x.expand(b, -1, -1, -1))
+    lse = fm.attend(q, many(k), many(k), scale=1.0, return_lse=True)[1]
+    want = 18 + math.log1p((lk - 1) * math.exp(-18.0))
+    # 18 itself is held to 2^-20
+    assert (lse.double() - want).abs().max() <= (512 + 31) * 2.0 ** -24 + 2.7e-6 + 2.0 ** -20 * 2
