@@ -701,6 +701,7 @@ attend_few_kernel(const __grid_constant__ CUtensorMap map_sk, const __grid_const
         }
         const float c = p.scale * kLog2e;
         const float slack = fminf((float)FEW_SLACK_BITS / c, 1e30f);
+        float mc[2] = {0.f, 0.f};   // FEW_WEIGHT_BITS - c m
         // this lane's row address in ldmatrix: matrix lane / 8, row lane % 8 of the warp's 16 keys
         const int mi = lane >> 3, mr = lane & 7;
         const int krow = warp * 16 + (mi >> 1) * 8 + mr, kpiece = mi & 1;   // keys: (0-7, d 0-7), (0-7, d 8-15), (8-15, ..)
@@ -750,6 +751,12 @@ attend_few_kernel(const __grid_constant__ CUtensorMap map_sk, const __grid_const
                 const float f0 = g0 ? ex2((m[0] - top[0]) * c) : 1.f, f1 = g1 ? ex2((m[1] - top[1]) * c) : 1.f;
                 if (g0) m[0] = top[0];
                 if (g1) m[1] = top[1];
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    // scaled scores beyond fp32's range count as infinite, as in the tiles
+                    const float m2 = m[e] * c;
+                    mc[e] = m2 == -CUDART_INF_F ? 0.f : m2 == CUDART_INF_F ? CUDART_NAN_F : (float)FEW_WEIGHT_BITS<T> - m2;
+                }
                 l[0] *= f0;
                 l[1] *= f1;
 #pragma unroll
@@ -765,10 +772,7 @@ attend_few_kernel(const __grid_constant__ CUtensorMap map_sk, const __grid_const
             for (int h = 0; h < 2; h++)
 #pragma unroll
                 for (int e = 0; e < 2; e++) {
-                    // scaled scores beyond fp32's range count as infinite, as in the tiles
-                    const float m2 = m[e] * c;
-                    const float mc = m2 == -CUDART_INF_F ? 0.f : m2 == CUDART_INF_F ? CUDART_NAN_F : (float)FEW_WEIGHT_BITS<T> - m2;
-                    const float x = ex2(fmaf(s[h][2 * e], c, mc)), y = ex2(fmaf(s[h][2 * e + 1], c, mc));
+                    const float x = ex2(fmaf(s[h][2 * e], c, mc[e])), y = ex2(fmaf(s[h][2 * e + 1], c, mc[e]));
                     l[e] += x + y;
                     w[2 * h + e] = pack2<T>(x, y);
                 }
