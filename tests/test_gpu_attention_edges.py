@@ -369,3 +369,57 @@ def test_log_sums_of_a_million_keys(fm, dtype):
     want = 18 + math.log1p((lk - 1) * math.exp(-18.0))
     # 18 itself is held to 2^-20
     assert (lse.double() - want).abs().max() <= (512 + 31) * 2.0 ** -24 + 2.7e-6 + 2.0 ** -20 * 2
+
+
+# ---- groups of odd size ----------------------------------------------------------------------------
+
+
+GROUPS = [(2, 3, 300, 65, 1, 64, (300, 77)), (1, 5, 1000, 96, 1, 128, None), (2, 1, 4000, 127, 1, 72, (4000, 1)), (1, 40, 513, 200, 2, 64, None),
+          (3, 70, 140, 34, 2, 128, (140, 0, 129)), (1, 300, 200, 65, 1, 64, None)]
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("shape", GROUPS, ids=str)
+def test_groups_that_do_not_fill_their_tiles(fm, shape, dtype):
+    # 65 to 127 heads a key head: a gradient tile of 64 and one that is part empty; 17, 100: a queries' tile with rows left over
+    b, lq, lk, h, hk, d, n = shape
+    dt = TYPES[dtype]
+    q, k, v = rand(1, dt, b, lq, h, d, scale=1.5), rand(2, dt, b, lk, hk, d), rand(3, dt, b, lk, hk, d)
+    grad = rand(4, dt, b, lq, h, d)
+    n = lens(*n) if n else None
+    out, lse = fm.attend(q, k, v, key_lengths=n, return_lse=True)
+    check_out(out, lse, R.attend(q, k, v, n), dt, lk)
+    check_grads(fm.attend_backward(grad, q, k, v, out, lse, key_lengths=n), R.backward(grad, q, k, v, n), dt)
+    for causal in (False, True):
+        row = R.softmax(R.scores(q, k, n, 1 / math.sqrt(d), causal))[1].permute(0, 2, 1).float().contiguous()
+        got, want = fm.attention_mass(q, k, row, key_lengths=n, causal=causal), R.mass(q, k, row, n, causal=causal)
+        assert ((got.double() - want).abs() <= 1e-5 * want.abs() + 1e-7).all()
+    pk, pv = rand(5, dt, 333, hk, d), rand(6, dt, 333, hk, d)
+    out, lse = fm.attend_shared(q, pk, pv, k, v, n, return_lse=True)
+    check_out(out, lse, R.attend(q, k, v, n, causal=True, shared=(pk, pv)), dt, 333 + lk)
+    fm.check_attention_status()
+
+
+# ---- eviction --------------------------------------------------------------------------------------
+
+
+def test_evicted_rows_and_rows_behind_the_end_do_not_come_through(fm):
+    # NaN and infinities in rows behind the end, and in rows that are evicted, reach nothing; in rows that stay they come through
+    dt = torch.float16
+    b, lk, hk, d, keep = 3, 500, 2, 64, 40
+    k, v = rand(1, dt, b, lk, hk, d), rand(2, dt, b, lk, hk, d)
+    m = rand(3, torch.float32, b, hk, lk).abs() + 0.5
+    n = lens(500, 300, 17)
+    want = fm.evict(k, v, m, n, keep, recent=5)
+    kept = torch.zeros(b, hk, lk + 1, dtype=torch.bool, device="cuda").scatter_(2, want[3].long() % (lk + 1), True)[..., :lk]
+    gone = ~kept.permute(0, 2, 1)
+    k2, v2, m2 = k.clone(), v.clone(), m.clone()
+    k2[gone], v2[gone] = math.nan, math.inf
+    for i, x in enumerate(n.tolist()):
+        m2[i, :, x:] = math.nan
+        m2[i, 0, x:] = math.inf
+    got = fm.evict(k2, v2, m2, n, keep, recent=5)
+    assert all(torch.equal(x, y) for x, y in zip(want, got))
+    k2 = k.clone()
+    k2[0, -1] = math.nan                                     # among the recent ones
+    assert torch.isnan(fm.evict(k2, v, m, n, keep, recent=5)[0][0, keep - 1]).all()
