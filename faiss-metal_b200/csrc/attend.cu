@@ -938,8 +938,10 @@ struct AttendPlan {
 // How a segment's work is cut: ranges of keys that fill the SMs, of at least MIN_TILES tiles; and by which kernel.  Blocks of more than
 // 16 rows may go to either: the few-rows kernel starts and ends sooner, but reads the keys again for every block.  What is measured
 // (us, bf16, d = 128): a tile CTA 7 and 1.7 a tile of 128 keys, one an SM; a few-rows CTA 3.5 and 0.5 a tile of 64, two an SM; joining parts
-// 4.5.  E.g. few-rows / tiles: 2 units of 64 rows and 4,096 keys 10.6 / 15.2, of 48 rows and 16,384 keys 21.8 / 18.8; 8 units of 512
-// rows and 256 keys 8.5 / 12.6, 512 keys 18.4 / 15.4.
+// 4.5.  Few-rows / tiles at d = 128, then at d = 64: 2 units of 64 rows over 4,096 keys 10.6 / 15.7, 9.2 / 13.9; 2 of 48 over 16,384 16.7 / 18.4,
+// 14.1 / 16.9; 8 of 512 over 256 8.3 / 12.9, 6.0 / 10.8; 8 of 512 over 512 19.2 / 16.0, 14.7 / 13.5; 64 of 48 over 512 17.8 / 13.8, 13.6 /
+// 11.9; 148 of 64 over 1,024 43.8 / 20.9, 30.6 / 18.8.  Both cost less at d = 64, in much the same measure: of twelve such pairs at d = 128, 64 and 32
+// each the faster side was taken every time.
 constexpr int MIN_TILES = 2;
 constexpr int FEW_MIN_TILES = 4;
 constexpr double TILE_START_US = 7, TILE_US = 1.7, FEW_START_US = 3.5, FEW_US = 0.5, JOIN_US = 4.5;
