@@ -284,6 +284,22 @@ def test_keys_whose_scores_are_minus_infinity(fm, lq):
 
 
 @pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("b,t,p,n,h,hk,d", [(300, 1, 300_000, 40, 16, 2, 64), (300, 1, 300_000, 40, 16, 2, 128), (40, 300, 0, 70_000, 2, 1, 64),
+                                            (40, 300, 70_000, 40_000, 2, 1, 128)])
+def test_sums_of_long_prefixes_and_prompts(fm, b, t, p, n, h, hk, d, dtype):
+    dt = TYPES[dtype]
+    q, pk, pv = rand(1, dt, b, t, h, d, scale=1.5), rand(2, dt, p, hk, d), rand(3, dt, p, hk, d)
+    k, v = rand(4, dt, 1, n, hk, d).expand(b, -1, -1, -1), rand(5, dt, 1, n, hk, d).expand(b, -1, -1, -1)
+    length = torch.tensor([max(n - 37 * i, t) for i in range(b)], dtype=torch.int32, device="cuda")
+    out, lse = fm.attend_shared(q, pk, pv, k, v, length, return_lse=True)
+    for i in (0, 1, b - 1):
+        one = slice(i, i + 1)
+        check_out(out[one], lse[one], R.attend(q[one], k[one], v[one], length[one], causal=True, shared=(pk, pv)), dt, p + n)
+    assert torch.equal(out, fm.attend_shared(q, pk, pv, k, v, length))
+    fm.check_attention_status()
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
 def test_sums_of_many_queries_in_the_gradient(fm, dtype):
     """One query's weight times its output gradient is 64 at key 0; 500,000 others give 1.8e-6 each, 0.9 together: just below 2^-25 of the sum."""
     dt = TYPES[dtype]
