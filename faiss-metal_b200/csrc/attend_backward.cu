@@ -548,37 +548,40 @@ grad_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ C
 }
 
 // ---- fp16: grad_range_kernel: the units' largest rows (UnitRange) --------------------------------
-// A CTA takes rows of a unit, of do and q or of v, LANES lanes a row and four rows a lane.  A maximum does not depend on the order.  Rows that are
-// not finite, or zero, do not count: their terms are NaN, or 0, whatever the factors.
+// A CTA takes rows of a unit, of do and q or of v, LANES lanes a row and eight loads a lane.  A maximum does not depend on the order.  Rows that
+// are not finite, or zero, do not count: their terms are NaN, or 0, whatever the factors.
 template <int LANES>
-constexpr int RANGE_ROWS = 4 * 256 / LANES;
+constexpr int RANGE_ROWS = 4 * 256 / LANES;   // of queries; twice as many of values
 template <int LANES>
 __global__ void __launch_bounds__(256, 5) grad_range_kernel(AttView g, AttView q, AttView v, AttLengths len, uint32_t units, uint32_t kv_heads,
                                                             uint32_t group, int d, uint32_t* range) {
     constexpr int ROWS = RANGE_ROWS<LANES>;
     const int sub = threadIdx.x % LANES, slot = threadIdx.x / LANES;
     const uint32_t rows = (uint32_t)len.queries * group;
-    const uint32_t row_blocks = (rows + ROWS - 1) / ROWS, blocks = row_blocks + (uint32_t)((len.n + ROWS - 1) / ROWS);
+    const uint32_t row_blocks = (rows + ROWS - 1) / ROWS, blocks = row_blocks + (uint32_t)((len.n + 2 * ROWS - 1) / (2 * ROWS));
     for (uint32_t item = blockIdx.x; item < units * blocks; item += gridDim.x) {   // below 2^31: b200f_attend_backward sees to it
         const uint32_t unit = item / blocks, block = item - unit * blocks, b = unit / kv_heads, kvh = unit - b * kv_heads;
         uint32_t most = 0;
-        auto take = [&](bool query, uint32_t row0, uint32_t end) __attribute__((always_inline)) {
-            uint4 x[4], y[4];
+        auto take = [&](auto query_c, uint32_t row0, uint32_t end) __attribute__((always_inline)) {
+            constexpr bool query = decltype(query_c)::value;
+            constexpr int N = query ? 4 : 8;
+            uint4 x[N], y[4];
 #pragma unroll
-            for (int k = 0; k < 4; k++) {
+            for (int k = 0; k < N; k++) {
                 const uint32_t r = row0 + 256 / LANES * k + slot;
-                x[k] = y[k] = make_uint4(0, 0, 0, 0);
+                x[k] = make_uint4(0, 0, 0, 0);
+                if (query) y[k % 4] = make_uint4(0, 0, 0, 0);
                 if (r < end && sub * 8 < d) {
                     const uint32_t t = query ? r / group : r, h = query ? kvh * group + (r - t * group) : kvh;
                     x[k] = *reinterpret_cast<const uint4*>((query ? g : v).at(b, t, h) + sub * 8);
-                    if (query) y[k] = *reinterpret_cast<const uint4*>(q.at(b, t, h) + sub * 8);
+                    if (query) y[k % 4] = *reinterpret_cast<const uint4*>(q.at(b, t, h) + sub * 8);
                 }
             }
 #pragma unroll
-            for (int k = 0; k < 4; k++) {
+            for (int k = 0; k < N; k++) {
                 float square = 0.f, top = 1.f;
                 add_square(x[k], &square);
-                if (query) top = 0.f, add_largest(y[k], &top);
+                if (query) top = 0.f, add_largest(y[k % 4], &top);
 #pragma unroll
                 for (int o = LANES / 2; o > 0; o >>= 1) {
                     square += __shfl_xor_sync(0xffffffffu, square, o);
@@ -588,15 +591,15 @@ __global__ void __launch_bounds__(256, 5) grad_range_kernel(AttView g, AttView q
             }
         };
         if (block < row_blocks) {
-            take(true, block * ROWS, rows);
+            take(std::true_type(), block * ROWS, rows);
         } else {
-            const uint32_t row0 = (block - row_blocks) * ROWS, end = (uint32_t)len.of(b);
+            const uint32_t row0 = (block - row_blocks) * 2 * ROWS, end = (uint32_t)len.of(b);
             if (row0 >= end) continue;
-            take(false, row0, end);
+            take(std::false_type(), row0, end);
         }
         most = __reduce_max_sync(0xffffffffu, most);
         uint32_t* const to = range + (block < row_blocks ? 0 : units) + unit;
-        if ((threadIdx.x & 31) == 0 && most > __ldcg(to)) atomicMax(to, most);
+        if ((threadIdx.x & 31) == 0 && most) atomicMax(to, most);
     }
 }
 
@@ -778,7 +781,7 @@ int launch_backward(const B200FAttendBackwardArgs& a, const GradPlan& pl, GradPa
         if (HALF) {
             B200F_CUDA_TRY(cudaMemsetAsync(range, 0, 2 * units * 4, st));
             const int64_t per = a.d <= 64 ? RANGE_ROWS<8> : RANGE_ROWS<16>, most = (int64_t)cached_sm_count() * 24;
-            const int64_t items = units * (ceil_div64(a.queries * pl.rt.group, per) + ceil_div64(a.n, per));
+            const int64_t items = units * (ceil_div64(a.queries * pl.rt.group, per) + ceil_div64(a.n, 2 * per));
             auto* const kernel = a.d <= 64 ? grad_range_kernel<8> : grad_range_kernel<16>;
             kernel<<<(unsigned)(items < most ? items : most), 256, 0, st>>>(p.g, p.q, v, p.len, (uint32_t)units, (uint32_t)a.kv_heads,
                                                                             (uint32_t)pl.rt.group, a.d, range);
