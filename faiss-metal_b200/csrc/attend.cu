@@ -33,6 +33,9 @@ constexpr float WEIGHTS_MAX = 32768.f;     // fp16 weights end at 65504
 // what lies below 2^-25, with 1,000,000 such keys 1.5 % of a row.  96 weights of 2^8 add up to less than WEIGHTS_MAX.
 template <typename T>
 constexpr int TILE_WEIGHT_BITS = std::is_same<T, __half>::value ? 8 : 0;
+// Up to this scaled reference c m the weights are exp2(c s - c m), one operation before the exponential; c m is rounded, by 2^-12 at most here.  Beyond, where
+// it would be off by whole powers of two, a row has c (s - m), and a new look at its maximum in every tile.
+constexpr float NEAR_REFERENCE = 4096.f;
 // ends of sequences are weighed with the reference as it is up to this power of two
 template <typename T>
 constexpr float TILE_MASKED_BITS = std::is_same<T, __half>::value ? 12.f : 8.f;
@@ -83,7 +86,7 @@ struct TileParams {
     uint16_t* out;
     float* lse;
     float* part_o;         // [parts][rows_total][d], null: the one part is the result
-    float* part_lse;       // [parts][rows_total], base 2
+    float2* part_sum;      // [parts][rows_total]: the reference, as a score before scaling, and the sum of the weights against it
     float* sums;           // [rows_total][d]: of streams of more than SUM_TILES tiles, where there is one part (others have part_o's rows)
     int32_t* status;
 };
@@ -396,9 +399,9 @@ attend_tile_kernel(const __grid_constant__ CUtensorMap map_sk, const __grid_cons
         };
         uint32_t s[4][32];
         // weights of 32 keys to tensor memory; returns their sum
-        auto weigh = [&](auto mix, uint32_t (&x)[32], float mc_now, int i) __attribute__((always_inline)) {
+        auto weigh = [&](auto mix, uint32_t (&x)[32], float mc_now, float from, int i) __attribute__((always_inline)) {
             uint32_t w[16];
-            const float2 z = weigh32<T, decltype(mix)::value>(x, c, mc_now, w);
+            const float2 z = weigh32<T, decltype(mix)::value>(x, c, mc_now, from, w);
             tc_st16(tp + 16 * i, w);
             return z.x + z.y;
         };
@@ -429,7 +432,7 @@ attend_tile_kernel(const __grid_constant__ CUtensorMap map_sk, const __grid_cons
                         mbar_arrive_if(lane == 0, bar_free + t * 8);
                     }
                     if (!masked) {
-                        sum += weigh(std::true_type(), s[i], mc, i);
+                        sum += weigh(std::true_type(), s[i], mc, 0.f, i);
                     } else {
 #pragma unroll
                         for (int e = 0; e < 32; e++)
@@ -451,7 +454,10 @@ attend_tile_kernel(const __grid_constant__ CUtensorMap map_sk, const __grid_cons
                     l *= f;
                     // scaled scores beyond fp32's range count as infinite: +INF makes the row NaN, -INF weighs nothing
                     const float m2 = m * c;
-                    mc = fabsf(m2) == CUDART_INF_F ? CUDART_NAN_F : (float)TILE_WEIGHT_BITS<T> - m2;
+                    const bool far = !(fabsf(m2) <= NEAR_REFERENCE);
+                    mc = far ? CUDART_NAN_F : (float)TILE_WEIGHT_BITS<T> - m2;   // far: the next sum is NaN and comes here
+                    const float from = !far || m2 == -CUDART_INF_F ? 0.f : m2 == CUDART_INF_F ? CUDART_NAN_F : m;
+                    const float add = !far ? mc : m2 == -CUDART_INF_F ? 0.f : (float)TILE_WEIGHT_BITS<T>;
                     // O holds what came before: the previous tile's product is done (APART: waited for, else since the scores are there); the first part's
                     // may be under way
                     if (moved && h == 1) {
@@ -471,7 +477,7 @@ attend_tile_kernel(const __grid_constant__ CUtensorMap map_sk, const __grid_cons
                     sum = 0.f;
 #pragma unroll
                     for (int i = h ? PART : 0; i < (h ? 4 : PART); i++)
-                        sum += weigh(std::false_type(), s[i], m2 == -CUDART_INF_F ? 0.f : mc, i);
+                        sum += weigh(std::false_type(), s[i], add, from, i);
                 }
                 l += sum;
                 tc_wait_st();
@@ -498,7 +504,7 @@ attend_tile_kernel(const __grid_constant__ CUtensorMap map_sk, const __grid_cons
                 if (whole) {
                     if (p.lse) p.lse[grow] = lse2 * kLn2;
                 } else {
-                    p.part_lse[part * p.rows_total + grow] = lse2;
+                    p.part_sum[part * p.rows_total + grow] = make_float2(m, l * (1.f / (float)(1 << TILE_WEIGHT_BITS<T>)));
                 }
             }
             // results: through shared memory (the stream's query tile is done with), so that whole rows are written
@@ -700,8 +706,7 @@ attend_few_kernel(const __grid_constant__ CUtensorMap map_sk, const __grid_const
             }
         }
         const float c = p.scale * kLog2e;
-        const float slack = fminf((float)FEW_SLACK_BITS / c, 1e30f);
-        float mc[2] = {0.f, 0.f};   // FEW_WEIGHT_BITS - c m
+        float from[2] = {0.f, 0.f};   // the reference, where there is one
         // this lane's row address in ldmatrix: matrix lane / 8, row lane % 8 of the warp's 16 keys
         const int mi = lane >> 3, mr = lane & 7;
         const int krow = warp * 16 + (mi >> 1) * 8 + mr, kpiece = mi & 1;   // keys: (0-7, d 0-7), (0-7, d 8-15), (8-15, ..)
@@ -746,7 +751,7 @@ attend_few_kernel(const __grid_constant__ CUtensorMap map_sk, const __grid_const
                 top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 1));
                 top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 2));
             }
-            const bool g0 = top[0] > m[0] + slack, g1 = top[1] > m[1] + slack;
+            const bool g0 = (top[0] - m[0]) * c > (float)FEW_SLACK_BITS, g1 = (top[1] - m[1]) * c > (float)FEW_SLACK_BITS;
             if (__any_sync(0xffffffffu, g0 || g1)) {
                 const float f0 = g0 ? ex2((m[0] - top[0]) * c) : 1.f, f1 = g1 ? ex2((m[1] - top[1]) * c) : 1.f;
                 if (g0) m[0] = top[0];
@@ -755,7 +760,7 @@ attend_few_kernel(const __grid_constant__ CUtensorMap map_sk, const __grid_const
                 for (int e = 0; e < 2; e++) {
                     // scaled scores beyond fp32's range count as infinite, as in the tiles
                     const float m2 = m[e] * c;
-                    mc[e] = m2 == -CUDART_INF_F ? 0.f : m2 == CUDART_INF_F ? CUDART_NAN_F : (float)FEW_WEIGHT_BITS<T> - m2;
+                    from[e] = m2 == -CUDART_INF_F ? 0.f : m2 == CUDART_INF_F ? CUDART_NAN_F : m[e];
                 }
                 l[0] *= f0;
                 l[1] *= f1;
@@ -772,7 +777,8 @@ attend_few_kernel(const __grid_constant__ CUtensorMap map_sk, const __grid_const
             for (int h = 0; h < 2; h++)
 #pragma unroll
                 for (int e = 0; e < 2; e++) {
-                    const float x = ex2(fmaf(s[h][2 * e], c, mc[e])), y = ex2(fmaf(s[h][2 * e + 1], c, mc[e]));
+                    const float x = ex2(fmaf(s[h][2 * e] - from[e], c, (float)FEW_WEIGHT_BITS<T>));
+                    const float y = ex2(fmaf(s[h][2 * e + 1] - from[e], c, (float)FEW_WEIGHT_BITS<T>));
                     l[e] += x + y;
                     w[2 * h + e] = pack2<T>(x, y);
                 }
@@ -803,14 +809,14 @@ attend_few_kernel(const __grid_constant__ CUtensorMap map_sk, const __grid_const
     __syncthreads();
     if (!*abort_flag) {
         float* const po = reinterpret_cast<float*>(smem);                       // [4][FEW_ROWS][DP]
-        float* const pm = po + 4 * FEW_ROWS * DP, * const pl = pm + 4 * FEW_ROWS;   // base-2 maximum, sum
+        float* const pm = po + 4 * FEW_ROWS * DP, * const pl = pm + 4 * FEW_ROWS;   // reference, sum
+        const float c = p.scale * kLog2e;
         if (warp < 4) {
-            const float c = p.scale * kLog2e;
 #pragma unroll
             for (int e = 0; e < 2; e++) {
                 const int r = (lane >> 2) + 8 * e;
                 if ((lane & 3) == 0) {
-                    pm[warp * FEW_ROWS + r] = m[e] == -CUDART_INF_F ? -CUDART_INF_F : m[e] * c;
+                    pm[warp * FEW_ROWS + r] = m[e];
                     pl[warp * FEW_ROWS + r] = l[e];
                 }
 #pragma unroll
@@ -830,7 +836,7 @@ attend_few_kernel(const __grid_constant__ CUtensorMap map_sk, const __grid_const
                 const float lx = pl[x * FEW_ROWS + r];
                 if (lx == 0.f) continue;   // saw nothing
                 // a sum that is not 0 with maximum -INF: NaN came in
-                const float mx = pm[x * FEW_ROWS + r], f = mx == top ? 1.f : ex2(mx - top);
+                const float mx = pm[x * FEW_ROWS + r], f = mx == top ? 1.f : ex2((mx - top) * c);
                 total = fmaf(f, lx, total);
                 const float* const src = po + (x * FEW_ROWS + r) * DP + c0;
 #pragma unroll
@@ -840,7 +846,7 @@ attend_few_kernel(const __grid_constant__ CUtensorMap map_sk, const __grid_const
             const float inv = none ? 0.f : 1.f / total;
             const RowAt at = row_at(p, shared, unit, row0 + r);
             const int64_t grow = (at.b * p.queries + at.t) * p.heads + at.h;
-            const float lse2 = none ? -CUDART_INF_F : log2f(total) - (float)FEW_WEIGHT_BITS<T> + (top == -CUDART_INF_F ? 0.f : top);
+            const float lse2 = none ? -CUDART_INF_F : log2f(total) - (float)FEW_WEIGHT_BITS<T> + (top == -CUDART_INF_F ? 0.f : top * c);
 #pragma unroll
             for (int e = 0; e < 8; e++) acc[e] = none ? 0.f : acc[e] * inv;
             if (!p.part_o) {
@@ -851,7 +857,7 @@ attend_few_kernel(const __grid_constant__ CUtensorMap map_sk, const __grid_const
                 float4* const dst = reinterpret_cast<float4*>(p.part_o + (part * p.rows_total + grow) * p.d + c0);
                 dst[0] = make_float4(acc[0], acc[1], acc[2], acc[3]);
                 dst[1] = make_float4(acc[4], acc[5], acc[6], acc[7]);
-                if (c0 == 0) p.part_lse[part * p.rows_total + grow] = lse2;
+                if (c0 == 0) p.part_sum[part * p.rows_total + grow] = make_float2(top, total * (1.f / (float)(1 << FEW_WEIGHT_BITS<T>)));
             }
         }
     }
@@ -860,10 +866,11 @@ attend_few_kernel(const __grid_constant__ CUtensorMap map_sk, const __grid_const
 
 // ---- attend_join_kernel: partial results of a row become its result ------------------
 // W warps a row, each W-th part, so that many parts are on their way at once (1,000 rows of 37 parts: 31 us with a warp a row).
-// 8 warps a CTA, or W = 32.
+// 8 warps a CTA, or W = 32.  Parts bring references and sums, not their log-sums: where scores are large, these differ by less than
+// their rounding.
 template <typename T>
-__global__ void __launch_bounds__(1024) attend_join_kernel(const float* part_o, const float* part_lse, int parts, int64_t rows, int d, int W,
-                                                          uint16_t* out, float* lse) {
+__global__ void __launch_bounds__(1024) attend_join_kernel(const float* part_o, const float2* part_sum, int parts, int64_t rows, int d, int W,
+                                                          float c, uint16_t* out, float* lse) {
     __shared__ float4 acc_s[32][32];
     __shared__ float total_s[32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -872,27 +879,27 @@ __global__ void __launch_bounds__(1024) attend_join_kernel(const float* part_o, 
     pdl_trigger();
     const bool in = row < rows;
     float top = -CUDART_INF_F;
-    bool nan = false;
+    bool some = false;
     if (in) {
         for (int i = lane; i < parts; i += 32) {
-            const float x = __ldcg(part_lse + i * rows + row);
-            top = fmaxf(top, x);
-            nan |= x != x;
+            const float2 x = __ldcg(part_sum + i * rows + row);
+            if (x.y == 0.f) continue;   // saw nothing
+            top = fmaxf(top, x.x);
+            some = true;
         }
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    nan = __any_sync(0xffffffffu, nan);
-    const bool some = top != -CUDART_INF_F || nan;
+    some = __any_sync(0xffffffffu, some);
     float total = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
     const bool mine = lane * 4 < d;
     if (in && some) {
 #pragma unroll 4
         for (int i = warp % W; i < parts; i += W) {
-            const float x = __ldcg(part_lse + i * rows + row);
-            const float w = ex2(x - top);
-            if (x == -CUDART_INF_F) continue;   // nothing was written there
+            const float2 x = __ldcg(part_sum + i * rows + row);
+            if (x.y == 0.f) continue;   // nothing was written there
+            const float w = x.y * (x.x == top ? 1.f : ex2((x.x - top) * c));
             total += w;
             if (mine) {
                 const float4 o = __ldcg(reinterpret_cast<const float4*>(part_o + (i * rows + row) * d) + lane);
@@ -922,7 +929,7 @@ __global__ void __launch_bounds__(1024) attend_join_kernel(const float* part_o, 
     if (mine)
         *reinterpret_cast<uint2*>(out + row * d + lane * 4) =
                 make_uint2(pack2<T>(acc.x * inv, acc.y * inv), pack2<T>(acc.z * inv, acc.w * inv));
-    if (lane == 0 && lse) lse[row] = some ? (top + log2f(total)) * kLn2 : -CUDART_INF_F;
+    if (lane == 0 && lse) lse[row] = some ? ((top == -CUDART_INF_F ? 0.f : top * c) + log2f(total)) * kLn2 : -CUDART_INF_F;
 }
 
 // ---- host ---------------------------------------------------------------------------------------
@@ -1048,7 +1055,7 @@ AttendPlan plan_attend(const B200FAttendArgs& a) {
     const int64_t rows = a.batch * a.queries * a.heads;
     pl.scratch = 256;
     if (pl.sums) pl.scratch = (size_t)(256 + rows * a.d * 4);
-    if (pl.parts > 1) pl.scratch = (size_t)(round_up64(pl.parts * rows * 4, 256) + pl.parts * rows * a.d * 4);
+    if (pl.parts > 1) pl.scratch = (size_t)(round_up64(pl.parts * rows * 8, 256) + pl.parts * rows * a.d * 4);
     return pl;
 }
 
@@ -1083,8 +1090,8 @@ int launch_attend(const CUtensorMap* maps, const TileParams& p, const AttendPlan
     if (e == cudaSuccess && pl.parts > 1) {
         const int W = pl.parts > 64 ? 32 : pl.parts > 16 ? 8 : pl.parts > 8 ? 4 : pl.parts > 4 ? 2 : 1, warps = W > 8 ? W : 8;
         e = launch_kernel(attend_join_kernel<T>, dim3((unsigned)ceil_div64(p.rows_total, warps / W)), 32 * warps, 0, Launch(st, true),
-                          static_cast<const float*>(p.part_o), static_cast<const float*>(p.part_lse), pl.parts, p.rows_total, p.d, W, p.out,
-                          p.lse);
+                          static_cast<const float*>(p.part_o), static_cast<const float2*>(p.part_sum), pl.parts, p.rows_total, p.d, W,
+                          p.scale * kLog2e, p.out, p.lse);
         count_launch();
     }
     if (e != cudaSuccess) {
@@ -1146,8 +1153,8 @@ extern "C" int b200f_attend(const B200FAttendArgs* a) {
     p.lse = a->lse;
     p.status = a->status;
     if (pl.parts > 1) {
-        p.part_lse = static_cast<float*>(a->scratch);
-        p.part_o = p.part_lse + round_up64(pl.parts * p.rows_total, 64);
+        p.part_sum = static_cast<float2*>(a->scratch);
+        p.part_o = static_cast<float*>(a->scratch) + round_up64(pl.parts * p.rows_total * 2, 64);
     }
     if (pl.sums) p.sums = static_cast<float*>(a->scratch);
     const cudaStream_t st = (cudaStream_t)a->stream;

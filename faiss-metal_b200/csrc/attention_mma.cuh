@@ -182,20 +182,23 @@ __device__ __forceinline__ float2 ex2_fma(float2 y) {
                        __uint_as_float(__float_as_uint(r.y) * 8388608u + __float_as_uint(z.y)));
 }
 
-// w = exp2(x c + mc) of 32 values, packed; returns their sums.  In groups of eight, and each step for the whole group before the next:
+// w = exp2((x - from) c + mc) of 32 values, packed; returns their sums.  MIX: from is 0.  In groups of eight, and each step for the whole group before the next:
 // the compiler keeps this order, and an exponential's result takes some 40 cycles (a warp alone on its scheduler: 1,090
 // cycles for 64 values step by step, 600 this way; the exponential unit takes 512).
 // MIX: two of eight by ex2_fma, which takes the load off that unit; -INF gives 2^-126, +INF and NaN a large sum.
 template <typename T, bool MIX>
-__device__ __forceinline__ float2 weigh32(const uint32_t (&x)[32], float c, float mc, uint32_t* w) {
+__device__ __forceinline__ float2 weigh32(const uint32_t (&x)[32], float c, float mc, float from, uint32_t* w) {
     const float2 c2 = make_float2(c, c), mc2 = make_float2(mc, mc);
     float2 add[4];
 #pragma unroll
     for (int g = 0; g < 16; g += 4) {
         float2 y[4];
 #pragma unroll
-        for (int e = 0; e < 4; e++)
-            y[e] = fma2(make_float2(__uint_as_float(x[2 * (g + e)]), __uint_as_float(x[2 * (g + e) + 1])), c2, mc2);
+        for (int e = 0; e < 4; e++) {
+            y[e] = make_float2(__uint_as_float(x[2 * (g + e)]), __uint_as_float(x[2 * (g + e) + 1]));
+            if (!MIX) y[e] = add2(y[e], make_float2(-from, -from));
+            y[e] = fma2(y[e], c2, mc2);
+        }
 #pragma unroll
         for (int e = 0; e < (MIX ? 3 : 4); e++) {
             y[e].x = ex2(y[e].x);

@@ -339,6 +339,8 @@ int b200f_remap_labels_block_cyclic(int64_t* labels, int64_t count, int64_t bloc
  * A query that sees nothing has output 0 and log-sum -INF.  A value within its sequence's length that is infinite or NaN may reach
  * any query of the sequence, those before it included: their weight is 0, and 0 * NaN is NaN.  A score that leaves fp32's range when it is
  * multiplied by scale * log2(e) counts as infinite: +INF makes its row NaN, a key of -INF weighs nothing.
+ * Weights of the forward pass come from differences of scores, however large these are; the gradient and the accumulated weights take theirs
+ * from the fp32 log-sum, exp(s - lse), good to 2^-22 |lse| of themselves.
  *
  * Arithmetic: products of 16-bit operands, fp32 accumulation; weights and, in the backward pass, score
  * gradients are rounded to the operands' type before they are multiplied; sums, log-sums and normalisation

@@ -439,3 +439,33 @@ def test_evicted_rows_and_rows_behind_the_end_do_not_come_through(fm):
     k2 = k.clone()
     k2[0, -1] = math.nan                                     # among the recent ones
     assert torch.isnan(fm.evict(k2, v, m, n, keep, recent=5)[0][0, keep - 1]).all()
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("scale", [1.0, 3e3, 7e5, 1e8, 3e12, 1e20, 1e30, 1e37])
+@pytest.mark.parametrize("lq,lk", [(4, 300), (700, 300), (700, 1200), (60, 9000)])
+def test_ties_of_large_scores(fm, lq, lk, scale, dtype):
+    """Keys of equal score, whatever its size, share a row: at the end of a rise, in different tiles, warps and ranges.  Scores are products of two
+    numbers, exact in fp32; the next lower one lies a sixteenth below."""
+    dt = TYPES[dtype]
+    a, c = (torch.tensor(x, dtype=dt).item() for x in (1.1, 0.7))
+    q = torch.zeros(1, lq, 1, 64, dtype=dt, device="cuda")
+    q[..., 0] = a
+    q[0, 1::2] *= -1
+    k, v = torch.zeros(1, lk, 1, 64, dtype=dt, device="cuda"), rand(3, dt, 1, lk, 1, 64)
+    k[..., 0] = torch.linspace(-0.9, 0.9, lk, device="cuda").to(dt).clamp(-c + c / 16, c - c / 16).view(1, lk, 1)
+    ties = torch.tensor([3, 17, 40, 129, 200, lk // 2, lk - 20, lk - 1], device="cuda").unique()
+    k[0, ties, 0, 0] = c
+    lows = torch.tensor([2, 30, 131, lk // 2 + 1, lk - 3], device="cuda").unique()
+    k[0, lows, 0, 0] = -c
+    out, lse = fm.attend(q, k, v, scale=scale, return_lse=True)
+    # with the maximum taken off first: at 1e20 a 64-bit log-sum does not hold the number of ties any more
+    s = R.scores(q, k, None, scale, False)
+    p, vv = torch.softmax(s, -1), R.heads_first(v, 1)
+    want, size, want_lse = (p @ vv).permute(0, 2, 1, 3), (p @ vv.abs()).permute(0, 2, 1, 3), torch.logsumexp(s, -1).permute(0, 2, 1)
+    u = unit(dt)
+    # scores are held to 2^-24 of themselves where tiles, warps and ranges meet; beyond 2^13 only equal ones share a row
+    near = min(abs(a * c * scale) * 2.0 ** -22, 0.0 if a * c * scale / 16 > 30 else 1.0)
+    assert ((out.double() - want).abs() <= u * want.abs() + (1.1 * u + near + 3e-6) * size + 2.0 ** -24).all()
+    assert ((lse.double() - want_lse).abs() <= 1e-6 * want_lse.abs() + 2e-5).all()
+    fm.check_attention_status()
