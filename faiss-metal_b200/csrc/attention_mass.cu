@@ -11,14 +11,13 @@ namespace {
 // Scores with the keys in the rows of the tile, S = K Q^T, so that a key belongs to a thread and its weights are added up in a
 // register.  FEW (all query rows of a key head in one tile): the queries stay in shared memory, key tiles stream past: one read of
 // the keys is the bound.  Else a key tile stays and tiles of query rows stream past; exponentials bound it.  S has two buffers, each with
-// its own four warps.  Two CTAs share an SM, so that one's start and end hide behind the other.  With FEW, d > 64 and
-// more than 48 packed rows a CTA has an SM to itself: its three key tiles and query rows take more than half of the shared memory.
+// its own four warps.  Two CTAs share an SM, so that one's start and end hide behind the other.
 // Measured: FEW (bf16, d = 128, 32 sequences of one query, 32 heads on 8 key heads, up to 8,192 keys) 57 us, 5.7 TB/s; else (fp16, d = 64, 2 x 1,111
 // queries, 16 heads on 4 key heads, 2,049 keys) 37 us.  A quarter of the exponentials by ex2_fma, or loads of S in two buffers: 7 %
 // slower.
 constexpr int MASS_THREADS = 384;   // TMA, MMA, two warps for log-sums; 2 x 4 warps
 constexpr int MASS_SLOTS = 128;     // query rows of a tile
-constexpr int MASS_RING = 5;        // streamed tiles at most (launch_mass)
+constexpr int MASS_RING = 5;        // streamed tiles at most: what half an SM's shared memory takes (launch_mass)
 constexpr int MASS_STATS = 4;       // query tiles whose log-sums are fetched ahead
 constexpr int MASS_STAT = MASS_STATS * MASS_SLOTS * 8;
 
@@ -364,7 +363,9 @@ int check_mass(const B200FAttentionMassArgs* a) {
 template <typename T, int DP, bool FEW>
 int launch_mass(const CUtensorMap* maps, MassParams p, int64_t items, cudaStream_t st) {
     const int key_bytes = DP / 64 * ATT_CHUNK, query_bytes = DP / 64 * p.cols * 128;   // multiples of 1024
-    p.ring = DP == 64 ? 5 : FEW ? 3 : 2;
+    // two CTAs an SM: with more than 48 query rows of d > 64 a third key tile would leave room for one (16 x 8,192 keys of 8 heads, 52 / 64 /
+    // 128 rows: 71.3 / 72.1 / 87.4 us with three, 54.4 / 54.7 / 65.4 us with two)
+    p.ring = DP == 64 ? 5 : FEW && p.cols <= 48 ? 3 : 2;
     p.a_off = 0;
     p.ring_off = FEW ? query_bytes : key_bytes;
     p.stage = FEW ? key_bytes : query_bytes;

@@ -469,3 +469,21 @@ def test_ties_of_large_scores(fm, lq, lk, scale, dtype):
     assert ((out.double() - want).abs() <= u * want.abs() + (1.1 * u + near + 3e-6) * size + 2.0 ** -24).all()
     assert ((lse.double() - want_lse).abs() <= 1e-6 * want_lse.abs() + 2e-5).all()
     fm.check_attention_status()
+
+
+# ---- accumulated weights of every number of rows in a tile ------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("lq,h,hk", [(12, 8, 2), (49, 2, 2), (13, 8, 2), (16, 16, 4), (97, 1, 1), (1, 128, 1), (32, 8, 2)])
+def test_accumulated_weights_of_wide_rows(fm, lq, h, hk, dtype):
+    # 48 to 128 packed rows of d = 128 over many key tiles: the rings of three and of two
+    dt = TYPES[dtype]
+    b, lk, d = 3, 3333, 128
+    q, k, n = rand(1, dt, b, lq, h, d, scale=1.5), rand(2, dt, b, lk, hk, d), lens(3333, 1024, 129)
+    for causal in (False, True):
+        lse = R.softmax(R.scores(q, k, n, 1 / math.sqrt(d), causal))[1].permute(0, 2, 1).float().contiguous()
+        got, want = fm.attention_mass(q, k, lse, key_lengths=n, causal=causal), R.mass(q, k, lse, n, causal=causal)
+        assert ((got.double() - want).abs() <= 1e-5 * want.abs() + 1e-7).all()
+        assert torch.equal(got, fm.attention_mass(q, k, lse, key_lengths=n, causal=causal))
+    fm.check_attention_status()
