@@ -20,7 +20,7 @@ namespace {
 // keys go to the tensor cores while those of the others are computed.
 // d <= 64 leaves tensor memory for P beside S (APART): the next scores are computed as soon as these are in registers, and the way
 // round is the softmax alone.
-// Measured (bf16, d = 128, 8 x 2,048 queries of 16 heads on 4 key heads, 4,096 keys): 500 us, 1,100 TFLOP/s, at the 1.48 GHz that
+// Measured (bf16, d = 128, 8 x 2,048 queries of 16 heads on 4 key heads, 4,096 keys): 513 us, 1,070 TFLOP/s, at the 1.48 GHz that
 // the power limit leaves; 2,820 cycles for both streams' tiles, 2,048 of them of the tensor cores.  Slower when measured
 // against the kernel of that time: tiles of 64 keys in two buffers a stream (789 us against 620), two threads a row (3,640 cycles
 // against 3,360), an issuing warp a stream (647 us against 588).

@@ -20,7 +20,7 @@ namespace {
 // Products of 64 columns with both operands in shared memory run at 2/3 of the full rate, which its bandwidth bounds: KEYS spends 1,280
 // of its 1,326 cycles a tile on them (1,024 at full rate), tensor memory being full.  Without acc2 there is room: A1 and A2 lie in
 // tensor memory, and 768 of a tile's 923 cycles are the tensor cores'.
-// Measured (bf16, d = 128, 8 x 2,048 queries of 16 heads on 4 key heads, 4,096 keys): 1,660 us, 830 TFLOP/s of the 5 products that the
+// Measured (bf16, d = 128, 8 x 2,048 queries of 16 heads on 4 key heads, 4,096 keys): 1,650 us, 830 TFLOP/s of the 5 products that the
 // gradient needs, 1,160 of the 7 that run, at the clock that the power limit leaves.
 constexpr int GRAD_THREADS = 384;   // TMA, MMA, two spare warps; 2 x 4 warps
 constexpr int GRAD_ROWS = 64;       // rows of a streamed tile
@@ -122,8 +122,8 @@ __device__ __forceinline__ UnitRange unit_range(const uint32_t* range, int64_t u
 
 // Score gradients of 32 columns from `col` on, ds = p (dp - delta), and the weights p.  KEYS: the columns' statistics lie at `mstat` in shared
 // memory, minus log-sums, minus deltas and, fp16, what undoes the move of the query row, 2^-x: c and `factor` are of rows that were not
-// moved, the deltas hold their factor already (16 bits are enough for a power of two, and the products leave shared memory little time: fp16,
-// the case measured above, 1,610 us with both factors read as floats, 1,570 so, 1,475 without any).  Else the row's own.  Steps by groups, as in weigh32.
+// moved, the deltas hold their factor already (16 bits are enough for a power of two, and the products leave shared memory little time: the
+// case measured above in fp16, L2 flushed in between, 1,610 us with both factors read as floats, 1,570 so, 1,475 without any).  Else the row's own.  Steps by groups, as in weigh32.
 template <typename T, bool KEYS>
 __device__ __forceinline__ void grad32(const uint32_t (&s)[32], const uint32_t (&dp)[32], float c, float factor, uint32_t mstat, int col,
                                        float mlse, float mdelta, uint32_t (&wp)[16], uint32_t (&ws)[16]) {
