@@ -21,7 +21,7 @@ namespace {
 // d <= 64 leaves tensor memory for P beside S (APART): the next scores are computed as soon as these are in registers, and the way
 // round is the softmax alone.
 // Measured (bf16, d = 128, 8 x 2,048 queries of 16 heads on 4 key heads, 4,096 keys): 513 us, 1,070 TFLOP/s, at the 1.48 GHz that
-// the power limit leaves; 2,820 cycles for both streams' tiles, 2,048 of them of the tensor cores.  Slower when measured
+// the power limit leaves; 2,850 cycles for both streams' tiles, 2,048 of them of the tensor cores.  Slower when measured
 // against the kernel of that time: tiles of 64 keys in two buffers a stream (789 us against 620), two threads a row (3,640 cycles
 // against 3,360), an issuing warp a stream (647 us against 588).
 constexpr int TILE_THREADS = 384;          // TMA, MMA, two spare warps (setmaxnreg is by four); 2 x 4 softmax warps
